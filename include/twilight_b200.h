@@ -464,6 +464,138 @@ int tw_decode_attention_noalloc(const void* q, const void* k, const void* v,
                                 int max_seqlen_k, int head_dim, int dtype, float softmax_scale,
                                 void* out, int out_dtype, float* lse, void* stream);
 
+/* ---- paged KV cache: step plan, row write, attention -------------------------------------------------
+ * No counterpart in the reference, whose cache is one contiguous slab per head
+ * (hi/slab_cache.py:37-74) and whose prompt attention is the model's own: an
+ * addition of this library for several requests that share a pool of pages in
+ * device memory, and for prompts that are processed in chunks.
+ *
+ * POOL.  Page i holds page_size token rows of every KV head; row o of head h
+ * of page i is at k_pages / v_pages + i*page_stride + h*head_stride +
+ * o*token_stride elements (head_dim contiguous elements), the same strides for
+ * K and V.  Both [page][head][row][D] and [page][row][head][D] orders are such
+ * strides, and so are K and V interleaved in one allocation.  Pointers are
+ * 16-byte aligned, strides positive multiples of 8 elements.
+ * BLOCK TABLE.  Token j of request b is row j % page_size of page
+ * block_table[b*table_stride + j / page_size].  Entries past the request's
+ * last page are never read.  SLOT = page*page_size + row (int64); -1: none. */
+typedef struct tw_paged_pool {
+  void* k_pages;
+  void* v_pages;
+  int64_t page_stride;
+  int64_t head_stride;
+  int64_t token_stride;
+  int64_t num_pages;
+  int32_t page_size;
+  int32_t kv_heads;
+  int32_t head_dim;  /* 128 */
+  int32_t dtype;     /* TW_F16 / TW_BF16 */
+} tw_paged_pool;
+size_t tw_paged_pool_size(void);
+
+/* One serving step's block tables and slot map, built on the device in one
+ * launch from the requests' lengths.  lens [B]: tokens held; new_lens [B]:
+ * tokens to add, or < 0 for a request that has ended.  free_pages [num_pages]
+ * with *free_count entries is a stack of unused pages.
+ *   1. Ended requests' pages are pushed on the stack in request order (their
+ *      kv_lens become 0; their table rows stay as they are).
+ *   2. In request order each request takes the pages its new tokens need from
+ *      the top of the stack and gets them written to its table row.  A request
+ *      whose pages would not fit the table's width is refused, and so is,
+ *      once the pages wanted so far exceed the stack, each one that wants any:
+ *      it keeps its old length, its tokens get slot -1, and *error_flag
+ *      becomes TW_ERR_CAPACITY.
+ *   3. kv_lens [B] = lens + new_lens, cu_q [B+1] = prefix sums of the new
+ *      lengths, *free_count_out = pages left, and for each new token (rows
+ *      cu_q[b] .. cu_q[b+1]) slots / positions [tokens_cap]: its slot and its
+ *      position in its request.  Rows past the last token get slot -1 and
+ *      position 0; more tokens than tokens_cap set TW_ERR_CAPACITY.
+ * A page id outside [0, num_pages) that a token would be given sets
+ * TW_ERR_INVALID_INDEX and slot -1.  *error_flag keeps the largest code.
+ * Outputs must not overlap inputs other than block_table and free_pages, which
+ * are updated in place; a repeated call on the same inputs gives the same
+ * outputs.  requests <= 8192. */
+typedef struct tw_paged_step_args {
+  const int32_t* lens;
+  const int32_t* new_lens;
+  int32_t* block_table;
+  int64_t table_stride;
+  int32_t table_width;
+  int32_t requests;
+  int32_t page_size;
+  int32_t tokens_cap;
+  int32_t* free_pages;
+  int64_t num_pages;
+  const int32_t* free_count;
+  int32_t* kv_lens;
+  int32_t* cu_q;
+  int64_t* slots;
+  int32_t* positions;
+  int32_t* free_count_out;
+  int32_t* error_flag;
+} tw_paged_step_args;
+int tw_paged_step(const tw_paged_step_args* args, void* stream);
+size_t tw_paged_step_args_size(void);
+
+/* Rows k / v [tokens][kv_heads][D] (element strides given, D contiguous) to
+ * their slots of the pool.  Slot -1 is skipped; another slot outside the pool
+ * is skipped and sets *error_flag.  Two equal slots leave one of the rows. */
+int tw_paged_write(const tw_paged_pool* pool, const void* k, int64_t k_token_stride,
+                   int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                   int64_t v_head_stride, const int64_t* slots, int64_t tokens,
+                   int32_t* error_flag, void* stream);
+
+/* Attention of each request's new tokens (rows [cu_q[b], cu_q[b+1]) of q and
+ * out) over its paged tokens, the new ones included: kv_lens[b] counts them.
+ * Row i of a request with n rows is at position p = kv_lens[b] - n + i and
+ * sees the keys [max(0, p - window + 1), p] (window 0: [0, p]), none when
+ * p < 0:
+ *   out[t][h] = softmax(scale * q[t][h] . K^T) . V,  lse = log sum exp
+ * with KV head h / (q_heads / kv_heads).  A row that sees no key, and every
+ * row at or past cu_q[B], gets out 0 and lse -inf.  What rows the mask hides
+ * hold (NaN included) does not reach a result.
+ * tokens: rows of q and out, at least cu_q[B] (which may be less: padding).
+ * max_q_len, max_kv_len: upper bounds of the requests' lengths (they size the
+ * launch); a longer request sets *error_flag to TW_ERR_BAD_ARG and its rows
+ * are not computed.  A page id outside the pool sets TW_ERR_INVALID_INDEX and
+ * is not read (its keys count as zero rows), and so does a kv_len beyond the
+ * table (which is cut).  workspace: >= tw_paged_attention_workspace_size(...)
+ * bytes, 16-byte aligned, no initial content; calls that share one must not
+ * overlap.  out_dtype: the pool's dtype or TW_F32.  lse, error_flag may be
+ * NULL.  page_size a multiple of 8, q_heads / kv_heads <= 64; q and out
+ * 16-byte aligned, their strides multiples of 8 elements. */
+typedef struct tw_paged_attention_args {
+  tw_paged_pool pool;
+  const void* q;
+  int64_t q_token_stride;
+  int64_t q_head_stride;
+  const int32_t* block_table;
+  int64_t table_stride;
+  int32_t table_width;
+  int32_t requests;
+  const int32_t* cu_q;
+  const int32_t* kv_lens;
+  int32_t tokens;
+  int32_t q_heads;
+  int32_t max_q_len;
+  int32_t max_kv_len;
+  int32_t window;
+  float softmax_scale;
+  void* out;
+  int64_t out_token_stride;
+  int64_t out_head_stride;
+  int32_t out_dtype;
+  int32_t reserved; /* 0 */
+  float* lse;       /* [tokens][q_heads] or NULL */
+  int32_t* error_flag;
+  void* workspace;
+  size_t workspace_bytes;
+} tw_paged_attention_args;
+size_t tw_paged_attention_workspace_size(int requests, int tokens, int q_heads, int kv_heads,
+                                         int max_q_len, int max_kv_len, int head_dim);
+int tw_paged_attention(const tw_paged_attention_args* args, void* stream);
+size_t tw_paged_attention_args_size(void);
+
 #ifdef __cplusplus
 }
 #endif

@@ -65,6 +65,41 @@ class RowReuse(ctypes.Structure):
     ]
 
 
+class PagedPool(ctypes.Structure):
+    """tw_paged_pool of include/twilight_b200.h."""
+
+    _fields_ = [
+        ("k_pages", P), ("v_pages", P), ("page_stride", I64), ("head_stride", I64),
+        ("token_stride", I64), ("num_pages", I64), ("page_size", I32T), ("kv_heads", I32T),
+        ("head_dim", I32T), ("dtype", I32T),
+    ]
+
+
+class PagedStepArgs(ctypes.Structure):
+    """tw_paged_step_args of include/twilight_b200.h."""
+
+    _fields_ = [
+        ("lens", P), ("new_lens", P), ("block_table", P), ("table_stride", I64),
+        ("table_width", I32T), ("requests", I32T), ("page_size", I32T), ("tokens_cap", I32T),
+        ("free_pages", P), ("num_pages", I64), ("free_count", P), ("kv_lens", P), ("cu_q", P),
+        ("slots", P), ("positions", P), ("free_count_out", P), ("error_flag", P),
+    ]
+
+
+class PagedAttentionArgs(ctypes.Structure):
+    """tw_paged_attention_args of include/twilight_b200.h."""
+
+    _fields_ = [
+        ("pool", PagedPool), ("q", P), ("q_token_stride", I64), ("q_head_stride", I64),
+        ("block_table", P), ("table_stride", I64), ("table_width", I32T), ("requests", I32T),
+        ("cu_q", P), ("kv_lens", P), ("tokens", I32T), ("q_heads", I32T), ("max_q_len", I32T),
+        ("max_kv_len", I32T), ("window", I32T), ("softmax_scale", FLT), ("out", P),
+        ("out_token_stride", I64), ("out_head_stride", I64), ("out_dtype", I32T),
+        ("reserved", I32T), ("lse", P), ("error_flag", P), ("workspace", P),
+        ("workspace_bytes", SZ),
+    ]
+
+
 # name -> (restype, argtypes); mirrors include/twilight_b200.h
 SIGNATURES = {
     "tw_status_string": (ctypes.c_char_p, [I32]),
@@ -104,6 +139,13 @@ SIGNATURES = {
     "tw_row_reuse_size": (SZ, []),
     "tw_qkv_rope": (I32, [P, P, P, P, I32, I32, I32, I32, P, P, I32, P, P, P, P]),
     "tw_decode_attention_noalloc": (I32, [P, P, P, P, I32, I32, I32, I32, I32, FLT, P, I32, P, P]),
+    "tw_paged_pool_size": (SZ, []),
+    "tw_paged_step": (I32, [ctypes.POINTER(PagedStepArgs), P]),
+    "tw_paged_step_args_size": (SZ, []),
+    "tw_paged_write": (I32, [ctypes.POINTER(PagedPool), P, I64, I64, P, I64, I64, P, I64, P, P]),
+    "tw_paged_attention_workspace_size": (SZ, [I32, I32, I32, I32, I32, I32, I32]),
+    "tw_paged_attention": (I32, [ctypes.POINTER(PagedAttentionArgs), P]),
+    "tw_paged_attention_args_size": (SZ, []),
 }
 
 _lib = None

@@ -324,3 +324,177 @@ def qkv_rope(hidden: torch.Tensor, w_q: torch.Tensor, w_k: torch.Tensor, w_v: to
         _ptr(hidden), _ptr(w_q), _ptr(w_k), _ptr(w_v), H, n_q, n_kv, HEAD_DIM, _ptr(cos), _ptr(sin),
         _kv_code(dt), _ptr(q_out), _ptr(k_out), _ptr(v_out), _stream(hidden.device)), "qkv_rope")
     return q_out, k_out, v_out
+
+
+# ------------------------------------------------------------- paged cache --
+
+def _i32(name: str, t: torch.Tensor, *shape: int | None) -> None:
+    """t is an int32 CUDA tensor of this shape (None: any extent), rows contiguous."""
+    if not t.is_cuda:
+        raise ValueError("twilight ops require CUDA tensors (no CPU fallback)")
+    if t.dtype != torch.int32 or t.dim() != len(shape) or (t.shape[-1] > 1 and t.stride(-1) != 1) \
+            or any(n is not None and n != m for n, m in zip(shape, t.shape)):
+        want = ", ".join("*" if n is None else str(n) for n in shape)
+        raise ValueError(f"{name} must be int32 [{want}] with contiguous rows, "
+                         f"got {t.dtype} {tuple(t.shape)}")
+
+
+def _same_device(device: torch.device, *tensors: torch.Tensor | None) -> None:
+    if any(t is not None and t.device != device for t in tensors):
+        raise ValueError("all tensors of a call must be on one CUDA device")
+    if device.index != torch.cuda.current_device():
+        raise ValueError(f"the tensors are on {device}: make it the current device")
+
+
+def _rows_strides(name: str, t: torch.Tensor) -> tuple[int, int]:
+    """(token, head) strides of [tokens, heads, 128] rows; an extent of 1 has none of its own."""
+    token, head, inner = t.stride()
+    if inner != 1:
+        raise ValueError(f"{name} needs contiguous rows of {HEAD_DIM} elements")
+    if t.shape[1] <= 1:
+        head = HEAD_DIM
+    if t.shape[0] <= 1:
+        token = head * max(t.shape[1], 1)
+    if token <= 0 or head <= 0 or token % 8 or head % 8 or t.data_ptr() % 16:
+        raise ValueError(f"{name} needs 16-byte aligned rows (positive strides in multiples of 8)")
+    return token, head
+
+
+def _paged_pool(k_pages: torch.Tensor, v_pages: torch.Tensor) -> "_lib.PagedPool":
+    """tw_paged_pool of [pages, kv_heads, page_size, 128] tensors (any order of strides)."""
+    if not (k_pages.is_cuda and v_pages.is_cuda):
+        raise ValueError("twilight ops require CUDA tensors (no CPU fallback)")
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype \
+            or k_pages.shape[3] != HEAD_DIM or 0 in k_pages.shape:
+        raise ValueError(f"k_pages and v_pages must be [pages, kv_heads, page_size, {HEAD_DIM}] "
+                         "of one dtype")
+    pages, heads, size, _ = k_pages.shape
+    strides = []
+    for i, (n, s, t) in enumerate(zip(k_pages.shape, k_pages.stride(), v_pages.stride())):
+        if n > 1 and s != t:
+            raise ValueError("k_pages and v_pages must have the same strides")
+        # a dimension of one page, head or row has no stride of its own
+        strides.append(s if n > 1 else HEAD_DIM)
+    if strides[3] != 1 or any(s <= 0 or s % 8 for s in strides[:3]) or \
+            (k_pages.data_ptr() | v_pages.data_ptr()) % 16:
+        raise ValueError("pages need contiguous 16-byte aligned rows (strides in multiples of 8)")
+    return _lib.PagedPool(k_pages.data_ptr(), v_pages.data_ptr(), strides[0], strides[1],
+                          strides[2], pages, size, heads, HEAD_DIM, _kv_code(k_pages.dtype))
+
+
+def paged_step(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor,
+               free_pages: torch.Tensor, free_count: torch.Tensor, *, page_size: int,
+               kv_lens: torch.Tensor, cu_q: torch.Tensor, slots: torch.Tensor,
+               positions: torch.Tensor, free_count_out: torch.Tensor,
+               error_flag: torch.Tensor | None = None) -> None:
+    """Block tables and slot map of one serving step, in one launch (tw_paged_step).
+
+    lens / new_lens [B] int32 (tokens held, tokens to add; new < 0: the request
+    has ended and its pages go back), block_table [B, W] and the page stack
+    free_pages [num_pages] with free_count [1] entries are updated; outputs
+    kv_lens [B], cu_q [B+1], free_count_out [1] and, per new token, slots
+    (int64, -1: none) and positions [tokens_cap].  A refused request or a full
+    output sets error_flag to TW_ERR_CAPACITY."""
+    B = lens.shape[0] if lens.dim() == 1 else -1
+    _i32("lens", lens, None)
+    _i32("new_lens", new_lens, B)
+    _i32("block_table", block_table, B, None)
+    _i32("free_pages", free_pages, None)
+    _i32("free_count", free_count, 1)
+    _i32("kv_lens", kv_lens, B)
+    _i32("cu_q", cu_q, B + 1)
+    _i32("free_count_out", free_count_out, 1)
+    if slots.dtype != torch.int64 or slots.dim() != 1 or not slots.is_contiguous():
+        raise ValueError("slots must be int64 [tokens_cap]")
+    _i32("positions", positions, slots.shape[0])
+    _same_device(lens.device, new_lens, block_table, free_pages, free_count, kv_lens, cu_q, slots,
+                 positions, free_count_out, error_flag)
+    W = block_table.shape[1]
+    args = _lib.PagedStepArgs(
+        lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(),
+        block_table.stride(0) if B > 1 else W, W, B, page_size, slots.shape[0],
+        free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(), kv_lens.data_ptr(),
+        cu_q.data_ptr(), slots.data_ptr(), positions.data_ptr(), free_count_out.data_ptr(),
+        _ptr(error_flag))
+    _lib.check(lib().tw_paged_step(ctypes.byref(args), _stream(lens.device)), "paged_step")
+
+
+def paged_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_pages: torch.Tensor,
+                v_pages: torch.Tensor, *, error_flag: torch.Tensor | None = None) -> None:
+    """New rows k / v [T, kv_heads, 128] (strided views of a projection are fine) to
+    slots [T] int64 of the pool [pages, kv_heads, page_size, 128] (tw_paged_write);
+    slot -1 is skipped."""
+    pool = _paged_pool(k_pages, v_pages)
+    if k.dim() != 3 or k.shape != v.shape or k.shape[1:] != (pool.kv_heads, HEAD_DIM) or \
+            k.dtype != k_pages.dtype or v.dtype != k_pages.dtype:
+        raise ValueError("k and v must be [T, kv_heads, 128] in the pool's dtype")
+    if slots.dtype != torch.int64 or slots.shape != k.shape[:1] or not slots.is_contiguous():
+        raise ValueError("slots must be int64 [T]")
+    _same_device(k_pages.device, v_pages, k, v, slots, error_flag)
+    _lib.check(lib().tw_paged_write(
+        ctypes.byref(pool), k.data_ptr(), *_rows_strides("k", k), v.data_ptr(),
+        *_rows_strides("v", v), slots.data_ptr(), k.shape[0], _ptr(error_flag),
+        _stream(k_pages.device)), "paged_write")
+
+
+def paged_attention_workspace_bytes(requests: int, tokens: int, q_heads: int, kv_heads: int,
+                                    max_q_len: int, max_kv_len: int) -> int:
+    return int(lib().tw_paged_attention_workspace_size(requests, tokens, q_heads, kv_heads,
+                                                       max_q_len, max_kv_len, HEAD_DIM))
+
+
+def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                    block_table: torch.Tensor, cu_q: torch.Tensor, kv_lens: torch.Tensor, *,
+                    max_q_len: int, max_kv_len: int, window: int = 0,
+                    softmax_scale: float | None = None, out: torch.Tensor | None = None,
+                    out_dtype: torch.dtype | None = None, lse: torch.Tensor | None = None,
+                    workspace: torch.Tensor | None = None,
+                    error_flag: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention of each request's new tokens over its paged tokens, the
+    new ones included (tw_paged_attention): one token each, chunks of prompts,
+    or both in one call.
+
+    q [T, q_heads, 128] (token and head strides free), pool [pages, kv_heads,
+    page_size, 128], block_table [B, W] int32, cu_q [B+1] and kv_lens [B] int32
+    on the device; max_q_len / max_kv_len bound the requests' lengths.  window
+    > 0: each token sees the last `window` positions only.  Returns out
+    [T, q_heads, 128] (q's dtype or float32); lse [T, q_heads] fp32 receives the
+    log-sum-exp.  Without a workspace one is allocated for the call."""
+    pool = _paged_pool(k_pages, v_pages)
+    if q.dim() != 3 or q.shape[2] != HEAD_DIM or q.dtype != k_pages.dtype or \
+            q.shape[1] == 0 or q.shape[1] % pool.kv_heads:
+        raise ValueError("q must be [T, q_heads, 128] in the pool's dtype, q_heads a multiple of "
+                         "kv_heads")
+    T, Hq, _ = q.shape
+    _i32("kv_lens", kv_lens, None)
+    B = kv_lens.shape[0]
+    _i32("cu_q", cu_q, B + 1)
+    _i32("block_table", block_table, B, None)
+    if out is None:
+        out = torch.empty((T, Hq, HEAD_DIM), dtype=out_dtype or q.dtype, device=q.device)
+    elif out.shape != q.shape or (out_dtype is not None and out.dtype != out_dtype):
+        raise ValueError("out must have q's shape (and out_dtype)")
+    if out.dtype not in (q.dtype, torch.float32):
+        raise ValueError("out must have q's dtype or float32")
+    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (T, Hq)
+                            or not lse.is_contiguous()):
+        raise ValueError("lse must be float32 [T, q_heads]")
+    if workspace is None:
+        need = paged_attention_workspace_bytes(B, T, Hq, pool.kv_heads, max_q_len, max_kv_len)
+        if need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    elif not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous")
+    _same_device(q.device, k_pages, v_pages, block_table, cu_q, kv_lens, out, lse, workspace,
+                 error_flag)
+    W = block_table.shape[1]
+    args = _lib.PagedAttentionArgs(
+        pool, q.data_ptr(), *_rows_strides("q", q), block_table.data_ptr(),
+        block_table.stride(0) if B > 1 else W, W, B, cu_q.data_ptr(), kv_lens.data_ptr(), T, Hq,
+        max_q_len, max_kv_len, window,
+        softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(HEAD_DIM),
+        out.data_ptr(), *_rows_strides("out", out), DTYPE_CODES[out.dtype], 0, _ptr(lse),
+        _ptr(error_flag), _ptr(workspace),
+        0 if workspace is None else workspace.numel() * workspace.element_size())
+    _lib.check(lib().tw_paged_attention(ctypes.byref(args), _stream(q.device)), "paged_attention")
+    return out
