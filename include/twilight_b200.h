@@ -478,7 +478,8 @@ int tw_decode_attention_noalloc(const void* q, const void* k, const void* v,
  * 16-byte aligned, strides positive multiples of 8 elements.
  * BLOCK TABLE.  Token j of request b is row j % page_size of page
  * block_table[b*table_stride + j / page_size].  Entries past the request's
- * last page are never read.  SLOT = page*page_size + row (int64); -1: none. */
+ * last page, and those of pages that no row sees any more (window), are never
+ * used.  SLOT = page*page_size + row (int64); -1: none. */
 typedef struct tw_paged_pool {
   void* k_pages;
   void* v_pages;
@@ -555,9 +556,10 @@ int tw_paged_write(const tw_paged_pool* pool, const void* k, int64_t k_token_str
  * row at or past cu_q[B], gets out 0 and lse -inf.  What rows the mask hides
  * hold (NaN included) does not reach a result.
  * tokens: rows of q and out, at least cu_q[B] (which may be less: padding).
- * max_q_len, max_kv_len: upper bounds of the requests' lengths (they size the
- * launch); a longer request sets *error_flag to TW_ERR_BAD_ARG and its rows
- * are not computed.  A page id outside the pool sets TW_ERR_INVALID_INDEX and
+ * max_q_len: an upper bound of the requests' new tokens (it chooses the
+ * kernels); a longer request sets *error_flag to TW_ERR_BAD_ARG and its rows
+ * are not computed.  max_kv_len: the longest kv_lens, which sizes the launch;
+ * with longer ones the results are the same, later.  A page id outside the pool sets TW_ERR_INVALID_INDEX and
  * is not read (its keys count as zero rows), and so does a kv_len beyond the
  * table (which is cut).  workspace: >= tw_paged_attention_workspace_size(...)
  * bytes, 16-byte aligned, no initial content; calls that share one must not
@@ -592,7 +594,7 @@ typedef struct tw_paged_attention_args {
   size_t workspace_bytes;
 } tw_paged_attention_args;
 size_t tw_paged_attention_workspace_size(int requests, int tokens, int q_heads, int kv_heads,
-                                         int max_q_len, int max_kv_len, int head_dim);
+                                         int max_q_len, int max_kv_len, int window, int head_dim);
 int tw_paged_attention(const tw_paged_attention_args* args, void* stream);
 size_t tw_paged_attention_args_size(void);
 

@@ -285,6 +285,18 @@ def test_window(tw, cuda, window, new, kv):
     b.check(out, lse, window=window)
 
 
+@pytest.mark.parametrize("page", [8, 16, 128])
+def test_pages_before_the_window_may_be_gone(tw, cuda, page):
+    new, kv, window = [1, 1, 40], [900, 300, 640], 100
+    b = Batch(cuda, new, kv, q_heads=8, kv_heads=2, page=page, dtype=torch.bfloat16)
+    whole, lse, _ = b.run(tw, window=window)
+    b.check(whole, lse, window=window)
+    for r in range(3):
+        b.table[r, :(kv[r] - new[r] - window + 1) // page] = -1
+    out, again, error = b.run(tw, window=window)
+    assert error == 0 and torch.equal(out, whole) and torch.equal(again, lse)
+
+
 @pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("new,kv", [([1], [5000]), ([3], [5003]), ([200], [3200]), ([8], [2048])])
 def test_long_contexts_with_few_rows(tw, cuda, out_dtype, new, kv):

@@ -143,7 +143,7 @@ SIGNATURES = {
     "tw_paged_step": (I32, [ctypes.POINTER(PagedStepArgs), P]),
     "tw_paged_step_args_size": (SZ, []),
     "tw_paged_write": (I32, [ctypes.POINTER(PagedPool), P, I64, I64, P, I64, I64, P, I64, P, P]),
-    "tw_paged_attention_workspace_size": (SZ, [I32, I32, I32, I32, I32, I32, I32]),
+    "tw_paged_attention_workspace_size": (SZ, [I32, I32, I32, I32, I32, I32, I32, I32]),
     "tw_paged_attention": (I32, [ctypes.POINTER(PagedAttentionArgs), P]),
     "tw_paged_attention_args_size": (SZ, []),
 }

@@ -1,26 +1,19 @@
-// Attention of new tokens over a paged KV cache.
+// Attention of new tokens over a paged KV cache: argument checks, how the call
+// is divided, and the merge of split rows.
 //
-// Row (t, h): token t of request b at position p sees the keys [lo, p];
-// out = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m), s_j = scale * q . k_j,
-// with the running maximum m and sum of one pass over the keys.
-#include <math_constants.h>
-
-#include "paged.cuh"
+// Row (t, h): token t of request b at position p sees the keys [low, p];
+// out = sum_j 2^(s_j - m) v_j / sum_j 2^(s_j - m), s_j = scale * log2(e) * q . k_j.
+#include "paged_attention.cuh"
 
 namespace tw {
 
-constexpr int kRowWarps = 8;  // rows per CTA of the row kernel
+constexpr int kRowWarps = 8;  // rows per CTA
 
-struct PagedRows {
-  const int32_t* table;  // the request's row of the block table
-  int first;             // first row of q of the request
-  int n;                 // its new tokens
-  int kv;                // its tokens, the new ones included
-};
-
+// Requests of many new tokens, one warp per row.
 template <typename T, typename Out>
 __global__ void __launch_bounds__(kRowWarps * 32)
-paged_row_kernel(tw_paged_attention_args a, float scale_log2) {
+paged_row_kernel(const __grid_constant__ PagedWork w) {
+  const tw_paged_attention_args& a = w.a;
   pdl_wait();
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31;
@@ -28,64 +21,125 @@ paged_row_kernel(tw_paged_attention_args a, float scale_log2) {
   if (row >= (int64_t)a.tokens * a.q_heads) return;
   const int t = (int)(row / a.q_heads);
   const int h = (int)(row - (int64_t)t * a.q_heads);
-  const int g = h / (a.q_heads / a.pool.kv_heads);
-  float acc[4] = {0.f, 0.f, 0.f, 0.f};
-  float m = -CUDART_INF_F, l = 0.f;
   const int b = first_above(a.cu_q + 1, a.requests, t);
-  if (b < a.requests) {
-    const int n = a.cu_q[b + 1] - a.cu_q[b];
-    const int64_t cap = (int64_t)a.table_width * a.pool.page_size;
-    int kv = a.kv_lens[b];
-    if (kv > cap) {
-      kv = (int)cap;
-      raise_error(a.error_flag, TW_ERR_INVALID_INDEX);
+  if (b >= a.requests) return;
+  const PagedRequest rq = paged_request(a, b);
+  if (rq.n <= w.few_tokens) return;
+  const int p = rq.kv - rq.n + (t - rq.first);
+  if (lane == 0)
+    for (int j = paged_low(a, max(rq.kv - rq.n, 0)); j < rq.kv; j += a.pool.page_size) {
+      const int page = a.block_table[(int64_t)b * a.table_stride + j / a.pool.page_size];
+      if (page < 0 || page >= a.pool.num_pages) raise_error(a.error_flag, TW_ERR_INVALID_INDEX);
     }
-    const int p = kv - n + (t - a.cu_q[b]);
-    const int lo = a.window > 0 ? max(0, p - a.window + 1) : 0;
-    const T* q = (const T*)a.q + (int64_t)t * a.q_token_stride + (int64_t)h * a.q_head_stride;
-    float x[4];
+  const PagedRow x = paged_one_row<T>(w, b, t, h, paged_low(a, p), p + 1);
+  float o[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = to_f32<T>(q[lane * 4 + i]) * scale_log2;
-    const int32_t* table = a.block_table + (int64_t)b * a.table_stride;
-    for (int j = lo; j <= p; ++j) {
-      const int i = j / a.pool.page_size;
-      const int page = table[i];
-      const bool ok = page >= 0 && page < a.pool.num_pages;
-      if (!ok) raise_error(a.error_flag, TW_ERR_INVALID_INDEX);
-      const int64_t at = (int64_t)page * a.pool.page_stride + (int64_t)g * a.pool.head_stride +
-                         (int64_t)(j - i * a.pool.page_size) * a.pool.token_stride + lane * 4;
-      float s = 0.f, v[4];
+  for (int c = 0; c < 4; ++c) o[c] = x.l == 0.f ? 0.f : x.acc[c] / x.l;
+  paged_store_row<Out, 4>(a, t, h, lane * 4, o, x.l == 0.f ? -CUDART_INF_F : x.m + log2f(x.l));
+}
+
+// Joins the ranges of split rows: out = sum_s 2^(lse_s - M) o_s / sum_s 2^(lse_s - M).
+// A warp per row; the ranges are added in order, so the bits do not depend on
+// which was ready first.
+template <typename Out>
+__global__ void __launch_bounds__(kRowWarps * 32)
+paged_merge_kernel(const __grid_constant__ PagedWork w) {
+  const tw_paged_attention_args& a = w.a;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int lane = threadIdx.x & 31;
+  const int64_t row = (int64_t)blockIdx.x * kRowWarps + (threadIdx.x >> 5);
+  if (row >= (int64_t)a.requests * a.pool.kv_heads * w.few_rows) return;
+  const int r = (int)(row % w.few_rows);
+  const int unit = (int)(row / w.few_rows);
+  const int b = unit / a.pool.kv_heads;
+  const int g = unit - b * a.pool.kv_heads;
+  const PagedRequest rq = paged_request(a, b);
+  if (rq.n > w.few_tokens || r >= rq.n * w.group) return;
+  const int parts = paged_range(a, rq, w.few, 0).parts;
+  if (parts == 1) return;  // the range wrote the result itself
+  const float* lse = w.few.part_lse + row * w.few.splits;
+  const float* po = w.few.part_o + row * w.few.splits * kHeadDim + lane * 4;
+  float m = -CUDART_INF_F;
+  for (int s = lane; s < parts; s += 32) m = fmaxf(m, lse[s]);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        s = fmaf(x[c], ok ? to_f32<T>(((const T*)a.pool.k_pages)[at + c]) : 0.f, s);
-        v[c] = ok ? to_f32<T>(((const T*)a.pool.v_pages)[at + c]) : 0.f;
-      }
-#pragma unroll
-      for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-      const float m_new = fmaxf(m, s);
-      const float m_use = m_new == -CUDART_INF_F ? 0.f : m_new;
-      const float keep = exp2f(m - m_use);
-      const float e = exp2f(s - m_use);
-      m = m_new;
-      l = fmaf(l, keep, e);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) acc[c] = fmaf(acc[c], keep, e * v[c]);
-    }
+  for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+  const float u = m == -CUDART_INF_F ? 0.f : m;
+  float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+  for (int s = 0; s < parts; ++s) {
+    const float f = ex2(lse[s] - u);
+    const float4 x = *reinterpret_cast<const float4*>(po + (int64_t)s * kHeadDim);
+    l += f;
+    o[0] = fmaf(x.x, f, o[0]);
+    o[1] = fmaf(x.y, f, o[1]);
+    o[2] = fmaf(x.z, f, o[2]);
+    o[3] = fmaf(x.w, f, o[3]);
   }
-  Out* out = (Out*)a.out + (int64_t)t * a.out_token_stride + (int64_t)h * a.out_head_stride;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-  for (int c = 0; c < 4; ++c) out[lane * 4 + c] = from_f32<Out>(l == 0.f ? 0.f : acc[c] / l);
-  if (a.lse && lane == 0)
-    a.lse[row] = l == 0.f ? -CUDART_INF_F : (m + log2f(l)) * 0.6931471805599453f;
+  for (int c = 0; c < 4; ++c) o[c] *= inv;
+  paged_store_row<Out, 4>(a, rq.first + r / w.group, g * w.group + r % w.group, lane * 4, o,
+                          l == 0.f ? -CUDART_INF_F : m + log2f(l));
 }
 
 template <typename T, typename Out>
-int launch_paged_rows(const tw_paged_attention_args& a, float scale_log2, cudaStream_t stream) {
-  const int64_t rows = (int64_t)a.tokens * a.q_heads;
+static int launch_rows(const PagedWork& w, cudaStream_t stream) {
+  const int64_t rows = (int64_t)w.a.tokens * w.a.q_heads;
   const int64_t ctas = (rows + kRowWarps - 1) / kRowWarps;
   if (ctas > INT32_MAX) return TW_ERR_UNSUPPORTED;
   return launch_pdl(paged_row_kernel<T, Out>, dim3((unsigned)ctas), dim3(kRowWarps * 32), 0,
-                    stream, a, scale_log2);
+                    stream, w);
+}
+
+template <typename Out>
+static int launch_merge(const PagedWork& w, cudaStream_t stream) {
+  const int64_t rows = (int64_t)w.a.requests * w.a.pool.kv_heads * w.few_rows;
+  const int64_t ctas = (rows + kRowWarps - 1) / kRowWarps;
+  if (ctas > INT32_MAX) return TW_ERR_UNSUPPORTED;
+  return launch_pdl(paged_merge_kernel<Out>, dim3((unsigned)ctas), dim3(kRowWarps * 32), 0, stream,
+                    w);
+}
+
+// ---- division of a call -----------------------------------------------------------
+constexpr int kFewRows = 16;  // rows of one warp-level product
+
+static int div_up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+
+static size_t part_bytes(int64_t rows, const PagedSplit& sp) {
+  return sp.splits > 1 ? (size_t)rows * sp.splits * (kHeadDim + 4) * sizeof(float) : 0;
+}
+
+// Ranges of the token kernel.  Its 2 CTAs per SM share the device; one request
+// (or a few) is cut so that all of them get a range, no shorter than 256 keys
+// (the pipeline's fill and the merge cost about that); many requests are cut
+// into twice the CTAs, because their lengths differ; and no range is longer
+// than 4096 keys, so that one long request among many short ones does not
+// leave the others waiting.
+static PagedSplit split_few(int requests, int kv_heads, int max_keys) {
+  const int64_t units = (int64_t)requests * kv_heads;
+  const int64_t ctas = 2 * 148 * (requests > 1 ? 2 : 1);
+  int64_t chunk = div_up(units * max_keys, ctas);
+  chunk = chunk < 256 ? 256 : chunk > 4096 ? 4096 : chunk;
+  PagedSplit sp = {};
+  sp.chunk = div_up(chunk, kTileKeys) * kTileKeys;
+  sp.splits = max_keys > sp.chunk ? div_up(max_keys, sp.chunk) : 1;
+  return sp;
+}
+
+// Fills the division of `w` from the call's sizes; returns the workspace bytes.
+static size_t plan_paged(PagedWork& w, int requests, int tokens, int q_heads, int kv_heads,
+                         int max_q_len, int max_kv_len, int window) {
+  w.group = q_heads / kv_heads;
+  const int most = max_q_len < tokens ? max_q_len : tokens;
+  w.few_tokens = kFewRows / w.group < most ? kFewRows / w.group : most;
+  w.few_rows = w.few_tokens * w.group;
+  // keys that a request's rows see, from a tile's begin on
+  int64_t keys = max_kv_len;
+  if (window > 0 && keys > (int64_t)window + most + kTileKeys)
+    keys = (int64_t)window + most + kTileKeys;
+  w.few = split_few(requests, kv_heads, (int)(keys > 0 ? keys : 1));
+  return part_bytes((int64_t)requests * kv_heads * w.few_rows, w.few);
 }
 
 }  // namespace tw
@@ -96,8 +150,13 @@ extern "C" size_t tw_paged_attention_args_size(void) { return sizeof(tw_paged_at
 
 extern "C" size_t tw_paged_attention_workspace_size(int requests, int tokens, int q_heads,
                                                     int kv_heads, int max_q_len, int max_kv_len,
-                                                    int head_dim) {
-  return 0;
+                                                    int window, int head_dim) {
+  if (requests <= 0 || tokens <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0 ||
+      q_heads / kv_heads > 64 || max_q_len < 0 || max_kv_len < 0 || window < 0 ||
+      head_dim != kHeadDim)
+    return 0;
+  PagedWork w = {};
+  return plan_paged(w, requests, tokens, q_heads, kv_heads, max_q_len, max_kv_len, window);
 }
 
 extern "C" int tw_paged_attention(const tw_paged_attention_args* args, void* stream) {
@@ -119,12 +178,43 @@ extern "C" int tw_paged_attention(const tw_paged_attention_args* args, void* str
       !paged_stride_ok(a.q_head_stride) || !paged_stride_ok(a.out_token_stride) ||
       !paged_stride_ok(a.out_head_stride))
     return TW_ERR_BAD_ARG;
-  const float scale_log2 = a.softmax_scale * 1.4426950408889634f;
-  cudaStream_t st = (cudaStream_t)stream;
+  PagedWork w = {};
+  w.a = a;
+  w.scale_log2 = a.softmax_scale * 1.4426950408889634f;
+  const size_t need = plan_paged(w, a.requests, a.tokens, a.q_heads, a.pool.kv_heads, a.max_q_len,
+                                 a.max_kv_len, a.window);
+  if (need > 0) {
+    if (!a.workspace || a.workspace_bytes < need) return TW_ERR_CAPACITY;
+    if (!aligned16(a.workspace)) return TW_ERR_BAD_ARG;
+    const int64_t rows = (int64_t)a.requests * a.pool.kv_heads * w.few_rows;
+    w.few.part_o = (float*)a.workspace;
+    w.few.part_lse = w.few.part_o + rows * w.few.splits * kHeadDim;
+  }
+  // one box: the rows that a page and a tile of 64 keys have in common
+  w.box = 64;
+  while (a.pool.page_size % w.box != 0) w.box /= 2;
+  PagedMaps maps;
+  const cuuint64_t dims[4] = {(cuuint64_t)kHeadDim, (cuuint64_t)a.pool.page_size,
+                              (cuuint64_t)a.pool.kv_heads, (cuuint64_t)a.pool.num_pages};
+  const cuuint64_t strides[3] = {(cuuint64_t)a.pool.token_stride * 2,
+                                 (cuuint64_t)a.pool.head_stride * 2,
+                                 (cuuint64_t)a.pool.page_stride * 2};
+  const cuuint32_t box[4] = {64, (cuuint32_t)w.box, 1, 1};
+  int st = encode_rows_map(&maps.k, a.pool.dtype, 4, a.pool.k_pages, dims, strides, box);
+  if (st == TW_OK) st = encode_rows_map(&maps.v, a.pool.dtype, 4, a.pool.v_pages, dims, strides, box);
+  if (st != TW_OK) return st;
+  cudaStream_t s = (cudaStream_t)stream;
+  st = launch_paged_token(w, maps, s);
+  if (st != TW_OK) return st;
+  if (w.few.splits > 1 && w.few_rows > 0) {
+    st = a.out_dtype == TW_F32    ? launch_merge<float>(w, s)
+         : a.pool.dtype == TW_F16 ? launch_merge<__half>(w, s)
+                                  : launch_merge<__nv_bfloat16>(w, s);
+    if (st != TW_OK) return st;
+  }
+  if (a.max_q_len <= w.few_tokens) return TW_OK;
   if (a.pool.dtype == TW_F16)
-    return a.out_dtype == TW_F32 ? launch_paged_rows<__half, float>(a, scale_log2, st)
-                                 : launch_paged_rows<__half, __half>(a, scale_log2, st);
-  return a.out_dtype == TW_F32
-             ? launch_paged_rows<__nv_bfloat16, float>(a, scale_log2, st)
-             : launch_paged_rows<__nv_bfloat16, __nv_bfloat16>(a, scale_log2, st);
+    return a.out_dtype == TW_F32 ? launch_rows<__half, float>(w, s) : launch_rows<__half, __half>(w, s);
+  return a.out_dtype == TW_F32 ? launch_rows<__nv_bfloat16, float>(w, s)
+                               : launch_rows<__nv_bfloat16, __nv_bfloat16>(w, s);
 }

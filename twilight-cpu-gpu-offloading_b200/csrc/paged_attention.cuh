@@ -1,0 +1,171 @@
+// What the kernels of the paged attention share: a call's work, a request's
+// rows and keys, the split of the keys, and the one-row form.
+#pragma once
+
+#include <math_constants.h>
+
+#include "async.cuh"
+#include "paged.cuh"
+
+namespace tw {
+
+constexpr int kTileKeys = 128;  // splits begin at multiples of this
+
+// How one kernel of the call divides a request's keys: ranges of `chunk` keys
+// (a multiple of kTileKeys), `splits` of them at most.  A request of the call
+// that is longer than max_kv_len said gets its rest in the last range.
+struct PagedSplit {
+  int chunk;
+  int splits;
+  float* part_o;    // [rows][splits][D], each range's softmax-weighted mean of V
+  float* part_lse;  // [rows][splits], its log2 sum of exponentials
+};
+
+struct PagedWork {
+  tw_paged_attention_args a;
+  float scale_log2;  // softmax_scale * log2(e)
+  int group;         // query heads per KV head
+  int few_tokens;    // requests with at most this many new tokens: token kernel
+  int few_rows;      // few_tokens * group
+  int box;           // token rows of one TMA box
+  PagedSplit few;    // rows: (request * kv_heads + head) * few_rows + row
+  PagedSplit many;   // rows: token * q_heads + head
+};
+
+struct PagedRequest {
+  int first, n;  // its rows of q: [first, first + n)
+  int kv;        // its tokens, the new ones included
+};
+
+// Lengths as the call gives them, cut to what its buffers hold.
+__device__ __forceinline__ PagedRequest paged_request(const tw_paged_attention_args& a, int b) {
+  PagedRequest r;
+  r.first = min(max(a.cu_q[b], 0), a.tokens);
+  r.n = max(min(a.cu_q[b + 1], a.tokens) - r.first, 0);
+  const long long cap = (long long)a.table_width * a.pool.page_size;
+  r.kv = max(a.kv_lens[b], 0);
+  if (r.kv > cap) {
+    r.kv = (int)cap;
+    raise_error(a.error_flag, TW_ERR_INVALID_INDEX);
+  }
+  return r;
+}
+
+// Keys that the row at position p sees: [low(p), p].
+__device__ __forceinline__ int paged_low(const tw_paged_attention_args& a, int p) {
+  return a.window > 0 ? max(0, p - a.window + 1) : 0;
+}
+
+// 2^x by the special-function unit (relative error 2^-22; 2^-inf = 0).
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+struct PagedRange {
+  int begin, end;  // keys
+  int parts;       // ranges that the request is divided into
+};
+
+// Range `s` of a request's keys.
+__device__ __forceinline__ PagedRange paged_range(const tw_paged_attention_args& a,
+                                                  const PagedRequest& r, const PagedSplit& sp,
+                                                  int s) {
+  const int low = paged_low(a, max(r.kv - r.n, 0)) / kTileKeys * kTileKeys;
+  PagedRange x;
+  x.parts = min(max((r.kv - low + sp.chunk - 1) / sp.chunk, 1), sp.splits);
+  x.begin = low + s * sp.chunk;
+  x.end = s == x.parts - 1 ? r.kv : min(r.kv, x.begin + sp.chunk);
+  return x;
+}
+
+// Softmax-weighted sum of V over the keys [low, high) for one row, by a warp:
+// lane l holds dimensions 4l .. 4l + 3.  One pass with the running maximum m
+// (in log2 units) and sum l.
+struct PagedRow {
+  float acc[4];
+  float m, l;
+};
+template <typename T>
+__device__ __noinline__ PagedRow paged_one_row(const PagedWork& w, int b, int t, int h, int low,
+                                               int high) {
+  const tw_paged_attention_args& a = w.a;
+  const int lane = threadIdx.x & 31;
+  const T* q = (const T*)a.q + (int64_t)t * a.q_token_stride + (int64_t)h * a.q_head_stride;
+  const int32_t* table = a.block_table + (int64_t)b * a.table_stride;
+  const int64_t head = (int64_t)(h / w.group) * a.pool.head_stride;
+  PagedRow r = {{0.f, 0.f, 0.f, 0.f}, -CUDART_INF_F, 0.f};
+  float x[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = to_f32<T>(q[lane * 4 + i]);
+  for (int j = low; j < high; ++j) {
+    const int i = j / a.pool.page_size;
+    const int page = table[i];
+    const bool ok = page >= 0 && page < a.pool.num_pages;
+    const int64_t at = (int64_t)page * a.pool.page_stride + head +
+                       (int64_t)(j - i * a.pool.page_size) * a.pool.token_stride + lane * 4;
+    float s = 0.f, v[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      s = fmaf(x[c], ok ? to_f32<T>(((const T*)a.pool.k_pages)[at + c]) : 0.f, s);
+      v[c] = ok ? to_f32<T>(((const T*)a.pool.v_pages)[at + c]) : 0.f;
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+    s *= w.scale_log2;
+    const float m_new = fmaxf(r.m, s);
+    const float m_use = m_new == -CUDART_INF_F ? 0.f : m_new;
+    const float keep = ex2(r.m - m_use);
+    const float e = ex2(s - m_use);
+    r.m = m_new;
+    r.l = fmaf(r.l, keep, e);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) r.acc[c] = fmaf(r.acc[c], keep, e * v[c]);
+  }
+  return r;
+}
+
+// Result of a row whose keys are one range: out and lse.  `n` consecutive
+// dimensions from d0; lse by the thread with d0 == 0.
+template <typename Out, int N>
+__device__ __forceinline__ void paged_store_row(const tw_paged_attention_args& a, int t, int h,
+                                                int d0, const float (&o)[N], float lse2) {
+  Out* out = (Out*)a.out + (int64_t)t * a.out_token_stride + (int64_t)h * a.out_head_stride + d0;
+  constexpr int kVec = 16 / sizeof(Out);
+  if constexpr (N % kVec == 0) {
+#pragma unroll
+    for (int c = 0; c < N; c += kVec) {
+      __align__(16) Out x[kVec];
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) x[i] = from_f32<Out>(o[c + i]);
+      *reinterpret_cast<uint4*>(out + c) = *reinterpret_cast<uint4*>(x);
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < N; ++c) out[c] = from_f32<Out>(o[c]);
+  }
+  if (a.lse && d0 == 0)
+    a.lse[(int64_t)t * a.q_heads + h] = lse2 * 0.6931471805599453f;  // log2 -> ln
+}
+
+// A range's result of a row, for the merge.
+template <int N>
+__device__ __forceinline__ void paged_store_part(const PagedSplit& sp, int64_t row, int s, int d0,
+                                                 const float (&o)[N], float lse2) {
+  float* to = sp.part_o + (row * sp.splits + s) * kHeadDim + d0;
+#pragma unroll
+  for (int c = 0; c < N; c += 4)
+    *reinterpret_cast<float4*>(to + c) = make_float4(o[c], o[c + 1], o[c + 2], o[c + 3]);
+  if (d0 == 0) sp.part_lse[row * sp.splits + s] = lse2;
+}
+
+// The maps of the pool's K and V: [page][head][row][D] boxes of `box` rows of
+// one head of one page, 64 elements wide.
+struct PagedMaps {
+  CUtensorMap k, v;
+};
+
+int launch_paged_token(const PagedWork& w, const PagedMaps& maps, cudaStream_t stream);
+
+}  // namespace tw

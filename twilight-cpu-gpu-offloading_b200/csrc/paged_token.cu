@@ -1,0 +1,437 @@
+// Paged attention of requests with few new rows per KV head (a token each, as
+// in decoding, or a few): at most 16 rows (tokens x query heads of the group).
+//
+// Mathematics: for each range of keys, one pass with a running reference m and
+// sum l per row: p_j = 2^(s_j - m), l += p_j, O += p_j v_j, both scaled when m
+// moves.  m moves only when a score exceeds it by more than 8 (p stays below
+// 2^8, far from overflow in either 16-bit type), so the accumulators are
+// rarely rescaled.  A range leaves O / l and m + log2 l; ranges are joined by
+// weights 2^(lse_s - max).
+//
+// Bound: HBM, every K / V row of the visible keys read once per KV head
+// (512 bytes a key); the 16-row products are 4 % of what the tensor cores
+// could do in that time, so the warp-level mma.sync (one 16 x 8 x 16 product
+// per instruction, operands and results in registers) is enough and needs no
+// round trip through tensor memory.
+//
+// Layout: a CTA takes one KV head of one request and one range of its keys.
+// One warp fetches 64-key tiles (K and V, 32 KB) into a ring of three stages
+// by TMA, a box for each page piece; four warps take 16 keys of every tile
+// each, keep m, l and O of all 16 rows in registers, and join at the end
+// through shared memory.  Two CTAs are resident per SM: up to 192 KB in flight.
+#include "paged_attention.cuh"
+
+namespace tw {
+
+constexpr int kTokRows = 16;
+constexpr int kTokTile = 64;       // keys per stage
+constexpr int kTokStages = 3;
+constexpr int kTokWarps = 4;       // consumers
+constexpr int kTokThreads = (kTokWarps + 1) * 32;
+constexpr int kTokHalf = kTokTile * 128;          // 64 of the 128 dimensions of a tile
+constexpr int kTokStageBytes = 4 * kTokHalf;      // K lo, K hi, V lo, V hi
+constexpr int kTokRowPad = kHeadDim + 4;          // floats per row of the join
+constexpr int kTokSmem = kTokStages * kTokStageBytes + 1024;  // + alignment of the swizzle
+constexpr int kPadCtas = 8;        // CTAs that clear the rows past the last token
+constexpr float kMoveBy = 8.0f;    // log2 units
+
+template <typename T> struct MmaType;
+template <> struct MmaType<__half> {
+  static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                             uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+template <> struct MmaType<__nv_bfloat16> {
+  static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                             uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+
+// Offset of element (row, d) of a [64 rows][128] tile stored as two halves of
+// 128-byte rows with the 16-byte columns of each row XORed by row % 8.
+__device__ __forceinline__ uint32_t tok_offset(int row, int d) {
+  return (uint32_t)((d >> 6) * kTokHalf + row * 128 + (((d & 63) * 2) ^ ((row & 7) << 4)));
+}
+
+__device__ __forceinline__ void consumer_sync() {
+  asm volatile("bar.sync 1, %0;" ::"n"(kTokWarps * 32) : "memory");
+}
+
+template <typename T, typename Out>
+__global__ void __launch_bounds__(kTokThreads, 2)
+paged_token_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ PagedMaps maps) {
+  extern __shared__ char s_raw[];
+  __shared__ uint64_t s_full[kTokStages], s_empty[kTokStages];
+  __shared__ float s_m[kTokWarps][kTokRows], s_l[kTokWarps][kTokRows];
+  __shared__ volatile int s_abort;
+  __shared__ int s_bad_rows;
+  const tw_paged_attention_args& a = w.a;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int kv_heads = a.pool.kv_heads;
+  const int64_t cta = blockIdx.x;
+  const int64_t units = (int64_t)a.requests * kv_heads * w.few.splits;
+  pdl_wait();
+  pdl_launch_dependents();
+
+  if (cta >= units) {  // rows past the last token: out 0, lse -inf
+    const int end = min(max(a.cu_q[a.requests], 0), a.tokens);
+    const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+    const int64_t rows = (int64_t)(a.tokens - end) * a.q_heads;
+    for (int64_t i = (cta - units) * kTokThreads + tid; i < rows * 32;
+         i += (int64_t)kPadCtas * kTokThreads) {
+      const int64_t row = i >> 5;
+      const int t = end + (int)(row / a.q_heads);
+      paged_store_row<Out, 4>(a, t, (int)(row % a.q_heads), (int)(i & 31) * 4, zero,
+                              -CUDART_INF_F);
+    }
+    return;
+  }
+  const int split = (int)(cta % w.few.splits);
+  const int unit = (int)(cta / w.few.splits);
+  const int b = unit / kv_heads;
+  const int g = unit - b * kv_heads;
+  const PagedRequest rq = paged_request(a, b);
+  if (rq.n == 0) return;
+  if (rq.n > w.few_tokens) {
+    if (rq.n > a.max_q_len && tid == 0) raise_error(a.error_flag, TW_ERR_BAD_ARG);
+    return;
+  }
+  const PagedRange range = paged_range(a, rq, w.few, split);
+  if (split >= range.parts) return;
+  const int R = w.group;
+  const int rows = rq.n * R;
+  // keys that some row sees, in this range
+  const int low = max(range.begin, paged_low(a, max(rq.kv - rq.n, 0)));
+  const int tile0 = low / kTokTile * kTokTile;
+  const int tiles = range.end > low ? (range.end - tile0 + kTokTile - 1) / kTokTile : 0;
+
+  char* smem = (char*)(((uintptr_t)s_raw + 1023) & ~(uintptr_t)1023);
+  const uint32_t ring = smem_addr(smem);
+  if (tid == 0) {
+    for (int i = 0; i < kTokStages; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&s_empty[i], kTokWarps);
+    }
+    s_abort = 0;
+    s_bad_rows = 0;
+    mbar_init_fence();
+  }
+  __syncthreads();
+
+  if (warp == kTokWarps) {
+    // ---- producer: lane l copies one box of K or V of each tile
+    const int boxes = kTokTile / w.box;
+    const int matrix = lane / (2 * boxes);  // 0 K, 1 V, more: idle
+    const int half = (lane / boxes) & 1;
+    const int box = lane % boxes;
+    const CUtensorMap* map = matrix == 0 ? &maps.k : &maps.v;
+    const int32_t* table = a.block_table + (int64_t)b * a.table_stride;
+    const uint32_t dst = ring + (2 * matrix + half) * kTokHalf + box * w.box * 128;
+    if (lane == 0) prefetch_map(&maps.k);
+    if (lane == 1) prefetch_map(&maps.v);
+    const int stride = w.box;
+    int key = tile0 + box * stride;
+    int page = 0;
+    // boxes wholly before the first visible key are not read: a page that slid out
+    // of the window may be gone
+    const int skipped = (low - tile0) / stride;
+    if (matrix < 2 && key < range.end && box >= skipped) page = table[key / a.pool.page_size];
+    int i = 0;
+    for (; i < tiles; ++i) {
+      const int stage = i % kTokStages;
+      const int now_key = key, now_page = page;
+      key += kTokTile;
+      if (matrix < 2 && i + 1 < tiles && key < range.end) page = table[key / a.pool.page_size];
+      if (i >= kTokStages &&
+          !mbar_wait(&s_empty[stage], (uint32_t)((i / kTokStages - 1) & 1), &s_abort))
+        break;
+      if (lane == 0) {
+        const int valid = min(range.end - (tile0 + i * kTokTile), kTokTile);
+        const int count = (valid + stride - 1) / stride - (i == 0 ? skipped : 0);
+        mbar_arrive_expect(&s_full[stage], (uint32_t)(count * stride * 4 * 128));
+      }
+      __syncwarp();
+      if (matrix < 2 && now_key < range.end && (i > 0 || box >= skipped)) {
+        int p = now_page;
+        if (p < 0 || p >= a.pool.num_pages) {
+          raise_error(a.error_flag, TW_ERR_INVALID_INDEX);
+          p = (int)a.pool.num_pages;  // out of the map's range: zeros
+        }
+        tma_load_4d(map, dst + stage * kTokStageBytes, &s_full[stage], half * 64,
+                    now_key % a.pool.page_size, g, p);
+      }
+    }
+    if (s_abort) {
+      // give up: wait (with the same limit) for the copies in flight
+      volatile int never = 0;
+      for (int j = max(0, i - kTokStages); j < i; ++j)
+        mbar_wait(&s_full[j % kTokStages], (uint32_t)((j / kTokStages) & 1), &never);
+    }
+    return;
+  }
+
+  // ---- consumers: fragments of the 16 query rows, row r = token * R + head
+  uint32_t qf[8][4];
+  const int r0 = lane >> 2, r1 = r0 + 8;
+  const int c0 = (lane & 3) * 2;
+  {
+    const T* q0 = (const T*)a.q + (int64_t)(rq.first + r0 / R) * a.q_token_stride +
+                  (int64_t)(g * R + r0 % R) * a.q_head_stride + c0;
+    const T* q1 = (const T*)a.q + (int64_t)(rq.first + r1 / R) * a.q_token_stride +
+                  (int64_t)(g * R + r1 % R) * a.q_head_stride + c0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      qf[k][0] = r0 < rows ? *reinterpret_cast<const uint32_t*>(q0 + k * 16) : 0u;
+      qf[k][1] = r1 < rows ? *reinterpret_cast<const uint32_t*>(q1 + k * 16) : 0u;
+      qf[k][2] = r0 < rows ? *reinterpret_cast<const uint32_t*>(q0 + k * 16 + 8) : 0u;
+      qf[k][3] = r1 < rows ? *reinterpret_cast<const uint32_t*>(q1 + k * 16 + 8) : 0u;
+    }
+  }
+  // visible keys of the thread's two rows (rows past the last see what row 0 sees)
+  const int p0 = rq.kv - rq.n + (r0 < rows ? r0 / R : 0);
+  const int p1 = rq.kv - rq.n + (r1 < rows ? r1 / R : 0);
+  const int low0 = paged_low(a, p0), low1 = paged_low(a, p1);
+  // keys that every row sees: tiles inside need no mask
+  const int all_low = paged_low(a, rq.kv - 1), all_high = rq.kv - rq.n + 1;
+
+  float acc[16][4];
+#pragma unroll
+  for (int d = 0; d < 16; ++d)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) acc[d][c] = 0.f;
+  float m0 = -CUDART_INF_F, m1 = -CUDART_INF_F, l0 = 0.f, l1 = 0.f;
+  const int wrow = warp * 16;  // the warp's keys of a tile
+  const uint32_t k_at = ring + tok_offset(wrow + (lane >> 4) * 8 + (lane & 7), 0);
+  const int k_col = ((lane >> 3) & 1) * 16;  // bytes
+  const int k_xor = (lane & 7) << 4;
+  const uint32_t v_at = ring + 2 * kTokHalf + (wrow + ((lane >> 3) & 1) * 8 + (lane & 7)) * 128;
+  const int v_col = (lane >> 4) * 16;
+
+  for (int i = 0; i < tiles; ++i) {
+    const int stage = i % kTokStages;
+    const uint32_t base = stage * kTokStageBytes;
+    const int key0 = tile0 + i * kTokTile + wrow;  // the warp's first key
+    if (!mbar_wait(&s_full[stage], (uint32_t)((i / kTokStages) & 1), &s_abort)) break;
+    if (key0 < range.end && key0 + 16 > low) {
+      const bool edge = key0 < all_low || key0 + 16 > all_high || key0 < low ||
+                        key0 + 16 > range.end;
+      float s[2][4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) s[0][c] = s[1][c] = 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        uint32_t kb[4];
+        ldmatrix4(kb, k_at - (((lane & 7) << 4)) + base + (k >> 2) * kTokHalf +
+                          ((((k & 3) * 32) + k_col) ^ k_xor));
+        MmaType<T>::mma(s[0], qf[k], kb[0], kb[1]);
+        MmaType<T>::mma(s[1], qf[k], kb[2], kb[3]);
+      }
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) s[n][c] *= w.scale_log2;
+      if (edge) {
+        // hide what a row does not see, and clear V rows that none sees: what
+        // they hold (NaN included) must not meet a weight of zero
+        const int first = key0 + c0;
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int j = first + n * 8 + (c & 1);
+            const bool seen = c < 2 ? (j >= low0 && j <= p0) : (j >= low1 && j <= p1);
+            if (!seen || j < range.begin || j >= range.end) s[n][c] = -CUDART_INF_F;
+          }
+        const int row = lane >> 1;
+        const int j = key0 + row;
+        if (j < low || j >= range.end) {
+          char* z = smem + base + 2 * kTokHalf + (lane & 1) * kTokHalf + (wrow + row) * 128;
+#pragma unroll
+          for (int c = 0; c < 8; ++c)
+            reinterpret_cast<uint4*>(z)[c] = make_uint4(0u, 0u, 0u, 0u);
+        }
+        __syncwarp();
+      }
+      float t0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
+      float t1 = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
+#pragma unroll
+      for (int off = 1; off < 4; off <<= 1) {
+        t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, off));
+        t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, off));
+      }
+      const bool move0 = t0 > m0 + kMoveBy, move1 = t1 > m1 + kMoveBy;
+      if (__any_sync(0xffffffffu, move0 || move1)) {
+        const float n0 = move0 ? t0 : m0, n1 = move1 ? t1 : m1;
+        // an unmoved reference keeps its sums (-inf - -inf would be NaN)
+        const float f0 = move0 ? ex2(m0 - n0) : 1.f, f1 = move1 ? ex2(m1 - n1) : 1.f;
+        m0 = n0;
+        m1 = n1;
+        l0 *= f0;
+        l1 *= f1;
+#pragma unroll
+        for (int d = 0; d < 16; ++d) {
+          acc[d][0] *= f0;
+          acc[d][1] *= f0;
+          acc[d][2] *= f1;
+          acc[d][3] *= f1;
+        }
+      }
+      const float u0 = m0 == -CUDART_INF_F ? 0.f : m0, u1 = m1 == -CUDART_INF_F ? 0.f : m1;
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        s[n][0] = ex2(s[n][0] - u0);
+        s[n][1] = ex2(s[n][1] - u0);
+        s[n][2] = ex2(s[n][2] - u1);
+        s[n][3] = ex2(s[n][3] - u1);
+        l0 += s[n][0] + s[n][1];
+        l1 += s[n][2] + s[n][3];
+      }
+      // weights rounded to the 16-bit type for the product (the sum l keeps them
+      // in 32 bits): half a unit each, of either sign
+      const uint32_t pf[4] = {MmaType<T>::pack(s[0][0], s[0][1]), MmaType<T>::pack(s[0][2], s[0][3]),
+                              MmaType<T>::pack(s[1][0], s[1][1]), MmaType<T>::pack(s[1][2], s[1][3])};
+#pragma unroll
+      for (int d = 0; d < 8; ++d) {
+        uint32_t vb[4];
+        ldmatrix4_trans(vb, v_at + base + (d >> 2) * kTokHalf +
+                                ((((d & 3) * 32) + v_col) ^ k_xor));
+        MmaType<T>::mma(acc[2 * d], pf, vb[0], vb[1]);
+        MmaType<T>::mma(acc[2 * d + 1], pf, vb[2], vb[3]);
+      }
+      if (edge) fence_async_smem();  // the cleared rows, before the next copy into them
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&s_empty[stage]);
+  }
+
+  // ---- join the four warps
+  if (s_abort && lane == 0) raise_error(a.error_flag, TW_ERR_TIMEOUT);
+#pragma unroll
+  for (int off = 1; off < 4; off <<= 1) {
+    l0 += __shfl_xor_sync(0xffffffffu, l0, off);
+    l1 += __shfl_xor_sync(0xffffffffu, l1, off);
+  }
+  consumer_sync();  // the ring is free: every tile has been read
+  float* s_o = reinterpret_cast<float*>(smem);  // [warps][rows][kTokRowPad]
+#pragma unroll
+  for (int d = 0; d < 16; ++d) {
+    float* o = s_o + (warp * kTokRows + r0) * kTokRowPad + d * 8 + c0;
+    *reinterpret_cast<float2*>(o) = make_float2(acc[d][0], acc[d][1]);
+    *reinterpret_cast<float2*>(o + 8 * kTokRowPad) = make_float2(acc[d][2], acc[d][3]);
+  }
+  if ((lane & 3) == 0) {
+    s_m[warp][r0] = m0;
+    s_m[warp][r1] = m1;
+    s_l[warp][r0] = l0;
+    s_l[warp][r1] = l1;
+  }
+  consumer_sync();
+  const bool joined = range.parts == 1;
+  {
+    const int r = tid >> 3, d0 = (tid & 7) * 16;
+    float m = -CUDART_INF_F;
+#pragma unroll
+    for (int k = 0; k < kTokWarps; ++k) m = fmaxf(m, s_m[k][r]);
+    const float u = m == -CUDART_INF_F ? 0.f : m;
+    float l = 0.f, o[16];
+#pragma unroll
+    for (int c = 0; c < 16; ++c) o[c] = 0.f;
+#pragma unroll
+    for (int k = 0; k < kTokWarps; ++k) {
+      const float f = ex2(s_m[k][r] - u);
+      l = fmaf(s_l[k][r], f, l);
+      const float* x = s_o + (k * kTokRows + r) * kTokRowPad + d0;
+#pragma unroll
+      for (int c = 0; c < 16; ++c) o[c] = fmaf(x[c], f, o[c]);
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    float odd = 0.f;
+#pragma unroll
+    for (int c = 0; c < 16; ++c) {
+      o[c] *= inv;
+      odd = fmaf(o[c], 0.f, odd);  // NaN when one is not finite
+    }
+    const float lse2 = l == 0.f ? -CUDART_INF_F : m + log2f(l);
+    if (r < rows) {
+      const int t = rq.first + r / R, h = g * R + r % R;
+      if (joined)
+        paged_store_row<Out, 16>(a, t, h, d0, o, lse2);
+      else
+        paged_store_part<16>(w.few, (int64_t)unit * w.few_rows + r, split, d0, o, lse2);
+      // A row that is not finite may owe it to a V row that another token sees
+      // and this one does not (weight 0 times infinity or NaN).
+      if (rq.n > 1 && odd != 0.f) atomicOr(&s_bad_rows, 1 << r);
+    }
+  }
+  if (rq.n == 1) return;
+  consumer_sync();
+  for (int bad = s_bad_rows; bad; bad &= bad - 1) {
+    const int r = __ffs(bad) - 1;
+    if (r % kTokWarps != warp) continue;
+    const int t = rq.first + r / R, h = g * R + r % R;
+    const int p = rq.kv - rq.n + r / R;
+    const PagedRow x = paged_one_row<T>(w, b, t, h, max(range.begin, paged_low(a, p)),
+                                        min(range.end, p + 1));
+    float o[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) o[c] = x.l == 0.f ? 0.f : x.acc[c] / x.l;
+    const float lse2 = x.l == 0.f ? -CUDART_INF_F : x.m + log2f(x.l);
+    if (joined)
+      paged_store_row<Out, 4>(a, t, h, lane * 4, o, lse2);
+    else
+      paged_store_part<4>(w.few, (int64_t)unit * w.few_rows + r, split, lane * 4, o, lse2);
+  }
+}
+
+template <typename T, typename Out>
+static int launch(const PagedWork& w, const PagedMaps& maps, cudaStream_t stream) {
+  static DynSmemOptIn opt_in;
+  const auto kernel = paged_token_kernel<T, Out>;
+  const int rc = ensure_dyn_smem((const void*)kernel, opt_in, kTokSmem);
+  if (rc != TW_OK) return rc;
+  const int64_t ctas = (int64_t)w.a.requests * w.a.pool.kv_heads * w.few.splits + kPadCtas;
+  if (ctas > INT32_MAX) return TW_ERR_UNSUPPORTED;
+  return launch_pdl(kernel, dim3((unsigned)ctas), dim3(kTokThreads), (size_t)kTokSmem, stream, w,
+                    maps);
+}
+
+int launch_paged_token(const PagedWork& w, const PagedMaps& maps, cudaStream_t stream) {
+  if (w.a.pool.dtype == TW_F16)
+    return w.a.out_dtype == TW_F32 ? launch<__half, float>(w, maps, stream)
+                                   : launch<__half, __half>(w, maps, stream);
+  return w.a.out_dtype == TW_F32 ? launch<__nv_bfloat16, float>(w, maps, stream)
+                                 : launch<__nv_bfloat16, __nv_bfloat16>(w, maps, stream);
+}
+
+}  // namespace tw

@@ -438,9 +438,9 @@ def paged_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_pages: 
 
 
 def paged_attention_workspace_bytes(requests: int, tokens: int, q_heads: int, kv_heads: int,
-                                    max_q_len: int, max_kv_len: int) -> int:
+                                    max_q_len: int, max_kv_len: int, window: int = 0) -> int:
     return int(lib().tw_paged_attention_workspace_size(requests, tokens, q_heads, kv_heads,
-                                                       max_q_len, max_kv_len, HEAD_DIM))
+                                                       max_q_len, max_kv_len, window, HEAD_DIM))
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -456,7 +456,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 
     q [T, q_heads, 128] (token and head strides free), pool [pages, kv_heads,
     page_size, 128], block_table [B, W] int32, cu_q [B+1] and kv_lens [B] int32
-    on the device; max_q_len / max_kv_len bound the requests' lengths.  window
+    on the device; max_q_len bounds the requests' new tokens, max_kv_len is their
+    longest kv_lens (it sizes the launch).  window
     > 0: each token sees the last `window` positions only.  Returns out
     [T, q_heads, 128] (q's dtype or float32); lse [T, q_heads] fp32 receives the
     log-sum-exp.  Without a workspace one is allocated for the call."""
@@ -480,7 +481,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
                             or not lse.is_contiguous()):
         raise ValueError("lse must be float32 [T, q_heads]")
     if workspace is None:
-        need = paged_attention_workspace_bytes(B, T, Hq, pool.kv_heads, max_q_len, max_kv_len)
+        need = paged_attention_workspace_bytes(B, T, Hq, pool.kv_heads, max_q_len, max_kv_len,
+                                               window)
         if need:
             workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
     elif not workspace.is_contiguous():
