@@ -21,7 +21,7 @@ CSRC = PKG / "csrc"
 LIB = PKG / "libtwilight_b200.so"
 SOURCES = ["quest.cu", "int4.cu", "topp_union.cu", "gather.cu", "attention.cu", "frontend.cu",
            "capi.cu", "paged.cu", "paged_attention.cu",
-           "paged_token.cu"]
+           "paged_token.cu", "paged_chunk.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",

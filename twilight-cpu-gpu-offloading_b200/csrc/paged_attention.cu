@@ -7,59 +7,49 @@
 
 namespace tw {
 
-constexpr int kRowWarps = 8;  // rows per CTA
-
-// Requests of many new tokens, one warp per row.
-template <typename T, typename Out>
-__global__ void __launch_bounds__(kRowWarps * 32)
-paged_row_kernel(const __grid_constant__ PagedWork w) {
-  const tw_paged_attention_args& a = w.a;
-  pdl_wait();
-  pdl_launch_dependents();
-  const int lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * kRowWarps + (threadIdx.x >> 5);
-  if (row >= (int64_t)a.tokens * a.q_heads) return;
-  const int t = (int)(row / a.q_heads);
-  const int h = (int)(row - (int64_t)t * a.q_heads);
-  const int b = first_above(a.cu_q + 1, a.requests, t);
-  if (b >= a.requests) return;
-  const PagedRequest rq = paged_request(a, b);
-  if (rq.n <= w.few_tokens) return;
-  const int p = rq.kv - rq.n + (t - rq.first);
-  if (lane == 0)
-    for (int j = paged_low(a, max(rq.kv - rq.n, 0)); j < rq.kv; j += a.pool.page_size) {
-      const int page = a.block_table[(int64_t)b * a.table_stride + j / a.pool.page_size];
-      if (page < 0 || page >= a.pool.num_pages) raise_error(a.error_flag, TW_ERR_INVALID_INDEX);
-    }
-  const PagedRow x = paged_one_row<T>(w, b, t, h, paged_low(a, p), p + 1);
-  float o[4];
-#pragma unroll
-  for (int c = 0; c < 4; ++c) o[c] = x.l == 0.f ? 0.f : x.acc[c] / x.l;
-  paged_store_row<Out, 4>(a, t, h, lane * 4, o, x.l == 0.f ? -CUDART_INF_F : x.m + log2f(x.l));
-}
+constexpr int kRowWarps = 8;  // rows per CTA of the merge
 
 // Joins the ranges of split rows: out = sum_s 2^(lse_s - M) o_s / sum_s 2^(lse_s - M).
 // A warp per row; the ranges are added in order, so the bits do not depend on
 // which was ready first.
-template <typename Out>
+template <typename Out, bool kFew>
 __global__ void __launch_bounds__(kRowWarps * 32)
 paged_merge_kernel(const __grid_constant__ PagedWork w) {
   const tw_paged_attention_args& a = w.a;
+  const PagedSplit& sp = kFew ? w.few : w.many;
   pdl_wait();
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31;
   const int64_t row = (int64_t)blockIdx.x * kRowWarps + (threadIdx.x >> 5);
-  if (row >= (int64_t)a.requests * a.pool.kv_heads * w.few_rows) return;
-  const int r = (int)(row % w.few_rows);
-  const int unit = (int)(row / w.few_rows);
-  const int b = unit / a.pool.kv_heads;
-  const int g = unit - b * a.pool.kv_heads;
-  const PagedRequest rq = paged_request(a, b);
-  if (rq.n > w.few_tokens || r >= rq.n * w.group) return;
-  const int parts = paged_range(a, rq, w.few, 0).parts;
+  int t, h;
+  PagedRequest rq;
+  PagedKeys keys;
+  if (kFew) {
+    if (row >= (int64_t)a.requests * a.pool.kv_heads * w.few_rows) return;
+    const int r = (int)(row % w.few_rows);
+    const int unit = (int)(row / w.few_rows);
+    const int b = unit / a.pool.kv_heads;
+    rq = paged_request(a, b);
+    if (rq.n > w.few_tokens || r >= rq.n * w.group) return;
+    t = rq.first + r / w.group;
+    h = (unit - b * a.pool.kv_heads) * w.group + r % w.group;
+    keys = paged_keys(a, rq, 0, rq.n);
+  } else {
+    if (row >= (int64_t)a.tokens * a.q_heads) return;
+    t = (int)(row / a.q_heads);
+    h = (int)(row - (int64_t)t * a.q_heads);
+    const int b = first_above(a.cu_q + 1, a.requests, t);
+    if (b >= a.requests) return;
+    rq = paged_request(a, b);
+    if (rq.n <= w.few_tokens || rq.n > a.max_q_len) return;
+    const int tokens = paged_chunk_tokens(w.group);
+    const int begin = (t - rq.first) / tokens * tokens;
+    keys = paged_keys(a, rq, begin, min(rq.n - begin, tokens));
+  }
+  const int parts = paged_range(sp, keys.low, keys.high, 0).parts;
   if (parts == 1) return;  // the range wrote the result itself
-  const float* lse = w.few.part_lse + row * w.few.splits;
-  const float* po = w.few.part_o + row * w.few.splits * kHeadDim + lane * 4;
+  const float* lse = sp.part_lse + row * sp.splits;
+  const float* po = sp.part_o + row * sp.splits * kHeadDim + lane * 4;
   float m = -CUDART_INF_F;
   for (int s = lane; s < parts; s += 32) m = fmaxf(m, lse[s]);
 #pragma unroll
@@ -79,26 +69,17 @@ paged_merge_kernel(const __grid_constant__ PagedWork w) {
   const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
   for (int c = 0; c < 4; ++c) o[c] *= inv;
-  paged_store_row<Out, 4>(a, rq.first + r / w.group, g * w.group + r % w.group, lane * 4, o,
-                          l == 0.f ? -CUDART_INF_F : m + log2f(l));
+  paged_store_row<Out, 4>(a, t, h, lane * 4, o, l == 0.f ? -CUDART_INF_F : m + log2f(l));
 }
 
-template <typename T, typename Out>
-static int launch_rows(const PagedWork& w, cudaStream_t stream) {
-  const int64_t rows = (int64_t)w.a.tokens * w.a.q_heads;
+template <bool kFew>
+static int launch_merge(const PagedWork& w, int64_t rows, cudaStream_t stream) {
   const int64_t ctas = (rows + kRowWarps - 1) / kRowWarps;
   if (ctas > INT32_MAX) return TW_ERR_UNSUPPORTED;
-  return launch_pdl(paged_row_kernel<T, Out>, dim3((unsigned)ctas), dim3(kRowWarps * 32), 0,
-                    stream, w);
-}
-
-template <typename Out>
-static int launch_merge(const PagedWork& w, cudaStream_t stream) {
-  const int64_t rows = (int64_t)w.a.requests * w.a.pool.kv_heads * w.few_rows;
-  const int64_t ctas = (rows + kRowWarps - 1) / kRowWarps;
-  if (ctas > INT32_MAX) return TW_ERR_UNSUPPORTED;
-  return launch_pdl(paged_merge_kernel<Out>, dim3((unsigned)ctas), dim3(kRowWarps * 32), 0, stream,
-                    w);
+  const auto kernel = w.a.out_dtype == TW_F32   ? paged_merge_kernel<float, kFew>
+                      : w.a.out_dtype == TW_F16 ? paged_merge_kernel<__half, kFew>
+                                                : paged_merge_kernel<__nv_bfloat16, kFew>;
+  return launch_pdl(kernel, dim3((unsigned)ctas), dim3(kRowWarps * 32), 0, stream, w);
 }
 
 // ---- division of a call -----------------------------------------------------------
@@ -116,7 +97,7 @@ static size_t part_bytes(int64_t rows, const PagedSplit& sp) {
 // into twice the CTAs, because their lengths differ; and no range is longer
 // than 4096 keys, so that one long request among many short ones does not
 // leave the others waiting.
-static PagedSplit split_few(int requests, int kv_heads, int max_keys) {
+static PagedSplit split_few(int requests, int kv_heads, int64_t max_keys) {
   const int64_t units = (int64_t)requests * kv_heads;
   const int64_t ctas = 2 * 148 * (requests > 1 ? 2 : 1);
   int64_t chunk = div_up(units * max_keys, ctas);
@@ -127,19 +108,57 @@ static PagedSplit split_few(int requests, int kv_heads, int max_keys) {
   return sp;
 }
 
-// Fills the division of `w` from the call's sizes; returns the workspace bytes.
-static size_t plan_paged(PagedWork& w, int requests, int tokens, int q_heads, int kv_heads,
-                         int max_q_len, int max_kv_len, int window) {
+// Ranges of the chunk kernel: one, unless its CTAs would leave SMs idle.  Then
+// the keys are cut so that about all SMs get one, no shorter than 512 keys.
+static PagedSplit split_many(int64_t units, int64_t keys) {
+  PagedSplit sp = {};
+  const int64_t most = units < 148 ? 148 / units : 1;
+  int64_t chunk = div_up(keys, most);
+  chunk = chunk < 512 ? 512 : chunk;
+  sp.chunk = div_up(chunk, kTileKeys) * kTileKeys;
+  sp.splits = most > 1 && keys > sp.chunk ? div_up(keys, sp.chunk) : 1;
+  return sp;
+}
+
+struct PagedPlan {
+  int64_t few_rows, many_rows;  // rows with partial results
+  size_t bytes;                 // of the workspace
+};
+
+// Divides a call by its sizes.
+static PagedPlan plan_paged(PagedWork& w, int requests, int tokens, int q_heads, int kv_heads,
+                            int max_q_len, int max_kv_len, int window) {
   w.group = q_heads / kv_heads;
-  const int most = max_q_len < tokens ? max_q_len : tokens;
+  const int most = max_q_len < 1 ? 1 : max_q_len < tokens ? max_q_len : tokens;
   w.few_tokens = kFewRows / w.group < most ? kFewRows / w.group : most;
+  if (requests == 1 && most > w.few_tokens) w.few_tokens = 0;  // one request: one kernel
   w.few_rows = w.few_tokens * w.group;
-  // keys that a request's rows see, from a tile's begin on
-  int64_t keys = max_kv_len;
-  if (window > 0 && keys > (int64_t)window + most + kTileKeys)
-    keys = (int64_t)window + most + kTileKeys;
-  w.few = split_few(requests, kv_heads, (int)(keys > 0 ? keys : 1));
-  return part_bytes((int64_t)requests * kv_heads * w.few_rows, w.few);
+  // keys that a CTA's rows see, from a tile's begin on (1: there may be none)
+  const int64_t cap = (int64_t)max_kv_len > 0 ? max_kv_len : 1;
+  auto seen = [&](int64_t rows) {
+    const int64_t x = (int64_t)window + rows + kTileKeys;
+    return window > 0 && x < cap ? x : cap;
+  };
+  PagedPlan plan = {};
+  if (w.few_tokens > 0) {
+    w.few = split_few(requests, kv_heads, seen(w.few_tokens));
+    plan.few_rows = (int64_t)requests * kv_heads * w.few_rows;
+  }
+  if (most > w.few_tokens) {
+    const int each = paged_chunk_tokens(w.group);
+    const int64_t slots = requests == 1 ? div_up(tokens, each) : tokens / each + requests;
+    w.many = split_many(slots * kv_heads, seen(each));
+    plan.many_rows = (int64_t)tokens * q_heads;
+  }
+  plan.bytes = part_bytes(plan.few_rows, w.few) + part_bytes(plan.many_rows, w.many);
+  return plan;
+}
+
+static void place_parts(PagedSplit& sp, int64_t rows, float*& at) {
+  if (sp.splits <= 1) return;
+  sp.part_o = at;
+  sp.part_lse = at + rows * sp.splits * kHeadDim;
+  at += part_bytes(rows, sp) / sizeof(float);
 }
 
 }  // namespace tw
@@ -156,7 +175,7 @@ extern "C" size_t tw_paged_attention_workspace_size(int requests, int tokens, in
       head_dim != kHeadDim)
     return 0;
   PagedWork w = {};
-  return plan_paged(w, requests, tokens, q_heads, kv_heads, max_q_len, max_kv_len, window);
+  return plan_paged(w, requests, tokens, q_heads, kv_heads, max_q_len, max_kv_len, window).bytes;
 }
 
 extern "C" int tw_paged_attention(const tw_paged_attention_args* args, void* stream) {
@@ -181,14 +200,14 @@ extern "C" int tw_paged_attention(const tw_paged_attention_args* args, void* str
   PagedWork w = {};
   w.a = a;
   w.scale_log2 = a.softmax_scale * 1.4426950408889634f;
-  const size_t need = plan_paged(w, a.requests, a.tokens, a.q_heads, a.pool.kv_heads, a.max_q_len,
-                                 a.max_kv_len, a.window);
-  if (need > 0) {
-    if (!a.workspace || a.workspace_bytes < need) return TW_ERR_CAPACITY;
+  const PagedPlan plan = plan_paged(w, a.requests, a.tokens, a.q_heads, a.pool.kv_heads,
+                                    a.max_q_len, a.max_kv_len, a.window);
+  if (plan.bytes > 0) {
+    if (!a.workspace || a.workspace_bytes < plan.bytes) return TW_ERR_CAPACITY;
     if (!aligned16(a.workspace)) return TW_ERR_BAD_ARG;
-    const int64_t rows = (int64_t)a.requests * a.pool.kv_heads * w.few_rows;
-    w.few.part_o = (float*)a.workspace;
-    w.few.part_lse = w.few.part_o + rows * w.few.splits * kHeadDim;
+    float* at = (float*)a.workspace;
+    place_parts(w.few, plan.few_rows, at);
+    place_parts(w.many, plan.many_rows, at);
   }
   // one box: the rows that a page and a tile of 64 keys have in common
   w.box = 64;
@@ -204,17 +223,14 @@ extern "C" int tw_paged_attention(const tw_paged_attention_args* args, void* str
   if (st == TW_OK) st = encode_rows_map(&maps.v, a.pool.dtype, 4, a.pool.v_pages, dims, strides, box);
   if (st != TW_OK) return st;
   cudaStream_t s = (cudaStream_t)stream;
-  st = launch_paged_token(w, maps, s);
-  if (st != TW_OK) return st;
-  if (w.few.splits > 1 && w.few_rows > 0) {
-    st = a.out_dtype == TW_F32    ? launch_merge<float>(w, s)
-         : a.pool.dtype == TW_F16 ? launch_merge<__half>(w, s)
-                                  : launch_merge<__nv_bfloat16>(w, s);
+  if (w.many.splits > 0) {
+    st = launch_paged_chunk(w, maps, s);
+    if (st == TW_OK && w.many.splits > 1) st = launch_merge<false>(w, plan.many_rows, s);
     if (st != TW_OK) return st;
   }
-  if (a.max_q_len <= w.few_tokens) return TW_OK;
-  if (a.pool.dtype == TW_F16)
-    return a.out_dtype == TW_F32 ? launch_rows<__half, float>(w, s) : launch_rows<__half, __half>(w, s);
-  return a.out_dtype == TW_F32 ? launch_rows<__nv_bfloat16, float>(w, s)
-                               : launch_rows<__nv_bfloat16, __nv_bfloat16>(w, s);
+  if (w.few.splits > 0) {
+    st = launch_paged_token(w, maps, s);
+    if (st == TW_OK && w.few.splits > 1) st = launch_merge<true>(w, plan.few_rows, s);
+  }
+  return st;
 }

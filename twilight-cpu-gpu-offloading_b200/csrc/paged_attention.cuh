@@ -25,7 +25,7 @@ struct PagedWork {
   tw_paged_attention_args a;
   float scale_log2;  // softmax_scale * log2(e)
   int group;         // query heads per KV head
-  int few_tokens;    // requests with at most this many new tokens: token kernel
+  int few_tokens;    // requests with at most this many new tokens: token kernel (0: none)
   int few_rows;      // few_tokens * group
   int box;           // token rows of one TMA box
   PagedSplit few;    // rows: (request * kv_heads + head) * few_rows + row
@@ -65,19 +65,28 @@ __device__ __forceinline__ float ex2(float x) {
 
 struct PagedRange {
   int begin, end;  // keys
-  int parts;       // ranges that the request is divided into
+  int parts;       // ranges that [low, high) is divided into
 };
 
-// Range `s` of a request's keys.
-__device__ __forceinline__ PagedRange paged_range(const tw_paged_attention_args& a,
-                                                  const PagedRequest& r, const PagedSplit& sp,
-                                                  int s) {
-  const int low = paged_low(a, max(r.kv - r.n, 0)) / kTileKeys * kTileKeys;
+// Range `part` of the keys [low, high).
+__device__ __forceinline__ PagedRange paged_range(const PagedSplit& sp, int low, int high,
+                                                  int part) {
+  low = low / kTileKeys * kTileKeys;
   PagedRange x;
-  x.parts = min(max((r.kv - low + sp.chunk - 1) / sp.chunk, 1), sp.splits);
-  x.begin = low + s * sp.chunk;
-  x.end = s == x.parts - 1 ? r.kv : min(r.kv, x.begin + sp.chunk);
+  x.parts = min(max((high - low + sp.chunk - 1) / sp.chunk, 1), sp.splits);
+  x.begin = low + part * sp.chunk;
+  x.end = part == x.parts - 1 ? high : min(high, x.begin + sp.chunk);
   return x;
+}
+
+// Keys that some of the rows [i, i + n) of a request see.
+struct PagedKeys {
+  int low, high;
+};
+__device__ __forceinline__ PagedKeys paged_keys(const tw_paged_attention_args& a,
+                                                const PagedRequest& r, int i, int n) {
+  const int p = r.kv - r.n + i;
+  return {paged_low(a, max(p, 0)), max(p + n, 0)};
 }
 
 // Softmax-weighted sum of V over the keys [low, high) for one row, by a warp:
@@ -166,6 +175,25 @@ struct PagedMaps {
   CUtensorMap k, v;
 };
 
+// Rows past the last token: out 0, lse -inf.  For CTA `cta` of kPadCtas.
+constexpr int kPadCtas = 8;
+template <typename Out>
+__device__ __forceinline__ void paged_clear_padding(const tw_paged_attention_args& a, int cta) {
+  const int end = min(max(a.cu_q[a.requests], 0), a.tokens);
+  const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+  const int64_t rows = (int64_t)(a.tokens - end) * a.q_heads;
+  for (int64_t i = (int64_t)cta * blockDim.x + threadIdx.x; i < rows * 32;
+       i += (int64_t)kPadCtas * blockDim.x) {
+    const int64_t row = i >> 5;
+    paged_store_row<Out, 4>(a, end + (int)(row / a.q_heads), (int)(row % a.q_heads),
+                            (int)(i & 31) * 4, zero, -CUDART_INF_F);
+  }
+}
+
+// New tokens that a CTA of the chunk kernel takes: 2 x 128 rows.
+__host__ __device__ __forceinline__ int paged_chunk_tokens(int group) { return 2 * (128 / group); }
+
 int launch_paged_token(const PagedWork& w, const PagedMaps& maps, cudaStream_t stream);
+int launch_paged_chunk(const PagedWork& w, const PagedMaps& maps, cudaStream_t stream);
 
 }  // namespace tw

@@ -1,0 +1,474 @@
+// Paged attention of requests with many new tokens: chunks of prompts.
+//
+// Mathematics as in the token kernel (reference m that moves only when a score
+// exceeds it by more than 8 in log2 units, sum l, O), on 128 x 128 products.
+//
+// Bound: the tensor cores, 4 D flops per visible (row, key): S = Q K^T and
+// O += P V.  Next to them the special-function unit, one 2^x per pair, which
+// takes as long as the two products (16 a clock against 8192 flops a clock).
+//
+// Layout: a CTA takes 2 x 128 rows of one KV head, a row being a (token, query
+// head of the group) pair, so K and V are read once for all heads of the group
+// and each tile of 128 keys once for both halves.  One thread issues all
+// products; a warp copies Q once and K / V tiles by TMA into a ring of five
+// 32 KB slots, page piece by page piece; two warpgroups take one half each, a
+// thread one row: it reads its row of S from tensor memory, writes the weights
+// P back over it in 16 bits, and the product with V takes P from there.  The
+// halves alternate: while one computes its weights, the tensor cores work for
+// the other.
+#include "paged_attention.cuh"
+#include "tensor.cuh"
+
+namespace tw {
+
+constexpr int kChRows = 128;                      // rows of a half
+constexpr int kChSoftmax = 256;                   // threads 0..255: the halves' rows
+constexpr int kChMmaWarp = 8, kChLoadWarp = 9;
+constexpr int kChThreads = 320;
+constexpr int kChHalfTile = 128 * 128;            // bytes: 128 rows of 64 elements
+constexpr int kChTileBytes = 2 * kChHalfTile;
+constexpr int kChSlots = 5;
+constexpr int kChSmem = (2 + kChSlots) * kChTileBytes + 1024;
+constexpr int kChColumns = 512;                   // S0, S1, O0, O1: 128 columns each
+constexpr float kChMoveBy = 8.0f;                 // log2 units
+
+template <typename T> struct Pack16;
+template <> struct Pack16<__half> {
+  static constexpr bool kBf16 = false;
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+template <> struct Pack16<__nv_bfloat16> {
+  static constexpr bool kBf16 = true;
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+
+__device__ __forceinline__ void softmax_sync() {
+  asm volatile("bar.sync 1, %0;" ::"n"(kChSoftmax) : "memory");
+}
+
+struct ChunkShared {
+  uint64_t full[kChSlots], empty[kChSlots];
+  uint64_t q_full, ragged;      // Q is there; a tile whose V rows get cleared is there
+  uint64_t s_full[2], p_full[2];  // scores / weights of a half
+  uint64_t o_full, drain;
+  uint32_t tmem;
+  volatile int abort;
+  unsigned bad[8];              // rows to be done again, a word per warp
+};
+
+template <typename T, typename Out>
+__global__ void __launch_bounds__(kChThreads, 1)
+paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ PagedMaps maps,
+                   const __grid_constant__ CUtensorMap q_map) {
+  extern __shared__ char s_raw[];
+  __shared__ ChunkShared sh;
+  const tw_paged_attention_args& a = w.a;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int kv_heads = a.pool.kv_heads;
+  const int R = w.group;
+  const int tokens = paged_chunk_tokens(R), half_tokens = tokens / 2;
+  pdl_wait();
+  pdl_launch_dependents();
+
+  // The CTA's request: a request with rows [c, d) owns the slots from
+  // c / tokens + b on, one per `tokens` rows, and no two requests share one.
+  // The last slots come first: within a request they see the most keys.
+  const int64_t cta = blockIdx.x;
+  const int split = (int)(cta % w.many.splits);
+  const int g = (int)(cta / w.many.splits % kv_heads);
+  const int slots = a.tokens / tokens + a.requests;
+  const int64_t ctas = (int64_t)slots * kv_heads * w.many.splits;
+  if (cta >= ctas) {
+    paged_clear_padding<Out>(a, (int)(cta - ctas));
+    return;
+  }
+  const int slot = slots - 1 - (int)(cta / w.many.splits / kv_heads);
+  int b = 0;
+  for (int lo = 0, hi = a.requests; lo < hi;) {  // last b whose first slot is <= slot
+    const int mid = (lo + hi) >> 1;
+    if (a.cu_q[mid] / tokens + mid <= slot) {
+      b = mid;
+      lo = mid + 1;
+    } else {
+      hi = mid;
+    }
+  }
+  const PagedRequest rq = paged_request(a, b);
+  const int begin = (slot - (rq.first / tokens + b)) * tokens;  // first token of the CTA
+  if (rq.n <= w.few_tokens || begin >= rq.n || begin < 0) return;
+  if (rq.n > a.max_q_len) {
+    if (tid == 0) raise_error(a.error_flag, TW_ERR_BAD_ARG);
+    return;
+  }
+  const int here = min(rq.n - begin, tokens);    // tokens of the CTA
+  const PagedKeys keys = paged_keys(a, rq, begin, here);
+  const PagedRange range = paged_range(w.many, keys.low, keys.high, split);
+  if (split >= range.parts) return;
+  const int halves = here > half_tokens ? 2 : 1;
+  const int p_first = rq.kv - rq.n + begin;      // position of the first token
+  const int low = max(range.begin, keys.low), high = range.end;
+  const int key0 = low / kTileKeys * kTileKeys;
+  const int tiles = high > low ? (high - key0 + kTileKeys - 1) / kTileKeys : 0;
+
+  char* smem = (char*)(((uintptr_t)s_raw + 1023) & ~(uintptr_t)1023);
+  const uint32_t q_at = smem_addr(smem);
+  const uint32_t ring = q_at + 2 * kChTileBytes;
+  if (warp == kChMmaWarp) tmem_alloc(&sh.tmem, kChColumns);
+  if (tid == 0) {
+    for (int i = 0; i < kChSlots; ++i) {
+      mbar_init(&sh.full[i], 1);
+      mbar_init(&sh.empty[i], 1);
+    }
+    mbar_init(&sh.q_full, 1);
+    mbar_init(&sh.ragged, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh.s_full[i], 1);
+      mbar_init(&sh.p_full[i], kChRows);
+    }
+    mbar_init(&sh.o_full, 1);
+    mbar_init(&sh.drain, 1);
+    sh.abort = 0;
+    mbar_init_fence();
+  }
+  if (tid < 8) sh.bad[tid] = 0;
+  tmem_fence_before();
+  __syncthreads();
+  tmem_fence_after();
+  const uint32_t tmem = sh.tmem;
+
+  if (warp == kChLoadWarp) {
+    // ---- copies.  Slot n % kChSlots: n = 2j is K tile j, n = 2j + 1 is V tile j.
+    if (lane == 0) {
+      prefetch_map(&q_map);
+      prefetch_map(&maps.k);
+      prefetch_map(&maps.v);
+      mbar_arrive_expect(&sh.q_full, (uint32_t)(halves * R * half_tokens * kHeadDim * 2));
+      for (int i = 0; i < halves && tiles > 0; ++i)
+        for (int d = 0; d < 2; ++d)
+          tma_load_3d(&q_map, q_at + i * kChTileBytes + d * kChHalfTile, &sh.q_full, d * 64, g * R,
+                      rq.first + begin + i * half_tokens);
+    }
+    const int boxes = kTileKeys / w.box;  // per tile and 64 dimensions; 2 * boxes <= 32
+    const int dim_half = lane / boxes;    // 0, 1; more: idle
+    const int box = lane % boxes;
+    const int32_t* table = a.block_table + (int64_t)b * a.table_stride;
+    const uint32_t dst = ring + dim_half * kChHalfTile + box * w.box * 128;
+    // boxes wholly before the first visible key are not read: a page that slid out
+    // of the window may be gone
+    const int skipped = (low - key0) / w.box;
+    int key = key0 + box * w.box;
+    int page = 0;
+    if (dim_half < 2 && key < high && box >= skipped) page = table[key / a.pool.page_size];
+    int n = 0, done_ragged = 0;
+    bool ok = true;
+    for (int j = 0; j < tiles && ok; ++j) {
+      const int at = key, from = page;
+      const bool mine = dim_half < 2 && at < high && (j > 0 || box >= skipped);
+      key += kTileKeys;
+      if (dim_half < 2 && j + 1 < tiles && key < high) page = table[key / a.pool.page_size];
+      int p = from;
+      if (mine && (p < 0 || p >= a.pool.num_pages)) {
+        raise_error(a.error_flag, TW_ERR_INVALID_INDEX);
+        p = (int)a.pool.num_pages;  // out of the map's range: zeros
+      }
+      const int first = key0 + j * kTileKeys;
+      const int valid = min(high - first, kTileKeys);
+      const int count = (valid + w.box - 1) / w.box - (j == 0 ? skipped : 0);
+      const uint32_t bytes = (uint32_t)(count * w.box * kHeadDim * 2);
+      const bool ragged = first < low || valid < kTileKeys;
+#pragma unroll 1
+      for (int m = 0; m < 2; ++m, ++n) {
+        const int s = n % kChSlots;
+        if (n >= kChSlots &&
+            !__all_sync(0xffffffffu, mbar_wait(&sh.empty[s],
+                                               (uint32_t)((n / kChSlots - 1) & 1), &sh.abort))) {
+          ok = false;
+          break;
+        }
+        uint64_t* bar = m == 1 && ragged ? &sh.ragged : &sh.full[s];
+        if (lane == 0) mbar_arrive_expect(bar, bytes);
+        __syncwarp();
+        if (mine)
+          tma_load_4d(m == 0 ? &maps.k : &maps.v, dst + s * kChTileBytes, bar, dim_half * 64,
+                      at % a.pool.page_size, g, p);
+        if (m == 1 && ragged) {
+          // V rows that no row sees: what they hold (NaN included) must not meet a
+          // weight of zero
+          if (!__all_sync(0xffffffffu,
+                          mbar_wait(bar, (uint32_t)(done_ragged & 1), &sh.abort))) {
+            ok = false;
+            break;
+          }
+          ++done_ragged;
+          char* tile = smem + (2 + s) * kChTileBytes;
+          for (int i = lane; i < kTileKeys * 16; i += 32) {
+            const int row = i >> 4;
+            if (first + row < low || row >= valid)
+              reinterpret_cast<uint4*>(tile + ((i >> 3) & 1) * kChHalfTile + row * 128)[i & 7] =
+                  make_uint4(0u, 0u, 0u, 0u);
+          }
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.full[s]);
+        }
+      }
+    }
+    if (!ok || sh.abort) {
+      // give up: wait (with the same limit) for the copies in flight
+      volatile int never = 0;
+      mbar_wait(&sh.q_full, 0, &never);
+      for (int i = max(0, n - kChSlots); i < n; ++i)
+        mbar_wait(&sh.full[i % kChSlots], (uint32_t)((i / kChSlots) & 1), &never);
+    }
+  } else if (warp == kChMmaWarp) {
+    // ---- products, all issued by one thread
+    if (lane == 0 && tiles > 0) {
+      constexpr uint32_t desc_s = product_desc(Pack16<T>::kBf16, kTileKeys, false);
+      constexpr uint32_t desc_o = product_desc(Pack16<T>::kBf16, kHeadDim, true);
+      // S of half i from Q_i and the K tile in ring slot s
+      auto scores = [&](int i, int s) {
+        const uint32_t qa = q_at + i * kChTileBytes, ka = ring + s * kChTileBytes;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const uint32_t off = (k >> 2) * kChHalfTile + (k & 3) * 32;
+          mma_smem(tmem + i * 128, operand_desc(qa + off, 16, 1024), operand_desc(ka + off, 16, 1024),
+                   desc_s, k > 0);
+        }
+        mma_commit(&sh.s_full[i]);
+      };
+      auto values = [&](int i, int s, bool add) {
+        const uint32_t va = ring + s * kChTileBytes;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          mma_tmem(tmem + 256 + i * 128, tmem + i * 128 + k * 8,
+                   operand_desc(va + k * 2048, kChHalfTile, 1024), desc_o, add || k > 0);
+      };
+      auto wait_slot = [&](int n) {
+        return mbar_wait(&sh.full[n % kChSlots], (uint32_t)((n / kChSlots) & 1), &sh.abort);
+      };
+      bool ok = mbar_wait(&sh.q_full, 0, &sh.abort) && wait_slot(0);
+      if (ok) {
+        tmem_fence_after();
+        for (int i = 0; i < halves; ++i) scores(i, 0);
+        mma_commit(&sh.empty[0]);
+      }
+      for (int j = 0; j < tiles && ok; ++j) {
+        const int nv = 2 * j + 1, nk = 2 * j + 2;
+        if (!wait_slot(nv)) break;
+        if (j + 1 < tiles && !wait_slot(nk)) break;
+        for (int i = 0; i < halves; ++i) {
+          ok = mbar_wait(&sh.p_full[i], (uint32_t)(j & 1), &sh.abort);
+          if (!ok) break;
+          tmem_fence_after();
+          values(i, nv % kChSlots, j > 0);
+          if (i == halves - 1) mma_commit(&sh.empty[nv % kChSlots]);
+          if (j + 1 < tiles) scores(i, nk % kChSlots);
+        }
+        if (ok && j + 1 < tiles) mma_commit(&sh.empty[nk % kChSlots]);
+      }
+      if (!sh.abort) {
+        mma_commit(&sh.o_full);
+      } else {
+        volatile int never = 0;
+        mma_commit(&sh.drain);
+        mbar_wait(&sh.drain, 0, &never);
+      }
+    }
+  } else {
+    // ---- weights: a thread per row
+    const int i = warp >> 2;              // half
+    const int r = tid & (kChRows - 1);    // row of the half
+    const int token = r / R, head = r - token * R;
+    const int ti = i * half_tokens + token;  // token of the CTA
+    const bool live = token < half_tokens && ti < here;
+    const int p = p_first + ti;           // keys [see, p] (rows that are not live: any)
+    const int see = paged_low(a, p);
+    // keys that all rows of the half see: tiles inside need no mask
+    const int p_half = p_first + i * half_tokens;
+    const int all_low = paged_low(a, p_half + half_tokens - 1), all_high = p_half + 1;
+    const uint32_t my = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t s_col = my + i * 128, o_col = my + 256 + i * 128;
+    float m = -CUDART_INF_F;
+    uint64_t l2[2] = {0ull, 0ull};
+    const uint64_t scale2 = pair(w.scale_log2, w.scale_log2);
+    bool ok = true;
+    if (i < halves) {
+      for (int j = 0; j < tiles; ++j) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&sh.s_full[i], (uint32_t)(j & 1), &sh.abort));
+        if (!ok) break;
+        tmem_fence_after();
+        float s[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32(s[c], s_col + c * 32);
+        tmem_wait_ld();
+        const int first = key0 + j * kTileKeys;
+        if (first < all_low || first < low || first + kTileKeys > min(all_high, high)) {
+          const int from = max(see, low) - first, to = min(p + 1, high) - first;
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int x = 0; x < 32; ++x)
+              if (c * 32 + x < from || c * 32 + x >= to) s[c][x] = -CUDART_INF_F;
+        }
+        float top[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          top[c] = fmaxf(s[c][0], s[c][1]);
+#pragma unroll
+          for (int x = 2; x < 32; x += 2) top[c] = fmaxf(top[c], fmaxf(s[c][x], s[c][x + 1]));
+        }
+        const float t = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * w.scale_log2;
+        const bool move = t > m + kChMoveBy;
+        if (__any_sync(0xffffffffu, move)) {
+          const float f = move ? ex2(m - t) : 1.f;
+          if (move) m = t;
+          const uint64_t f2 = pair(f, f);
+          l2[0] = mul2(l2[0], f2);
+          l2[1] = mul2(l2[1], f2);
+          if (j > 0) {  // O of the tiles so far is complete: S of this one came after it
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              float o[32];
+              tmem_ld32(o, o_col + c * 32);
+              tmem_wait_ld();
+              uint32_t u[32];
+#pragma unroll
+              for (int x = 0; x < 32; ++x) u[x] = __float_as_uint(o[x] * f);
+              tmem_st32(o_col + c * 32, u);
+            }
+          }
+        }
+        const float u = m == -CUDART_INF_F ? 0.f : -m;
+        const uint64_t u2 = pair(u, u);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          // weights rounded to the 16-bit type for the product (the sum l keeps
+          // them in 32 bits): half a unit each, of either sign
+          uint32_t packed[16];
+#pragma unroll
+          for (int x = 0; x < 32; x += 2) {
+            float e0, e1;
+            unpair(fma2(pair(s[c][x], s[c][x + 1]), scale2, u2), e0, e1);
+            e0 = ex2(e0);
+            e1 = ex2(e1);
+            l2[(x >> 1) & 1] = add2(l2[(x >> 1) & 1], pair(e0, e1));
+            packed[x >> 1] = Pack16<T>::pack(e0, e1);
+          }
+          tmem_st16(s_col + c * 16, packed);
+        }
+        tmem_wait_st();
+        tmem_fence_before();
+        mbar_arrive(&sh.p_full[i]);
+      }
+    }
+    float l = 0.f;
+    {
+      float x0, x1;
+      unpair(add2(l2[0], l2[1]), x0, x1);
+      l = x0 + x1;
+    }
+    if (tiles > 0 && ok)
+      ok = __all_sync(0xffffffffu, mbar_wait(&sh.o_full, 0, &sh.abort));
+    tmem_fence_after();
+    if (!ok && lane == 0) raise_error(a.error_flag, TW_ERR_TIMEOUT);
+    const int t = rq.first + begin + ti, h = g * R + head;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float lse2 = l == 0.f ? -CUDART_INF_F : m + log2f(l);
+    const bool joined = range.parts == 1;
+    const int64_t row = (int64_t)t * a.q_heads + h;
+    if (i < halves) {
+      float odd = 0.f;
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        float o[32];
+        if (tiles > 0) {
+          tmem_ld32(o, o_col + c * 32);
+          tmem_wait_ld();
+        }
+#pragma unroll
+        for (int x = 0; x < 32; ++x) {
+          o[x] = l == 0.f ? 0.f : o[x] * inv;
+          odd = fmaf(o[x], 0.f, odd);  // NaN when one is not finite
+        }
+        if (live) {
+          if (joined)
+            paged_store_row<Out, 32>(a, t, h, c * 32, o, lse2);
+          else
+            paged_store_part<32>(w.many, row, split, c * 32, o, lse2);
+        }
+      }
+      // A row that is not finite may owe it to a V row that another token sees
+      // and this one does not (weight 0 times infinity or NaN).
+      const unsigned again = __ballot_sync(0xffffffffu, live && odd != 0.f);
+      if (lane == 0) sh.bad[warp] = again;
+    }
+    softmax_sync();
+    for (int x = 0; x < 8; ++x) {
+      for (unsigned bad = sh.bad[x]; bad; bad &= bad - 1) {
+        const int rr = (x & 3) * 32 + __ffs(bad) - 1;
+        if (rr % 8 != warp) continue;
+        const int tt = (x >> 2) * half_tokens + rr / R;
+        const int hh = g * R + rr % R;
+        const int pp = p_first + tt;
+        const PagedRow y = paged_one_row<T>(w, b, rq.first + begin + tt, hh,
+                                            max(range.begin, paged_low(a, pp)),
+                                            min(range.end, pp + 1));
+        float o[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[c] = y.l == 0.f ? 0.f : y.acc[c] / y.l;
+        const float z = y.l == 0.f ? -CUDART_INF_F : y.m + log2f(y.l);
+        if (joined)
+          paged_store_row<Out, 4>(a, rq.first + begin + tt, hh, lane * 4, o, z);
+        else
+          paged_store_part<4>(w.many, (int64_t)(rq.first + begin + tt) * a.q_heads + hh, split,
+                              lane * 4, o, z);
+      }
+    }
+    tmem_fence_before();
+  }
+  __syncwarp();
+  __syncthreads();
+  if (warp == kChMmaWarp) {
+    tmem_fence_after();
+    tmem_free(tmem, kChColumns);
+  }
+}
+
+template <typename T, typename Out>
+static int launch_chunk(const PagedWork& w, const PagedMaps& maps, cudaStream_t stream) {
+  const int tokens = paged_chunk_tokens(w.group);
+  CUtensorMap q_map;
+  const cuuint64_t dims[3] = {(cuuint64_t)kHeadDim, (cuuint64_t)w.a.q_heads,
+                              (cuuint64_t)w.a.tokens};
+  const cuuint64_t strides[2] = {(cuuint64_t)w.a.q_head_stride * 2,
+                                 (cuuint64_t)w.a.q_token_stride * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)w.group, (cuuint32_t)tokens / 2};
+  int rc = encode_rows_map(&q_map, w.a.pool.dtype, 3, w.a.q, dims, strides, box);
+  if (rc != TW_OK) return rc;
+  static DynSmemOptIn opt_in;
+  const auto kernel = paged_chunk_kernel<T, Out>;
+  rc = ensure_dyn_smem((const void*)kernel, opt_in, kChSmem);
+  if (rc != TW_OK) return rc;
+  const int64_t ctas = ((int64_t)w.a.tokens / tokens + w.a.requests) * w.a.pool.kv_heads *
+                           w.many.splits +
+                       (w.few_tokens > 0 ? 0 : kPadCtas);
+  if (ctas > INT32_MAX) return TW_ERR_UNSUPPORTED;
+  return launch_pdl(kernel, dim3((unsigned)ctas), dim3(kChThreads), (size_t)kChSmem, stream, w,
+                    maps, q_map);
+}
+
+int launch_paged_chunk(const PagedWork& w, const PagedMaps& maps, cudaStream_t stream) {
+  if (w.a.pool.dtype == TW_F16)
+    return w.a.out_dtype == TW_F32 ? launch_chunk<__half, float>(w, maps, stream)
+                                   : launch_chunk<__half, __half>(w, maps, stream);
+  return w.a.out_dtype == TW_F32 ? launch_chunk<__nv_bfloat16, float>(w, maps, stream)
+                                 : launch_chunk<__nv_bfloat16, __nv_bfloat16>(w, maps, stream);
+}
+
+}  // namespace tw

@@ -32,7 +32,6 @@ constexpr int kTokHalf = kTokTile * 128;          // 64 of the 128 dimensions of
 constexpr int kTokStageBytes = 4 * kTokHalf;      // K lo, K hi, V lo, V hi
 constexpr int kTokRowPad = kHeadDim + 4;          // floats per row of the join
 constexpr int kTokSmem = kTokStages * kTokStageBytes + 1024;  // + alignment of the swizzle
-constexpr int kPadCtas = 8;        // CTAs that clear the rows past the last token
 constexpr float kMoveBy = 8.0f;    // log2 units
 
 template <typename T> struct MmaType;
@@ -104,17 +103,8 @@ paged_token_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
   pdl_wait();
   pdl_launch_dependents();
 
-  if (cta >= units) {  // rows past the last token: out 0, lse -inf
-    const int end = min(max(a.cu_q[a.requests], 0), a.tokens);
-    const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-    const int64_t rows = (int64_t)(a.tokens - end) * a.q_heads;
-    for (int64_t i = (cta - units) * kTokThreads + tid; i < rows * 32;
-         i += (int64_t)kPadCtas * kTokThreads) {
-      const int64_t row = i >> 5;
-      const int t = end + (int)(row / a.q_heads);
-      paged_store_row<Out, 4>(a, t, (int)(row % a.q_heads), (int)(i & 31) * 4, zero,
-                              -CUDART_INF_F);
-    }
+  if (cta >= units) {
+    paged_clear_padding<Out>(a, (int)(cta - units));
     return;
   }
   const int split = (int)(cta % w.few.splits);
@@ -127,12 +117,12 @@ paged_token_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
     if (rq.n > a.max_q_len && tid == 0) raise_error(a.error_flag, TW_ERR_BAD_ARG);
     return;
   }
-  const PagedRange range = paged_range(a, rq, w.few, split);
+  const PagedKeys keys = paged_keys(a, rq, 0, rq.n);
+  const PagedRange range = paged_range(w.few, keys.low, keys.high, split);
   if (split >= range.parts) return;
   const int R = w.group;
   const int rows = rq.n * R;
-  // keys that some row sees, in this range
-  const int low = max(range.begin, paged_low(a, max(rq.kv - rq.n, 0)));
+  const int low = max(range.begin, keys.low);  // first key that some row sees, in this range
   const int tile0 = low / kTokTile * kTokTile;
   const int tiles = range.end > low ? (range.end - tile0 + kTokTile - 1) / kTokTile : 0;
 
@@ -174,7 +164,8 @@ paged_token_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
       key += kTokTile;
       if (matrix < 2 && i + 1 < tiles && key < range.end) page = table[key / a.pool.page_size];
       if (i >= kTokStages &&
-          !mbar_wait(&s_empty[stage], (uint32_t)((i / kTokStages - 1) & 1), &s_abort))
+          !__all_sync(0xffffffffu, mbar_wait(&s_empty[stage],
+                                             (uint32_t)((i / kTokStages - 1) & 1), &s_abort)))
         break;
       if (lane == 0) {
         const int valid = min(range.end - (tile0 + i * kTokTile), kTokTile);
@@ -242,7 +233,9 @@ paged_token_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
     const int stage = i % kTokStages;
     const uint32_t base = stage * kTokStageBytes;
     const int key0 = tile0 + i * kTokTile + wrow;  // the warp's first key
-    if (!mbar_wait(&s_full[stage], (uint32_t)((i / kTokStages) & 1), &s_abort)) break;
+    if (!__all_sync(0xffffffffu,
+                    mbar_wait(&s_full[stage], (uint32_t)((i / kTokStages) & 1), &s_abort)))
+      break;
     if (key0 < range.end && key0 + 16 > low) {
       const bool edge = key0 < all_low || key0 + 16 > all_high || key0 < low ||
                         key0 + 16 > range.end;
