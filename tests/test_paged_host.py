@@ -4,6 +4,7 @@ host (no kernel is launched)."""
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import pytest
 
@@ -13,6 +14,30 @@ def test_struct_sizes(tw):
     assert ctypes.sizeof(L.PagedPool) == lib.tw_paged_pool_size()
     assert ctypes.sizeof(L.PagedStepArgs) == lib.tw_paged_step_args_size()
     assert ctypes.sizeof(L.PagedAttentionArgs) == lib.tw_paged_attention_args_size()
+
+
+def flat(cls):
+    """(offset, size, is float) of every field, the nested ones' too."""
+    for name, kind in cls._fields_:
+        field = getattr(cls, name)
+        if issubclass(kind, ctypes.Structure):
+            yield from ((field.offset + o, n, f) for o, n, f in flat(kind))
+        else:
+            yield field.offset, field.size, kind is ctypes.c_float
+
+
+@pytest.mark.parametrize("cls,fmt", [("PagedPool", "PAGED_POOL_FORMAT"),
+                                     ("PagedStepArgs", "PAGED_STEP_FORMAT"),
+                                     ("PagedAttentionArgs", "PAGED_ATTENTION_FORMAT")])
+def test_packed_layout(tw, cls, fmt):
+    """The formats that the wrappers pack are the structs, field by field."""
+    cls, fmt = getattr(tw._lib, cls), getattr(tw._lib, fmt)
+    assert struct.calcsize(fmt) == ctypes.sizeof(cls)
+    fields = list(flat(cls))
+    assert len(fields) == len(fmt)
+    for i, (offset, size, is_float) in enumerate(fields):
+        assert struct.calcsize(fmt[:i + 1]) - struct.calcsize(fmt[i]) == offset
+        assert struct.calcsize(fmt[i]) == size and (fmt[i] == "f") == is_float
 
 
 def pool(L, **change):

@@ -100,7 +100,13 @@ class PagedAttentionArgs(ctypes.Structure):
     ]
 
 
-# name -> (restype, argtypes); mirrors include/twilight_b200.h
+# The same structs as struct.Struct formats: packing one is several times faster
+# than filling a ctypes.Structure, and these calls are made once per layer.
+PAGED_POOL_FORMAT = "QQqqqqiiii"
+PAGED_STEP_FORMAT = "QQQqiiiiQqQQQQQQQ"
+PAGED_ATTENTION_FORMAT = PAGED_POOL_FORMAT + "QqqQqiiQQiiiiifQqqiiQQQQ"
+
+# name -> (restype, argtypes); a struct pointer is P: packed bytes or byref(struct); mirrors include/twilight_b200.h
 SIGNATURES = {
     "tw_status_string": (ctypes.c_char_p, [I32]),
     "tw_last_cuda_error": (I32, []),
@@ -140,11 +146,11 @@ SIGNATURES = {
     "tw_qkv_rope": (I32, [P, P, P, P, I32, I32, I32, I32, P, P, I32, P, P, P, P]),
     "tw_decode_attention_noalloc": (I32, [P, P, P, P, I32, I32, I32, I32, I32, FLT, P, I32, P, P]),
     "tw_paged_pool_size": (SZ, []),
-    "tw_paged_step": (I32, [ctypes.POINTER(PagedStepArgs), P]),
+    "tw_paged_step": (I32, [P, P]),
     "tw_paged_step_args_size": (SZ, []),
-    "tw_paged_write": (I32, [ctypes.POINTER(PagedPool), P, I64, I64, P, I64, I64, P, I64, P, P]),
+    "tw_paged_write": (I32, [P, P, I64, I64, P, I64, I64, P, I64, P, P]),
     "tw_paged_attention_workspace_size": (SZ, [I32, I32, I32, I32, I32, I32, I32, I32]),
-    "tw_paged_attention": (I32, [ctypes.POINTER(PagedAttentionArgs), P]),
+    "tw_paged_attention": (I32, [P, P]),
     "tw_paged_attention_args_size": (SZ, []),
 }
 

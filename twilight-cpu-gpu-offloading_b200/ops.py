@@ -6,7 +6,9 @@ libtwilight_b200.so; a CPU tensor is rejected, never computed on the host.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
+import struct
 
 import torch
 
@@ -14,6 +16,7 @@ from . import _lib
 
 HEAD_DIM = 128
 DTYPE_CODES = {torch.float16: _lib.TW_F16, torch.bfloat16: _lib.TW_BF16, torch.float32: _lib.TW_F32}
+_SCALE = 1.0 / math.sqrt(HEAD_DIM)
 SCALE_RECIPROCAL = 0   # "/ 15" as torch on CUDA: x * fp32(1/15)
 SCALE_DIVIDE = 1       # "/ 15" as torch on CPU: IEEE division
 
@@ -327,59 +330,84 @@ def qkv_rope(hidden: torch.Tensor, w_q: torch.Tensor, w_k: torch.Tensor, w_v: to
 
 
 # ------------------------------------------------------------- paged cache --
+# These calls are made for every step and layer, and a short one's kernel takes a
+# few microseconds.  So each has one expression of all checks (the message is
+# worked out only when it fails) and packs its arguments in one go.
 
-def _i32(name: str, t: torch.Tensor, *shape: int | None) -> None:
-    """t is an int32 CUDA tensor of this shape (None: any extent), rows contiguous."""
-    if not t.is_cuda:
+_PACK_POOL = struct.Struct(_lib.PAGED_POOL_FORMAT).pack
+_PACK_STEP = struct.Struct(_lib.PAGED_STEP_FORMAT).pack
+_PACK_ATTENTION = struct.Struct(_lib.PAGED_ATTENTION_FORMAT).pack
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _device_index(t: torch.Tensor) -> int:
+    """The current device's index, which has to be t's."""
+    dev = t.get_device()
+    if dev < 0:
         raise ValueError("twilight ops require CUDA tensors (no CPU fallback)")
-    if t.dtype != torch.int32 or t.dim() != len(shape) or (t.shape[-1] > 1 and t.stride(-1) != 1) \
-            or any(n is not None and n != m for n, m in zip(shape, t.shape)):
-        want = ", ".join("*" if n is None else str(n) for n in shape)
-        raise ValueError(f"{name} must be int32 [{want}] with contiguous rows, "
-                         f"got {t.dtype} {tuple(t.shape)}")
+    if dev != torch.cuda.current_device():
+        raise ValueError(f"the tensors are on cuda:{dev}: make it the current device")
+    return dev
 
 
-def _same_device(device: torch.device, *tensors: torch.Tensor | None) -> None:
-    if any(t is not None and t.device != device for t in tensors):
-        raise ValueError("all tensors of a call must be on one CUDA device")
-    if device.index != torch.cuda.current_device():
-        raise ValueError(f"the tensors are on {device}: make it the current device")
+def _explain(dev: int, *wanted) -> None:
+    """Raises for the first tensor that is not as wanted: (name, tensor, dtype, shape);
+    a tensor of None is optional, an extent of None is any."""
+    for name, t, dtype, shape in wanted:
+        if t is None:
+            continue
+        if t.get_device() < 0:
+            raise ValueError("twilight ops require CUDA tensors (no CPU fallback)")
+        if t.get_device() != dev:
+            raise ValueError(f"{name} must be on the device of the other tensors, cuda:{dev}")
+        if t.dtype != dtype or t.dim() != len(shape) or \
+                any(n is not None and n != m for n, m in zip(shape, t.shape)) or \
+                not (t[0] if t.dim() > 1 and t.shape[0] else t).is_contiguous():
+            want = ", ".join("*" if n is None else str(n) for n in shape)
+            raise ValueError(f"{name} must be {dtype} [{want}] with contiguous rows, got "
+                             f"{t.dtype} {list(t.shape)}")
+    raise ValueError("unexpected tensors")
 
 
 def _rows_strides(name: str, t: torch.Tensor) -> tuple[int, int]:
     """(token, head) strides of [tokens, heads, 128] rows; an extent of 1 has none of its own."""
     token, head, inner = t.stride()
+    tokens, heads, _ = t.shape
     if inner != 1:
         raise ValueError(f"{name} needs contiguous rows of {HEAD_DIM} elements")
-    if t.shape[1] <= 1:
+    if heads <= 1:
         head = HEAD_DIM
-    if t.shape[0] <= 1:
-        token = head * max(t.shape[1], 1)
-    if token <= 0 or head <= 0 or token % 8 or head % 8 or t.data_ptr() % 16:
+    if tokens <= 1:
+        token = head * (heads or 1)
+    if token <= 0 or head <= 0 or (token | head) & 7 or t.data_ptr() & 15:
         raise ValueError(f"{name} needs 16-byte aligned rows (positive strides in multiples of 8)")
     return token, head
 
 
-def _paged_pool(k_pages: torch.Tensor, v_pages: torch.Tensor) -> "_lib.PagedPool":
-    """tw_paged_pool of [pages, kv_heads, page_size, 128] tensors (any order of strides)."""
-    if not (k_pages.is_cuda and v_pages.is_cuda):
-        raise ValueError("twilight ops require CUDA tensors (no CPU fallback)")
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype \
-            or k_pages.shape[3] != HEAD_DIM or 0 in k_pages.shape:
+def _paged_pool(dev: int, k_pages: torch.Tensor, v_pages: torch.Tensor) -> tuple:
+    """The fields of tw_paged_pool for [pages, kv_heads, page_size, 128] tensors (any
+    order of strides)."""
+    shape, strides = k_pages.shape, k_pages.stride()
+    if len(shape) != 4 or shape != v_pages.shape or k_pages.dtype != v_pages.dtype \
+            or shape[3] != HEAD_DIM or 0 in shape:
         raise ValueError(f"k_pages and v_pages must be [pages, kv_heads, page_size, {HEAD_DIM}] "
                          "of one dtype")
-    pages, heads, size, _ = k_pages.shape
-    strides = []
-    for i, (n, s, t) in enumerate(zip(k_pages.shape, k_pages.stride(), v_pages.stride())):
-        if n > 1 and s != t:
-            raise ValueError("k_pages and v_pages must have the same strides")
-        # a dimension of one page, head or row has no stride of its own
-        strides.append(s if n > 1 else HEAD_DIM)
-    if strides[3] != 1 or any(s <= 0 or s % 8 for s in strides[:3]) or \
-            (k_pages.data_ptr() | v_pages.data_ptr()) % 16:
+    if k_pages.get_device() != dev or v_pages.get_device() != dev:
+        _explain(dev, ("k_pages", k_pages, k_pages.dtype, shape),
+                 ("v_pages", v_pages, v_pages.dtype, shape))
+    if 1 in shape:  # an extent of 1 has no stride of its own
+        other = tuple(HEAD_DIM if n == 1 else s for n, s in zip(shape, v_pages.stride()))
+        strides = tuple(HEAD_DIM if n == 1 else s for n, s in zip(shape, strides))
+    else:
+        other = v_pages.stride()
+    if strides != other:
+        raise ValueError("k_pages and v_pages must have the same strides")
+    page, head, token, inner = strides
+    k, v = k_pages.data_ptr(), v_pages.data_ptr()
+    if inner != 1 or page <= 0 or head <= 0 or token <= 0 or (page | head | token) & 7 or \
+            (k | v) & 15:
         raise ValueError("pages need contiguous 16-byte aligned rows (strides in multiples of 8)")
-    return _lib.PagedPool(k_pages.data_ptr(), v_pages.data_ptr(), strides[0], strides[1],
-                          strides[2], pages, size, heads, HEAD_DIM, _kv_code(k_pages.dtype))
+    return k, v, page, head, token, shape[0], shape[2], shape[1], HEAD_DIM, _kv_code(k_pages.dtype)
 
 
 def paged_step(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor,
@@ -395,28 +423,45 @@ def paged_step(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Te
     kv_lens [B], cu_q [B+1], free_count_out [1] and, per new token, slots
     (int64, -1: none) and positions [tokens_cap].  A refused request or a full
     output sets error_flag to TW_ERR_CAPACITY."""
+    dev = _device_index(lens)
+    i32 = torch.int32
     B = lens.shape[0] if lens.dim() == 1 else -1
-    _i32("lens", lens, None)
-    _i32("new_lens", new_lens, B)
-    _i32("block_table", block_table, B, None)
-    _i32("free_pages", free_pages, None)
-    _i32("free_count", free_count, 1)
-    _i32("kv_lens", kv_lens, B)
-    _i32("cu_q", cu_q, B + 1)
-    _i32("free_count_out", free_count_out, 1)
-    if slots.dtype != torch.int64 or slots.dim() != 1 or not slots.is_contiguous():
-        raise ValueError("slots must be int64 [tokens_cap]")
-    _i32("positions", positions, slots.shape[0])
-    _same_device(lens.device, new_lens, block_table, free_pages, free_count, kv_lens, cu_q, slots,
-                 positions, free_count_out, error_flag)
+    each, cap = (B,), slots.shape
+    if not (lens.dtype is new_lens.dtype is block_table.dtype is free_pages.dtype is
+            free_count.dtype is kv_lens.dtype is cu_q.dtype is positions.dtype is
+            free_count_out.dtype is i32 and slots.dtype is torch.int64
+            and new_lens.shape == each and kv_lens.shape == each and cu_q.shape == (B + 1,)
+            and free_pages.dim() == 1 and free_count.shape == (1,)
+            and free_count_out.shape == (1,) and len(cap) == 1 and positions.shape == cap
+            and block_table.dim() == 2 and block_table.shape[0] == B
+            and (block_table.stride(1) == 1 or block_table.shape[1] == 1)
+            and lens.is_contiguous() and new_lens.is_contiguous() and free_pages.is_contiguous()
+            and kv_lens.is_contiguous() and cu_q.is_contiguous() and slots.is_contiguous()
+            and positions.is_contiguous()
+            and dev == new_lens.get_device() == block_table.get_device() ==
+            free_pages.get_device() == free_count.get_device() == kv_lens.get_device() ==
+            cu_q.get_device() == slots.get_device() == positions.get_device() ==
+            free_count_out.get_device()
+            and (error_flag is None
+                 or (error_flag.get_device() == dev and error_flag.dtype is i32))):
+        _explain(dev, ("lens", lens, i32, (None,)), ("new_lens", new_lens, i32, each),
+                 ("block_table", block_table, i32, (B, None)),
+                 ("free_pages", free_pages, i32, (None,)), ("free_count", free_count, i32, (1,)),
+                 ("kv_lens", kv_lens, i32, each), ("cu_q", cu_q, i32, (B + 1,)),
+                 ("slots", slots, torch.int64, (None,)),
+                 ("positions", positions, i32, cap[:1]),
+                 ("free_count_out", free_count_out, i32, (1,)),
+                 ("error_flag", error_flag, i32, (1,)))
     W = block_table.shape[1]
-    args = _lib.PagedStepArgs(
+    args = _PACK_STEP(
         lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(),
-        block_table.stride(0) if B > 1 else W, W, B, page_size, slots.shape[0],
-        free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(), kv_lens.data_ptr(),
-        cu_q.data_ptr(), slots.data_ptr(), positions.data_ptr(), free_count_out.data_ptr(),
-        _ptr(error_flag))
-    _lib.check(lib().tw_paged_step(ctypes.byref(args), _stream(lens.device)), "paged_step")
+        block_table.stride(0) if B > 1 else W, W, B, page_size, cap[0], free_pages.data_ptr(),
+        free_pages.shape[0], free_count.data_ptr(), kv_lens.data_ptr(), cu_q.data_ptr(),
+        slots.data_ptr(), positions.data_ptr(), free_count_out.data_ptr(),
+        0 if error_flag is None else error_flag.data_ptr())
+    status = lib().tw_paged_step(args, _raw_stream(dev))
+    if status:
+        _lib.check(status, "paged_step")
 
 
 def paged_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_pages: torch.Tensor,
@@ -424,21 +469,33 @@ def paged_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_pages: 
     """New rows k / v [T, kv_heads, 128] (strided views of a projection are fine) to
     slots [T] int64 of the pool [pages, kv_heads, page_size, 128] (tw_paged_write);
     slot -1 is skipped."""
-    pool = _paged_pool(k_pages, v_pages)
-    if k.dim() != 3 or k.shape != v.shape or k.shape[1:] != (pool.kv_heads, HEAD_DIM) or \
-            k.dtype != k_pages.dtype or v.dtype != k_pages.dtype:
-        raise ValueError("k and v must be [T, kv_heads, 128] in the pool's dtype")
-    if slots.dtype != torch.int64 or slots.shape != k.shape[:1] or not slots.is_contiguous():
-        raise ValueError("slots must be int64 [T]")
-    _same_device(k_pages.device, v_pages, k, v, slots, error_flag)
-    _lib.check(lib().tw_paged_write(
-        ctypes.byref(pool), k.data_ptr(), *_rows_strides("k", k), v.data_ptr(),
-        *_rows_strides("v", v), slots.data_ptr(), k.shape[0], _ptr(error_flag),
-        _stream(k_pages.device)), "paged_write")
+    dev = _device_index(k)
+    pool = _paged_pool(dev, k_pages, v_pages)
+    shape, dtype = k.shape, k_pages.dtype
+    if not (len(shape) == 3 and shape == v.shape and shape[1] == pool[7] and shape[2] == HEAD_DIM
+            and k.dtype is v.dtype is dtype and slots.dtype is torch.int64
+            and slots.shape == shape[:1] and slots.is_contiguous()
+            and dev == v.get_device() == slots.get_device()
+            and (error_flag is None
+                 or (error_flag.get_device() == dev and error_flag.dtype is torch.int32))):
+        rows = (None, pool[7], HEAD_DIM)
+        _explain(dev, ("k", k[:0], dtype, rows), ("v", v[:0], dtype, rows),
+                 ("slots", slots, torch.int64, shape[:1]),
+                 ("error_flag", error_flag, torch.int32, (1,)))
+    k_token, k_head = _rows_strides("k", k)
+    v_token, v_head = _rows_strides("v", v)
+    status = lib().tw_paged_write(
+        _PACK_POOL(*pool), k.data_ptr(), k_token, k_head, v.data_ptr(), v_token, v_head,
+        slots.data_ptr(), shape[0], None if error_flag is None else error_flag.data_ptr(),
+        _raw_stream(dev))
+    if status:
+        _lib.check(status, "paged_write")
 
 
+@functools.lru_cache(maxsize=1024)
 def paged_attention_workspace_bytes(requests: int, tokens: int, q_heads: int, kv_heads: int,
                                     max_q_len: int, max_kv_len: int, window: int = 0) -> int:
+    """Bytes of the workspace of a paged_attention call of these sizes (0: none needed)."""
     return int(lib().tw_paged_attention_workspace_size(requests, tokens, q_heads, kv_heads,
                                                        max_q_len, max_kv_len, window, HEAD_DIM))
 
@@ -457,46 +514,62 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     q [T, q_heads, 128] (token and head strides free), pool [pages, kv_heads,
     page_size, 128], block_table [B, W] int32, cu_q [B+1] and kv_lens [B] int32
     on the device; max_q_len bounds the requests' new tokens, max_kv_len is their
-    longest kv_lens (it sizes the launch).  window
-    > 0: each token sees the last `window` positions only.  Returns out
-    [T, q_heads, 128] (q's dtype or float32); lse [T, q_heads] fp32 receives the
-    log-sum-exp.  Without a workspace one is allocated for the call."""
-    pool = _paged_pool(k_pages, v_pages)
-    if q.dim() != 3 or q.shape[2] != HEAD_DIM or q.dtype != k_pages.dtype or \
-            q.shape[1] == 0 or q.shape[1] % pool.kv_heads:
+    longest kv_lens (it sizes the launch).  window > 0: each token sees the last
+    `window` positions only.  Returns out [T, q_heads, 128] (q's dtype or
+    float32); lse [T, q_heads] fp32 receives the log-sum-exp.  Without a
+    workspace one is allocated for the call."""
+    dev = _device_index(q)
+    pool = _paged_pool(dev, k_pages, v_pages)
+    shape, dtype, i32 = q.shape, q.dtype, torch.int32
+    if len(shape) != 3 or shape[2] != HEAD_DIM or dtype is not k_pages.dtype or \
+            shape[1] == 0 or shape[1] % pool[7]:
         raise ValueError("q must be [T, q_heads, 128] in the pool's dtype, q_heads a multiple of "
                          "kv_heads")
-    T, Hq, _ = q.shape
-    _i32("kv_lens", kv_lens, None)
+    T, Hq, _ = shape
+    if kv_lens.dim() != 1:
+        raise ValueError("kv_lens must be [requests]")
     B = kv_lens.shape[0]
-    _i32("cu_q", cu_q, B + 1)
-    _i32("block_table", block_table, B, None)
+    if not (kv_lens.dtype is cu_q.dtype is block_table.dtype is i32 and cu_q.shape == (B + 1,)
+            and block_table.dim() == 2 and block_table.shape[0] == B
+            and (block_table.stride(1) == 1 or block_table.shape[1] == 1)
+            and kv_lens.is_contiguous() and cu_q.is_contiguous()
+            and dev == kv_lens.get_device() == cu_q.get_device() == block_table.get_device()
+            and (lse is None or (lse.dtype is torch.float32 and lse.shape == (T, Hq)
+                                 and lse.is_contiguous() and lse.get_device() == dev))
+            and (error_flag is None
+                 or (error_flag.get_device() == dev and error_flag.dtype is i32))):
+        _explain(dev, ("kv_lens", kv_lens, i32, (None,)), ("cu_q", cu_q, i32, (B + 1,)),
+                 ("block_table", block_table, i32, (B, None)),
+                 ("lse", lse, torch.float32, (T, Hq)), ("error_flag", error_flag, i32, (1,)))
     if out is None:
-        out = torch.empty((T, Hq, HEAD_DIM), dtype=out_dtype or q.dtype, device=q.device)
-    elif out.shape != q.shape or (out_dtype is not None and out.dtype != out_dtype):
-        raise ValueError("out must have q's shape (and out_dtype)")
-    if out.dtype not in (q.dtype, torch.float32):
+        out = torch.empty(shape, dtype=out_dtype or dtype, device=q.device)
+        out_token, out_head = Hq * HEAD_DIM, HEAD_DIM
+    else:
+        if out.shape != shape or out.get_device() != dev or \
+                (out_dtype is not None and out.dtype is not out_dtype):
+            raise ValueError("out must have q's shape and device (and out_dtype)")
+        out_token, out_head = _rows_strides("out", out)
+    if out.dtype is not dtype and out.dtype is not torch.float32:
         raise ValueError("out must have q's dtype or float32")
-    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (T, Hq)
-                            or not lse.is_contiguous()):
-        raise ValueError("lse must be float32 [T, q_heads]")
     if workspace is None:
-        need = paged_attention_workspace_bytes(B, T, Hq, pool.kv_heads, max_q_len, max_kv_len,
-                                               window)
+        need = paged_attention_workspace_bytes(B, T, Hq, pool[7], max_q_len, max_kv_len, window)
         if need:
             workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-    elif not workspace.is_contiguous():
-        raise ValueError("workspace must be contiguous")
-    _same_device(q.device, k_pages, v_pages, block_table, cu_q, kv_lens, out, lse, workspace,
-                 error_flag)
+    else:
+        need = workspace.numel() * workspace.element_size()
+        if workspace.get_device() != dev or not workspace.is_contiguous():
+            raise ValueError("workspace must be contiguous, on q's device")
     W = block_table.shape[1]
-    args = _lib.PagedAttentionArgs(
-        pool, q.data_ptr(), *_rows_strides("q", q), block_table.data_ptr(),
+    q_token, q_head = _rows_strides("q", q)
+    args = _PACK_ATTENTION(
+        *pool, q.data_ptr(), q_token, q_head, block_table.data_ptr(),
         block_table.stride(0) if B > 1 else W, W, B, cu_q.data_ptr(), kv_lens.data_ptr(), T, Hq,
         max_q_len, max_kv_len, window,
-        softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(HEAD_DIM),
-        out.data_ptr(), *_rows_strides("out", out), DTYPE_CODES[out.dtype], 0, _ptr(lse),
-        _ptr(error_flag), _ptr(workspace),
-        0 if workspace is None else workspace.numel() * workspace.element_size())
-    _lib.check(lib().tw_paged_attention(ctypes.byref(args), _stream(q.device)), "paged_attention")
+        _SCALE if softmax_scale is None else softmax_scale, out.data_ptr(), out_token, out_head,
+        DTYPE_CODES[out.dtype], 0, 0 if lse is None else lse.data_ptr(),
+        0 if error_flag is None else error_flag.data_ptr(),
+        0 if workspace is None else workspace.data_ptr(), need)
+    status = lib().tw_paged_attention(args, _raw_stream(dev))
+    if status:
+        _lib.check(status, "paged_attention")
     return out
