@@ -12,6 +12,19 @@ __device__ __forceinline__ uint32_t smem_addr(const void* p) {
   return (uint32_t)__cvta_generic_to_shared(p);
 }
 
+// True in one thread of a converged warp.  Copies and products take their operands
+// from uniform registers: under this test the compiler knows that one thread issues
+// them, under `lane == 0` it would emit a loop over the warp's values for each.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(one));
+  return one != 0;
+}
+
 __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(bar)), "r"(count)
                : "memory");
@@ -48,28 +61,26 @@ __device__ __forceinline__ unsigned long long global_ns() {
 // A wait ends after two seconds whatever happens; the caller then gives up.
 constexpr unsigned long long kWaitLimitNs = 2000000000ull;
 
-static __device__ __noinline__ bool mbar_wait_slow(uint64_t* bar, uint32_t parity,
-                                            volatile int* abort_flag) {
-  const unsigned long long start = global_ns();
-  for (;;) {
-    for (int i = 0; i < 64; ++i)
-      if (mbar_try(bar, parity)) return true;
-    if (*abort_flag) return false;
-    if (global_ns() - start > kWaitLimitNs) {
-      *abort_flag = 1;
-      return false;
-    }
-  }
-}
-
 // Waits for the phase of this parity to complete.  False: the wait ran out, or
 // another thread's did (abort_flag, in shared memory, tells the others).
+// Inlined, like all of a kernel that splits its registers by setmaxnreg: a call
+// would hold the whole kernel to one register count.
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity,
                                           volatile int* abort_flag) {
+  unsigned long long start = 0;
 #pragma unroll 1
-  for (int i = 0; i < 16; ++i)
+  for (unsigned i = 1;; ++i) {
     if (mbar_try(bar, parity)) return true;
-  return mbar_wait_slow(bar, parity, abort_flag);
+    if ((i & 63) == 0) {
+      if (*abort_flag) return false;
+      const unsigned long long now = global_ns();
+      if (start == 0) start = now;
+      if (now - start > kWaitLimitNs) {
+        *abort_flag = 1;
+        return false;
+      }
+    }
+  }
 }
 
 // Orders this thread's shared-memory accesses before later ones of the copy

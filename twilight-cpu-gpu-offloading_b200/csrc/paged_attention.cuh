@@ -97,7 +97,7 @@ struct PagedRow {
   float m, l;
 };
 template <typename T>
-__device__ __noinline__ PagedRow paged_one_row(const PagedWork& w, int b, int t, int h, int low,
+__device__ __forceinline__ PagedRow paged_one_row(const PagedWork& w, int b, int t, int h, int low,
                                                int high) {
   const tw_paged_attention_args& a = w.a;
   const int lane = threadIdx.x & 31;

@@ -19,18 +19,24 @@
 #include "paged_attention.cuh"
 #include "tensor.cuh"
 
+#include <type_traits>
+
 namespace tw {
 
 constexpr int kChRows = 128;                      // rows of a half
 constexpr int kChSoftmax = 256;                   // threads 0..255: the halves' rows
-constexpr int kChMmaWarp = 8, kChLoadWarp = 9;
-constexpr int kChThreads = 320;
+constexpr int kChMmaWarp = 8, kChKeyWarp = 9, kChValueWarp = 10;
+constexpr int kChThreads = 384;                   // one warp of the third group is idle
+// Registers: the launch gives 168 to each of 384 threads; the warpgroups of the
+// rows take from the third: 216 + 216 + 72 = 3 * 168.
+constexpr int kChRowRegs = 216, kChIssueRegs = 72;
 constexpr int kChHalfTile = 128 * 128;            // bytes: 128 rows of 64 elements
 constexpr int kChTileBytes = 2 * kChHalfTile;
 constexpr int kChSlots = 5;
 constexpr int kChSmem = (2 + kChSlots) * kChTileBytes + 1024;
 constexpr int kChColumns = 512;                   // S0, S1, O0, O1: 128 columns each
 constexpr float kChMoveBy = 8.0f;                 // log2 units
+constexpr int kChFma = 4;                         // one pair in this many on the FMA pipe
 
 template <typename T> struct Pack16;
 template <> struct Pack16<__half> {
@@ -55,7 +61,8 @@ __device__ __forceinline__ void softmax_sync() {
 struct ChunkShared {
   uint64_t full[kChSlots], empty[kChSlots];
   uint64_t q_full, ragged;      // Q is there; a tile whose V rows get cleared is there
-  uint64_t s_full[2], p_full[2];  // scores / weights of a half
+  uint64_t s_full[2];           // scores of a half
+  uint64_t p_full[2][2];        // weights of a half: keys 0..63, 64..127 of the tile
   uint64_t o_full, drain;
   uint32_t tmem;
   volatile int abort;
@@ -129,7 +136,8 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
     mbar_init(&sh.ragged, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sh.s_full[i], 1);
-      mbar_init(&sh.p_full[i], kChRows);
+      mbar_init(&sh.p_full[i][0], 4);
+      mbar_init(&sh.p_full[i][1], 4);
     }
     mbar_init(&sh.o_full, 1);
     mbar_init(&sh.drain, 1);
@@ -142,81 +150,98 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
   tmem_fence_after();
   const uint32_t tmem = sh.tmem;
 
-  if (warp == kChLoadWarp) {
-    // ---- copies.  Slot n % kChSlots: n = 2j is K tile j, n = 2j + 1 is V tile j.
-    if (lane == 0) {
-      prefetch_map(&q_map);
-      prefetch_map(&maps.k);
-      prefetch_map(&maps.v);
-      mbar_arrive_expect(&sh.q_full, (uint32_t)(halves * R * half_tokens * kHeadDim * 2));
-      for (int i = 0; i < halves && tiles > 0; ++i)
-        for (int d = 0; d < 2; ++d)
-          tma_load_3d(&q_map, q_at + i * kChTileBytes + d * kChHalfTile, &sh.q_full, d * 64, g * R,
-                      rq.first + begin + i * half_tokens);
+  // (the register split inside the branches: past a join the smaller number holds)
+  if (warp >= kChMmaWarp) {
+  shrink_registers<kChIssueRegs>();
+  if (warp == kChKeyWarp || warp == kChValueWarp) {
+    // ---- copies: one warp those of Q and K, one those of V.  Ring slot n % kChSlots:
+    // n = 2j is K tile j, n = 2j + 1 is V tile j.
+    const bool values = warp == kChValueWarp;
+    const CUtensorMap* map = values ? &maps.v : &maps.k;
+    if (elect_one()) {
+      prefetch_map(map);
+      if (!values) {
+        mbar_arrive_expect(&sh.q_full, (uint32_t)(halves * R * half_tokens * kHeadDim * 2));
+        for (int i = 0; i < halves && tiles > 0; ++i)
+          for (int d = 0; d < 2; ++d)
+            tma_load_3d(&q_map, q_at + i * kChTileBytes + d * kChHalfTile, &sh.q_full, d * 64,
+                        g * R, rq.first + begin + i * half_tokens);
+      }
     }
-    const int boxes = kTileKeys / w.box;  // per tile and 64 dimensions; 2 * boxes <= 32
-    const int dim_half = lane / boxes;    // 0, 1; more: idle
-    const int box = lane % boxes;
+    __syncwarp();
+    // lane l < boxes knows the page of box l of the next tile
+    const int boxes = kTileKeys / w.box;
     const int32_t* table = a.block_table + (int64_t)b * a.table_stride;
-    const uint32_t dst = ring + dim_half * kChHalfTile + box * w.box * 128;
+    const uint32_t box_bytes = (uint32_t)w.box * 128;  // of 64 dimensions
     // boxes wholly before the first visible key are not read: a page that slid out
     // of the window may be gone
     const int skipped = (low - key0) / w.box;
-    int key = key0 + box * w.box;
+    int key = key0 + lane * w.box;
     int page = 0;
-    if (dim_half < 2 && key < high && box >= skipped) page = table[key / a.pool.page_size];
-    int n = 0, done_ragged = 0;
+    if (lane < boxes && key < high && lane >= skipped) page = table[key / a.pool.page_size];
+    int n = values ? 1 : 0;
+    uint32_t done_ragged = 0;
     bool ok = true;
-    for (int j = 0; j < tiles && ok; ++j) {
-      const int at = key, from = page;
-      const bool mine = dim_half < 2 && at < high && (j > 0 || box >= skipped);
-      key += kTileKeys;
-      if (dim_half < 2 && j + 1 < tiles && key < high) page = table[key / a.pool.page_size];
-      int p = from;
-      if (mine && (p < 0 || p >= a.pool.num_pages)) {
+    for (int j = 0; j < tiles; ++j, n += 2) {
+      int p = page;
+      if (lane < boxes && key < high && (j > 0 || lane >= skipped) &&
+          (p < 0 || p >= a.pool.num_pages)) {
         raise_error(a.error_flag, TW_ERR_INVALID_INDEX);
         p = (int)a.pool.num_pages;  // out of the map's range: zeros
       }
+      key += kTileKeys;
+      if (lane < boxes && j + 1 < tiles && key < high) page = table[key / a.pool.page_size];
       const int first = key0 + j * kTileKeys;
       const int valid = min(high - first, kTileKeys);
-      const int count = (valid + w.box - 1) / w.box - (j == 0 ? skipped : 0);
-      const uint32_t bytes = (uint32_t)(count * w.box * kHeadDim * 2);
-      const bool ragged = first < low || valid < kTileKeys;
-#pragma unroll 1
-      for (int m = 0; m < 2; ++m, ++n) {
-        const int s = n % kChSlots;
-        if (n >= kChSlots &&
-            !__all_sync(0xffffffffu, mbar_wait(&sh.empty[s],
-                                               (uint32_t)((n / kChSlots - 1) & 1), &sh.abort))) {
-          ok = false;
-          break;
+      const int from = j == 0 ? skipped : 0, to = (valid + w.box - 1) / w.box;
+      const bool ragged = values && (first < low || valid < kTileKeys);
+      const int s = n % kChSlots;
+      if (n >= kChSlots) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&sh.empty[s], (uint32_t)((n / kChSlots - 1) & 1),
+                                               &sh.abort));
+        if (!ok) break;
+      }
+      uint64_t* bar = ragged ? &sh.ragged : &sh.full[s];
+      if (elect_one()) mbar_arrive_expect(bar, (uint32_t)(to - from) * box_bytes * 2);
+      uint32_t dst = ring + s * kChTileBytes + from * box_bytes;
+      int row = (first + from * w.box) % a.pool.page_size;  // of the next box in its page
+      for (int x = from; x < to; x += 4) {  // four boxes a turn: their pages at once
+        int px[4];
+#pragma unroll
+        for (int y = 0; y < 4; ++y) px[y] = __shfl_sync(0xffffffffu, p, x + y);
+        int rx[4];
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          rx[y] = row;
+          row += w.box;
+          if (row == a.pool.page_size) row = 0;
         }
-        uint64_t* bar = m == 1 && ragged ? &sh.ragged : &sh.full[s];
-        if (lane == 0) mbar_arrive_expect(bar, bytes);
+        if (elect_one()) {
+#pragma unroll
+          for (int y = 0; y < 4; ++y)
+            if (x + y < to) {
+              tma_load_4d(map, dst + y * box_bytes, bar, 0, rx[y], g, px[y]);
+              tma_load_4d(map, dst + kChHalfTile + y * box_bytes, bar, 64, rx[y], g, px[y]);
+            }
+        }
+        dst += 4 * box_bytes;
+      }
+      if (ragged) {
+        // V rows that no row sees: what they hold (NaN included) must not meet a
+        // weight of zero
+        ok = __all_sync(0xffffffffu, mbar_wait(bar, done_ragged & 1, &sh.abort));
+        if (!ok) break;
+        ++done_ragged;
+        char* tile = smem + (2 + s) * kChTileBytes;
+        for (int i = lane; i < kTileKeys * 16; i += 32) {
+          const int r = i >> 4;
+          if (first + r < low || r >= valid)
+            reinterpret_cast<uint4*>(tile + ((i >> 3) & 1) * kChHalfTile + r * 128)[i & 7] =
+                make_uint4(0u, 0u, 0u, 0u);
+        }
+        fence_async_smem();
         __syncwarp();
-        if (mine)
-          tma_load_4d(m == 0 ? &maps.k : &maps.v, dst + s * kChTileBytes, bar, dim_half * 64,
-                      at % a.pool.page_size, g, p);
-        if (m == 1 && ragged) {
-          // V rows that no row sees: what they hold (NaN included) must not meet a
-          // weight of zero
-          if (!__all_sync(0xffffffffu,
-                          mbar_wait(bar, (uint32_t)(done_ragged & 1), &sh.abort))) {
-            ok = false;
-            break;
-          }
-          ++done_ragged;
-          char* tile = smem + (2 + s) * kChTileBytes;
-          for (int i = lane; i < kTileKeys * 16; i += 32) {
-            const int row = i >> 4;
-            if (first + row < low || row >= valid)
-              reinterpret_cast<uint4*>(tile + ((i >> 3) & 1) * kChHalfTile + row * 128)[i & 7] =
-                  make_uint4(0u, 0u, 0u, 0u);
-          }
-          fence_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sh.full[s]);
-        }
+        if (lane == 0) mbar_arrive(&sh.full[s]);
       }
     }
     if (!ok || sh.abort) {
@@ -228,7 +253,7 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
     }
   } else if (warp == kChMmaWarp) {
     // ---- products, all issued by one thread
-    if (lane == 0 && tiles > 0) {
+    if (tiles > 0 && elect_one()) {
       constexpr uint32_t desc_s = product_desc(Pack16<T>::kBf16, kTileKeys, false);
       constexpr uint32_t desc_o = product_desc(Pack16<T>::kBf16, kHeadDim, true);
       // S of half i from Q_i and the K tile in ring slot s
@@ -242,10 +267,10 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
         }
         mma_commit(&sh.s_full[i]);
       };
-      auto values = [&](int i, int s, bool add) {
+      auto values = [&](int i, int s, int part, bool add) {
         const uint32_t va = ring + s * kChTileBytes;
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
+        for (int k = part * 4; k < part * 4 + 4; ++k)
           mma_tmem(tmem + 256 + i * 128, tmem + i * 128 + k * 8,
                    operand_desc(va + k * 2048, kChHalfTile, 1024), desc_o, add || k > 0);
       };
@@ -263,10 +288,14 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
         if (!wait_slot(nv)) break;
         if (j + 1 < tiles && !wait_slot(nk)) break;
         for (int i = 0; i < halves; ++i) {
-          ok = mbar_wait(&sh.p_full[i], (uint32_t)(j & 1), &sh.abort);
+          ok = mbar_wait(&sh.p_full[i][0], (uint32_t)(j & 1), &sh.abort);
           if (!ok) break;
           tmem_fence_after();
-          values(i, nv % kChSlots, j > 0);
+          values(i, nv % kChSlots, 0, j > 0);
+          ok = mbar_wait(&sh.p_full[i][1], (uint32_t)(j & 1), &sh.abort);
+          if (!ok) break;
+          tmem_fence_after();
+          values(i, nv % kChSlots, 1, true);
           if (i == halves - 1) mma_commit(&sh.empty[nv % kChSlots]);
           if (j + 1 < tiles) scores(i, nk % kChSlots);
         }
@@ -280,7 +309,9 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
         mbar_wait(&sh.drain, 0, &never);
       }
     }
+  }
   } else {
+    grow_registers<kChRowRegs>();
     // ---- weights: a thread per row
     const int i = warp >> 2;              // half
     const int r = tid & (kChRows - 1);    // row of the half
@@ -308,7 +339,8 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
         for (int c = 0; c < 4; ++c) tmem_ld32(s[c], s_col + c * 32);
         tmem_wait_ld();
         const int first = key0 + j * kTileKeys;
-        if (first < all_low || first < low || first + kTileKeys > min(all_high, high)) {
+        const bool edge = first < all_low || first < low || first + kTileKeys > min(all_high, high);
+        if (edge) {
           const int from = max(see, low) - first, to = min(p + 1, high) - first;
 #pragma unroll
           for (int c = 0; c < 4; ++c)
@@ -319,11 +351,12 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
         float top[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          top[c] = fmaxf(s[c][0], s[c][1]);
+          top[c] = max3_nan(s[c][0], s[c][1], s[c][2]);
 #pragma unroll
-          for (int x = 2; x < 32; x += 2) top[c] = fmaxf(top[c], fmaxf(s[c][x], s[c][x + 1]));
+          for (int x = 3; x < 31; x += 2) top[c] = max3_nan(top[c], s[c][x], s[c][x + 1]);
+          top[c] = max3_nan(top[c], s[c][31], s[c][31]);
         }
-        const float t = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * w.scale_log2;
+        const float t = max3_nan(max3_nan(top[0], top[1], top[2]), top[3], top[3]) * w.scale_log2;
         const bool move = t > m + kChMoveBy;
         if (__any_sync(0xffffffffu, move)) {
           const float f = move ? ex2(m - t) : 1.f;
@@ -346,25 +379,45 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
         }
         const float u = m == -CUDART_INF_F ? 0.f : -m;
         const uint64_t u2 = pair(u, u);
+        // Weights, rounded to the 16-bit type for the product (the sum l keeps them
+        // in 32 bits): half a unit each, of either sign.  Where all is finite, one
+        // pair in kChFma goes through the FMA pipe instead of the special-function
+        // unit, which alone would take as long as the products.
+        auto weights = [&](auto plain) {
+          // an operand of its own for each form, or the compiler computes all 64
+          // products before it branches and spills them
+          uint64_t by = scale2;
+          asm volatile("// form %1" : "+l"(by) : "n"((int)decltype(plain)::value));
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          // weights rounded to the 16-bit type for the product (the sum l keeps
-          // them in 32 bits): half a unit each, of either sign
-          uint32_t packed[16];
+          for (int c = 0; c < 4; ++c) {
+            uint32_t packed[16];
 #pragma unroll
-          for (int x = 0; x < 32; x += 2) {
-            float e0, e1;
-            unpair(fma2(pair(s[c][x], s[c][x + 1]), scale2, u2), e0, e1);
-            e0 = ex2(e0);
-            e1 = ex2(e1);
-            l2[(x >> 1) & 1] = add2(l2[(x >> 1) & 1], pair(e0, e1));
-            packed[x >> 1] = Pack16<T>::pack(e0, e1);
+            for (int x = 0; x < 32; x += 2) {
+              const uint64_t y = fma2(pair(s[c][x], s[c][x + 1]), by, u2);
+              float e0, e1;
+              if (decltype(plain)::value && (x >> 1) % kChFma == kChFma - 1) {
+                ex2_fma(y, e0, e1);
+              } else {
+                unpair(y, e0, e1);
+                e0 = ex2(e0);
+                e1 = ex2(e1);
+              }
+              l2[(x >> 1) & 1] = add2(l2[(x >> 1) & 1], pair(e0, e1));
+              packed[x >> 1] = Pack16<T>::pack(e0, e1);
+            }
+            tmem_st16(s_col + c * 16, packed);
+            if (c & 1) {  // the product with V takes 64 keys at a time
+              tmem_wait_st();
+              tmem_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&sh.p_full[i][c >> 1]);
+            }
           }
-          tmem_st16(s_col + c * 16, packed);
-        }
-        tmem_wait_st();
-        tmem_fence_before();
-        mbar_arrive(&sh.p_full[i]);
+        };
+        if (__all_sync(0xffffffffu, !edge && t == t && fabsf(m) < CUDART_INF_F))
+          weights(std::true_type{});
+        else
+          weights(std::false_type{});
       }
     }
     float l = 0.f;
