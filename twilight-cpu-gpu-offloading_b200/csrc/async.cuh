@@ -41,15 +41,27 @@ __device__ __forceinline__ void mbar_arrive_expect(uint64_t* bar, uint32_t bytes
                "r"(bytes)
                : "memory");
 }
+// One look at a barrier's phase.  kSuspend: the thread may sleep for a while first,
+// which spares power (what bounds a kernel of products) but wakes later.
+template <bool kSuspend>
 __device__ __forceinline__ bool mbar_try(uint64_t* bar, uint32_t parity) {
   uint32_t done;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(done)
-      : "r"(smem_addr(bar)), "r"(parity)
-      : "memory");
+  if constexpr (kSuspend)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(smem_addr(bar)), "r"(parity)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(smem_addr(bar)), "r"(parity)
+        : "memory");
   return done != 0;
 }
 __device__ __forceinline__ unsigned long long global_ns() {
@@ -65,12 +77,13 @@ constexpr unsigned long long kWaitLimitNs = 2000000000ull;
 // another thread's did (abort_flag, in shared memory, tells the others).
 // Inlined, like all of a kernel that splits its registers by setmaxnreg: a call
 // would hold the whole kernel to one register count.
+template <bool kSuspend = true>
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity,
                                           volatile int* abort_flag) {
   unsigned long long start = 0;
 #pragma unroll 1
   for (unsigned i = 1;; ++i) {
-    if (mbar_try(bar, parity)) return true;
+    if (mbar_try<kSuspend>(bar, parity)) return true;
     if ((i & 63) == 0) {
       if (*abort_flag) return false;
       const unsigned long long now = global_ns();

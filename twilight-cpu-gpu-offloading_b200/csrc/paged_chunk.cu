@@ -36,7 +36,7 @@ constexpr int kChSlots = 5;
 constexpr int kChSmem = (2 + kChSlots) * kChTileBytes + 1024;
 constexpr int kChColumns = 512;                   // S0, S1, O0, O1: 128 columns each
 constexpr float kChMoveBy = 8.0f;                 // log2 units
-constexpr int kChFma = 4;                         // one pair in this many on the FMA pipe
+constexpr int kChFma = 8;                         // one pair in this many on the FMA pipe
 
 template <typename T> struct Pack16;
 template <> struct Pack16<__half> {

@@ -164,7 +164,7 @@ paged_token_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
       key += kTokTile;
       if (matrix < 2 && i + 1 < tiles && key < range.end) page = table[key / a.pool.page_size];
       if (i >= kTokStages &&
-          !__all_sync(0xffffffffu, mbar_wait(&s_empty[stage],
+          !__all_sync(0xffffffffu, mbar_wait<false>(&s_empty[stage],
                                              (uint32_t)((i / kTokStages - 1) & 1), &s_abort)))
         break;
       if (lane == 0) {
@@ -187,7 +187,7 @@ paged_token_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
       // give up: wait (with the same limit) for the copies in flight
       volatile int never = 0;
       for (int j = max(0, i - kTokStages); j < i; ++j)
-        mbar_wait(&s_full[j % kTokStages], (uint32_t)((j / kTokStages) & 1), &never);
+        mbar_wait<false>(&s_full[j % kTokStages], (uint32_t)((j / kTokStages) & 1), &never);
     }
     return;
   }
@@ -234,7 +234,7 @@ paged_token_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
     const uint32_t base = stage * kTokStageBytes;
     const int key0 = tile0 + i * kTokTile + wrow;  // the warp's first key
     if (!__all_sync(0xffffffffu,
-                    mbar_wait(&s_full[stage], (uint32_t)((i / kTokStages) & 1), &s_abort)))
+                    mbar_wait<false>(&s_full[stage], (uint32_t)((i / kTokStages) & 1), &s_abort)))
       break;
     if (key0 < range.end && key0 + 16 > low) {
       const bool edge = key0 < all_low || key0 + 16 > all_high || key0 < low ||
