@@ -9,6 +9,7 @@
 
 namespace tw {
 
+constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kTileKeys = 128;  // splits begin at multiples of this
 
 // How one kernel of the call divides a request's keys: ranges of `chunk` keys
@@ -155,7 +156,7 @@ __device__ __forceinline__ void paged_store_row(const tw_paged_attention_args& a
     for (int c = 0; c < N; ++c) out[c] = from_f32<Out>(o[c]);
   }
   if (a.lse && d0 == 0)
-    a.lse[(int64_t)t * a.q_heads + h] = lse2 * 0.6931471805599453f;  // log2 -> ln
+    a.lse[(int64_t)t * a.q_heads + h] = lse2 * kLn2;
 }
 
 // A range's result of a row, for the merge.

@@ -58,6 +58,36 @@ __device__ __forceinline__ void softmax_sync() {
   asm volatile("bar.sync 1, %0;" ::"n"(kChSoftmax) : "memory");
 }
 
+// The warp's 32 rows on their way out: 16-byte columns XORed by row % 8.
+template <typename Out>
+__device__ __forceinline__ void stage_row(char* smem, int warp, int row, int quarter,
+                                          const float (&o)[32]) {
+  constexpr int kVec = 16 / sizeof(Out);  // elements of a column
+  char* base = smem + (warp * 32 + row) * (kHeadDim * (int)sizeof(Out));
+#pragma unroll
+  for (int c = 0; c < 32 / kVec; ++c) {
+    __align__(16) Out x[kVec];
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) x[e] = from_f32<Out>(o[c * kVec + e]);
+    const int column = (quarter * (32 / kVec) + c) ^ (row & 7);
+    *reinterpret_cast<uint4*>(base + column * 16) = *reinterpret_cast<uint4*>(x);
+  }
+}
+template <typename Out, typename Place>
+__device__ __forceinline__ void write_rows(const char* smem, int warp, int lane, Place place) {
+  constexpr int kColumns = kHeadDim * (int)sizeof(Out) / 16;  // 16 or 32
+  constexpr int kRows = 32 / kColumns;                        // rows a turn
+  const int column = lane % kColumns;
+#pragma unroll 4
+  for (int x = 0; x < 32; x += kRows) {
+    const int row = x + lane / kColumns;
+    Out* to = place(row);
+    if (to)
+      reinterpret_cast<uint4*>(to)[column] = *reinterpret_cast<const uint4*>(
+          smem + (warp * 32 + row) * (kHeadDim * (int)sizeof(Out)) + ((column ^ (row & 7)) * 16));
+  }
+}
+
 struct ChunkShared {
   uint64_t full[kChSlots], empty[kChSlots];
   uint64_t q_full, ragged;      // Q is there; a tile whose V rows get cleared is there
@@ -80,53 +110,9 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
   const int kv_heads = a.pool.kv_heads;
   const int R = w.group;
   const int tokens = paged_chunk_tokens(R), half_tokens = tokens / 2;
-  pdl_wait();
-  pdl_launch_dependents();
-
-  // The CTA's request: a request with rows [c, d) owns the slots from
-  // c / tokens + b on, one per `tokens` rows, and no two requests share one.
-  // The last slots come first: within a request they see the most keys.
-  const int64_t cta = blockIdx.x;
-  const int split = (int)(cta % w.many.splits);
-  const int g = (int)(cta / w.many.splits % kv_heads);
-  const int slots = a.tokens / tokens + a.requests;
-  const int64_t ctas = (int64_t)slots * kv_heads * w.many.splits;
-  if (cta >= ctas) {
-    paged_clear_padding<Out>(a, (int)(cta - ctas));
-    return;
-  }
-  const int slot = slots - 1 - (int)(cta / w.many.splits / kv_heads);
-  int b = 0;
-  for (int lo = 0, hi = a.requests; lo < hi;) {  // last b whose first slot is <= slot
-    const int mid = (lo + hi) >> 1;
-    if (a.cu_q[mid] / tokens + mid <= slot) {
-      b = mid;
-      lo = mid + 1;
-    } else {
-      hi = mid;
-    }
-  }
-  const PagedRequest rq = paged_request(a, b);
-  const int begin = (slot - (rq.first / tokens + b)) * tokens;  // first token of the CTA
-  if (rq.n <= w.few_tokens || begin >= rq.n || begin < 0) return;
-  if (rq.n > a.max_q_len) {
-    if (tid == 0) raise_error(a.error_flag, TW_ERR_BAD_ARG);
-    return;
-  }
-  const int here = min(rq.n - begin, tokens);    // tokens of the CTA
-  const PagedKeys keys = paged_keys(a, rq, begin, here);
-  const PagedRange range = paged_range(w.many, keys.low, keys.high, split);
-  if (split >= range.parts) return;
-  const int halves = here > half_tokens ? 2 : 1;
-  const int p_first = rq.kv - rq.n + begin;      // position of the first token
-  const int low = max(range.begin, keys.low), high = range.end;
-  const int key0 = low / kTileKeys * kTileKeys;
-  const int tiles = high > low ? (high - key0 + kTileKeys - 1) / kTileKeys : 0;
-
   char* smem = (char*)(((uintptr_t)s_raw + 1023) & ~(uintptr_t)1023);
   const uint32_t q_at = smem_addr(smem);
   const uint32_t ring = q_at + 2 * kChTileBytes;
-  if (warp == kChMmaWarp) tmem_alloc(&sh.tmem, kChColumns);
   if (tid == 0) {
     for (int i = 0; i < kChSlots; ++i) {
       mbar_init(&sh.full[i], 1);
@@ -145,6 +131,61 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
     mbar_init_fence();
   }
   if (tid < 8) sh.bad[tid] = 0;
+  pdl_wait();
+  pdl_launch_dependents();
+
+  // The CTA's request: a request with rows [c, d) owns the slots from
+  // c / tokens + b on, one per `tokens` rows, and no two requests share one.
+  // The last slots come first: within a request they see the most keys.
+  const int64_t cta = blockIdx.x;
+  const int split = (int)(cta % w.many.splits);
+  const int g = (int)(cta / w.many.splits % kv_heads);
+  const int slots = a.tokens / tokens + a.requests;
+  const int64_t ctas = (int64_t)slots * kv_heads * w.many.splits;
+  if (cta >= ctas) {
+    paged_clear_padding<Out>(a, (int)(cta - ctas));
+    return;
+  }
+  const int slot = slots - 1 - (int)(cta / w.many.splits / kv_heads);
+  // last b whose first slot is <= slot: 32 candidates a round
+  int b = 0;
+  for (int n = a.requests; n > 1;) {
+    const int stride = (n + 31) / 32;
+    const int i = lane * stride;
+    const bool at_most = i < n && a.cu_q[b + i] / tokens + b + i <= slot;
+    const int k = max(__popc(__ballot_sync(0xffffffffu, at_most)) - 1, 0);
+    b += k * stride;
+    n = min(stride, n - k * stride);
+  }
+  const PagedRequest rq = paged_request(a, b);
+  const int begin = (slot - (rq.first / tokens + b)) * tokens;  // first token of the CTA
+  if (rq.n <= w.few_tokens || begin >= rq.n || begin < 0) return;
+  if (rq.n > a.max_q_len) {
+    if (tid == 0) raise_error(a.error_flag, TW_ERR_BAD_ARG);
+    return;
+  }
+  const int here = min(rq.n - begin, tokens);    // tokens of the CTA
+  const PagedKeys keys = paged_keys(a, rq, begin, here);
+  const PagedRange range = paged_range(w.many, keys.low, keys.high, split);
+  if (split >= range.parts) return;
+  const int halves = here > half_tokens ? 2 : 1;
+  const int p_first = rq.kv - rq.n + begin;      // position of the first token
+  const int low = max(range.begin, keys.low), high = range.end;
+  const int key0 = low / kTileKeys * kTileKeys;
+  const int tiles = high > low ? (high - key0 + kTileKeys - 1) / kTileKeys : 0;
+
+  // Lane l < boxes of a copying warp knows the page of box l of the next tile.
+  // Boxes wholly before the first visible key are not read: a page that slid out
+  // of the window may be gone.
+  const int boxes = kTileKeys / w.box;
+  const int skipped = (low - key0) / w.box;
+  const int32_t* table = a.block_table + (int64_t)b * a.table_stride;
+  int key = key0 + lane * w.box;
+  int page = 0;
+  if ((warp == kChKeyWarp || warp == kChValueWarp) && lane < boxes && key < high &&
+      lane >= skipped)
+    page = table[key / a.pool.page_size];
+  if (warp == kChMmaWarp) tmem_alloc(&sh.tmem, kChColumns);
   tmem_fence_before();
   __syncthreads();
   tmem_fence_after();
@@ -169,16 +210,7 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
       }
     }
     __syncwarp();
-    // lane l < boxes knows the page of box l of the next tile
-    const int boxes = kTileKeys / w.box;
-    const int32_t* table = a.block_table + (int64_t)b * a.table_stride;
     const uint32_t box_bytes = (uint32_t)w.box * 128;  // of 64 dimensions
-    // boxes wholly before the first visible key are not read: a page that slid out
-    // of the window may be gone
-    const int skipped = (low - key0) / w.box;
-    int key = key0 + lane * w.box;
-    int page = 0;
-    if (lane < boxes && key < high && lane >= skipped) page = table[key / a.pool.page_size];
     int n = values ? 1 : 0;
     uint32_t done_ragged = 0;
     bool ok = true;
@@ -342,11 +374,20 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
         const bool edge = first < all_low || first < low || first + kTileKeys > min(all_high, high);
         if (edge) {
           const int from = max(see, low) - first, to = min(p + 1, high) - first;
+          if (__any_sync(0xffffffffu, to < kTileKeys)) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
+            for (int c = 0; c < 4; ++c)
 #pragma unroll
-            for (int x = 0; x < 32; ++x)
-              if (c * 32 + x < from || c * 32 + x >= to) s[c][x] = -CUDART_INF_F;
+              for (int x = 0; x < 32; ++x)
+                if (c * 32 + x >= to) s[c][x] = -CUDART_INF_F;
+          }
+          if (__any_sync(0xffffffffu, from > 0)) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int x = 0; x < 32; ++x)
+                if (c * 32 + x < from) s[c][x] = -CUDART_INF_F;
+          }
         }
         float top[4];
 #pragma unroll
@@ -434,27 +475,59 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const float lse2 = l == 0.f ? -CUDART_INF_F : m + log2f(l);
     const bool joined = range.parts == 1;
-    const int64_t row = (int64_t)t * a.q_heads + h;
     if (i < halves) {
+      // Rows go through shared memory (Q and the ring are free: all products are
+      // done), so that a warp writes whole rows to memory: a thread writing its own
+      // row 16 bytes at a time took 3.5 us for the 256 rows.
       float odd = 0.f;
-#pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
-        float o[32];
+      {
+        float o[4][32];
         if (tiles > 0) {
-          tmem_ld32(o, o_col + c * 32);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_ld32(o[c], o_col + c * 32);
           tmem_wait_ld();
         }
 #pragma unroll
-        for (int x = 0; x < 32; ++x) {
-          o[x] = l == 0.f ? 0.f : o[x] * inv;
-          odd = fmaf(o[x], 0.f, odd);  // NaN when one is not finite
-        }
-        if (live) {
+        for (int c = 0; c < 4; ++c) {
+#pragma unroll
+          for (int x = 0; x < 32; ++x) {
+            o[c][x] = l == 0.f ? 0.f : o[c][x] * inv;
+            odd = fmaf(o[c][x], 0.f, odd);  // NaN when one is not finite
+          }
           if (joined)
-            paged_store_row<Out, 32>(a, t, h, c * 32, o, lse2);
+            stage_row<Out>(smem, warp, lane, c, o[c]);
           else
-            paged_store_part<32>(w.many, row, split, c * 32, o, lse2);
+            stage_row<float>(smem, warp, lane, c, o[c]);
         }
+      }
+      if (live) {
+        const int64_t row = (int64_t)t * a.q_heads + h;
+        if (!joined)
+          w.many.part_lse[row * w.many.splits + split] = lse2;
+        else if (a.lse)
+          a.lse[row] = lse2 * kLn2;
+      }
+      __syncwarp();
+      // row x of the warp: token y / R by multiplication (exact for y < 128, R <= 64)
+      const unsigned by_r = (65536u + R - 1) / R;
+      const int y0 = (warp & 3) * 32, t0 = rq.first + begin + i * half_tokens;
+      const int rows = min(half_tokens, here - i * half_tokens) * R;
+      if (joined) {
+        Out* to = (Out*)a.out + (int64_t)t0 * a.out_token_stride +
+                  (int64_t)(g * R) * a.out_head_stride;
+        write_rows<Out>(smem, warp, lane, [&](int x) -> Out* {
+          const int y = y0 + x, k = (int)(y * by_r >> 16);
+          return y < rows ? to + (int64_t)k * a.out_token_stride + (y - k * R) * a.out_head_stride
+                          : nullptr;
+        });
+      } else {
+        float* to = w.many.part_o +
+                    (((int64_t)t0 * a.q_heads + g * R) * w.many.splits + split) * kHeadDim;
+        write_rows<float>(smem, warp, lane, [&](int x) -> float* {
+          const int y = y0 + x, k = (int)(y * by_r >> 16);
+          return y < rows ? to + ((int64_t)k * a.q_heads + (y - k * R)) * w.many.splits * kHeadDim
+                          : nullptr;
+        });
       }
       // A row that is not finite may owe it to a V row that another token sees
       // and this one does not (weight 0 times infinity or NaN).
@@ -462,7 +535,9 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
       if (lane == 0) sh.bad[warp] = again;
     }
     softmax_sync();
-    for (int x = 0; x < 8; ++x) {
+    const bool redo = __any_sync(0xffffffffu, sh.bad[lane & 7] != 0);
+#pragma unroll 1
+    for (int x = 0; redo && x < 8; ++x) {
       for (unsigned bad = sh.bad[x]; bad; bad &= bad - 1) {
         const int rr = (x & 3) * 32 + __ffs(bad) - 1;
         if (rr % 8 != warp) continue;
