@@ -77,13 +77,12 @@ constexpr unsigned long long kWaitLimitNs = 2000000000ull;
 // another thread's did (abort_flag, in shared memory, tells the others).
 // Inlined, like all of a kernel that splits its registers by setmaxnreg: a call
 // would hold the whole kernel to one register count.
-template <bool kSuspend = true>
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity,
-                                          volatile int* abort_flag) {
+template <typename Look>
+__device__ __forceinline__ bool wait_until(Look look, volatile int* abort_flag) {
   unsigned long long start = 0;
 #pragma unroll 1
   for (unsigned i = 1;; ++i) {
-    if (mbar_try<kSuspend>(bar, parity)) return true;
+    if (look()) return true;
     if ((i & 63) == 0) {
       if (*abort_flag) return false;
       const unsigned long long now = global_ns();
@@ -94,6 +93,11 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity,
       }
     }
   }
+}
+template <bool kSuspend = true>
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity,
+                                          volatile int* abort_flag) {
+  return wait_until([&] { return mbar_try<kSuspend>(bar, parity); }, abort_flag);
 }
 
 // Orders this thread's shared-memory accesses before later ones of the copy

@@ -7,46 +7,54 @@
 
 namespace tw {
 
-constexpr int kRowWarps = 8;  // rows per CTA of the merge
+constexpr int kMergeWarps = 4;  // of a row
 
 // Joins the ranges of split rows: out = sum_s 2^(lse_s - M) o_s / sum_s 2^(lse_s - M).
-// A warp per row; the ranges are added in order, so the bits do not depend on
-// which was ready first.
+// A CTA per row, its warps taking every fourth range, so that a row's loads are in
+// flight together (one warp alone: 3 us for 37 ranges).  The ranges are added in
+// an order that does not depend on which was ready first.
+// Every CTA waits for the kernel before it, also one without work: what follows in
+// the stream takes the end of this kernel for the end of that one.
+__device__ __forceinline__ void merge_nothing() {
+  pdl_wait();
+  pdl_launch_dependents();
+}
+
 template <typename Out, bool kFew>
-__global__ void __launch_bounds__(kRowWarps * 32)
+__global__ void __launch_bounds__(kMergeWarps * 32)
 paged_merge_kernel(const __grid_constant__ PagedWork w) {
   const tw_paged_attention_args& a = w.a;
   const PagedSplit& sp = kFew ? w.few : w.many;
-  pdl_wait();
-  pdl_launch_dependents();
-  const int lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * kRowWarps + (threadIdx.x >> 5);
+  // The lengths are older than the kernel before this one, which waited for what
+  // wrote them; the partial results are not.
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row = blockIdx.x;
   int t, h;
   PagedRequest rq;
   PagedKeys keys;
   if (kFew) {
-    if (row >= (int64_t)a.requests * a.pool.kv_heads * w.few_rows) return;
     const int r = (int)(row % w.few_rows);
     const int unit = (int)(row / w.few_rows);
     const int b = unit / a.pool.kv_heads;
     rq = paged_request(a, b);
-    if (rq.n > w.few_tokens || r >= rq.n * w.group) return;
+    if (rq.n > w.few_tokens || r >= rq.n * w.group) return merge_nothing();
     t = rq.first + r / w.group;
     h = (unit - b * a.pool.kv_heads) * w.group + r % w.group;
     keys = paged_keys(a, rq, 0, rq.n);
   } else {
-    if (row >= (int64_t)a.tokens * a.q_heads) return;
     t = (int)(row / a.q_heads);
     h = (int)(row - (int64_t)t * a.q_heads);
     const int b = first_above(a.cu_q + 1, a.requests, t);
-    if (b >= a.requests) return;
+    if (b >= a.requests) return merge_nothing();
     rq = paged_request(a, b);
-    if (rq.n <= w.few_tokens || rq.n > a.max_q_len) return;
+    if (rq.n <= w.few_tokens || rq.n > a.max_q_len) return merge_nothing();
     const int tokens = paged_chunk_tokens(w.group);
     const int begin = (t - rq.first) / tokens * tokens;
     keys = paged_keys(a, rq, begin, min(rq.n - begin, tokens));
   }
   const int parts = paged_range(sp, keys.low, keys.high, 0).parts;
+  pdl_wait();
+  pdl_launch_dependents();
   if (parts == 1) return;  // the range wrote the result itself
   const float* lse = sp.part_lse + row * sp.splits;
   const float* po = sp.part_o + row * sp.splits * kHeadDim + lane * 4;
@@ -57,7 +65,7 @@ paged_merge_kernel(const __grid_constant__ PagedWork w) {
   const float u = m == -CUDART_INF_F ? 0.f : m;
   float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
-  for (int s = 0; s < parts; ++s) {
+  for (int s = warp; s < parts; s += kMergeWarps) {
     const float f = ex2(lse[s] - u);
     const float4 x = *reinterpret_cast<const float4*>(po + (int64_t)s * kHeadDim);
     l += f;
@@ -65,6 +73,21 @@ paged_merge_kernel(const __grid_constant__ PagedWork w) {
     o[1] = fmaf(x.y, f, o[1]);
     o[2] = fmaf(x.z, f, o[2]);
     o[3] = fmaf(x.w, f, o[3]);
+  }
+  __shared__ float s_l[kMergeWarps];
+  __shared__ float4 s_o[kMergeWarps][32];
+  if (lane == 0) s_l[warp] = l;
+  s_o[warp][lane] = make_float4(o[0], o[1], o[2], o[3]);
+  __syncthreads();
+  if (warp != 0) return;
+#pragma unroll
+  for (int k = 1; k < kMergeWarps; ++k) {
+    const float4 x = s_o[k][lane];
+    l += s_l[k];
+    o[0] += x.x;
+    o[1] += x.y;
+    o[2] += x.z;
+    o[3] += x.w;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
@@ -74,12 +97,11 @@ paged_merge_kernel(const __grid_constant__ PagedWork w) {
 
 template <bool kFew>
 static int launch_merge(const PagedWork& w, int64_t rows, cudaStream_t stream) {
-  const int64_t ctas = (rows + kRowWarps - 1) / kRowWarps;
-  if (ctas > INT32_MAX) return TW_ERR_UNSUPPORTED;
+  if (rows > INT32_MAX) return TW_ERR_UNSUPPORTED;
   const auto kernel = w.a.out_dtype == TW_F32   ? paged_merge_kernel<float, kFew>
                       : w.a.out_dtype == TW_F16 ? paged_merge_kernel<__half, kFew>
                                                 : paged_merge_kernel<__nv_bfloat16, kFew>;
-  return launch_pdl(kernel, dim3((unsigned)ctas), dim3(kRowWarps * 32), 0, stream, w);
+  return launch_pdl(kernel, dim3((unsigned)rows), dim3(kMergeWarps * 32), 0, stream, w);
 }
 
 // ---- division of a call -----------------------------------------------------------

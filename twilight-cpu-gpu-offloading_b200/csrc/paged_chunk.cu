@@ -369,7 +369,8 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
         float s[4][32];
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld32(s[c], s_col + c * 32);
-        tmem_wait_ld();
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_wait_ld(s[c]);
         const int first = key0 + j * kTileKeys;
         const bool edge = first < all_low || first < low || first + kTileKeys > min(all_high, high);
         if (edge) {
@@ -410,7 +411,7 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
             for (int c = 0; c < 4; ++c) {
               float o[32];
               tmem_ld32(o, o_col + c * 32);
-              tmem_wait_ld();
+              tmem_wait_ld(o);
               uint32_t u[32];
 #pragma unroll
               for (int x = 0; x < 32; ++x) u[x] = __float_as_uint(o[x] * f);
@@ -485,7 +486,8 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
         if (tiles > 0) {
 #pragma unroll
           for (int c = 0; c < 4; ++c) tmem_ld32(o[c], o_col + c * 32);
-          tmem_wait_ld();
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_wait_ld(o[c]);
         }
 #pragma unroll
         for (int c = 0; c < 4; ++c) {

@@ -98,19 +98,41 @@ paged_token_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
   const tw_paged_attention_args& a = w.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int kv_heads = a.pool.kv_heads;
-  const int64_t cta = blockIdx.x;
-  const int64_t units = (int64_t)a.requests * kv_heads * w.few.splits;
+  if (tid == 0) {
+    for (int i = 0; i < kTokStages; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&s_empty[i], kTokWarps);
+    }
+    s_abort = 0;
+    s_bad_rows = 0;
+    mbar_init_fence();
+  }
+  if (tid == kTokWarps * 32) {
+    prefetch_map(&maps.k);
+    prefetch_map(&maps.v);
+  }
   pdl_wait();
   pdl_launch_dependents();
 
-  if (cta >= units) {
-    paged_clear_padding<Out>(a, (int)(cta - units));
+  // the first CTAs, which are done at once
+  if (blockIdx.x < kPadCtas) {
+    paged_clear_padding<Out>(a, blockIdx.x);
     return;
   }
+  const int64_t cta = blockIdx.x - kPadCtas;
   const int split = (int)(cta % w.few.splits);
   const int unit = (int)(cta / w.few.splits);
   const int b = unit / kv_heads;
   const int g = unit - b * kv_heads;
+  // The producer's first page, where it has to be without a window, together with
+  // the lengths: one round trip less before the first copy.
+  const int boxes = kTokTile / w.box;
+  const int box = lane % boxes;
+  const int32_t* table = a.block_table + (int64_t)b * a.table_stride;
+  const int guess = split * w.few.chunk + box * w.box;
+  int page = 0;
+  if (warp == kTokWarps && a.window == 0 && guess / a.pool.page_size < a.table_width)
+    page = table[guess / a.pool.page_size];
   const PagedRequest rq = paged_request(a, b);
   if (rq.n == 0) return;
   if (rq.n > w.few_tokens) {
@@ -128,35 +150,21 @@ paged_token_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
 
   char* smem = (char*)(((uintptr_t)s_raw + 1023) & ~(uintptr_t)1023);
   const uint32_t ring = smem_addr(smem);
-  if (tid == 0) {
-    for (int i = 0; i < kTokStages; ++i) {
-      mbar_init(&s_full[i], 1);
-      mbar_init(&s_empty[i], kTokWarps);
-    }
-    s_abort = 0;
-    s_bad_rows = 0;
-    mbar_init_fence();
-  }
   __syncthreads();
 
   if (warp == kTokWarps) {
     // ---- producer: lane l copies one box of K or V of each tile
-    const int boxes = kTokTile / w.box;
     const int matrix = lane / (2 * boxes);  // 0 K, 1 V, more: idle
     const int half = (lane / boxes) & 1;
-    const int box = lane % boxes;
     const CUtensorMap* map = matrix == 0 ? &maps.k : &maps.v;
-    const int32_t* table = a.block_table + (int64_t)b * a.table_stride;
     const uint32_t dst = ring + (2 * matrix + half) * kTokHalf + box * w.box * 128;
-    if (lane == 0) prefetch_map(&maps.k);
-    if (lane == 1) prefetch_map(&maps.v);
     const int stride = w.box;
     int key = tile0 + box * stride;
-    int page = 0;
     // boxes wholly before the first visible key are not read: a page that slid out
     // of the window may be gone
     const int skipped = (low - tile0) / stride;
-    if (matrix < 2 && key < range.end && box >= skipped) page = table[key / a.pool.page_size];
+    if (key != guess || a.window != 0)
+      page = matrix < 2 && key < range.end && box >= skipped ? table[key / a.pool.page_size] : 0;
     int i = 0;
     for (; i < tiles; ++i) {
       const int stage = i % kTokStages;

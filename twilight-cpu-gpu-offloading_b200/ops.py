@@ -338,6 +338,21 @@ _PACK_POOL = struct.Struct(_lib.PAGED_POOL_FORMAT).pack
 _PACK_STEP = struct.Struct(_lib.PAGED_STEP_FORMAT).pack
 _PACK_ATTENTION = struct.Struct(_lib.PAGED_ATTENTION_FORMAT).pack
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
+
+# Workspaces of paged_attention calls that brought none, per (device, stream): calls on
+# one stream follow one another, and a larger one takes the place of a smaller.
+_paged_workspaces: dict[tuple[int, int], torch.Tensor] = {}
+
+
+def _paged_workspace(dev: int, stream: int, need: int) -> torch.Tensor:
+    if torch.cuda.is_current_stream_capturing():  # a graph keeps its own
+        return torch.empty(need, dtype=torch.uint8, device=torch.device("cuda", dev))
+    kept = _paged_workspaces.get((dev, stream))
+    if kept is None or kept.numel() < need:
+        kept = torch.empty(need, dtype=torch.uint8, device=torch.device("cuda", dev))
+        _paged_workspaces[dev, stream] = kept
+    return kept
 
 
 def _device_index(t: torch.Tensor) -> int:
@@ -345,7 +360,7 @@ def _device_index(t: torch.Tensor) -> int:
     dev = t.get_device()
     if dev < 0:
         raise ValueError("twilight ops require CUDA tensors (no CPU fallback)")
-    if dev != torch.cuda.current_device():
+    if dev != _current_device():
         raise ValueError(f"the tensors are on cuda:{dev}: make it the current device")
     return dev
 
@@ -517,7 +532,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     longest kv_lens (it sizes the launch).  window > 0: each token sees the last
     `window` positions only.  Returns out [T, q_heads, 128] (q's dtype or
     float32); lse [T, q_heads] fp32 receives the log-sum-exp.  Without a
-    workspace one is allocated for the call."""
+    workspace one is taken that is kept for the current stream."""
     dev = _device_index(q)
     pool = _paged_pool(dev, k_pages, v_pages)
     shape, dtype, i32 = q.shape, q.dtype, torch.int32
@@ -542,7 +557,10 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
                  ("block_table", block_table, i32, (B, None)),
                  ("lse", lse, torch.float32, (T, Hq)), ("error_flag", error_flag, i32, (1,)))
     if out is None:
-        out = torch.empty(shape, dtype=out_dtype or dtype, device=q.device)
+        if (out_dtype is None or out_dtype is dtype) and q.is_contiguous():
+            out = torch.empty_like(q)  # half the time of torch.empty
+        else:
+            out = torch.empty(shape, dtype=out_dtype or dtype, device=q.device)
         out_token, out_head = Hq * HEAD_DIM, HEAD_DIM
     else:
         if out.shape != shape or out.get_device() != dev or \
@@ -551,10 +569,11 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         out_token, out_head = _rows_strides("out", out)
     if out.dtype is not dtype and out.dtype is not torch.float32:
         raise ValueError("out must have q's dtype or float32")
+    stream = _raw_stream(dev)
     if workspace is None:
         need = paged_attention_workspace_bytes(B, T, Hq, pool[7], max_q_len, max_kv_len, window)
         if need:
-            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+            workspace = _paged_workspace(dev, stream, need)
     else:
         need = workspace.numel() * workspace.element_size()
         if workspace.get_device() != dev or not workspace.is_contiguous():
@@ -569,7 +588,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         DTYPE_CODES[out.dtype], 0, 0 if lse is None else lse.data_ptr(),
         0 if error_flag is None else error_flag.data_ptr(),
         0 if workspace is None else workspace.data_ptr(), need)
-    status = lib().tw_paged_attention(args, _raw_stream(dev))
+    status = lib().tw_paged_attention(args, stream)
     if status:
         _lib.check(status, "paged_attention")
     return out
