@@ -15,8 +15,8 @@
 // round trip through tensor memory.
 //
 // Layout: a CTA takes one KV head of one request and one range of its keys.
-// One warp fetches 64-key tiles (K and V, 32 KB) into a ring of three stages
-// by TMA, a box for each page piece; four warps take 16 keys of every tile
+// Two warps fetch 64-key tiles (K and V, 32 KB) into a ring of three stages by
+// TMA, a box for each page piece; four warps take 16 keys of every tile
 // each, keep m, l and O of all 16 rows in registers, and join at the end
 // through shared memory.  Two CTAs are resident per SM: up to 192 KB in flight.
 #include "paged_attention.cuh"
@@ -27,7 +27,7 @@ constexpr int kTokRows = 16;
 constexpr int kTokTile = 64;       // keys per stage
 constexpr int kTokStages = 3;
 constexpr int kTokWarps = 4;       // consumers
-constexpr int kTokThreads = (kTokWarps + 1) * 32;
+constexpr int kTokThreads = (kTokWarps + 2) * 32;  // and a warp that copies K, one V
 constexpr int kTokHalf = kTokTile * 128;          // 64 of the 128 dimensions of a tile
 constexpr int kTokStageBytes = 4 * kTokHalf;      // K lo, K hi, V lo, V hi
 constexpr int kTokRowPad = kHeadDim + 4;          // floats per row of the join
@@ -100,7 +100,7 @@ paged_token_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
   const int kv_heads = a.pool.kv_heads;
   if (tid == 0) {
     for (int i = 0; i < kTokStages; ++i) {
-      mbar_init(&s_full[i], 1);
+      mbar_init(&s_full[i], 2);
       mbar_init(&s_empty[i], kTokWarps);
     }
     s_abort = 0;
@@ -124,14 +124,15 @@ paged_token_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
   const int unit = (int)(cta / w.few.splits);
   const int b = unit / kv_heads;
   const int g = unit - b * kv_heads;
-  // The producer's first page, where it has to be without a window, together with
-  // the lengths: one round trip less before the first copy.
+  // Lane l < boxes of a copying warp knows the page of box l of the next tile; the
+  // first, where it has to be without a window, is read together with the lengths:
+  // one round trip less before the first copy.
   const int boxes = kTokTile / w.box;
   const int box = lane % boxes;
   const int32_t* table = a.block_table + (int64_t)b * a.table_stride;
   const int guess = split * w.few.chunk + box * w.box;
   int page = 0;
-  if (warp == kTokWarps && a.window == 0 && guess / a.pool.page_size < a.table_width)
+  if (warp >= kTokWarps && a.window == 0 && guess / a.pool.page_size < a.table_width)
     page = table[guess / a.pool.page_size];
   const PagedRequest rq = paged_request(a, b);
   if (rq.n == 0) return;
@@ -152,43 +153,56 @@ paged_token_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
   const uint32_t ring = smem_addr(smem);
   __syncthreads();
 
-  if (warp == kTokWarps) {
-    // ---- producer: lane l copies one box of K or V of each tile
-    const int matrix = lane / (2 * boxes);  // 0 K, 1 V, more: idle
-    const int half = (lane / boxes) & 1;
+  if (warp >= kTokWarps) {
+    // ---- copies: a warp those of K, a warp those of V
+    const int matrix = warp - kTokWarps;
     const CUtensorMap* map = matrix == 0 ? &maps.k : &maps.v;
-    const uint32_t dst = ring + (2 * matrix + half) * kTokHalf + box * w.box * 128;
-    const int stride = w.box;
-    int key = tile0 + box * stride;
+    const uint32_t box_bytes = (uint32_t)w.box * 128;  // of 64 dimensions
+    int key = tile0 + box * w.box;
     // boxes wholly before the first visible key are not read: a page that slid out
     // of the window may be gone
-    const int skipped = (low - tile0) / stride;
+    const int skipped = (low - tile0) / w.box;
     if (key != guess || a.window != 0)
-      page = matrix < 2 && key < range.end && box >= skipped ? table[key / a.pool.page_size] : 0;
+      page = key < range.end && box >= skipped ? table[key / a.pool.page_size] : 0;
     int i = 0;
     for (; i < tiles; ++i) {
       const int stage = i % kTokStages;
-      const int now_key = key, now_page = page;
+      int p = page;
+      if (lane < boxes && key < range.end && (i > 0 || box >= skipped) &&
+          (p < 0 || p >= a.pool.num_pages)) {
+        raise_error(a.error_flag, TW_ERR_INVALID_INDEX);
+        p = (int)a.pool.num_pages;  // out of the map's range: zeros
+      }
       key += kTokTile;
-      if (matrix < 2 && i + 1 < tiles && key < range.end) page = table[key / a.pool.page_size];
+      if (i + 1 < tiles && key < range.end) page = table[key / a.pool.page_size];
       if (i >= kTokStages &&
           !__all_sync(0xffffffffu, mbar_wait<false>(&s_empty[stage],
-                                             (uint32_t)((i / kTokStages - 1) & 1), &s_abort)))
+                                                    (uint32_t)((i / kTokStages - 1) & 1), &s_abort)))
         break;
-      if (lane == 0) {
-        const int valid = min(range.end - (tile0 + i * kTokTile), kTokTile);
-        const int count = (valid + stride - 1) / stride - (i == 0 ? skipped : 0);
-        mbar_arrive_expect(&s_full[stage], (uint32_t)(count * stride * 4 * 128));
-      }
-      __syncwarp();
-      if (matrix < 2 && now_key < range.end && (i > 0 || box >= skipped)) {
-        int p = now_page;
-        if (p < 0 || p >= a.pool.num_pages) {
-          raise_error(a.error_flag, TW_ERR_INVALID_INDEX);
-          p = (int)a.pool.num_pages;  // out of the map's range: zeros
+      const int first = tile0 + i * kTokTile;
+      const int from = i == 0 ? skipped : 0;
+      const int to = (min(range.end - first, kTokTile) + w.box - 1) / w.box;
+      int row = (first + from * w.box) % a.pool.page_size;  // of the next box in its page
+      uint32_t dst = ring + stage * kTokStageBytes + matrix * 2 * kTokHalf + from * box_bytes;
+      if (elect_one()) mbar_arrive_expect(&s_full[stage], (uint32_t)(to - from) * box_bytes * 2);
+      for (int x = from; x < to; x += 4) {  // four boxes a turn: their pages at once
+        int px[4], rx[4];
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          px[y] = __shfl_sync(0xffffffffu, p, x + y);
+          rx[y] = row;
+          row += w.box;
+          if (row == a.pool.page_size) row = 0;
         }
-        tma_load_4d(map, dst + stage * kTokStageBytes, &s_full[stage], half * 64,
-                    now_key % a.pool.page_size, g, p);
+        if (elect_one()) {
+#pragma unroll
+          for (int y = 0; y < 4; ++y)
+            if (x + y < to) {
+              tma_load_4d(map, dst + y * box_bytes, &s_full[stage], 0, rx[y], g, px[y]);
+              tma_load_4d(map, dst + kTokHalf + y * box_bytes, &s_full[stage], 64, rx[y], g, px[y]);
+            }
+        }
+        dst += 4 * box_bytes;
       }
     }
     if (s_abort) {
