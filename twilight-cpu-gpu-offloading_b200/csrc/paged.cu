@@ -18,7 +18,7 @@ namespace tw {
 // three dependent loads (lengths -> table or stack -> slot).
 constexpr int kStepThreads = 512;
 constexpr int kStepMaxRequests = 8192;
-constexpr int kStepTokensPerCta = 2048;
+constexpr int kStepTokensPerCta = kStepThreads;
 
 struct StepSums {
   long long tokens, wanted, returned;
@@ -148,7 +148,6 @@ __global__ void __launch_bounds__(kStepThreads) paged_step_kernel(tw_paged_step_
       raise_error(a.error_flag, TW_ERR_CAPACITY);
   }
   // per request: lengths and the pages it takes
-  long long taken_end = 0;
   for (int b = first; b < B; b += step) {
     const StepRequest r = step_request(a.lens[b], a.new_lens[b], a.page_size, a.table_width);
     const bool ok = served(b, r);
@@ -167,7 +166,7 @@ __global__ void __launch_bounds__(kStepThreads) paged_step_kernel(tw_paged_step_
   if (blockIdx.x == 0 && tid == 0) {
     // requests are served up to the first whose pages the stack does not hold
     const int n = first_above(s_wanted, B, saturate(top));
-    taken_end = n > 0 ? s_wanted[n - 1] : 0;
+    const long long taken_end = n > 0 ? s_wanted[n - 1] : 0;
     a.cu_q[0] = 0;
     *a.free_count_out = (int)min(top - taken_end, (long long)a.num_pages);
     if (total > a.tokens_cap) raise_error(a.error_flag, TW_ERR_CAPACITY);
@@ -175,34 +174,43 @@ __global__ void __launch_bounds__(kStepThreads) paged_step_kernel(tw_paged_step_
 }
 
 // ---- row write ------------------------------------------------------------------
-// One 16-byte vector of K and the same of V per thread and turn; the 16 threads
-// of a row write 256 contiguous bytes.  Bound: HBM (each byte read and written
-// once).
+// One 16-byte vector of K and the same of V per thread; the 16 threads of a row
+// write 256 contiguous bytes.  Bound: HBM (each byte read and written once).
 constexpr int kWriteThreads = 256;
 
 __global__ void __launch_bounds__(kWriteThreads)
-paged_write_kernel(tw_paged_pool pool, const uint4* __restrict__ k, int64_t k_token,
-                   int64_t k_head, const uint4* __restrict__ v, int64_t v_token, int64_t v_head,
-                   const int64_t* __restrict__ slots, int64_t vectors, int32_t* error_flag) {
+paged_write_kernel(const __grid_constant__ tw_paged_pool pool, const uint4* __restrict__ k,
+                   int64_t k_token, int64_t k_head, const uint4* __restrict__ v, int64_t v_token,
+                   int64_t v_head, const int64_t* __restrict__ slots, int64_t rows,
+                   int32_t* error_flag) {
   pdl_wait();
   pdl_launch_dependents();
-  const int64_t i = (int64_t)blockIdx.x * kWriteThreads + threadIdx.x;
-  if (i >= vectors) return;
-  const int c = (int)(i & (kVecPerRow16 - 1));
-  const int64_t row = i / kVecPerRow16;
-  const int64_t t = row / pool.kv_heads;
-  const int64_t h = row - t * pool.kv_heads;
+  const int c = threadIdx.x & (kVecPerRow16 - 1);
+  const int64_t row = (int64_t)blockIdx.x * (kWriteThreads / kVecPerRow16) +
+                      threadIdx.x / kVecPerRow16;
+  if (row >= rows) return;
+  int64_t t, h;
+  if (rows <= INT32_MAX) {  // a 64-bit division takes as long as a load
+    t = (unsigned)row / (unsigned)pool.kv_heads;
+    h = row - t * pool.kv_heads;
+  } else {
+    t = row / pool.kv_heads;
+    h = row - t * pool.kv_heads;
+  }
+  const uint4 kv = __ldcs(k + (t * k_token + h * k_head) / kPagedAlign + c);
+  const uint4 vv = __ldcs(v + (t * v_token + h * v_head) / kPagedAlign + c);
   const int64_t slot = slots[t];
   if (slot < 0 || slot >= pool.num_pages * pool.page_size) {
     if (slot != -1) raise_error(error_flag, TW_ERR_INVALID_INDEX);
     return;
   }
-  const int64_t page = slot / pool.page_size;
+  const int64_t page = slot <= INT32_MAX ? (unsigned)slot / (unsigned)pool.page_size
+                                         : slot / pool.page_size;
   const int64_t o = slot - page * pool.page_size;
   const int64_t to = (page * pool.page_stride + h * pool.head_stride + o * pool.token_stride) /
                          kPagedAlign + c;
-  reinterpret_cast<uint4*>(pool.k_pages)[to] = k[(t * k_token + h * k_head) / kPagedAlign + c];
-  reinterpret_cast<uint4*>(pool.v_pages)[to] = v[(t * v_token + h * v_head) / kPagedAlign + c];
+  reinterpret_cast<uint4*>(pool.k_pages)[to] = kv;
+  reinterpret_cast<uint4*>(pool.v_pages)[to] = vv;
 }
 
 }  // namespace tw
@@ -245,10 +253,10 @@ extern "C" int tw_paged_write(const tw_paged_pool* pool, const void* k, int64_t 
       !paged_stride_ok(k_head_stride) || !paged_stride_ok(v_token_stride) ||
       !paged_stride_ok(v_head_stride))
     return TW_ERR_BAD_ARG;
-  const int64_t vectors = tokens * pool->kv_heads * kVecPerRow16;
-  const int64_t ctas = (vectors + kWriteThreads - 1) / kWriteThreads;
+  const int64_t rows = tokens * pool->kv_heads;
+  const int64_t ctas = (rows * kVecPerRow16 + kWriteThreads - 1) / kWriteThreads;
   if (ctas > INT32_MAX) return TW_ERR_UNSUPPORTED;
   return launch_pdl(paged_write_kernel, dim3((unsigned)ctas), dim3(kWriteThreads), 0,
                     (cudaStream_t)stream, *pool, (const uint4*)k, k_token_stride, k_head_stride,
-                    (const uint4*)v, v_token_stride, v_head_stride, slots, vectors, error_flag);
+                    (const uint4*)v, v_token_stride, v_head_stride, slots, rows, error_flag);
 }

@@ -393,12 +393,12 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
         float top[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          top[c] = max3_nan(s[c][0], s[c][1], s[c][2]);
+          top[c] = max3(s[c][0], s[c][1], s[c][2]);
 #pragma unroll
-          for (int x = 3; x < 31; x += 2) top[c] = max3_nan(top[c], s[c][x], s[c][x + 1]);
-          top[c] = max3_nan(top[c], s[c][31], s[c][31]);
+          for (int x = 3; x < 31; x += 2) top[c] = max3(top[c], s[c][x], s[c][x + 1]);
+          top[c] = max3(top[c], s[c][31], s[c][31]);
         }
-        const float t = max3_nan(max3_nan(top[0], top[1], top[2]), top[3], top[3]) * w.scale_log2;
+        const float t = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * w.scale_log2;
         const bool move = t > m + kChMoveBy;
         if (__any_sync(0xffffffffu, move)) {
           const float f = move ? ex2(m - t) : 1.f;
@@ -456,7 +456,7 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
             }
           }
         };
-        if (__all_sync(0xffffffffu, !edge && t == t && fabsf(m) < CUDART_INF_F))
+        if (__all_sync(0xffffffffu, !edge && fabsf(m) < CUDART_INF_F))
           weights(std::true_type{});
         else
           weights(std::false_type{});

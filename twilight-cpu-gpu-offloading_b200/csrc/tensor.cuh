@@ -144,21 +144,26 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
 }
 
 
-// The largest of three; NaN when one is NaN.
-__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+// The largest of three.
+__device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
 
-// 2^x of a pair on the FMA pipe, for finite x <= 126 (below -126: 2^-126): n = x
+// 2^x of a pair on the FMA pipe, for x <= 126 (below -126: 2^-126; NaN: NaN): n = x
 // rounded to a whole number by adding 1.5 * 2^23, 2^(x - n) on [-1/2, 1/2] by the
-// polynomial of degree 4 with the smallest largest relative error there
-// (2.6e-6; Remez exchange), n added to the exponent bits.
+// polynomial of degree 4 with the smallest largest relative error there (2.6e-6;
+// Remez exchange), times 2^n put together from its bits.
 __device__ __forceinline__ void ex2_fma(uint64_t x2, float& e0, float& e1) {
   float x0, x1;
   unpair(x2, x0, x1);
-  x2 = pair(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
+  x2 = pair(max_nan(x0, -126.f), max_nan(x1, -126.f));
   const uint64_t round = pair(12582912.f, 12582912.f), back = pair(-12582912.f, -12582912.f);
   const uint64_t r = add2(x2, round);
   const uint64_t f = fma2(add2(r, back), pair(-1.f, -1.f), x2);
@@ -167,11 +172,11 @@ __device__ __forceinline__ void ex2_fma(uint64_t x2, float& e0, float& e1) {
   p = fma2(p, f, pair(0x1.ec06dap-3f, 0x1.ec06dap-3f));
   p = fma2(p, f, pair(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
   p = fma2(p, f, pair(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
-  float r0, r1, p0, p1;
+  float r0, r1;
   unpair(r, r0, r1);
-  unpair(p, p0, p1);
-  e0 = __int_as_float(__float_as_int(p0) + (__float_as_int(r0) << 23));
-  e1 = __int_as_float(__float_as_int(p1) + (__float_as_int(r1) << 23));
+  p = mul2(p, pair(__int_as_float((__float_as_int(r0) << 23) + 0x3f800000),
+                   __int_as_float((__float_as_int(r1) << 23) + 0x3f800000)));
+  unpair(p, e0, e1);
 }
 
 // Registers of a warpgroup's threads, all of which run this.
