@@ -9,17 +9,21 @@ Import by path (the directory name is not a Python identifier)::
 
 Public API mirrors the reference's offload caches (hi/quest_offload_cache.py,
 hi/twilight_offload_cache.py) and its varlen attention call (hi/mp.py:21-52).
-All compute runs in libtwilight_b200.so (C ABI: include/twilight_b200.h).
+PagedKVCache (this package's own) serves several requests from pages in device
+memory, prompts in chunks.  All compute runs in libtwilight_b200.so (C ABI: include/twilight_b200.h).
 """
 
 from . import _lib, ops
 from .attention import flash_attention_varlen_forward, sparse_gqa_decode_attention
 from .cache import QuestTopKOffloadedCache, TwilightMatchedBudgetOffloadedCache
+from .paged import PagedKVCache, PagedStep
 from .slab import MappedHostSlab, SequentialCacheState, SlabGeometry
 
 __all__ = [
     "QuestTopKOffloadedCache",
     "TwilightMatchedBudgetOffloadedCache",
+    "PagedKVCache",
+    "PagedStep",
     "SlabGeometry",
     "SequentialCacheState",
     "MappedHostSlab",
