@@ -245,14 +245,12 @@ extern "C" int tw_paged_attention(const tw_paged_attention_args* args, void* str
   if (st == TW_OK) st = encode_rows_map(&maps.v, a.pool.dtype, 4, a.pool.v_pages, dims, strides, box);
   if (st != TW_OK) return st;
   cudaStream_t s = (cudaStream_t)stream;
-  if (w.many.splits > 0) {
-    st = launch_paged_chunk(w, maps, s);
-    if (st == TW_OK && w.many.splits > 1) st = launch_merge<false>(w, plan.many_rows, s);
-    if (st != TW_OK) return st;
-  }
-  if (w.few.splits > 0) {
-    st = launch_paged_token(w, maps, s);
-    if (st == TW_OK && w.few.splits > 1) st = launch_merge<true>(w, plan.few_rows, s);
-  }
+  // The token kernel of a mixed call takes the SMs that the chunk kernel leaves idle
+  // at its end: 16 requests, 10 of them single tokens: 78 -> 63 us.
+  w.beside = w.many.splits > 0;
+  if (w.many.splits > 0) st = launch_paged_chunk(w, maps, s);
+  if (st == TW_OK && w.few.splits > 0) st = launch_paged_token(w, maps, s);
+  if (st == TW_OK && w.few.splits > 1) st = launch_merge<true>(w, plan.few_rows, s);
+  if (st == TW_OK && w.many.splits > 1) st = launch_merge<false>(w, plan.many_rows, s);
   return st;
 }

@@ -54,6 +54,11 @@ template <> struct Pack16<__nv_bfloat16> {
   }
 };
 
+// The lowest n bits (n <= 0: none, n >= 32: all).
+__device__ __forceinline__ uint32_t low_bits(int n) {
+  return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1;
+}
+
 __device__ __forceinline__ void softmax_sync() {
   asm volatile("bar.sync 1, %0;" ::"n"(kChSoftmax) : "memory");
 }
@@ -374,20 +379,14 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
         const int first = key0 + j * kTileKeys;
         const bool edge = first < all_low || first < low || first + kTileKeys > min(all_high, high);
         if (edge) {
+          // a bit per key, which predicates take eight at a time
           const int from = max(see, low) - first, to = min(p + 1, high) - first;
-          if (__any_sync(0xffffffffu, to < kTileKeys)) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
+          for (int c = 0; c < 4; ++c) {
+            const uint32_t seen = low_bits(to - c * 32) & ~low_bits(from - c * 32);
 #pragma unroll
-              for (int x = 0; x < 32; ++x)
-                if (c * 32 + x >= to) s[c][x] = -CUDART_INF_F;
-          }
-          if (__any_sync(0xffffffffu, from > 0)) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-#pragma unroll
-              for (int x = 0; x < 32; ++x)
-                if (c * 32 + x < from) s[c][x] = -CUDART_INF_F;
+            for (int x = 0; x < 32; ++x)
+              if (!(seen >> x & 1)) s[c][x] = -CUDART_INF_F;
           }
         }
         float top[4];
