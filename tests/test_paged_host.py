@@ -4,7 +4,6 @@ host (no kernel is launched)."""
 from __future__ import annotations
 
 import ctypes
-import struct
 
 import pytest
 
@@ -14,30 +13,6 @@ def test_struct_sizes(tw):
     assert ctypes.sizeof(L.PagedPool) == lib.tw_paged_pool_size()
     assert ctypes.sizeof(L.PagedStepArgs) == lib.tw_paged_step_args_size()
     assert ctypes.sizeof(L.PagedAttentionArgs) == lib.tw_paged_attention_args_size()
-
-
-def flat(cls):
-    """(offset, size, is float) of every field, the nested ones' too."""
-    for name, kind in cls._fields_:
-        field = getattr(cls, name)
-        if issubclass(kind, ctypes.Structure):
-            yield from ((field.offset + o, n, f) for o, n, f in flat(kind))
-        else:
-            yield field.offset, field.size, kind is ctypes.c_float
-
-
-@pytest.mark.parametrize("cls,fmt", [("PagedPool", "PAGED_POOL_FORMAT"),
-                                     ("PagedStepArgs", "PAGED_STEP_FORMAT"),
-                                     ("PagedAttentionArgs", "PAGED_ATTENTION_FORMAT")])
-def test_packed_layout(tw, cls, fmt):
-    """The formats that the wrappers pack are the structs, field by field."""
-    cls, fmt = getattr(tw._lib, cls), getattr(tw._lib, fmt)
-    assert struct.calcsize(fmt) == ctypes.sizeof(cls)
-    fields = list(flat(cls))
-    assert len(fields) == len(fmt)
-    for i, (offset, size, is_float) in enumerate(fields):
-        assert struct.calcsize(fmt[:i + 1]) - struct.calcsize(fmt[i]) == offset
-        assert struct.calcsize(fmt[i]) == size and (fmt[i] == "f") == is_float
 
 
 def pool(L, **change):
@@ -98,6 +73,19 @@ def test_null_and_empty_calls(tw):
                               None) == L.TW_OK
     assert lib.tw_paged_attention(ctypes.byref(a), None) == L.TW_OK
     assert lib.tw_paged_step(ctypes.byref(L.PagedStepArgs()), None) == L.TW_ERR_BAD_ARG
+
+
+def test_binding_checks_its_arguments(tw):
+    b = tw._lib.binding()
+    for call, n in ((b.paged_step, 12), (b.paged_write, 6), (b.paged_attention, 15)):
+        with pytest.raises(TypeError):
+            call()
+        args = [1 if n == 12 and i == 5 or n == 15 and i in (6, 7, 8) else None for i in range(n)]
+        assert call(*args) == -1  # no tensors
+    with pytest.raises(ValueError):
+        b.paged_step(*[1 << 40 if i == 5 else None for i in range(12)])
+    with pytest.raises(TypeError):
+        b.paged_attention(*[None] * 15)
 
 
 def test_cpu_tensors_are_refused(tw):

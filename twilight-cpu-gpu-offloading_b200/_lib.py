@@ -10,9 +10,12 @@ capacity errors (hi/quest_offload_cache.py:104-106).
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libtwilight_b200.so"
+BINDING_PATH = LIB_PATH.with_name("_binding.so")
 
 TW_OK = 0
 TW_ERR_INVALID_INDEX = 1
@@ -100,13 +103,7 @@ class PagedAttentionArgs(ctypes.Structure):
     ]
 
 
-# The same structs as struct.Struct formats: packing one is several times faster
-# than filling a ctypes.Structure, and these calls are made once per layer.
-PAGED_POOL_FORMAT = "QQqqqqiiii"
-PAGED_STEP_FORMAT = "QQQqiiiiQqQQQQQQQ"
-PAGED_ATTENTION_FORMAT = PAGED_POOL_FORMAT + "QqqQqiiQQiiiiifQqqiiQQQQ"
-
-# name -> (restype, argtypes); a struct pointer is P: packed bytes or byref(struct); mirrors include/twilight_b200.h
+# name -> (restype, argtypes); mirrors include/twilight_b200.h
 SIGNATURES = {
     "tw_status_string": (ctypes.c_char_p, [I32]),
     "tw_last_cuda_error": (I32, []),
@@ -146,15 +143,16 @@ SIGNATURES = {
     "tw_qkv_rope": (I32, [P, P, P, P, I32, I32, I32, I32, P, P, I32, P, P, P, P]),
     "tw_decode_attention_noalloc": (I32, [P, P, P, P, I32, I32, I32, I32, I32, FLT, P, I32, P, P]),
     "tw_paged_pool_size": (SZ, []),
-    "tw_paged_step": (I32, [P, P]),
+    "tw_paged_step": (I32, [ctypes.POINTER(PagedStepArgs), P]),
     "tw_paged_step_args_size": (SZ, []),
-    "tw_paged_write": (I32, [P, P, I64, I64, P, I64, I64, P, I64, P, P]),
+    "tw_paged_write": (I32, [ctypes.POINTER(PagedPool), P, I64, I64, P, I64, I64, P, I64, P, P]),
     "tw_paged_attention_workspace_size": (SZ, [I32, I32, I32, I32, I32, I32, I32, I32]),
-    "tw_paged_attention": (I32, [P, P]),
+    "tw_paged_attention": (I32, [ctypes.POINTER(PagedAttentionArgs), P]),
     "tw_paged_attention_args_size": (SZ, []),
 }
 
 _lib = None
+_binding = None
 
 
 class TwilightError(RuntimeError):
@@ -177,6 +175,25 @@ def load():
         fn.argtypes = argtypes
     _lib = lib
     return lib
+
+
+def binding():
+    """The compiled binding of the paged-cache calls (no fallback)."""
+    global _binding
+    if _binding is None:
+        import torch  # noqa: F401  (its libraries first)
+
+        load()
+        if not BINDING_PATH.exists():
+            raise ImportError(
+                f"{BINDING_PATH.name} is missing: build it with "
+                "`python twilight-cpu-gpu-offloading_b200/build.py` (there is no CPU fallback)")
+        loader = importlib.machinery.ExtensionFileLoader("_binding", str(BINDING_PATH))
+        spec = importlib.util.spec_from_file_location("_binding", BINDING_PATH, loader=loader)
+        module = importlib.util.module_from_spec(spec)
+        loader.exec_module(module)
+        _binding = module
+    return _binding
 
 
 def status_string(status: int) -> str:

@@ -3,7 +3,8 @@
     python twilight-cpu-gpu-offloading_b200/build.py
 
 nvcc cross-compiles for sm_100a without a GPU.  The shared library exports
-the C ABI declared in include/twilight_b200.h.
+the C ABI declared in include/twilight_b200.h; _binding.so calls it with torch
+tensors where a call through ctypes would take the host too long.
 """
 
 from __future__ import annotations
@@ -12,6 +13,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -19,6 +21,7 @@ PKG = Path(__file__).resolve().parent
 REPO = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libtwilight_b200.so"
+BINDING = PKG / "_binding.so"  # Python calls with torch tensors (csrc/binding.cpp)
 SOURCES = ["quest.cu", "int4.cu", "topp_union.cu", "gather.cu", "attention.cu", "frontend.cu",
            "capi.cu", "paged.cu", "paged_attention.cu",
            "paged_token.cu", "paged_chunk.cu"]
@@ -41,11 +44,27 @@ def sources() -> list[Path]:
     return [CSRC / s for s in SOURCES]
 
 
+def binding_command() -> list[str]:
+    """g++ against the headers and libraries of the installed torch."""
+    import torch
+    from torch.utils import cpp_extension
+
+    include = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"],
+               str(Path(nvcc()).resolve().parents[1] / "include")]
+    lib = Path(torch.__file__).resolve().parent / "lib"
+    return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            *[f"-I{p}" for p in include], str(CSRC / "binding.cpp"), "-o",
+            str(BINDING.with_suffix(".so.tmp")), f"-L{PKG}", f"-l:{LIB.name}",
+            "-Wl,-rpath,$ORIGIN", f"-L{lib}", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu",
+            "-ltorch_python"]
+
+
 def needs_build() -> bool:
-    if not LIB.exists():
+    if not LIB.exists() or not BINDING.exists():
         return True
-    mtime = LIB.stat().st_mtime
-    deps = sources() + list(CSRC.glob("*.cuh")) + [REPO / "include" / "twilight_b200.h"]
+    mtime = min(LIB.stat().st_mtime, BINDING.stat().st_mtime)
+    deps = sources() + list(CSRC.glob("*.cuh")) + [CSRC / "binding.cpp"] + [REPO / "include" / "twilight_b200.h"]
     return any(d.stat().st_mtime > mtime for d in deps)
 
 
@@ -76,6 +95,11 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         print(" ".join(link))
     subprocess.run(link, check=True)
     tmp.replace(LIB)
+    cmd = binding_command()
+    if verbose:
+        print(" ".join(cmd))
+    subprocess.run(cmd, check=True)
+    BINDING.with_suffix(".so.tmp").replace(BINDING)
     return LIB
 
 

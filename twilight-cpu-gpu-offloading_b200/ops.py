@@ -8,7 +8,6 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
-import struct
 
 import torch
 
@@ -16,7 +15,6 @@ from . import _lib
 
 HEAD_DIM = 128
 DTYPE_CODES = {torch.float16: _lib.TW_F16, torch.bfloat16: _lib.TW_BF16, torch.float32: _lib.TW_F32}
-_SCALE = 1.0 / math.sqrt(HEAD_DIM)
 SCALE_RECIPROCAL = 0   # "/ 15" as torch on CUDA: x * fp32(1/15)
 SCALE_DIVIDE = 1       # "/ 15" as torch on CPU: IEEE division
 
@@ -330,40 +328,9 @@ def qkv_rope(hidden: torch.Tensor, w_q: torch.Tensor, w_k: torch.Tensor, w_v: to
 
 
 # ------------------------------------------------------------- paged cache --
-# These calls are made for every step and layer, and a short one's kernel takes a
-# few microseconds.  So each has one expression of all checks (the message is
-# worked out only when it fails) and packs its arguments in one go.
-
-_PACK_POOL = struct.Struct(_lib.PAGED_POOL_FORMAT).pack
-_PACK_STEP = struct.Struct(_lib.PAGED_STEP_FORMAT).pack
-_PACK_ATTENTION = struct.Struct(_lib.PAGED_ATTENTION_FORMAT).pack
-_raw_stream = torch._C._cuda_getCurrentRawStream
-_current_device = torch._C._cuda_getDevice
-
-# Workspaces of paged_attention calls that brought none, per (device, stream): calls on
-# one stream follow one another, and a larger one takes the place of a smaller.
-_paged_workspaces: dict[tuple[int, int], torch.Tensor] = {}
-
-
-def _paged_workspace(dev: int, stream: int, need: int) -> torch.Tensor:
-    if torch.cuda.is_current_stream_capturing():  # a graph keeps its own
-        return torch.empty(need, dtype=torch.uint8, device=torch.device("cuda", dev))
-    kept = _paged_workspaces.get((dev, stream))
-    if kept is None or kept.numel() < need:
-        kept = torch.empty(need, dtype=torch.uint8, device=torch.device("cuda", dev))
-        _paged_workspaces[dev, stream] = kept
-    return kept
-
-
-def _device_index(t: torch.Tensor) -> int:
-    """The current device's index, which has to be t's."""
-    dev = t.get_device()
-    if dev < 0:
-        raise ValueError("twilight ops require CUDA tensors (no CPU fallback)")
-    if dev != _current_device():
-        raise ValueError(f"the tensors are on cuda:{dev}: make it the current device")
-    return dev
-
+# Called for every step and layer, so these go through the compiled binding
+# (csrc/binding.cpp), which unpacks and checks the tensors; what is wrong with them is
+# worked out here when it finds that something is.
 
 def _explain(dev: int, *wanted) -> None:
     """Raises for the first tensor that is not as wanted: (name, tensor, dtype, shape);
@@ -371,7 +338,9 @@ def _explain(dev: int, *wanted) -> None:
     for name, t, dtype, shape in wanted:
         if t is None:
             continue
-        if t.get_device() < 0:
+        if not isinstance(t, torch.Tensor):
+            raise ValueError(f"{name} must be a tensor")
+        if not t.is_cuda:
             raise ValueError("twilight ops require CUDA tensors (no CPU fallback)")
         if t.get_device() != dev:
             raise ValueError(f"{name} must be on the device of the other tensors, cuda:{dev}")
@@ -381,48 +350,42 @@ def _explain(dev: int, *wanted) -> None:
             want = ", ".join("*" if n is None else str(n) for n in shape)
             raise ValueError(f"{name} must be {dtype} [{want}] with contiguous rows, got "
                              f"{t.dtype} {list(t.shape)}")
-    raise ValueError("unexpected tensors")
 
 
-def _rows_strides(name: str, t: torch.Tensor) -> tuple[int, int]:
-    """(token, head) strides of [tokens, heads, 128] rows; an extent of 1 has none of its own."""
-    token, head, inner = t.stride()
-    tokens, heads, _ = t.shape
-    if inner != 1:
-        raise ValueError(f"{name} needs contiguous rows of {HEAD_DIM} elements")
-    if heads <= 1:
-        head = HEAD_DIM
-    if tokens <= 1:
-        token = head * (heads or 1)
-    if token <= 0 or head <= 0 or (token | head) & 7 or t.data_ptr() & 15:
-        raise ValueError(f"{name} needs 16-byte aligned rows (positive strides in multiples of 8)")
-    return token, head
+def _explain_device(t: torch.Tensor) -> int:
+    if not t.is_cuda:
+        raise ValueError("twilight ops require CUDA tensors (no CPU fallback)")
+    if t.get_device() != torch.cuda.current_device():
+        raise ValueError(f"the tensors are on {t.device}: make it the current device")
+    return t.get_device()
 
 
-def _paged_pool(dev: int, k_pages: torch.Tensor, v_pages: torch.Tensor) -> tuple:
-    """The fields of tw_paged_pool for [pages, kv_heads, page_size, 128] tensors (any
-    order of strides)."""
-    shape, strides = k_pages.shape, k_pages.stride()
-    if len(shape) != 4 or shape != v_pages.shape or k_pages.dtype != v_pages.dtype \
-            or shape[3] != HEAD_DIM or 0 in shape:
+def _explain_rows(dev: int, name: str, t: torch.Tensor, dtype: torch.dtype, *shape) -> None:
+    """[tokens, heads, 128] rows that may be strided."""
+    _explain(dev, (name, t[:0] if t.dim() else t, dtype, (None, *shape[1:])))
+    if shape[0] is not None and t.shape[0] != shape[0]:
+        raise ValueError(f"{name} must have {shape[0]} rows, got {t.shape[0]}")
+    if t.stride(2) != 1 or t.data_ptr() % 16 or \
+            any(n > 1 and (s <= 0 or s % 8) for n, s in zip(t.shape[:2], t.stride())):
+        raise ValueError(f"{name} needs contiguous 16-byte aligned rows of {HEAD_DIM} elements "
+                         "(positive strides in multiples of 8)")
+
+
+def _explain_pool(dev: int, k_pages: torch.Tensor, v_pages: torch.Tensor) -> None:
+    _kv_code(k_pages.dtype)
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype \
+            or k_pages.shape[3] != HEAD_DIM or 0 in k_pages.shape:
         raise ValueError(f"k_pages and v_pages must be [pages, kv_heads, page_size, {HEAD_DIM}] "
                          "of one dtype")
-    if k_pages.get_device() != dev or v_pages.get_device() != dev:
-        _explain(dev, ("k_pages", k_pages, k_pages.dtype, shape),
-                 ("v_pages", v_pages, v_pages.dtype, shape))
-    if 1 in shape:  # an extent of 1 has no stride of its own
-        other = tuple(HEAD_DIM if n == 1 else s for n, s in zip(shape, v_pages.stride()))
-        strides = tuple(HEAD_DIM if n == 1 else s for n, s in zip(shape, strides))
-    else:
-        other = v_pages.stride()
-    if strides != other:
+    for t in (k_pages, v_pages):
+        if not t.is_cuda or t.get_device() != dev:
+            raise ValueError(f"the pages must be on the device of the other tensors, cuda:{dev}")
+    strides = [(s, r) for n, s, r in zip(k_pages.shape, k_pages.stride(), v_pages.stride()) if n > 1]
+    if any(s != r for s, r in strides):
         raise ValueError("k_pages and v_pages must have the same strides")
-    page, head, token, inner = strides
-    k, v = k_pages.data_ptr(), v_pages.data_ptr()
-    if inner != 1 or page <= 0 or head <= 0 or token <= 0 or (page | head | token) & 7 or \
-            (k | v) & 15:
+    if any(s <= 0 or s % 8 for s, _ in strides[:-1]) or strides[-1][0] != 1 or \
+            (k_pages.data_ptr() | v_pages.data_ptr()) % 16:
         raise ValueError("pages need contiguous 16-byte aligned rows (strides in multiples of 8)")
-    return k, v, page, head, token, shape[0], shape[2], shape[1], HEAD_DIM, _kv_code(k_pages.dtype)
 
 
 def paged_step(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor,
@@ -438,45 +401,23 @@ def paged_step(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Te
     kv_lens [B], cu_q [B+1], free_count_out [1] and, per new token, slots
     (int64, -1: none) and positions [tokens_cap].  A refused request or a full
     output sets error_flag to TW_ERR_CAPACITY."""
-    dev = _device_index(lens)
-    i32 = torch.int32
-    B = lens.shape[0] if lens.dim() == 1 else -1
-    each, cap = (B,), slots.shape
-    if not (lens.dtype is new_lens.dtype is block_table.dtype is free_pages.dtype is
-            free_count.dtype is kv_lens.dtype is cu_q.dtype is positions.dtype is
-            free_count_out.dtype is i32 and slots.dtype is torch.int64
-            and new_lens.shape == each and kv_lens.shape == each and cu_q.shape == (B + 1,)
-            and free_pages.dim() == 1 and free_count.shape == (1,)
-            and free_count_out.shape == (1,) and len(cap) == 1 and positions.shape == cap
-            and block_table.dim() == 2 and block_table.shape[0] == B
-            and (block_table.stride(1) == 1 or block_table.shape[1] == 1)
-            and lens.is_contiguous() and new_lens.is_contiguous() and free_pages.is_contiguous()
-            and kv_lens.is_contiguous() and cu_q.is_contiguous() and slots.is_contiguous()
-            and positions.is_contiguous()
-            and dev == new_lens.get_device() == block_table.get_device() ==
-            free_pages.get_device() == free_count.get_device() == kv_lens.get_device() ==
-            cu_q.get_device() == slots.get_device() == positions.get_device() ==
-            free_count_out.get_device()
-            and (error_flag is None
-                 or (error_flag.get_device() == dev and error_flag.dtype is i32))):
-        _explain(dev, ("lens", lens, i32, (None,)), ("new_lens", new_lens, i32, each),
+    rc = _lib.binding().paged_step(lens, new_lens, block_table, free_pages, free_count, page_size,
+                                   kv_lens, cu_q, slots, positions, free_count_out, error_flag)
+    if rc is None:
+        return
+    if rc < 0:
+        i32, dev = torch.int32, _explain_device(lens)
+        B = lens.shape[0] if lens.dim() == 1 else -1
+        _explain(dev, ("lens", lens, i32, (None,)), ("new_lens", new_lens, i32, (B,)),
                  ("block_table", block_table, i32, (B, None)),
                  ("free_pages", free_pages, i32, (None,)), ("free_count", free_count, i32, (1,)),
-                 ("kv_lens", kv_lens, i32, each), ("cu_q", cu_q, i32, (B + 1,)),
+                 ("kv_lens", kv_lens, i32, (B,)), ("cu_q", cu_q, i32, (B + 1,)),
                  ("slots", slots, torch.int64, (None,)),
-                 ("positions", positions, i32, cap[:1]),
+                 ("positions", positions, i32, slots.shape[:1]),
                  ("free_count_out", free_count_out, i32, (1,)),
                  ("error_flag", error_flag, i32, (1,)))
-    W = block_table.shape[1]
-    args = _PACK_STEP(
-        lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(),
-        block_table.stride(0) if B > 1 else W, W, B, page_size, cap[0], free_pages.data_ptr(),
-        free_pages.shape[0], free_count.data_ptr(), kv_lens.data_ptr(), cu_q.data_ptr(),
-        slots.data_ptr(), positions.data_ptr(), free_count_out.data_ptr(),
-        0 if error_flag is None else error_flag.data_ptr())
-    status = lib().tw_paged_step(args, _raw_stream(dev))
-    if status:
-        _lib.check(status, "paged_step")
+        raise ValueError("paged_step: unexpected tensors")
+    _lib.check(rc, "paged_step")
 
 
 def paged_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_pages: torch.Tensor,
@@ -484,27 +425,19 @@ def paged_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_pages: 
     """New rows k / v [T, kv_heads, 128] (strided views of a projection are fine) to
     slots [T] int64 of the pool [pages, kv_heads, page_size, 128] (tw_paged_write);
     slot -1 is skipped."""
-    dev = _device_index(k)
-    pool = _paged_pool(dev, k_pages, v_pages)
-    shape, dtype = k.shape, k_pages.dtype
-    if not (len(shape) == 3 and shape == v.shape and shape[1] == pool[7] and shape[2] == HEAD_DIM
-            and k.dtype is v.dtype is dtype and slots.dtype is torch.int64
-            and slots.shape == shape[:1] and slots.is_contiguous()
-            and dev == v.get_device() == slots.get_device()
-            and (error_flag is None
-                 or (error_flag.get_device() == dev and error_flag.dtype is torch.int32))):
-        rows = (None, pool[7], HEAD_DIM)
-        _explain(dev, ("k", k[:0], dtype, rows), ("v", v[:0], dtype, rows),
-                 ("slots", slots, torch.int64, shape[:1]),
+    rc = _lib.binding().paged_write(k, v, slots, k_pages, v_pages, error_flag)
+    if rc is None:
+        return
+    if rc < 0:
+        dev = _explain_device(k)
+        _explain_pool(dev, k_pages, v_pages)
+        dtype, heads = k_pages.dtype, k_pages.shape[1]
+        _explain_rows(dev, "k", k, dtype, None, heads, HEAD_DIM)
+        _explain_rows(dev, "v", v, dtype, k.shape[0], heads, HEAD_DIM)
+        _explain(dev, ("slots", slots, torch.int64, k.shape[:1]),
                  ("error_flag", error_flag, torch.int32, (1,)))
-    k_token, k_head = _rows_strides("k", k)
-    v_token, v_head = _rows_strides("v", v)
-    status = lib().tw_paged_write(
-        _PACK_POOL(*pool), k.data_ptr(), k_token, k_head, v.data_ptr(), v_token, v_head,
-        slots.data_ptr(), shape[0], None if error_flag is None else error_flag.data_ptr(),
-        _raw_stream(dev))
-    if status:
-        _lib.check(status, "paged_write")
+        raise ValueError("paged_write: unexpected tensors")
+    _lib.check(rc, "paged_write")
 
 
 @functools.lru_cache(maxsize=1024)
@@ -533,62 +466,30 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     `window` positions only.  Returns out [T, q_heads, 128] (q's dtype or
     float32); lse [T, q_heads] fp32 receives the log-sum-exp.  Without a
     workspace one is taken that is kept for the current stream."""
-    dev = _device_index(q)
-    pool = _paged_pool(dev, k_pages, v_pages)
-    shape, dtype, i32 = q.shape, q.dtype, torch.int32
-    if len(shape) != 3 or shape[2] != HEAD_DIM or dtype is not k_pages.dtype or \
-            shape[1] == 0 or shape[1] % pool[7]:
-        raise ValueError("q must be [T, q_heads, 128] in the pool's dtype, q_heads a multiple of "
-                         "kv_heads")
-    T, Hq, _ = shape
-    if kv_lens.dim() != 1:
-        raise ValueError("kv_lens must be [requests]")
-    B = kv_lens.shape[0]
-    if not (kv_lens.dtype is cu_q.dtype is block_table.dtype is i32 and cu_q.shape == (B + 1,)
-            and block_table.dim() == 2 and block_table.shape[0] == B
-            and (block_table.stride(1) == 1 or block_table.shape[1] == 1)
-            and kv_lens.is_contiguous() and cu_q.is_contiguous()
-            and dev == kv_lens.get_device() == cu_q.get_device() == block_table.get_device()
-            and (lse is None or (lse.dtype is torch.float32 and lse.shape == (T, Hq)
-                                 and lse.is_contiguous() and lse.get_device() == dev))
-            and (error_flag is None
-                 or (error_flag.get_device() == dev and error_flag.dtype is i32))):
+    rc = _lib.binding().paged_attention(q, k_pages, v_pages, block_table, cu_q, kv_lens, max_q_len,
+                                        max_kv_len, window, softmax_scale, out, out_dtype, lse,
+                                        workspace, error_flag)
+    if not isinstance(rc, int):
+        return rc
+    if rc < 0:
+        dev = _explain_device(q)
+        _explain_pool(dev, k_pages, v_pages)
+        if q.dim() != 3 or q.shape[1] == 0 or q.shape[1] % k_pages.shape[1]:
+            raise ValueError("q must be [T, q_heads, 128], q_heads a multiple of kv_heads")
+        heads = q.shape[1]
+        _explain_rows(dev, "q", q, k_pages.dtype, None, heads, HEAD_DIM)
+        i32, B = torch.int32, kv_lens.shape[0] if kv_lens.dim() == 1 else -1
         _explain(dev, ("kv_lens", kv_lens, i32, (None,)), ("cu_q", cu_q, i32, (B + 1,)),
                  ("block_table", block_table, i32, (B, None)),
-                 ("lse", lse, torch.float32, (T, Hq)), ("error_flag", error_flag, i32, (1,)))
-    if out is None:
-        if (out_dtype is None or out_dtype is dtype) and q.is_contiguous():
-            out = torch.empty_like(q)  # half the time of torch.empty
-        else:
-            out = torch.empty(shape, dtype=out_dtype or dtype, device=q.device)
-        out_token, out_head = Hq * HEAD_DIM, HEAD_DIM
-    else:
-        if out.shape != shape or out.get_device() != dev or \
-                (out_dtype is not None and out.dtype is not out_dtype):
-            raise ValueError("out must have q's shape and device (and out_dtype)")
-        out_token, out_head = _rows_strides("out", out)
-    if out.dtype is not dtype and out.dtype is not torch.float32:
-        raise ValueError("out must have q's dtype or float32")
-    stream = _raw_stream(dev)
-    if workspace is None:
-        need = paged_attention_workspace_bytes(B, T, Hq, pool[7], max_q_len, max_kv_len, window)
-        if need:
-            workspace = _paged_workspace(dev, stream, need)
-    else:
-        need = workspace.numel() * workspace.element_size()
-        if workspace.get_device() != dev or not workspace.is_contiguous():
+                 ("lse", lse, torch.float32, (q.shape[0], heads)),
+                 ("error_flag", error_flag, i32, (1,)))
+        if (out.dtype if out is not None else out_dtype) not in (None, q.dtype, torch.float32) or \
+                (out is not None and out_dtype not in (None, out.dtype)):
+            raise ValueError("out must have q's dtype or float32 (and out_dtype)")
+        if out is not None:
+            _explain_rows(dev, "out", out, out.dtype, q.shape[0], heads, HEAD_DIM)
+        if workspace is not None and (workspace.get_device() != dev
+                                      or not workspace.is_contiguous()):
             raise ValueError("workspace must be contiguous, on q's device")
-    W = block_table.shape[1]
-    q_token, q_head = _rows_strides("q", q)
-    args = _PACK_ATTENTION(
-        *pool, q.data_ptr(), q_token, q_head, block_table.data_ptr(),
-        block_table.stride(0) if B > 1 else W, W, B, cu_q.data_ptr(), kv_lens.data_ptr(), T, Hq,
-        max_q_len, max_kv_len, window,
-        _SCALE if softmax_scale is None else softmax_scale, out.data_ptr(), out_token, out_head,
-        DTYPE_CODES[out.dtype], 0, 0 if lse is None else lse.data_ptr(),
-        0 if error_flag is None else error_flag.data_ptr(),
-        0 if workspace is None else workspace.data_ptr(), need)
-    status = lib().tw_paged_attention(args, stream)
-    if status:
-        _lib.check(status, "paged_attention")
-    return out
+        raise ValueError("paged_attention: unexpected tensors")
+    _lib.check(rc, "paged_attention")
