@@ -162,6 +162,15 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
     b += k * stride;
     n = min(stride, n - k * stride);
   }
+  // Lane l < boxes of a copying warp knows the page of box l of the next tile; the
+  // first, where it has to be without a window, is read together with the lengths.
+  const int boxes = kTileKeys / w.box;
+  const int32_t* table = a.block_table + (int64_t)b * a.table_stride;
+  const bool copies = (warp == kChKeyWarp || warp == kChValueWarp) && lane < boxes;
+  const int guess = split * w.many.chunk + lane * w.box;
+  int page = 0;
+  if (copies && a.window == 0 && guess / a.pool.page_size < a.table_width)
+    page = table[guess / a.pool.page_size];
   const PagedRequest rq = paged_request(a, b);
   const int begin = (slot - (rq.first / tokens + b)) * tokens;  // first token of the CTA
   if (rq.n <= w.few_tokens || begin >= rq.n || begin < 0) return;
@@ -179,17 +188,12 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
   const int key0 = low / kTileKeys * kTileKeys;
   const int tiles = high > low ? (high - key0 + kTileKeys - 1) / kTileKeys : 0;
 
-  // Lane l < boxes of a copying warp knows the page of box l of the next tile.
   // Boxes wholly before the first visible key are not read: a page that slid out
   // of the window may be gone.
-  const int boxes = kTileKeys / w.box;
   const int skipped = (low - key0) / w.box;
-  const int32_t* table = a.block_table + (int64_t)b * a.table_stride;
   int key = key0 + lane * w.box;
-  int page = 0;
-  if ((warp == kChKeyWarp || warp == kChValueWarp) && lane < boxes && key < high &&
-      lane >= skipped)
-    page = table[key / a.pool.page_size];
+  if (copies && (key != guess || a.window != 0))
+    page = key < high && lane >= skipped ? table[key / a.pool.page_size] : 0;
   if (warp == kChMmaWarp) tmem_alloc(&sh.tmem, kChColumns);
   tmem_fence_before();
   __syncthreads();
@@ -479,7 +483,8 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
       // Rows go through shared memory (Q and the ring are free: all products are
       // done), so that a warp writes whole rows to memory: a thread writing its own
       // row 16 bytes at a time took 3.5 us for the 256 rows.
-      float odd = 0.f;
+      uint64_t odd2 = 0ull;
+      const uint64_t inv2 = pair(inv, inv);
       {
         float o[4][32];
         if (tiles > 0) {
@@ -487,13 +492,19 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
           for (int c = 0; c < 4; ++c) tmem_ld32(o[c], o_col + c * 32);
 #pragma unroll
           for (int c = 0; c < 4; ++c) tmem_wait_ld(o[c]);
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int x = 0; x < 32; ++x) o[c][x] = 0.f;
         }
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
 #pragma unroll
-          for (int x = 0; x < 32; ++x) {
-            o[c][x] = l == 0.f ? 0.f : o[c][x] * inv;
-            odd = fmaf(o[c][x], 0.f, odd);  // NaN when one is not finite
+          for (int x = 0; x < 32; x += 2) {
+            const uint64_t y = mul2(pair(o[c][x], o[c][x + 1]), inv2);
+            odd2 = fma2(y, 0ull, odd2);  // NaN when one is not finite
+            unpair(y, o[c][x], o[c][x + 1]);
           }
           if (joined)
             stage_row<Out>(smem, warp, lane, c, o[c]);
@@ -532,7 +543,9 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
       }
       // A row that is not finite may owe it to a V row that another token sees
       // and this one does not (weight 0 times infinity or NaN).
-      const unsigned again = __ballot_sync(0xffffffffu, live && odd != 0.f);
+      float odd0, odd1;
+      unpair(odd2, odd0, odd1);
+      const unsigned again = __ballot_sync(0xffffffffu, live && odd0 + odd1 != 0.f);
       if (lane == 0) sh.bad[warp] = again;
     }
     softmax_sync();
