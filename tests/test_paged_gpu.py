@@ -372,6 +372,74 @@ def test_values_that_a_row_does_not_see_stay_out(tw, cuda, value, where, window)
         assert bool(((out[rows].double() - ref[rows]).abs() <= tol[rows]).all())
 
 
+@pytest.mark.parametrize("where", ["q", "k", "v"])
+def test_values_that_a_row_sees_reach_it(tw, cuda, where):
+    """NaN in what a row attends with is NaN in its result, and in no other row's."""
+    b = Batch(cuda, [90, 1, 2], [200, 70, 40], q_heads=8, kv_heads=2, page=16,
+              dtype=torch.float16)
+    if where == "q":
+        b.q[30, 3, 7] = math.nan
+    else:
+        pages = b.k_pages if where == "k" else b.v_pages
+        pages[b.table[0, 150 // 16].long(), 0, 150 % 16, 3] = math.nan
+        pages[b.table[1, 0].long(), :, 5] = math.nan
+    out, lse, error = b.run(tw)
+    assert error == 0
+    bad = torch.isnan(out).any(-1)
+    want = torch.zeros_like(bad)
+    if where == "q":
+        want[30, 3] = True
+    else:
+        want[40:90, :4] = True  # positions 150 .. 199, the four heads of KV head 0
+        want[90] = True
+    assert torch.equal(bad, want)
+
+
+def test_requests_longer_than_max_q_len_are_flagged(tw, cuda):
+    for new, most in (([3, 1], 1), ([100, 60], 60)):
+        b = Batch(cuda, new, [150, 150], q_heads=8, kv_heads=2, page=16, dtype=torch.float16)
+        good, _, _ = b.run(tw)
+        out, _, error = b.run(tw, max_q_len=most)
+        assert error == tw._lib.TW_ERR_BAD_ARG
+        assert torch.equal(out[new[0]:], good[new[0]:])
+
+
+@pytest.mark.parametrize("requests", [33, 150, 1500])
+def test_many_requests(tw, cuda, requests):
+    rng = random.Random(requests)
+    new = [rng.choice((0, 1, 1, 1, 3, rng.randint(10, 70))) for _ in range(requests)]
+    kv = [n + rng.randint(0, 60) for n in new]
+    b = Batch(cuda, new, kv, q_heads=6, kv_heads=1, page=16, dtype=torch.bfloat16, seed=requests)
+    out, lse, error = b.run(tw)
+    assert error == 0
+    ref = torch.empty_like(out)
+    for r in range(requests):  # each request alone
+        first, n = int(b.cu[r]), new[r]
+        if n:
+            ref[first:first + n] = tw.ops.paged_attention(
+                b.q[first:first + n], b.k_pages, b.v_pages, b.table[r:r + 1],
+                torch.tensor([0, n], dtype=torch.int32, device=cuda), b.kv[r:r + 1], max_q_len=n,
+                max_kv_len=kv[r])
+    # one kernel or the other, one range or several: the same within both roundings
+    assert (out.float() - ref.float()).abs().max().item() <= 4 * 2.0 ** -8 * ref.abs().max().item()
+    for r in rng.sample(range(requests), 10):
+        first, n = int(b.cu[r]), new[r]
+        if n == 0:
+            continue
+        o, z, tol, _ = paged_ref.attention(
+            b.q[first:first + n], b.k_pages, b.v_pages, b.table[r:r + 1],
+            torch.tensor([0, n], device=cuda), b.kv[r:r + 1])
+        assert bool(((out[first:first + n].double() - o).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("most", [1, 10 ** 6])
+def test_max_kv_len_only_sizes_the_launch(tw, cuda, most):
+    b = Batch(cuda, [1, 50], [3000, 700], q_heads=8, kv_heads=2, page=16, dtype=torch.bfloat16)
+    out, lse, error = b.run(tw, max_kv_len=most)
+    assert error == 0
+    b.check(out, lse)
+
+
 def test_strided_rows_and_another_stream(tw, cuda):
     b = Batch(cuda, [1, 70], [33, 170], q_heads=8, kv_heads=2, page=16, dtype=torch.float16)
     T = b.q.shape[0]

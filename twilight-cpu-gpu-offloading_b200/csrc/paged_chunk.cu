@@ -542,10 +542,11 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
         });
       }
       // A row that is not finite may owe it to a V row that another token sees
-      // and this one does not (weight 0 times infinity or NaN).
+      // and this one does not (weight 0 times infinity or NaN).  If its sum is not
+      // finite, its own scores are to blame.
       float odd0, odd1;
       unpair(odd2, odd0, odd1);
-      const unsigned again = __ballot_sync(0xffffffffu, live && odd0 + odd1 != 0.f);
+      const unsigned again = __ballot_sync(0xffffffffu, live && odd0 + odd1 != 0.f && fabsf(l) < CUDART_INF_F);
       if (lane == 0) sh.bad[warp] = again;
     }
     softmax_sync();

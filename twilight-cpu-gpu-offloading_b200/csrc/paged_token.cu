@@ -410,8 +410,9 @@ paged_token_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
       else
         paged_store_part<16>(w.few, (int64_t)unit * w.few_rows + r, split, d0, o, lse2);
       // A row that is not finite may owe it to a V row that another token sees
-      // and this one does not (weight 0 times infinity or NaN).
-      if (rq.n > 1 && odd != 0.f) atomicOr(&s_bad_rows, 1 << r);
+      // and this one does not (weight 0 times infinity or NaN).  If its sum is not
+      // finite, its own scores are to blame.
+      if (rq.n > 1 && odd != 0.f && fabsf(l) < CUDART_INF_F) atomicOr(&s_bad_rows, 1 << r);
     }
   }
   if (rq.n == 1) return;
