@@ -7,7 +7,8 @@
 
 namespace tw {
 
-constexpr int kMergeWarps = 4;  // of a row
+constexpr int kMergeWarps = 4;   // of a row
+constexpr int kMergeAhead = 10;  // ranges that a warp reads before it knows the maximum
 
 // Joins the ranges of split rows: out = sum_s 2^(lse_s - M) o_s / sum_s 2^(lse_s - M).
 // A CTA per row, its warps taking every fourth range, so that a row's loads are in
@@ -58,22 +59,35 @@ paged_merge_kernel(const __grid_constant__ PagedWork w) {
   if (parts == 1) return;  // the range wrote the result itself
   const float* lse = sp.part_lse + row * sp.splits;
   const float* po = sp.part_o + row * sp.splits * kHeadDim + lane * 4;
+  // the first ranges of the warp are under way while the maximum is worked out
+  float4 x[kMergeAhead];
+  float z[kMergeAhead];
+#pragma unroll
+  for (int k = 0; k < kMergeAhead; ++k) {
+    const int s = warp + k * kMergeWarps;
+    x[k] = s < parts ? *reinterpret_cast<const float4*>(po + (int64_t)s * kHeadDim)
+                     : make_float4(0.f, 0.f, 0.f, 0.f);
+    z[k] = s < parts ? lse[s] : -CUDART_INF_F;
+  }
   float m = -CUDART_INF_F;
   for (int s = lane; s < parts; s += 32) m = fmaxf(m, lse[s]);
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
   const float u = m == -CUDART_INF_F ? 0.f : m;
   float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-  for (int s = warp; s < parts; s += kMergeWarps) {
-    const float f = ex2(lse[s] - u);
-    const float4 x = *reinterpret_cast<const float4*>(po + (int64_t)s * kHeadDim);
+  auto take = [&](const float4& y, float lse_s) {
+    const float f = ex2(lse_s - u);
     l += f;
-    o[0] = fmaf(x.x, f, o[0]);
-    o[1] = fmaf(x.y, f, o[1]);
-    o[2] = fmaf(x.z, f, o[2]);
-    o[3] = fmaf(x.w, f, o[3]);
-  }
+    o[0] = fmaf(y.x, f, o[0]);
+    o[1] = fmaf(y.y, f, o[1]);
+    o[2] = fmaf(y.z, f, o[2]);
+    o[3] = fmaf(y.w, f, o[3]);
+  };
+#pragma unroll
+  for (int k = 0; k < kMergeAhead; ++k) take(x[k], z[k]);
+#pragma unroll 8
+  for (int s = warp + kMergeAhead * kMergeWarps; s < parts; s += kMergeWarps)
+    take(*reinterpret_cast<const float4*>(po + (int64_t)s * kHeadDim), lse[s]);
   __shared__ float s_l[kMergeWarps];
   __shared__ float4 s_o[kMergeWarps][32];
   if (lane == 0) s_l[warp] = l;
