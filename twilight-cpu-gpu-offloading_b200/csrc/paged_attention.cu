@@ -12,8 +12,10 @@ constexpr int kMergeAhead = 10;  // ranges that a warp reads before it knows the
 
 // Joins the ranges of split rows: out = sum_s 2^(lse_s - M) o_s / sum_s 2^(lse_s - M).
 // A CTA per row, its warps taking every fourth range, so that a row's loads are in
-// flight together (one warp alone: 3 us for 37 ranges).  The ranges are added in
-// an order that does not depend on which was ready first.
+// flight together.  The ranges are added in an order that does not depend on which
+// was ready first.  Bound: latency; 32 rows of 37 ranges cost about 3 us after the
+// token kernel, 1.6 us less than with loads that wait for the maximum and 5 us less
+// than with one warp a row.
 // Every CTA waits for the kernel before it, also one without work: what follows in
 // the stream takes the end of this kernel for the end of that one.
 __device__ __forceinline__ void merge_nothing() {

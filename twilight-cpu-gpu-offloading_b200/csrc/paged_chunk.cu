@@ -10,12 +10,17 @@
 // Layout: a CTA takes 2 x 128 rows of one KV head, a row being a (token, query
 // head of the group) pair, so K and V are read once for all heads of the group
 // and each tile of 128 keys once for both halves.  One thread issues all
-// products; a warp copies Q once and K / V tiles by TMA into a ring of five
-// 32 KB slots, page piece by page piece; two warpgroups take one half each, a
-// thread one row: it reads its row of S from tensor memory, writes the weights
-// P back over it in 16 bits, and the product with V takes P from there.  The
-// halves alternate: while one computes its weights, the tensor cores work for
-// the other.
+// products; two warps copy Q, and K and V tiles by TMA into a ring of five 32 KB
+// slots, page piece by page piece; two warpgroups take one half each, a thread
+// one row: it reads its row of S from tensor memory, writes the weights P back
+// over it in 16 bits, and the product with V takes P from there.  The halves
+// alternate: while one computes its weights, the tensor cores work for the
+// other.  (Two threads a row, or two issuing threads, measured slower.)
+//
+// Measured: 4096 tokens over a 32k context, 64 / 8 heads: 3.56 ms, 1.16
+// PFLOP/s, at the board's power limit (1.5 to 1.6 GHz); 2048 tokens, 32 / 8
+// heads: 1.0 ms there, 45 us as a prompt of their own.  The tensor pipe is busy
+// 68 % of a busy SM's cycles; a tile takes 1.8 us, and each CTA 6 us more.
 #include "paged_attention.cuh"
 #include "tensor.cuh"
 
