@@ -532,6 +532,25 @@ def test_pool_beyond_32_bit_offsets(tw, cuda):
     b.check(out, lse)
 
 
+@pytest.mark.parametrize("new,kv", [([1], [5000]), ([200], [4000])])
+def test_workspace(tw, cuda, new, kv):
+    """A workspace that the caller brings: as large as asked for, whatever it holds."""
+    b = Batch(cuda, new, kv, q_heads=8, kv_heads=2, page=16, dtype=torch.bfloat16)
+    need = tw.ops.paged_attention_workspace_bytes(1, new[0], 8, 2, new[0], kv[0])
+    assert need > 0
+    out, lse, _ = b.run(tw)
+    for fill in (0, 255):
+        ws = torch.full((need,), fill, dtype=torch.uint8, device=cuda)
+        again, _, error = b.run(tw, workspace=ws)
+        assert error == 0 and torch.equal(again, out)
+    with pytest.raises(RuntimeError, match="capacity"):
+        b.run(tw, workspace=ws[:need - 1])
+    with pytest.raises(ValueError):
+        b.run(tw, workspace=torch.empty(need + 4, dtype=torch.uint8, device=cuda)[4:])
+    with pytest.raises(ValueError):
+        b.run(tw, workspace=torch.empty(need, dtype=torch.uint8))
+
+
 def test_attention_refusals(tw, cuda):
     b = Batch(cuda, [2, 1], [20, 30], q_heads=8, kv_heads=2, page=16, dtype=torch.float16)
     args = dict(q=b.q, k_pages=b.k_pages, v_pages=b.v_pages, block_table=b.table, cu_q=b.cu,

@@ -7,12 +7,12 @@
 
 namespace tw {
 
-constexpr int kMergeWarps = 4;   // of a row
+constexpr int kMergeWarps = 4;   // of a CTA
 constexpr int kMergeAhead = 10;  // ranges that a warp reads before it knows the maximum
 
 // Joins the ranges of split rows: out = sum_s 2^(lse_s - M) o_s / sum_s 2^(lse_s - M).
-// A CTA per row, its warps taking every fourth range, so that a row's loads are in
-// flight together.  The ranges are added in an order that does not depend on which
+// Rows of few-token requests have many ranges: four warps a row take every fourth,
+// so that a row's loads are in flight together; the others get a warp each.  The ranges are added in an order that does not depend on which
 // was ready first.  Bound: latency; 32 rows of 37 ranges cost about 3 us after the
 // token kernel, 1.6 us less than with loads that wait for the maximum and 5 us less
 // than with one warp a row.
@@ -28,10 +28,12 @@ __global__ void __launch_bounds__(kMergeWarps * 32)
 paged_merge_kernel(const __grid_constant__ PagedWork w) {
   const tw_paged_attention_args& a = w.a;
   const PagedSplit& sp = kFew ? w.few : w.many;
+  constexpr int kWarps = kFew ? kMergeWarps : 1;  // of a row
   // The lengths are older than the kernel before this one, which waited for what
   // wrote them; the partial results are not.
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t row = blockIdx.x;
+  const int lane = threadIdx.x & 31, warp = kFew ? threadIdx.x >> 5 : 0;
+  const int64_t row = kFew ? blockIdx.x
+                           : (int64_t)blockIdx.x * kMergeWarps + (threadIdx.x >> 5);
   int t, h;
   PagedRequest rq;
   PagedKeys keys;
@@ -47,7 +49,7 @@ paged_merge_kernel(const __grid_constant__ PagedWork w) {
   } else {
     t = (int)(row / a.q_heads);
     h = (int)(row - (int64_t)t * a.q_heads);
-    const int b = first_above(a.cu_q + 1, a.requests, t);
+    const int b = t < a.tokens ? first_above(a.cu_q + 1, a.requests, t) : a.requests;
     if (b >= a.requests) return merge_nothing();
     rq = paged_request(a, b);
     if (rq.n <= w.few_tokens || rq.n > a.max_q_len) return merge_nothing();
@@ -66,7 +68,7 @@ paged_merge_kernel(const __grid_constant__ PagedWork w) {
   float z[kMergeAhead];
 #pragma unroll
   for (int k = 0; k < kMergeAhead; ++k) {
-    const int s = warp + k * kMergeWarps;
+    const int s = warp + k * kWarps;
     x[k] = s < parts ? *reinterpret_cast<const float4*>(po + (int64_t)s * kHeadDim)
                      : make_float4(0.f, 0.f, 0.f, 0.f);
     z[k] = s < parts ? lse[s] : -CUDART_INF_F;
@@ -88,22 +90,24 @@ paged_merge_kernel(const __grid_constant__ PagedWork w) {
 #pragma unroll
   for (int k = 0; k < kMergeAhead; ++k) take(x[k], z[k]);
 #pragma unroll 8
-  for (int s = warp + kMergeAhead * kMergeWarps; s < parts; s += kMergeWarps)
+  for (int s = warp + kMergeAhead * kWarps; s < parts; s += kWarps)
     take(*reinterpret_cast<const float4*>(po + (int64_t)s * kHeadDim), lse[s]);
-  __shared__ float s_l[kMergeWarps];
-  __shared__ float4 s_o[kMergeWarps][32];
-  if (lane == 0) s_l[warp] = l;
-  s_o[warp][lane] = make_float4(o[0], o[1], o[2], o[3]);
-  __syncthreads();
-  if (warp != 0) return;
+  if constexpr (kFew) {
+    __shared__ float s_l[kMergeWarps];
+    __shared__ float4 s_o[kMergeWarps][32];
+    if (lane == 0) s_l[warp] = l;
+    s_o[warp][lane] = make_float4(o[0], o[1], o[2], o[3]);
+    __syncthreads();
+    if (warp != 0) return;
 #pragma unroll
-  for (int k = 1; k < kMergeWarps; ++k) {
-    const float4 x = s_o[k][lane];
-    l += s_l[k];
-    o[0] += x.x;
-    o[1] += x.y;
-    o[2] += x.z;
-    o[3] += x.w;
+    for (int k = 1; k < kMergeWarps; ++k) {
+      const float4 y = s_o[k][lane];
+      l += s_l[k];
+      o[0] += y.x;
+      o[1] += y.y;
+      o[2] += y.z;
+      o[3] += y.w;
+    }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
@@ -113,11 +117,12 @@ paged_merge_kernel(const __grid_constant__ PagedWork w) {
 
 template <bool kFew>
 static int launch_merge(const PagedWork& w, int64_t rows, cudaStream_t stream) {
-  if (rows > INT32_MAX) return TW_ERR_UNSUPPORTED;
+  const int64_t ctas = kFew ? rows : (rows + kMergeWarps - 1) / kMergeWarps;
+  if (ctas > INT32_MAX) return TW_ERR_UNSUPPORTED;
   const auto kernel = w.a.out_dtype == TW_F32   ? paged_merge_kernel<float, kFew>
                       : w.a.out_dtype == TW_F16 ? paged_merge_kernel<__half, kFew>
                                                 : paged_merge_kernel<__nv_bfloat16, kFew>;
-  return launch_pdl(kernel, dim3((unsigned)rows), dim3(kMergeWarps * 32), 0, stream, w);
+  return launch_pdl(kernel, dim3((unsigned)ctas), dim3(kMergeWarps * 32), 0, stream, w);
 }
 
 // ---- division of a call -----------------------------------------------------------
@@ -146,15 +151,26 @@ static PagedSplit split_few(int requests, int kv_heads, int64_t max_keys) {
   return sp;
 }
 
-// Ranges of the chunk kernel: one, unless its CTAs would leave SMs idle.  Then
-// the keys are cut so that about all SMs get one, no shorter than 512 keys.
-static PagedSplit split_many(int64_t units, int64_t keys) {
+// Ranges of the chunk kernel: one, unless its CTAs would leave SMs idle.  A single
+// request's CTAs are known: its keys are cut so that about all SMs get one, into
+// ranges of 768 keys or more (a range costs 6 us besides its tiles, and the merge;
+// 560 tokens at 3k, 14 heads: 36 us in three ranges, 29 us in four).
+// Of several requests, those with few tokens get no CTA here, but how many that are
+// the host does not know: the keys are cut for twice the SMs, into ranges of 1536
+// keys or more (13 requests of 5k to 14k, five of them with up to 8 tokens: 173 us
+// whole, 105 us in two ranges).  More does not pay where all have
+// a CTA (6 requests at 5k to 7k, 64 heads, 160 CTAs: 201 us whole, 259 us in three
+// ranges), nor does evening out the last wave of a single request (256 CTAs at 32k:
+// 1.00 ms whole, 1.13 ms in four): the partial results' traffic costs more.
+static PagedSplit split_many(int requests, int64_t units, int64_t keys) {
   PagedSplit sp = {};
-  const int64_t most = units < 148 ? 148 / units : 1;
-  int64_t chunk = div_up(keys, most);
-  chunk = chunk < 512 ? 512 : chunk;
-  sp.chunk = div_up(chunk, kTileKeys) * kTileKeys;
-  sp.splits = most > 1 && keys > sp.chunk ? div_up(keys, sp.chunk) : 1;
+  const int64_t ctas = (requests > 1 ? 2 : 1) * 148;
+  int64_t n = units < ctas ? ctas / units : 1;
+  const int64_t least = requests > 1 ? 1536 : 768;
+  n = keys / least < n ? keys / least : n;
+  sp.chunk = n > 1 ? div_up(div_up(keys, n), kTileKeys) * kTileKeys
+                   : div_up(keys, kTileKeys) * kTileKeys;
+  sp.splits = n > 1 ? div_up(keys, sp.chunk) : 1;
   return sp;
 }
 
@@ -185,7 +201,7 @@ static PagedPlan plan_paged(PagedWork& w, int requests, int tokens, int q_heads,
   if (most > w.few_tokens) {
     const int each = paged_chunk_tokens(w.group);
     const int64_t slots = requests == 1 ? div_up(tokens, each) : tokens / each + requests;
-    w.many = split_many(slots * kv_heads, seen(each));
+    w.many = split_many(requests, slots * kv_heads, seen(each));
     plan.many_rows = (int64_t)tokens * q_heads;
   }
   plan.bytes = part_bytes(plan.few_rows, w.few) + part_bytes(plan.many_rows, w.many);
