@@ -432,7 +432,7 @@ def test_many_requests(tw, cuda, requests):
         assert bool(((out[first:first + n].double() - o).abs() <= tol).all())
 
 
-@pytest.mark.parametrize("most", [1, 10 ** 6])
+@pytest.mark.parametrize("most", [0, 1, 10 ** 6, 2 ** 31 - 1])
 def test_max_kv_len_only_sizes_the_launch(tw, cuda, most):
     b = Batch(cuda, [1, 50], [3000, 700], q_heads=8, kv_heads=2, page=16, dtype=torch.bfloat16)
     out, lse, error = b.run(tw, max_kv_len=most)

@@ -12,10 +12,12 @@ constexpr int kMergeAhead = 10;  // ranges that a warp reads before it knows the
 
 // Joins the ranges of split rows: out = sum_s 2^(lse_s - M) o_s / sum_s 2^(lse_s - M).
 // Rows of few-token requests have many ranges: four warps a row take every fourth,
-// so that a row's loads are in flight together; the others get a warp each.  The ranges are added in an order that does not depend on which
-// was ready first.  Bound: latency; 32 rows of 37 ranges cost about 3 us after the
-// token kernel, 1.6 us less than with loads that wait for the maximum and 5 us less
-// than with one warp a row.
+// so that a row's loads are in flight together; the others get a warp each.  The
+// ranges are added in an order that does not depend on which was ready first.
+// Bound: latency; 32 rows of 37 ranges cost about 3 us after the token kernel, 1.6 us
+// less than with loads that wait for the maximum and 5 us less than with one warp a
+// row.
+//
 // Every CTA waits for the kernel before it, also one without work: what follows in
 // the stream takes the end of this kernel for the end of that one.
 __device__ __forceinline__ void merge_nothing() {
@@ -128,7 +130,17 @@ static int launch_merge(const PagedWork& w, int64_t rows, cudaStream_t stream) {
 // ---- division of a call -----------------------------------------------------------
 constexpr int kFewRows = 16;  // rows of one warp-level product
 
-static int div_up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+static int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// `keys` keys in ranges of at least `chunk`, whole tiles, kMaxSplits at most.
+constexpr int kMaxSplits = 256;
+static PagedSplit cut(int64_t keys, int64_t chunk) {
+  chunk = chunk * kMaxSplits < keys ? div_up(keys, kMaxSplits) : chunk;
+  PagedSplit sp = {};
+  sp.chunk = (int)(div_up(chunk, kTileKeys) * kTileKeys);
+  sp.splits = (int)div_up(keys, sp.chunk);
+  return sp;
+}
 
 static size_t part_bytes(int64_t rows, const PagedSplit& sp) {
   return sp.splits > 1 ? (size_t)rows * sp.splits * (kHeadDim + 4) * sizeof(float) : 0;
@@ -145,10 +157,7 @@ static PagedSplit split_few(int requests, int kv_heads, int64_t max_keys) {
   const int64_t ctas = 2 * 148 * (requests > 1 ? 2 : 1);
   int64_t chunk = div_up(units * max_keys, ctas);
   chunk = chunk < 256 ? 256 : chunk > 4096 ? 4096 : chunk;
-  PagedSplit sp = {};
-  sp.chunk = div_up(chunk, kTileKeys) * kTileKeys;
-  sp.splits = max_keys > sp.chunk ? div_up(max_keys, sp.chunk) : 1;
-  return sp;
+  return cut(max_keys, chunk);
 }
 
 // Ranges of the chunk kernel: one, unless its CTAs would leave SMs idle.  A single
@@ -158,20 +167,16 @@ static PagedSplit split_few(int requests, int kv_heads, int64_t max_keys) {
 // Of several requests, those with few tokens get no CTA here, but how many that are
 // the host does not know: the keys are cut for twice the SMs, into ranges of 1536
 // keys or more (13 requests of 5k to 14k, five of them with up to 8 tokens: 173 us
-// whole, 105 us in two ranges).  More does not pay where all have
-// a CTA (6 requests at 5k to 7k, 64 heads, 160 CTAs: 201 us whole, 259 us in three
-// ranges), nor does evening out the last wave of a single request (256 CTAs at 32k:
-// 1.00 ms whole, 1.13 ms in four): the partial results' traffic costs more.
+// whole, 105 us in two ranges).  More does not pay where all have a CTA (6 requests
+// at 5k to 7k, 64 heads, 160 CTAs: 201 us whole, 259 us in three ranges), nor does
+// evening out the last wave of a single request (256 CTAs at 32k: 1.00 ms whole,
+// 1.13 ms in four): the partial results' traffic costs more.
 static PagedSplit split_many(int requests, int64_t units, int64_t keys) {
-  PagedSplit sp = {};
   const int64_t ctas = (requests > 1 ? 2 : 1) * 148;
   int64_t n = units < ctas ? ctas / units : 1;
   const int64_t least = requests > 1 ? 1536 : 768;
   n = keys / least < n ? keys / least : n;
-  sp.chunk = n > 1 ? div_up(div_up(keys, n), kTileKeys) * kTileKeys
-                   : div_up(keys, kTileKeys) * kTileKeys;
-  sp.splits = n > 1 ? div_up(keys, sp.chunk) : 1;
-  return sp;
+  return cut(keys, n > 1 ? div_up(keys, n) : keys);
 }
 
 struct PagedPlan {
@@ -188,7 +193,7 @@ static PagedPlan plan_paged(PagedWork& w, int requests, int tokens, int q_heads,
   if (requests == 1 && most > w.few_tokens) w.few_tokens = 0;  // one request: one kernel
   w.few_rows = w.few_tokens * w.group;
   // keys that a CTA's rows see, from a tile's begin on (1: there may be none)
-  const int64_t cap = (int64_t)max_kv_len > 0 ? max_kv_len : 1;
+  const int64_t cap = max_kv_len < 1 ? 1 : max_kv_len < (1 << 30) ? max_kv_len : 1 << 30;
   auto seen = [&](int64_t rows) {
     const int64_t x = (int64_t)window + rows + kTileKeys;
     return window > 0 && x < cap ? x : cap;
@@ -200,7 +205,8 @@ static PagedPlan plan_paged(PagedWork& w, int requests, int tokens, int q_heads,
   }
   if (most > w.few_tokens) {
     const int each = paged_chunk_tokens(w.group);
-    const int64_t slots = requests == 1 ? div_up(tokens, each) : tokens / each + requests;
+    const int64_t slots =
+        requests == 1 ? div_up(tokens, each) : (int64_t)tokens / each + requests;
     w.many = split_many(requests, slots * kv_heads, seen(each));
     plan.many_rows = (int64_t)tokens * q_heads;
   }

@@ -207,155 +207,155 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
 
   // (the register split inside the branches: past a join the smaller number holds)
   if (warp >= kChMmaWarp) {
-  shrink_registers<kChIssueRegs>();
-  if (warp == kChKeyWarp || warp == kChValueWarp) {
-    // ---- copies: one warp those of Q and K, one those of V.  Ring slot n % kChSlots:
-    // n = 2j is K tile j, n = 2j + 1 is V tile j.
-    const bool values = warp == kChValueWarp;
-    const CUtensorMap* map = values ? &maps.v : &maps.k;
-    if (elect_one()) {
-      prefetch_map(map);
-      if (!values) {
-        mbar_arrive_expect(&sh.q_full, (uint32_t)(halves * R * half_tokens * kHeadDim * 2));
-        for (int i = 0; i < halves && tiles > 0; ++i)
-          for (int d = 0; d < 2; ++d)
-            tma_load_3d(&q_map, q_at + i * kChTileBytes + d * kChHalfTile, &sh.q_full, d * 64,
-                        g * R, rq.first + begin + i * half_tokens);
-      }
-    }
-    __syncwarp();
-    const uint32_t box_bytes = (uint32_t)w.box * 128;  // of 64 dimensions
-    int n = values ? 1 : 0;
-    uint32_t done_ragged = 0;
-    bool ok = true;
-    for (int j = 0; j < tiles; ++j, n += 2) {
-      int p = page;
-      if (lane < boxes && key < high && (j > 0 || lane >= skipped) &&
-          (p < 0 || p >= a.pool.num_pages)) {
-        raise_error(a.error_flag, TW_ERR_INVALID_INDEX);
-        p = (int)a.pool.num_pages;  // out of the map's range: zeros
-      }
-      key += kTileKeys;
-      if (lane < boxes && j + 1 < tiles && key < high) page = table[key / a.pool.page_size];
-      const int first = key0 + j * kTileKeys;
-      const int valid = min(high - first, kTileKeys);
-      const int from = j == 0 ? skipped : 0, to = (valid + w.box - 1) / w.box;
-      const bool ragged = values && (first < low || valid < kTileKeys);
-      const int s = n % kChSlots;
-      if (n >= kChSlots) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&sh.empty[s], (uint32_t)((n / kChSlots - 1) & 1),
-                                               &sh.abort));
-        if (!ok) break;
-      }
-      uint64_t* bar = ragged ? &sh.ragged : &sh.full[s];
-      if (elect_one()) mbar_arrive_expect(bar, (uint32_t)(to - from) * box_bytes * 2);
-      uint32_t dst = ring + s * kChTileBytes + from * box_bytes;
-      int row = (first + from * w.box) % a.pool.page_size;  // of the next box in its page
-      for (int x = from; x < to; x += 4) {  // four boxes a turn: their pages at once
-        int px[4];
-#pragma unroll
-        for (int y = 0; y < 4; ++y) px[y] = __shfl_sync(0xffffffffu, p, x + y);
-        int rx[4];
-#pragma unroll
-        for (int y = 0; y < 4; ++y) {
-          rx[y] = row;
-          row += w.box;
-          if (row == a.pool.page_size) row = 0;
+    shrink_registers<kChIssueRegs>();
+    if (warp == kChKeyWarp || warp == kChValueWarp) {
+      // ---- copies: one warp those of Q and K, one those of V.  Ring slot n % kChSlots:
+      // n = 2j is K tile j, n = 2j + 1 is V tile j.
+      const bool values = warp == kChValueWarp;
+      const CUtensorMap* map = values ? &maps.v : &maps.k;
+      if (elect_one()) {
+        prefetch_map(map);
+        if (!values) {
+          mbar_arrive_expect(&sh.q_full, (uint32_t)(halves * R * half_tokens * kHeadDim * 2));
+          for (int i = 0; i < halves && tiles > 0; ++i)
+            for (int d = 0; d < 2; ++d)
+              tma_load_3d(&q_map, q_at + i * kChTileBytes + d * kChHalfTile, &sh.q_full, d * 64,
+                          g * R, rq.first + begin + i * half_tokens);
         }
-        if (elect_one()) {
-#pragma unroll
-          for (int y = 0; y < 4; ++y)
-            if (x + y < to) {
-              tma_load_4d(map, dst + y * box_bytes, bar, 0, rx[y], g, px[y]);
-              tma_load_4d(map, dst + kChHalfTile + y * box_bytes, bar, 64, rx[y], g, px[y]);
-            }
-        }
-        dst += 4 * box_bytes;
       }
-      if (ragged) {
-        // V rows that no row sees: what they hold (NaN included) must not meet a
-        // weight of zero
-        ok = __all_sync(0xffffffffu, mbar_wait(bar, done_ragged & 1, &sh.abort));
-        if (!ok) break;
-        ++done_ragged;
-        char* tile = smem + (2 + s) * kChTileBytes;
-        for (int i = lane; i < kTileKeys * 16; i += 32) {
-          const int r = i >> 4;
-          if (first + r < low || r >= valid)
-            reinterpret_cast<uint4*>(tile + ((i >> 3) & 1) * kChHalfTile + r * 128)[i & 7] =
-                make_uint4(0u, 0u, 0u, 0u);
+      __syncwarp();
+      const uint32_t box_bytes = (uint32_t)w.box * 128;  // of 64 dimensions
+      int n = values ? 1 : 0;
+      uint32_t done_ragged = 0;
+      bool ok = true;
+      for (int j = 0; j < tiles; ++j, n += 2) {
+        int p = page;
+        if (lane < boxes && key < high && (j > 0 || lane >= skipped) &&
+            (p < 0 || p >= a.pool.num_pages)) {
+          raise_error(a.error_flag, TW_ERR_INVALID_INDEX);
+          p = (int)a.pool.num_pages;  // out of the map's range: zeros
         }
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.full[s]);
-      }
-    }
-    if (!ok || sh.abort) {
-      // give up: wait (with the same limit) for the copies in flight
-      volatile int never = 0;
-      mbar_wait(&sh.q_full, 0, &never);
-      for (int i = max(0, n - kChSlots); i < n; ++i)
-        mbar_wait(&sh.full[i % kChSlots], (uint32_t)((i / kChSlots) & 1), &never);
-    }
-  } else if (warp == kChMmaWarp) {
-    // ---- products, all issued by one thread
-    if (tiles > 0 && elect_one()) {
-      constexpr uint32_t desc_s = product_desc(Pack16<T>::kBf16, kTileKeys, false);
-      constexpr uint32_t desc_o = product_desc(Pack16<T>::kBf16, kHeadDim, true);
-      // S of half i from Q_i and the K tile in ring slot s
-      auto scores = [&](int i, int s) {
-        const uint32_t qa = q_at + i * kChTileBytes, ka = ring + s * kChTileBytes;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const uint32_t off = (k >> 2) * kChHalfTile + (k & 3) * 32;
-          mma_smem(tmem + i * 128, operand_desc(qa + off, 16, 1024), operand_desc(ka + off, 16, 1024),
-                   desc_s, k > 0);
-        }
-        mma_commit(&sh.s_full[i]);
-      };
-      auto values = [&](int i, int s, int part, bool add) {
-        const uint32_t va = ring + s * kChTileBytes;
-#pragma unroll
-        for (int k = part * 4; k < part * 4 + 4; ++k)
-          mma_tmem(tmem + 256 + i * 128, tmem + i * 128 + k * 8,
-                   operand_desc(va + k * 2048, kChHalfTile, 1024), desc_o, add || k > 0);
-      };
-      auto wait_slot = [&](int n) {
-        return mbar_wait(&sh.full[n % kChSlots], (uint32_t)((n / kChSlots) & 1), &sh.abort);
-      };
-      bool ok = mbar_wait(&sh.q_full, 0, &sh.abort) && wait_slot(0);
-      if (ok) {
-        tmem_fence_after();
-        for (int i = 0; i < halves; ++i) scores(i, 0);
-        mma_commit(&sh.empty[0]);
-      }
-      for (int j = 0; j < tiles && ok; ++j) {
-        const int nv = 2 * j + 1, nk = 2 * j + 2;
-        if (!wait_slot(nv)) break;
-        if (j + 1 < tiles && !wait_slot(nk)) break;
-        for (int i = 0; i < halves; ++i) {
-          ok = mbar_wait(&sh.p_full[i][0], (uint32_t)(j & 1), &sh.abort);
+        key += kTileKeys;
+        if (lane < boxes && j + 1 < tiles && key < high) page = table[key / a.pool.page_size];
+        const int first = key0 + j * kTileKeys;
+        const int valid = min(high - first, kTileKeys);
+        const int from = j == 0 ? skipped : 0, to = (valid + w.box - 1) / w.box;
+        const bool ragged = values && (first < low || valid < kTileKeys);
+        const int s = n % kChSlots;
+        if (n >= kChSlots) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&sh.empty[s], (uint32_t)((n / kChSlots - 1) & 1),
+                                                 &sh.abort));
           if (!ok) break;
-          tmem_fence_after();
-          values(i, nv % kChSlots, 0, j > 0);
-          ok = mbar_wait(&sh.p_full[i][1], (uint32_t)(j & 1), &sh.abort);
-          if (!ok) break;
-          tmem_fence_after();
-          values(i, nv % kChSlots, 1, true);
-          if (i == halves - 1) mma_commit(&sh.empty[nv % kChSlots]);
-          if (j + 1 < tiles) scores(i, nk % kChSlots);
         }
-        if (ok && j + 1 < tiles) mma_commit(&sh.empty[nk % kChSlots]);
+        uint64_t* bar = ragged ? &sh.ragged : &sh.full[s];
+        if (elect_one()) mbar_arrive_expect(bar, (uint32_t)(to - from) * box_bytes * 2);
+        uint32_t dst = ring + s * kChTileBytes + from * box_bytes;
+        int row = (first + from * w.box) % a.pool.page_size;  // of the next box in its page
+        for (int x = from; x < to; x += 4) {  // four boxes a turn: their pages at once
+          int px[4];
+#pragma unroll
+          for (int y = 0; y < 4; ++y) px[y] = __shfl_sync(0xffffffffu, p, x + y);
+          int rx[4];
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            rx[y] = row;
+            row += w.box;
+            if (row == a.pool.page_size) row = 0;
+          }
+          if (elect_one()) {
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+              if (x + y < to) {
+                tma_load_4d(map, dst + y * box_bytes, bar, 0, rx[y], g, px[y]);
+                tma_load_4d(map, dst + kChHalfTile + y * box_bytes, bar, 64, rx[y], g, px[y]);
+              }
+          }
+          dst += 4 * box_bytes;
+        }
+        if (ragged) {
+          // V rows that no row sees: what they hold (NaN included) must not meet a
+          // weight of zero
+          ok = __all_sync(0xffffffffu, mbar_wait(bar, done_ragged & 1, &sh.abort));
+          if (!ok) break;
+          ++done_ragged;
+          char* tile = smem + (2 + s) * kChTileBytes;
+          for (int i = lane; i < kTileKeys * 16; i += 32) {
+            const int r = i >> 4;
+            if (first + r < low || r >= valid)
+              reinterpret_cast<uint4*>(tile + ((i >> 3) & 1) * kChHalfTile + r * 128)[i & 7] =
+                  make_uint4(0u, 0u, 0u, 0u);
+          }
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.full[s]);
+        }
       }
-      if (!sh.abort) {
-        mma_commit(&sh.o_full);
-      } else {
+      if (!ok || sh.abort) {
+        // give up: wait (with the same limit) for the copies in flight
         volatile int never = 0;
-        mma_commit(&sh.drain);
-        mbar_wait(&sh.drain, 0, &never);
+        mbar_wait(&sh.q_full, 0, &never);
+        for (int i = max(0, n - kChSlots); i < n; ++i)
+          mbar_wait(&sh.full[i % kChSlots], (uint32_t)((i / kChSlots) & 1), &never);
+      }
+    } else if (warp == kChMmaWarp) {
+      // ---- products, all issued by one thread
+      if (tiles > 0 && elect_one()) {
+        constexpr uint32_t desc_s = product_desc(Pack16<T>::kBf16, kTileKeys, false);
+        constexpr uint32_t desc_o = product_desc(Pack16<T>::kBf16, kHeadDim, true);
+        // S of half i from Q_i and the K tile in ring slot s
+        auto scores = [&](int i, int s) {
+          const uint32_t qa = q_at + i * kChTileBytes, ka = ring + s * kChTileBytes;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const uint32_t off = (k >> 2) * kChHalfTile + (k & 3) * 32;
+            mma_smem(tmem + i * 128, operand_desc(qa + off, 16, 1024),
+                     operand_desc(ka + off, 16, 1024), desc_s, k > 0);
+          }
+          mma_commit(&sh.s_full[i]);
+        };
+        auto values = [&](int i, int s, int part, bool add) {
+          const uint32_t va = ring + s * kChTileBytes;
+#pragma unroll
+          for (int k = part * 4; k < part * 4 + 4; ++k)
+            mma_tmem(tmem + 256 + i * 128, tmem + i * 128 + k * 8,
+                     operand_desc(va + k * 2048, kChHalfTile, 1024), desc_o, add || k > 0);
+        };
+        auto wait_slot = [&](int n) {
+          return mbar_wait(&sh.full[n % kChSlots], (uint32_t)((n / kChSlots) & 1), &sh.abort);
+        };
+        bool ok = mbar_wait(&sh.q_full, 0, &sh.abort) && wait_slot(0);
+        if (ok) {
+          tmem_fence_after();
+          for (int i = 0; i < halves; ++i) scores(i, 0);
+          mma_commit(&sh.empty[0]);
+        }
+        for (int j = 0; j < tiles && ok; ++j) {
+          const int nv = 2 * j + 1, nk = 2 * j + 2;
+          if (!wait_slot(nv)) break;
+          if (j + 1 < tiles && !wait_slot(nk)) break;
+          for (int i = 0; i < halves; ++i) {
+            ok = mbar_wait(&sh.p_full[i][0], (uint32_t)(j & 1), &sh.abort);
+            if (!ok) break;
+            tmem_fence_after();
+            values(i, nv % kChSlots, 0, j > 0);
+            ok = mbar_wait(&sh.p_full[i][1], (uint32_t)(j & 1), &sh.abort);
+            if (!ok) break;
+            tmem_fence_after();
+            values(i, nv % kChSlots, 1, true);
+            if (i == halves - 1) mma_commit(&sh.empty[nv % kChSlots]);
+            if (j + 1 < tiles) scores(i, nk % kChSlots);
+          }
+          if (ok && j + 1 < tiles) mma_commit(&sh.empty[nk % kChSlots]);
+        }
+        if (!sh.abort) {
+          mma_commit(&sh.o_full);
+        } else {
+          volatile int never = 0;
+          mma_commit(&sh.drain);
+          mbar_wait(&sh.drain, 0, &never);
+        }
       }
     }
-  }
   } else {
     grow_registers<kChRowRegs>();
     // ---- weights: a thread per row
@@ -551,7 +551,8 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
       // finite, its own scores are to blame.
       float odd0, odd1;
       unpair(odd2, odd0, odd1);
-      const unsigned again = __ballot_sync(0xffffffffu, live && odd0 + odd1 != 0.f && fabsf(l) < CUDART_INF_F);
+      const unsigned again = __ballot_sync(
+          0xffffffffu, live && odd0 + odd1 != 0.f && fabsf(l) < CUDART_INF_F);
       if (lane == 0) sh.bad[warp] = again;
     }
     softmax_sync();
