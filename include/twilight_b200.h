@@ -558,14 +558,15 @@ int tw_paged_write(const tw_paged_pool* pool, const void* k, int64_t k_token_str
  * tokens: rows of q and out, at least cu_q[B] (which may be less: padding).
  * max_q_len: an upper bound of the requests' new tokens (it chooses the
  * kernels); a longer request sets *error_flag to TW_ERR_BAD_ARG and its rows
- * are not computed.  max_kv_len: the longest kv_lens, which sizes launch and workspace;
- * with longer ones the results are the same, later.  A page id outside the pool sets TW_ERR_INVALID_INDEX and
- * is not read (its keys count as zero rows), and so does a kv_len beyond the
- * table (which is cut).  workspace: >= tw_paged_attention_workspace_size(...)
- * bytes, 16-byte aligned, no initial content; calls that share one must not
- * overlap.  out_dtype: the pool's dtype or TW_F32.  lse, error_flag may be
- * NULL.  page_size a multiple of 8, q_heads / kv_heads <= 64; q and out
- * 16-byte aligned, their strides multiples of 8 elements. */
+ * are not computed.  max_kv_len: the longest kv_lens, which sizes launch and
+ * workspace; with longer ones the results are the same, later.  A page id
+ * outside the pool sets TW_ERR_INVALID_INDEX and is not read (its keys count
+ * as zero rows), and so does a kv_len beyond the table (which is cut).
+ * workspace: >= tw_paged_attention_workspace_size(...) bytes, 16-byte aligned,
+ * no initial content; calls that share one must not overlap.  out_dtype: the
+ * pool's dtype or TW_F32.  lse, error_flag may be NULL.  page_size a multiple
+ * of 8, q_heads / kv_heads <= 64; q and out 16-byte aligned, their strides
+ * multiples of 8 elements. */
 typedef struct tw_paged_attention_args {
   tw_paged_pool pool;
   const void* q;
