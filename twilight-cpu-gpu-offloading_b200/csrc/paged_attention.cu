@@ -17,22 +17,16 @@ constexpr int kMergeAhead = 10;  // ranges that a warp reads before it knows the
 // Bound: latency; 32 rows of 37 ranges cost about 3 us after the token kernel, 1.6 us
 // less than with loads that wait for the maximum and 5 us less than with one warp a
 // row.
-//
-// Every CTA waits for the kernel before it, also one without work: what follows in
-// the stream takes the end of this kernel for the end of that one.
-__device__ __forceinline__ void merge_nothing() {
-  pdl_wait();
-  pdl_launch_dependents();
-}
-
 template <typename Out, bool kFew>
 __global__ void __launch_bounds__(kMergeWarps * 32)
 paged_merge_kernel(const __grid_constant__ PagedWork w) {
   const tw_paged_attention_args& a = w.a;
   const PagedSplit& sp = kFew ? w.few : w.many;
   constexpr int kWarps = kFew ? kMergeWarps : 1;  // of a row
-  // The lengths are older than the kernel before this one, which waited for what
-  // wrote them; the partial results are not.
+  // Every CTA waits, also one without work: what follows in the stream takes the end
+  // of this kernel for the end of the one before it.
+  pdl_wait();
+  pdl_launch_dependents();
   const int lane = threadIdx.x & 31, warp = kFew ? threadIdx.x >> 5 : 0;
   const int64_t row = kFew ? blockIdx.x
                            : (int64_t)blockIdx.x * kMergeWarps + (threadIdx.x >> 5);
@@ -44,7 +38,7 @@ paged_merge_kernel(const __grid_constant__ PagedWork w) {
     const int unit = (int)(row / w.few_rows);
     const int b = unit / a.pool.kv_heads;
     rq = paged_request(a, b);
-    if (rq.n > w.few_tokens || r >= rq.n * w.group) return merge_nothing();
+    if (rq.n > w.few_tokens || r >= rq.n * w.group) return;
     t = rq.first + r / w.group;
     h = (unit - b * a.pool.kv_heads) * w.group + r % w.group;
     keys = paged_keys(a, rq, 0, rq.n);
@@ -52,16 +46,14 @@ paged_merge_kernel(const __grid_constant__ PagedWork w) {
     t = (int)(row / a.q_heads);
     h = (int)(row - (int64_t)t * a.q_heads);
     const int b = t < a.tokens ? first_above(a.cu_q + 1, a.requests, t) : a.requests;
-    if (b >= a.requests) return merge_nothing();
+    if (b >= a.requests) return;
     rq = paged_request(a, b);
-    if (rq.n <= w.few_tokens || rq.n > a.max_q_len) return merge_nothing();
+    if (rq.n <= w.few_tokens || rq.n > a.max_q_len) return;
     const int tokens = paged_chunk_tokens(w.group);
     const int begin = (t - rq.first) / tokens * tokens;
     keys = paged_keys(a, rq, begin, min(rq.n - begin, tokens));
   }
   const int parts = paged_range(sp, keys.low, keys.high, 0).parts;
-  pdl_wait();
-  pdl_launch_dependents();
   if (parts == 1) return;  // the range wrote the result itself
   const float* lse = sp.part_lse + row * sp.splits;
   const float* po = sp.part_o + row * sp.splits * kHeadDim + lane * 4;
@@ -283,9 +275,6 @@ extern "C" int tw_paged_attention(const tw_paged_attention_args* args, void* str
   if (st == TW_OK) st = encode_rows_map(&maps.v, a.pool.dtype, 4, a.pool.v_pages, dims, strides, box);
   if (st != TW_OK) return st;
   cudaStream_t s = (cudaStream_t)stream;
-  // The token kernel of a mixed call takes the SMs that the chunk kernel leaves idle
-  // at its end: 16 requests, 10 of them single tokens: 78 -> 63 us.
-  w.beside = w.many.splits > 0;
   if (w.many.splits > 0) st = launch_paged_chunk(w, maps, s);
   if (st == TW_OK && w.few.splits > 0) st = launch_paged_token(w, maps, s);
   if (st == TW_OK && w.few.splits > 1) st = launch_merge<true>(w, plan.few_rows, s);

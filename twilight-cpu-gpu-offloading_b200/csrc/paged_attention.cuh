@@ -29,7 +29,6 @@ struct PagedWork {
   int few_tokens;    // requests with at most this many new tokens: token kernel (0: none)
   int few_rows;      // few_tokens * group
   int box;           // token rows of one TMA box
-  int beside;        // the token kernel runs beside the chunk kernel of the call
   PagedSplit few;    // rows: (request * kv_heads + head) * few_rows + row
   PagedSplit many;   // rows: token * q_heads + head
 };

@@ -116,17 +116,14 @@ paged_token_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
     prefetch_map(&maps.k);
     prefetch_map(&maps.v);
   }
-  // Beside the chunk kernel of the same call there is nothing to wait for: it has
-  // waited for what came before, and none of its CTAs is still to start.  One CTA
-  // ends after it, so that what follows in the stream takes the end of this kernel
-  // for the end of both.
-  if (!w.beside) pdl_wait();
+  // also in a mixed call, whose chunk kernel has waited for the lengths, the table, Q,
+  // K and V already: only a grid's own wait makes what came before visible to it
+  pdl_wait();
   pdl_launch_dependents();
 
   // the first CTAs, which are done at once
   if (blockIdx.x < kPadCtas) {
     paged_clear_padding<Out>(a, blockIdx.x);
-    if (w.beside && blockIdx.x == 0) pdl_wait();
     return;
   }
   const int64_t cta = blockIdx.x - kPadCtas;
