@@ -3,12 +3,52 @@ its buffers do not hold."""
 
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
 from test_paged_gpu import Batch, D
 
 pytestmark = pytest.mark.gpu
+
+
+def alike(a, b):
+    """The same bits (NaN included)."""
+    return torch.equal(a.view(torch.int32), b.view(torch.int32))
+
+
+# ---------------------------------------------------------- the same bits --
+
+@pytest.mark.parametrize("heads", [(8, 2), (6, 2), (14, 2), (5, 1)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_bits_do_not_depend_on_rows_after_the_request(tw, cuda, heads, dtype):
+    b = Batch(cuda, [50], [700], q_heads=heads[0], kv_heads=heads[1], page=16, dtype=dtype)
+    first = None
+    for fill in (0.0, math.nan, math.inf, 1e4):
+        after = torch.full((77, heads[0], D), fill, dtype=dtype, device=cuda)
+        out, lse, error = b.run(tw, q=torch.cat((b.q, after)), out_dtype=torch.float32)
+        assert error == 0
+        if first is None:
+            first = out[:50].clone(), lse[:50].clone()
+        assert alike(out[:50], first[0]) and alike(lse[:50], first[1]), fill
+
+
+@pytest.mark.parametrize("heads", [(6, 2), (14, 2), (5, 1), (24, 8)])
+def test_bits_do_not_depend_on_the_calls_before(tw, cuda, heads):
+    """What earlier kernels left in shared memory stays out of the arithmetic."""
+    b = Batch(cuda, [300], [900], q_heads=heads[0], kv_heads=heads[1], page=16,
+              dtype=torch.bfloat16)
+    filler = Batch(cuda, [2048], [2048], q_heads=32, kv_heads=8, page=64, dtype=torch.bfloat16)
+    first = None
+    for fill in (0.0, math.nan, math.inf, 3e38):
+        filler.q.fill_(fill)
+        filler.run(tw)
+        out, lse, error = b.run(tw, out_dtype=torch.float32)
+        assert error == 0
+        if first is None:
+            first = out.clone(), lse.clone()
+        assert alike(out, first[0]) and alike(lse, first[1]), fill
 
 
 # ------------------------------------------------------- workspace and order --

@@ -464,7 +464,10 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
             }
           }
         };
-        if (__all_sync(0xffffffffu, !edge && fabsf(m) < CUDART_INF_F))
+        // Rows that are not live have no say: theirs are another request's or padding
+        // rows of q, or (groups that do not divide 128) what an earlier kernel left in
+        // shared memory, and a result's bits must not depend on those.
+        if (__all_sync(0xffffffffu, !edge && (!live || fabsf(m) < CUDART_INF_F)))
           weights(std::true_type{});
         else
           weights(std::false_type{});
