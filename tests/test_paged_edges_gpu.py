@@ -51,6 +51,82 @@ def test_bits_do_not_depend_on_the_calls_before(tw, cuda, heads):
         assert alike(out, first[0]) and alike(lse, first[1]), fill
 
 
+# -------------------------------------------------- values not finite in V --
+
+def spoil(b, request, keys, value, dims=slice(5, 7)):
+    page = b.v_pages.shape[2]
+    for j in keys:
+        b.v_pages[b.table[request, j // page].long(), :, j % page, dims] = value
+
+
+def device_ms(call):
+    call()
+    best = math.inf
+    for _ in range(3):
+        begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        begin.record()
+        call()
+        end.record()
+        end.synchronize()
+        best = min(best, begin.elapsed_time(end))
+    return best
+
+
+@pytest.mark.parametrize("new,kv,window", [([256], [3000], 0), ([3, 1], [3000, 40], 0),
+                                           ([256], [3000], 1500)])
+@pytest.mark.parametrize("where", ["seen by all", "seen by some", "both", "everywhere"])
+def test_values_not_finite_cost_little(tw, cuda, new, kv, window, where):
+    """A call whose V holds NaN takes about as long as a clean one: at most ten times (rows
+    of the few keys in question are looked at once more), not a pass per row."""
+    b = Batch(cuda, new, kv, q_heads=8, kv_heads=2, page=16, dtype=torch.bfloat16)
+    call = lambda: b.run(tw, window=window)  # noqa: E731
+    clean = device_ms(call)
+    early, late = kv[0] - new[0] - 9, kv[0] - 1
+    spoil(b, 0, {"seen by all": [early], "seen by some": [late], "both": [early, late],
+                 "everywhere": range(kv[0])}[where], math.nan)
+    assert device_ms(call) < 10 * clean + 0.05
+    out, lse, error = b.run(tw, window=window)
+    assert error == 0
+    b.check(out, lse, window=window)
+
+
+@pytest.mark.parametrize("heads", [(8, 2), (6, 2), (2, 2), (64, 1)])
+@pytest.mark.parametrize("window", [0, 1, 20, 150])
+@pytest.mark.parametrize("new,kv", [([100, 3, 1], [190, 64, 120]), ([4], [4]), ([2, 4], [900, 5]),
+                                    ([290], [1600])])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_infinities_and_nan_reach_the_rows_that_see_them(tw, cuda, heads, window, new, kv, dtype):
+    """Signed infinities and NaN in some dimensions of V, seen by some rows of a request and
+    hidden from others: each result is what the sum over the visible keys gives."""
+    b = Batch(cuda, new, kv, q_heads=heads[0], kv_heads=heads[1], page=16, dtype=dtype, seed=7)
+    marks = []
+    for r, (n, m) in enumerate(zip(new, kv)):
+        for at, value, dim in ((m - 1, math.inf, 3), (m - n // 2 - 1, -math.inf, 3),
+                               (m - n, math.nan, 64), (max(0, m - n - 5), -math.inf, 127),
+                               (max(0, m - n - window), math.inf, 40), (m - 2, math.nan, 0)):
+            if at >= 0:
+                spoil(b, r, [at], value, dim)
+                marks.append((r, at, value, dim))
+    out, lse, error = b.run(tw, window=window, out_dtype=torch.float32)
+    assert error == 0
+    b.check(out, lse, window=window)
+    # which of them: with weights above zero the sum is the first infinity, NaN, or
+    # NaN where both signs meet
+    for r, (n, m) in enumerate(zip(new, kv)):
+        first = int(b.cu[r])
+        for i in range(n):
+            p = m - n + i
+            want = {}
+            held = {(at, dim): value for q, at, value, dim in marks if q == r}  # the last one put
+            for (at, dim), value in held.items():
+                if at <= p and (not window or at > p - window):
+                    want[dim] = want.get(dim, 0.0) + value
+            for dim, value in want.items():
+                got = out[first + i, :, dim]
+                same = torch.isnan(got) if math.isnan(value) else got == value
+                assert bool(same.all()), (r, i, dim, value)
+
+
 # ------------------------------------------------------- workspace and order --
 
 def test_inputs_that_the_kernel_before_writes(tw, cuda):

@@ -1,5 +1,5 @@
 // What the kernels of the paged attention share: a call's work, a request's
-// rows and keys, the split of the keys, and the one-row form.
+// rows and keys, the split of the keys, and values that are not finite.
 #pragma once
 
 #include <math_constants.h>
@@ -90,50 +90,39 @@ __device__ __forceinline__ PagedKeys paged_keys(const tw_paged_attention_args& a
   return {paged_low(a, max(p, 0)), max(p + n, 0)};
 }
 
-// Softmax-weighted sum of V over the keys [low, high) for one row, by a warp:
-// lane l holds dimensions 4l .. 4l + 3.  One pass with the running maximum m
-// (in log2 units) and sum l.
-struct PagedRow {
-  float acc[4];
-  float m, l;
-};
+// The infinities and NaN of a pair of 16-bit values (exponent all ones): bit 15, bit 31.
 template <typename T>
-__device__ __forceinline__ PagedRow paged_one_row(const PagedWork& w, int b, int t, int h, int low,
-                                               int high) {
-  const tw_paged_attention_args& a = w.a;
-  const int lane = threadIdx.x & 31;
-  const T* q = (const T*)a.q + (int64_t)t * a.q_token_stride + (int64_t)h * a.q_head_stride;
-  const int32_t* table = a.block_table + (int64_t)b * a.table_stride;
-  const int64_t head = (int64_t)(h / w.group) * a.pool.head_stride;
-  PagedRow r = {{0.f, 0.f, 0.f, 0.f}, -CUDART_INF_F, 0.f};
-  float x[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] = to_f32<T>(q[lane * 4 + i]);
-  for (int j = low; j < high; ++j) {
-    const int i = j / a.pool.page_size;
-    const int page = table[i];
-    const bool ok = page >= 0 && page < a.pool.num_pages;
-    const int64_t at = (int64_t)page * a.pool.page_stride + head +
-                       (int64_t)(j - i * a.pool.page_size) * a.pool.token_stride + lane * 4;
-    float s = 0.f, v[4];
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      s = fmaf(x[c], ok ? to_f32<T>(((const T*)a.pool.k_pages)[at + c]) : 0.f, s);
-      v[c] = ok ? to_f32<T>(((const T*)a.pool.v_pages)[at + c]) : 0.f;
-    }
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-    s *= w.scale_log2;
-    const float m_new = fmaxf(r.m, s);
-    const float m_use = m_new == -CUDART_INF_F ? 0.f : m_new;
-    const float keep = ex2(r.m - m_use);
-    const float e = ex2(s - m_use);
-    r.m = m_new;
-    r.l = fmaf(r.l, keep, e);
-#pragma unroll
-    for (int c = 0; c < 4; ++c) r.acc[c] = fmaf(r.acc[c], keep, e * v[c]);
-  }
-  return r;
+__device__ __forceinline__ uint32_t odd_halves(uint32_t two);
+template <>
+__device__ __forceinline__ uint32_t odd_halves<__half>(uint32_t two) {
+  return ((two & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
+}
+template <>
+__device__ __forceinline__ uint32_t odd_halves<__nv_bfloat16>(uint32_t two) {
+  return ((two & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t clear_odd(uint32_t& two) {
+  const uint32_t odd = odd_halves<T>(two);
+  two &= ~((odd >> 15) * 0xffffu);
+  return odd;
+}
+// Clears them in eight values; true: there were some.
+template <typename T>
+__device__ __forceinline__ bool clear_odd(uint4& x) {
+  return (clear_odd<T>(x.x) | clear_odd<T>(x.y) | clear_odd<T>(x.z) | clear_odd<T>(x.w)) != 0;
+}
+
+// V of key k of request b, KV head g; nullptr: its page is none.
+template <typename T>
+__device__ __forceinline__ const T* paged_value(const tw_paged_attention_args& a, int b, int g,
+                                                int k) {
+  const int i = k / a.pool.page_size;
+  const int page = a.block_table[(int64_t)b * a.table_stride + i];
+  if (page < 0 || page >= a.pool.num_pages) return nullptr;
+  return (const T*)a.pool.v_pages + (int64_t)page * a.pool.page_stride +
+         (int64_t)g * a.pool.head_stride +
+         (int64_t)(k - i * a.pool.page_size) * a.pool.token_stride;
 }
 
 // Result of a row whose keys are one range: out and lse.  `n` consecutive

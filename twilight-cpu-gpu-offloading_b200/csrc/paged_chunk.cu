@@ -11,11 +11,12 @@
 // head of the group) pair, so K and V are read once for all heads of the group
 // and each tile of 128 keys once for both halves.  One thread issues all
 // products; two warps copy Q, and K and V tiles by TMA into a ring of five 32 KB
-// slots, page piece by page piece; two warpgroups take one half each, a thread
-// one row: it reads its row of S from tensor memory, writes the weights P back
-// over it in 16 bits, and the product with V takes P from there.  The halves
-// alternate: while one computes its weights, the tensor cores work for the
-// other.  (Two threads a row, or two issuing threads, measured slower.)
+// slots, page piece by page piece; one warp looks over the V tiles that hold keys
+// which some row does not see; two warpgroups take one half each, a thread one
+// row: it reads its row of S from tensor memory, writes the weights P back over it
+// in 16 bits, and the product with V takes P from there.  The halves alternate:
+// while one computes its weights, the tensor cores work for the other.  (Two
+// threads a row, or two issuing threads, measured slower.)
 //
 // Measured: 4096 tokens over a 32k context, 64 / 8 heads: 3.56 ms, 1.16
 // PFLOP/s, at the board's power limit (1.5 to 1.6 GHz); 2048 tokens, 32 / 8
@@ -30,8 +31,8 @@ namespace tw {
 
 constexpr int kChRows = 128;                      // rows of a half
 constexpr int kChSoftmax = 256;                   // threads 0..255: the halves' rows
-constexpr int kChMmaWarp = 8, kChKeyWarp = 9, kChValueWarp = 10;
-constexpr int kChThreads = 384;                   // one warp of the third group is idle
+constexpr int kChMmaWarp = 8, kChKeyWarp = 9, kChValueWarp = 10, kChLookWarp = 11;
+constexpr int kChThreads = 384;
 // Registers: the launch gives 168 to each of 384 threads; the warpgroups of the
 // rows take from the third: 216 + 216 + 72 = 3 * 168.
 constexpr int kChRowRegs = 216, kChIssueRegs = 72;
@@ -50,12 +51,22 @@ template <> struct Pack16<__half> {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
   }
+  static __device__ __forceinline__ uint32_t add_zero_times(uint32_t two, uint32_t sum) {
+    uint32_t r;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(two), "r"(0u), "r"(sum));
+    return r;
+  }
 };
 template <> struct Pack16<__nv_bfloat16> {
   static constexpr bool kBf16 = true;
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ uint32_t add_zero_times(uint32_t two, uint32_t sum) {
+    uint32_t r;
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(two), "r"(0u), "r"(sum));
+    return r;
   }
 };
 
@@ -64,8 +75,12 @@ __device__ __forceinline__ uint32_t low_bits(int n) {
   return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1;
 }
 
-__device__ __forceinline__ void softmax_sync() {
-  asm volatile("bar.sync 1, %0;" ::"n"(kChSoftmax) : "memory");
+// The looking warp is done; the rows' threads wait for that.
+__device__ __forceinline__ void looked_arrive() {
+  asm volatile("bar.arrive 1, %0;" ::"n"(kChSoftmax + 32) : "memory");
+}
+__device__ __forceinline__ void looked_wait() {
+  asm volatile("bar.sync 1, %0;" ::"n"(kChSoftmax + 32) : "memory");
 }
 
 // The warp's 32 rows on their way out: 16-byte columns XORed by row % 8.
@@ -98,15 +113,44 @@ __device__ __forceinline__ void write_rows(const char* smem, int warp, int lane,
   }
 }
 
+// Adds the values of `v` that are not finite to a staged row.
+template <typename T, typename Out>
+__device__ __forceinline__ void add_odd_staged(char* smem, int warp, int row, const T* v) {
+  constexpr int kVec = 16 / sizeof(Out);
+  Out* base = reinterpret_cast<Out*>(smem + (warp * 32 + row) * (kHeadDim * (int)sizeof(Out)));
+#pragma unroll 1
+  for (int c = 0; c < kVecPerRow16; ++c) {
+    const uint4 x = reinterpret_cast<const uint4*>(v)[c];
+    if (!(odd_halves<T>(x.x) | odd_halves<T>(x.y) | odd_halves<T>(x.z) | odd_halves<T>(x.w)))
+      continue;
+#pragma unroll 1
+    for (int e = 0; e < 8; ++e) {
+      const int d = c * 8 + e;
+      const float y = to_f32<T>(v[d]);
+      Out* to = base + ((d / kVec) ^ (row & 7)) * kVec + d % kVec;
+      if (!(fabsf(y) < CUDART_INF_F)) *to = from_f32<Out>(to_f32<Out>(*to) + y);
+    }
+  }
+}
+
+// Keys of the CTA that hold a V value that is not finite and that some row does not see,
+// a bit each: [0]: later than the first token, by distance from it; [1]: before the last
+// token's window, by distance from the first key.
+struct ChunkOdd {
+  unsigned bits[2][8];  // at most 255 each: the CTA has at most 256 tokens
+  int any;
+};
+
 struct ChunkShared {
   uint64_t full[kChSlots], empty[kChSlots];
-  uint64_t q_full, ragged;      // Q is there; a tile whose V rows get cleared is there
+  uint64_t loaded[kChSlots];    // a V tile that has to be looked over is there
+  uint64_t q_full;
   uint64_t s_full[2];           // scores of a half
   uint64_t p_full[2][2];        // weights of a half: keys 0..63, 64..127 of the tile
   uint64_t o_full, drain;
   uint32_t tmem;
   volatile int abort;
-  unsigned bad[8];              // rows to be done again, a word per warp
+  ChunkOdd odd;
 };
 
 template <typename T, typename Out>
@@ -127,9 +171,9 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
     for (int i = 0; i < kChSlots; ++i) {
       mbar_init(&sh.full[i], 1);
       mbar_init(&sh.empty[i], 1);
+      mbar_init(&sh.loaded[i], 1);
     }
     mbar_init(&sh.q_full, 1);
-    mbar_init(&sh.ragged, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sh.s_full[i], 1);
       mbar_init(&sh.p_full[i][0], 4);
@@ -140,7 +184,8 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
     sh.abort = 0;
     mbar_init_fence();
   }
-  if (tid < 8) sh.bad[tid] = 0;
+  if (tid < 16) sh.odd.bits[tid >> 3][tid & 7] = 0;
+  if (tid == 16) sh.odd.any = 0;
   pdl_wait();
   pdl_launch_dependents();
 
@@ -193,6 +238,15 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
   const int key0 = low / kTileKeys * kTileKeys;
   const int tiles = high > low ? (high - key0 + kTileKeys - 1) / kTileKeys : 0;
 
+  // Tiles of V with rows that are not of the range, or that not all tokens see.  What
+  // those hold must not meet a weight of zero in the product (0 x NaN, 0 x infinity):
+  // the looking warp clears them and what is not finite in them before it hands a tile
+  // on, and the rows that do see such a value get it added at the end.
+  const int see_last = paged_low(a, max(p_first + here - 1, 0));
+  const auto look = [&](int first) {
+    return first < max(low, see_last) || first + kTileKeys > min(high, p_first + 1);
+  };
+
   // Boxes wholly before the first visible key are not read: a page that slid out
   // of the window may be gone.
   const int skipped = (low - key0) / w.box;
@@ -226,7 +280,7 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
       __syncwarp();
       const uint32_t box_bytes = (uint32_t)w.box * 128;  // of 64 dimensions
       int n = values ? 1 : 0;
-      uint32_t done_ragged = 0;
+      uint32_t looked = 0, turn = 0;  // a bit per slot: its last tile gets looked over; phase
       bool ok = true;
       for (int j = 0; j < tiles; ++j, n += 2) {
         int p = page;
@@ -240,14 +294,16 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
         const int first = key0 + j * kTileKeys;
         const int valid = min(high - first, kTileKeys);
         const int from = j == 0 ? skipped : 0, to = (valid + w.box - 1) / w.box;
-        const bool ragged = values && (first < low || valid < kTileKeys);
         const int s = n % kChSlots;
         if (n >= kChSlots) {
           ok = __all_sync(0xffffffffu, mbar_wait(&sh.empty[s], (uint32_t)((n / kChSlots - 1) & 1),
                                                  &sh.abort));
           if (!ok) break;
         }
-        uint64_t* bar = ragged ? &sh.ragged : &sh.full[s];
+        const bool passes = values && look(first);  // by the looking warp
+        uint64_t* bar = passes ? &sh.loaded[s] : &sh.full[s];
+        looked = passes ? looked | 1u << s : looked & ~(1u << s);
+        turn ^= (uint32_t)passes << s;
         if (elect_one()) mbar_arrive_expect(bar, (uint32_t)(to - from) * box_bytes * 2);
         uint32_t dst = ring + s * kChTileBytes + from * box_bytes;
         int row = (first + from * w.box) % a.pool.page_size;  // of the next box in its page
@@ -272,31 +328,77 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
           }
           dst += 4 * box_bytes;
         }
-        if (ragged) {
-          // V rows that no row sees: what they hold (NaN included) must not meet a
-          // weight of zero
-          ok = __all_sync(0xffffffffu, mbar_wait(bar, done_ragged & 1, &sh.abort));
-          if (!ok) break;
-          ++done_ragged;
-          char* tile = smem + (2 + s) * kChTileBytes;
-          for (int i = lane; i < kTileKeys * 16; i += 32) {
-            const int r = i >> 4;
-            if (first + r < low || r >= valid)
-              reinterpret_cast<uint4*>(tile + ((i >> 3) & 1) * kChHalfTile + r * 128)[i & 7] =
-                  make_uint4(0u, 0u, 0u, 0u);
-          }
-          fence_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sh.full[s]);
-        }
       }
       if (!ok || sh.abort) {
         // give up: wait (with the same limit) for the copies in flight
         volatile int never = 0;
         mbar_wait(&sh.q_full, 0, &never);
-        for (int i = max(0, n - kChSlots); i < n; ++i)
-          mbar_wait(&sh.full[i % kChSlots], (uint32_t)((i / kChSlots) & 1), &never);
+        for (int i = n - 2; i >= 0 && i > n - 2 - kChSlots; i -= 2) {
+          const int s = i % kChSlots;
+          if (looked >> s & 1)
+            mbar_wait(&sh.loaded[s], ~(turn >> s) & 1, &never);
+          else
+            mbar_wait(&sh.full[s], (uint32_t)((i / kChSlots) & 1), &never);
+        }
       }
+    } else if (warp == kChLookWarp) {
+      // ---- V tiles with keys that some row does not see
+      uint32_t turn = 0;
+      bool ok = true;
+      for (int j = 0; j < tiles && ok; ++j) {
+        const int first = key0 + j * kTileKeys;
+        if (!look(first)) continue;
+        const int s = (2 * j + 1) % kChSlots;
+        ok = __all_sync(0xffffffffu, mbar_wait(&sh.loaded[s], turn >> s & 1, &sh.abort));
+        if (!ok) break;
+        turn ^= 1u << s;
+        char* tile = smem + (2 + s) * kChTileBytes;
+        auto at = [&](int i) {  // 16-byte vector i of the tile's rows
+          return reinterpret_cast<uint4*>(tile + ((i >> 3) & 1) * kChHalfTile + (i >> 4) * 128) +
+                 (i & 7);
+        };
+        // rows [0, c0) and [c1, 128) are not of the range; [c0, before): not all tokens'
+        // windows begin so early; [after, c1): later than the first token
+        const int c0 = max(low - first, 0), c1 = min(high - first, kTileKeys);
+        const int after = min(max(p_first + 1 - first, c0), c1);
+        const int before = min(max(see_last - first, c0), after);
+        for (int i = lane; i < c0 * 16; i += 32) *at(i) = make_uint4(0u, 0u, 0u, 0u);
+        for (int i = c1 * 16 + lane; i < kTileKeys * 16; i += 32)
+          *at(i) = make_uint4(0u, 0u, 0u, 0u);
+        // is there any (0 times it is NaN): eight vectors on their way at a time
+        uint32_t sum[4] = {0u, 0u, 0u, 0u};
+        auto find = [&](int from, int to) {
+#pragma unroll 8
+          for (int i = from * 16 + lane; i < to * 16; i += 32) {
+            const uint4 x = *at(i);
+            sum[0] = Pack16<T>::add_zero_times(x.x, sum[0]);
+            sum[1] = Pack16<T>::add_zero_times(x.y, sum[1]);
+            sum[2] = Pack16<T>::add_zero_times(x.z, sum[2]);
+            sum[3] = Pack16<T>::add_zero_times(x.w, sum[3]);
+          }
+        };
+        find(c0, before);
+        find(after, c1);
+        const uint32_t odd = odd_halves<T>(sum[0]) | odd_halves<T>(sum[1]) |
+                             odd_halves<T>(sum[2]) | odd_halves<T>(sum[3]);
+        if (__any_sync(0xffffffffu, odd != 0)) {
+          if (lane == 0) sh.odd.any = 1;
+          for (int i = c0 * 16 + lane; i < c1 * 16; i += 32) {
+            const int r = i >> 4, k = first + r;
+            uint4 x = *at(i);
+            if ((r < before || r >= after) && clear_odd<T>(x)) {
+              *at(i) = x;
+              const int kind = r >= after ? 0 : 1;
+              const int bit = kind == 0 ? k - p_first : k - keys.low;
+              atomicOr(&sh.odd.bits[kind][bit >> 5], 1u << (bit & 31));
+            }
+          }
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.full[s]);
+      }
+      looked_arrive();
     } else if (warp == kChMmaWarp) {
       // ---- products, all issued by one thread
       if (tiles > 0 && elect_one()) {
@@ -487,11 +589,11 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const float lse2 = l == 0.f ? -CUDART_INF_F : m + log2f(l);
     const bool joined = range.parts == 1;
+    looked_wait();
     if (i < halves) {
       // Rows go through shared memory (Q and the ring are free: all products are
       // done), so that a warp writes whole rows to memory: a thread writing its own
       // row 16 bytes at a time took 3.5 us for the 256 rows.
-      uint64_t odd2 = 0ull;
       const uint64_t inv2 = pair(inv, inv);
       {
         float o[4][32];
@@ -511,13 +613,26 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
 #pragma unroll
           for (int x = 0; x < 32; x += 2) {
             const uint64_t y = mul2(pair(o[c][x], o[c][x + 1]), inv2);
-            odd2 = fma2(y, 0ull, odd2);  // NaN when one is not finite
             unpair(y, o[c][x], o[c][x + 1]);
           }
           if (joined)
             stage_row<Out>(smem, warp, lane, c, o[c]);
           else
             stage_row<float>(smem, warp, lane, c, o[c]);
+        }
+      }
+      // what was cleared before the product and this row does see
+#pragma unroll 1
+      for (int x = 0; sh.odd.any && x < 16; ++x) {
+#pragma unroll 1
+        for (unsigned bits = sh.odd.bits[x >> 3][x & 7]; bits; bits &= bits - 1) {
+          const int k = (x & 7) * 32 + __ffs(bits) - 1 + (x < 8 ? p_first : keys.low);
+          const T* v = live && k >= see && k <= p ? paged_value<T>(a, b, g, k) : nullptr;
+          if (!v) continue;
+          if (joined)
+            add_odd_staged<T, Out>(smem, warp, lane, v);
+          else
+            add_odd_staged<T, float>(smem, warp, lane, v);
         }
       }
       if (live) {
@@ -548,38 +663,6 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
           return y < rows ? to + ((int64_t)k * a.q_heads + (y - k * R)) * w.many.splits * kHeadDim
                           : nullptr;
         });
-      }
-      // A row that is not finite may owe it to a V row that another token sees
-      // and this one does not (weight 0 times infinity or NaN).  If its sum is not
-      // finite, its own scores are to blame.
-      float odd0, odd1;
-      unpair(odd2, odd0, odd1);
-      const unsigned again = __ballot_sync(
-          0xffffffffu, live && odd0 + odd1 != 0.f && fabsf(l) < CUDART_INF_F);
-      if (lane == 0) sh.bad[warp] = again;
-    }
-    softmax_sync();
-    const bool redo = __any_sync(0xffffffffu, sh.bad[lane & 7] != 0);
-#pragma unroll 1
-    for (int x = 0; redo && x < 8; ++x) {
-      for (unsigned bad = sh.bad[x]; bad; bad &= bad - 1) {
-        const int rr = (x & 3) * 32 + __ffs(bad) - 1;
-        if (rr % 8 != warp) continue;
-        const int tt = (x >> 2) * half_tokens + rr / R;
-        const int hh = g * R + rr % R;
-        const int pp = p_first + tt;
-        const PagedRow y = paged_one_row<T>(w, b, rq.first + begin + tt, hh,
-                                            max(range.begin, paged_low(a, pp)),
-                                            min(range.end, pp + 1));
-        float o[4];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) o[c] = y.l == 0.f ? 0.f : y.acc[c] / y.l;
-        const float z = y.l == 0.f ? -CUDART_INF_F : y.m + log2f(y.l);
-        if (joined)
-          paged_store_row<Out, 4>(a, rq.first + begin + tt, hh, lane * 4, o, z);
-        else
-          paged_store_part<4>(w.many, (int64_t)(rq.first + begin + tt) * a.q_heads + hh, split,
-                              lane * 4, o, z);
       }
     }
     tmem_fence_before();

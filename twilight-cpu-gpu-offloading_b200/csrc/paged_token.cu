@@ -99,7 +99,10 @@ paged_token_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
   __shared__ uint64_t s_full[kTokStages], s_empty[kTokStages];
   __shared__ float s_m[kTokWarps][kTokRows], s_l[kTokWarps][kTokRows];
   __shared__ volatile int s_abort;
-  __shared__ int s_bad_rows;
+  // Keys with a V value that is not finite and that some row does not see, a bit each:
+  // 1..15: later than the first token by so much; 16..30: before the last token's
+  // window, so much (less 16) after the first key.
+  __shared__ unsigned s_odd;
   const tw_paged_attention_args& a = w.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int kv_heads = a.pool.kv_heads;
@@ -109,7 +112,7 @@ paged_token_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
       mbar_init(&s_empty[i], kTokWarps);
     }
     s_abort = 0;
-    s_bad_rows = 0;
+    s_odd = 0;
     mbar_init_fence();
   }
   if (tid == kTokWarps * 32) {
@@ -284,8 +287,9 @@ paged_token_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
 #pragma unroll
         for (int c = 0; c < 4; ++c) s[n][c] *= w.scale_log2;
       if (edge) {
-        // hide what a row does not see, and clear V rows that none sees: what
-        // they hold (NaN included) must not meet a weight of zero
+        // hide what a row does not see, and clear V rows that none sees and what is not
+        // finite in those that some row does not see: that must not meet a weight of
+        // zero (the rows that do see such a value get it added at the end)
         const int first = key0 + c0;
 #pragma unroll
         for (int n = 0; n < 2; ++n)
@@ -297,11 +301,22 @@ paged_token_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
           }
         const int row = lane >> 1;
         const int j = key0 + row;
+        uint4* z = reinterpret_cast<uint4*>(smem + base + 2 * kTokHalf + (lane & 1) * kTokHalf +
+                                            (wrow + row) * 128);
         if (j < low || j >= range.end) {
-          char* z = smem + base + 2 * kTokHalf + (lane & 1) * kTokHalf + (wrow + row) * 128;
 #pragma unroll
-          for (int c = 0; c < 8; ++c)
-            reinterpret_cast<uint4*>(z)[c] = make_uint4(0u, 0u, 0u, 0u);
+          for (int c = 0; c < 8; ++c) z[c] = make_uint4(0u, 0u, 0u, 0u);
+        } else if (j >= all_high || j < all_low) {
+          bool odd = false;
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            uint4 x = z[c];
+            if (clear_odd<T>(x)) {
+              z[c] = x;
+              odd = true;
+            }
+          }
+          if (odd) atomicOr(&s_odd, 1u << (j >= all_high ? j - all_high + 1 : j - keys.low + 16));
         }
         __syncwarp();
       }
@@ -398,11 +413,20 @@ paged_token_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
       for (int c = 0; c < 16; ++c) o[c] = fmaf(x[c], f, o[c]);
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    float odd = 0.f;
 #pragma unroll
-    for (int c = 0; c < 16; ++c) {
-      o[c] *= inv;
-      odd = fmaf(o[c], 0.f, odd);  // NaN when one is not finite
+    for (int c = 0; c < 16; ++c) o[c] *= inv;
+    // what was cleared before the product and this row does see
+#pragma unroll 1
+    for (unsigned bits = r < rows ? s_odd : 0u; bits; bits &= bits - 1) {
+      const int bit = __ffs(bits) - 1, p = rq.kv - rq.n + r / R;
+      const int k = bit < 16 ? all_high + bit - 1 : keys.low + bit - 16;
+      const T* v = k >= paged_low(a, p) && k <= p ? paged_value<T>(a, b, g, k) : nullptr;
+      if (!v) continue;
+#pragma unroll
+      for (int c = 0; c < 16; ++c) {
+        const float y = to_f32<T>(v[d0 + c]);
+        if (!(fabsf(y) < CUDART_INF_F)) o[c] += y;
+      }
     }
     const float lse2 = l == 0.f ? -CUDART_INF_F : m + log2f(l);
     if (r < rows) {
@@ -411,29 +435,7 @@ paged_token_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
         paged_store_row<Out, 16>(a, t, h, d0, o, lse2);
       else
         paged_store_part<16>(w.few, (int64_t)unit * w.few_rows + r, split, d0, o, lse2);
-      // A row that is not finite may owe it to a V row that another token sees
-      // and this one does not (weight 0 times infinity or NaN).  If its sum is not
-      // finite, its own scores are to blame.
-      if (rq.n > 1 && odd != 0.f && fabsf(l) < CUDART_INF_F) atomicOr(&s_bad_rows, 1 << r);
     }
-  }
-  if (rq.n == 1) return;
-  consumer_sync();
-  for (int bad = s_bad_rows; bad; bad &= bad - 1) {
-    const int r = __ffs(bad) - 1;
-    if (r % kTokWarps != warp) continue;
-    const int t = rq.first + r / R, h = g * R + r % R;
-    const int p = rq.kv - rq.n + r / R;
-    const PagedRow x = paged_one_row<T>(w, b, t, h, max(range.begin, paged_low(a, p)),
-                                        min(range.end, p + 1));
-    float o[4];
-#pragma unroll
-    for (int c = 0; c < 4; ++c) o[c] = x.l == 0.f ? 0.f : x.acc[c] / x.l;
-    const float lse2 = x.l == 0.f ? -CUDART_INF_F : x.m + log2f(x.l);
-    if (joined)
-      paged_store_row<Out, 4>(a, t, h, lane * 4, o, lse2);
-    else
-      paged_store_part<4>(w.few, (int64_t)unit * w.few_rows + r, split, lane * 4, o, lse2);
   }
 }
 
