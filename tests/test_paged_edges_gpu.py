@@ -8,6 +8,7 @@ import math
 import pytest
 import torch
 
+import paged_ref
 from test_paged_gpu import Batch, D
 
 pytestmark = pytest.mark.gpu
@@ -125,6 +126,41 @@ def test_infinities_and_nan_reach_the_rows_that_see_them(tw, cuda, heads, window
                 got = out[first + i, :, dim]
                 same = torch.isnan(got) if math.isnan(value) else got == value
                 assert bool(same.all()), (r, i, dim, value)
+
+
+# ------------------------------------------------------------ small weights --
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("size", [1e3, 1e5, 1e6, 1e7, 4e7, 1e8, 3e9, 1e30])
+@pytest.mark.parametrize("new,kv", [([1], [200]), ([70], [400]), ([300], [2000])])
+def test_large_scores(tw, cuda, dtype, size, new, kv):
+    """Scores so large that their rounding moves an exponent by more than the types' range:
+    a row whose largest score stands out by more than the scores' own error is the V row of
+    that key, and any other row lies among the values it sees."""
+    b = Batch(cuda, new, kv, q_heads=4, kv_heads=1, page=16, dtype=dtype)
+    out, lse, error = b.run(tw, softmax_scale=size)
+    assert error == 0
+    assert bool(torch.isfinite(out).all()) and bool(torch.isfinite(lse).all())
+    j = torch.arange(kv[0], device=cuda)
+    rows = [pages[b.table[0, j // 16].long(), 0, j % 16].double() for pages in (b.k_pages,
+                                                                                b.v_pages)]
+    score = torch.einsum("thd,kd->thk", b.q.double(), rows[0]) * size
+    seen = j <= kv[0] - new[0] + torch.arange(new[0], device=cuda)[:, None]
+    score.masked_fill_(~seen[:, None], -math.inf)
+    best = score.topk(2, -1)
+    # as in paged_ref: a score's error in 32 bits, twice, and 40 for the others to vanish
+    slack = 260 * 2.0 ** -24 * (b.q.double().abs() @ rows[0].abs().T).amax(-1) * size + 40
+    alone = best.values[..., 0] - best.values[..., 1] > slack
+    assert size < 1e6 or bool(alone.any())
+    want = rows[1][best.indices[..., 0]]
+    unit = paged_ref.UNIT[dtype]
+    assert bool(((out.double() - want).abs() <= 2 * unit * want.abs())[alone].all())
+    low, high = rows[1].amin(0), rows[1].amax(0)
+    assert bool((out.double() >= low - 2 * unit * low.abs()).all())
+    assert bool((out.double() <= high + 2 * unit * high.abs()).all())
+    # lse: the largest score, but for log(keys)
+    top = best.values[..., 0]
+    assert bool(((lse.double() - top).abs() <= math.log(kv[0]) + slack).all())
 
 
 # ------------------------------------------------------- workspace and order --

@@ -42,6 +42,7 @@ constexpr int kChSlots = 5;
 constexpr int kChSmem = (2 + kChSlots) * kChTileBytes + 1024;
 constexpr int kChColumns = 512;                   // S0, S1, O0, O1: 128 columns each
 constexpr float kChMoveBy = 8.0f;                 // log2 units
+constexpr float kChNear = 1048576.0f;             // log2 units
 constexpr int kChFma = 8;                         // one pair in this many on the FMA pipe
 
 template <typename T> struct Pack16;
@@ -473,7 +474,10 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
     const int all_low = paged_low(a, p_half + half_tokens - 1), all_high = p_half + 1;
     const uint32_t my = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t s_col = my + i * 128, o_col = my + 256 + i * 128;
-    float m = -CUDART_INF_F;
+    // the reference scaled, as a score, and the score beyond which it moves (rounded
+    // down: no weight exceeds 2^kChMoveBy)
+    float m = -CUDART_INF_F, top_s = -CUDART_INF_F, move_at = -CUDART_INF_F;
+    const float move_by = fminf(kChMoveBy / w.scale_log2, 1e38f);
     uint64_t l2[2] = {0ull, 0ull};
     const uint64_t scale2 = pair(w.scale_log2, w.scale_log2);
     bool ok = true;
@@ -508,11 +512,17 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
           for (int x = 3; x < 31; x += 2) top[c] = max3(top[c], s[c][x], s[c][x + 1]);
           top[c] = max3(top[c], s[c][31], s[c][31]);
         }
-        const float t = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * w.scale_log2;
-        const bool move = t > m + kChMoveBy;
+        const float t = max3(max3(top[0], top[1], top[2]), top[3], top[3]);
+        const bool move = t > move_at;
         if (__any_sync(0xffffffffu, move)) {
-          const float f = move ? ex2(m - t) : 1.f;
-          if (move) m = t;
+          float f = 1.f;
+          if (move) {
+            const float m_new = t * w.scale_log2;
+            f = ex2(fabsf(m_new) < kChNear ? m - m_new : (top_s - t) * w.scale_log2);
+            m = m_new;
+            top_s = t;
+            move_at = __fadd_rd(t, move_by);
+          }
           const uint64_t f2 = pair(f, f);
           l2[0] = mul2(l2[0], f2);
           l2[1] = mul2(l2[1], f2);
@@ -529,7 +539,12 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
             }
           }
         }
-        const float u = m == -CUDART_INF_F ? 0.f : -m;
+        // An exponent is s * scale - m in one operation, whose product is not rounded, but
+        // m is: by up to 2^-5 while |m| < 2^20, the same for all weights, which the sum
+        // makes good.  Beyond that it would carry them out of range; there it is
+        // (s - top_s) * scale.
+        const bool near = fabsf(m) < kChNear;
+        const float u = near ? -m : 0.f;
         const uint64_t u2 = pair(u, u);
         // Weights, rounded to the 16-bit type for the product (the sum l keeps them
         // in 32 bits): half a unit each, of either sign.  Where all is finite, one
@@ -540,12 +555,16 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
           // products before it branches and spills them
           uint64_t by = scale2;
           asm volatile("// form %1" : "+l"(by) : "n"((int)decltype(plain)::value));
+          const float less = near || m == -CUDART_INF_F ? 0.f : -top_s;
+          const uint64_t less2 = pair(less, less);
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             uint32_t packed[16];
 #pragma unroll
             for (int x = 0; x < 32; x += 2) {
-              const uint64_t y = fma2(pair(s[c][x], s[c][x + 1]), by, u2);
+              uint64_t y = pair(s[c][x], s[c][x + 1]);
+              if (!decltype(plain)::value) y = add2(y, less2);
+              y = fma2(y, by, u2);
               float e0, e1;
               if (decltype(plain)::value && (x >> 1) % kChFma == kChFma - 1) {
                 ex2_fma(y, e0, e1);
@@ -569,7 +588,7 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
         // Rows that are not live have no say: theirs are another request's or padding
         // rows of q, or (groups that do not divide 128) what an earlier kernel left in
         // shared memory, and a result's bits must not depend on those.
-        if (__all_sync(0xffffffffu, !edge && (!live || fabsf(m) < CUDART_INF_F)))
+        if (__all_sync(0xffffffffu, !edge && (!live || near)))
           weights(std::true_type{});
         else
           weights(std::false_type{});
