@@ -9,7 +9,7 @@ import pytest
 import torch
 
 import paged_ref
-from test_paged_gpu import Batch, D
+from test_paged_gpu import Batch, D, put
 
 pytestmark = pytest.mark.gpu
 
@@ -129,6 +129,37 @@ def test_infinities_and_nan_reach_the_rows_that_see_them(tw, cuda, heads, window
 
 
 # ------------------------------------------------------------ small weights --
+
+@pytest.mark.parametrize("new,kv", [([1], [256]), ([64], [760])])
+def test_small_fp16_weights_count(tw, cuda, new, kv):
+    """One key of weight 1, all others of 2^-25.5 with large values: the others' share of the
+    sum is not lost in the 16-bit weights.
+
+    Tolerance: weights and V in 16 bits, 32-bit sums.  Weights are rounded relative to
+    themselves (unit 2^-11) or, below the smallest normal value, by at most 2^-25 of the
+    type, which is 2^-32 of the row's largest where that one stands at 2^7."""
+    n = kv[0]
+    b = Batch(cuda, new, kv, q_heads=4, kv_heads=1, page=16, dtype=torch.float16)
+    rows = torch.zeros(n, 1, D, dtype=torch.float16, device=cuda)
+    rows[0, 0, 0] = 17.6875  # 25.52 in log2 units
+    put(b.k_pages, b.table[0], rows)
+    values = torch.full((n, 1, D), 30000.0, dtype=torch.float16, device=cuda)
+    values[0] = 1.0
+    put(b.v_pages, b.table[0], values)
+    b.q.zero_()
+    b.q[..., 0] = 1.0
+    out, lse, error = b.run(tw, softmax_scale=1.0, out_dtype=torch.float32)
+    assert error == 0
+    seen = (n - new[0] + 1 + torch.arange(new[0], device=cuda)).double()[:, None, None]
+    small = math.exp(-17.6875)
+    total = 1.0 + (seen - 1) * small
+    ref = (1.0 + (seen - 1) * small * 30000.0) / total
+    tol = 2.0 ** -11 * ref + (seen - 1) * 2.0 ** -32 * 30000.0 + 2.0 ** -18 * ref
+    assert bool(((out.double() - ref).abs() <= tol).all()), \
+        float(((out.double() - ref).abs() / tol).max())
+    ref_lse = 17.6875 + torch.log(total[..., 0])
+    assert bool(((lse.double() - ref_lse).abs() <= 2.0 ** -18).all())
+
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("size", [1e3, 1e5, 1e6, 1e7, 4e7, 1e8, 3e9, 1e30])

@@ -106,7 +106,7 @@ paged_merge_kernel(const __grid_constant__ PagedWork w) {
   const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
   for (int c = 0; c < 4; ++c) o[c] *= inv;
-  paged_store_row<Out, 4>(a, t, h, lane * 4, o, l == 0.f ? -CUDART_INF_F : m + log2f(l));
+  paged_store_row<Out, 4>(a, t, h, lane * 4, o, paged_lse(m, l));
 }
 
 template <bool kFew>

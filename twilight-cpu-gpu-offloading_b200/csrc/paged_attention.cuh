@@ -90,6 +90,13 @@ __device__ __forceinline__ PagedKeys paged_keys(const tw_paged_attention_args& a
   return {paged_low(a, max(p, 0)), max(p + n, 0)};
 }
 
+// Weights stand this much above the reference, in log2 units: an fp16 weight below 2^-25
+// is nothing in the product with V, and 1e5 keys of little weight each can be a share of
+// a result.  The reference moves when a score exceeds it by 8, so weights stay within
+// 2^15, and what is lost lies below 2^-32 of the row's largest.  (bf16 has the range.)
+template <typename T> constexpr float kLift = 0.f;
+template <> constexpr float kLift<__half> = 7.f;
+
 // The infinities and NaN of a pair of 16-bit values (exponent all ones): bit 15, bit 31.
 template <typename T>
 __device__ __forceinline__ uint32_t odd_halves(uint32_t two);
@@ -125,11 +132,21 @@ __device__ __forceinline__ const T* paged_value(const tw_paged_attention_args& a
          (int64_t)(k - i * a.pool.page_size) * a.pool.token_stride;
 }
 
+// Log-sum-exp of a row with reference m (log2 units) and sum l, and the same in log2
+// units for the merge.  Rounded once: log2(l) is small beside m, and m + log2(l) times ln 2
+// would round at m's size twice.
+__device__ __forceinline__ float paged_lse(float m, float l) {
+  return l == 0.f ? -CUDART_INF_F : fmaf(m, kLn2, log2f(l) * kLn2);
+}
+__device__ __forceinline__ float paged_lse2(float m, float l) {
+  return l == 0.f ? -CUDART_INF_F : m + log2f(l);
+}
+
 // Result of a row whose keys are one range: out and lse.  `n` consecutive
 // dimensions from d0; lse by the thread with d0 == 0.
 template <typename Out, int N>
 __device__ __forceinline__ void paged_store_row(const tw_paged_attention_args& a, int t, int h,
-                                                int d0, const float (&o)[N], float lse2) {
+                                                int d0, const float (&o)[N], float lse) {
   Out* out = (Out*)a.out + (int64_t)t * a.out_token_stride + (int64_t)h * a.out_head_stride + d0;
   constexpr int kVec = 16 / sizeof(Out);
   if constexpr (N % kVec == 0) {
@@ -145,7 +162,7 @@ __device__ __forceinline__ void paged_store_row(const tw_paged_attention_args& a
     for (int c = 0; c < N; ++c) out[c] = from_f32<Out>(o[c]);
   }
   if (a.lse && d0 == 0)
-    a.lse[(int64_t)t * a.q_heads + h] = lse2 * kLn2;
+    a.lse[(int64_t)t * a.q_heads + h] = lse;
 }
 
 // A range's result of a row, for the merge.

@@ -474,11 +474,11 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
     const int all_low = paged_low(a, p_half + half_tokens - 1), all_high = p_half + 1;
     const uint32_t my = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t s_col = my + i * 128, o_col = my + 256 + i * 128;
-    // the reference scaled, as a score, and the score beyond which it moves (rounded
-    // down: no weight exceeds 2^kChMoveBy)
+    // the reference scaled (and lowered: weights stand above it), as a score, and the
+    // score beyond which it moves (rounded down: no weight exceeds 2^(kChMoveBy + kLift))
     float m = -CUDART_INF_F, top_s = -CUDART_INF_F, move_at = -CUDART_INF_F;
     const float move_by = fminf(kChMoveBy / w.scale_log2, 1e38f);
-    uint64_t l2[2] = {0ull, 0ull};
+    float l = 0.f;
     const uint64_t scale2 = pair(w.scale_log2, w.scale_log2);
     bool ok = true;
     if (i < halves) {
@@ -517,15 +517,13 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
         if (__any_sync(0xffffffffu, move)) {
           float f = 1.f;
           if (move) {
-            const float m_new = t * w.scale_log2;
+            const float m_new = t * w.scale_log2 - kLift<T>;
             f = ex2(fabsf(m_new) < kChNear ? m - m_new : (top_s - t) * w.scale_log2);
             m = m_new;
             top_s = t;
             move_at = __fadd_rd(t, move_by);
           }
-          const uint64_t f2 = pair(f, f);
-          l2[0] = mul2(l2[0], f2);
-          l2[1] = mul2(l2[1], f2);
+          l *= f;
           if (j > 0) {  // O of the tiles so far is complete: S of this one came after it
 #pragma unroll 1
             for (int c = 0; c < 4; ++c) {
@@ -544,13 +542,16 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
         // makes good.  Beyond that it would carry them out of range; there it is
         // (s - top_s) * scale.
         const bool near = fabsf(m) < kChNear;
-        const float u = near ? -m : 0.f;
+        const float u = near ? -m : kLift<T>;
         const uint64_t u2 = pair(u, u);
         // Weights, rounded to the 16-bit type for the product (the sum l keeps them
         // in 32 bits): half a unit each, of either sign.  Where all is finite, one
         // pair in kChFma goes through the FMA pipe instead of the special-function
         // unit, which alone would take as long as the products.
+        // A tile's weights are summed by themselves first: beside a large l each alone
+        // could be less than its last bit.
         auto weights = [&](auto plain) {
+          uint64_t l2[2] = {0ull, 0ull};
           // an operand of its own for each form, or the compiler computes all 64
           // products before it branches and spills them
           uint64_t by = scale2;
@@ -584,6 +585,9 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
               if (lane == 0) mbar_arrive(&sh.p_full[i][c >> 1]);
             }
           }
+          float x0, x1;
+          unpair(add2(l2[0], l2[1]), x0, x1);
+          l += x0 + x1;
         };
         // Rows that are not live have no say: theirs are another request's or padding
         // rows of q, or (groups that do not divide 128) what an earlier kernel left in
@@ -594,19 +598,12 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
           weights(std::false_type{});
       }
     }
-    float l = 0.f;
-    {
-      float x0, x1;
-      unpair(add2(l2[0], l2[1]), x0, x1);
-      l = x0 + x1;
-    }
     if (tiles > 0 && ok)
       ok = __all_sync(0xffffffffu, mbar_wait(&sh.o_full, 0, &sh.abort));
     tmem_fence_after();
     if (!ok && lane == 0) raise_error(a.error_flag, TW_ERR_TIMEOUT);
     const int t = rq.first + begin + ti, h = g * R + head;
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    const float lse2 = l == 0.f ? -CUDART_INF_F : m + log2f(l);
     const bool joined = range.parts == 1;
     looked_wait();
     if (i < halves) {
@@ -657,9 +654,9 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
       if (live) {
         const int64_t row = (int64_t)t * a.q_heads + h;
         if (!joined)
-          w.many.part_lse[row * w.many.splits + split] = lse2;
+          w.many.part_lse[row * w.many.splits + split] = paged_lse2(m, l);
         else if (a.lse)
-          a.lse[row] = lse2 * kLn2;
+          a.lse[row] = paged_lse(m, l);
       }
       __syncwarp();
       // row x of the warp: token y / R by multiplication (exact for y < 128, R <= 64)

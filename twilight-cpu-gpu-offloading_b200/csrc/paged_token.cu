@@ -3,10 +3,10 @@
 //
 // Mathematics: for each range of keys, one pass with a running reference m and
 // sum l per row: p_j = 2^(s_j - m), l += p_j, O += p_j v_j, both scaled when m
-// moves.  m moves only when a score exceeds it by more than 8 (p stays below
-// 2^8, far from overflow in either 16-bit type), so the accumulators are
-// rarely rescaled.  A range leaves O / l and m + log2 l; ranges are joined by
-// weights 2^(lse_s - max).
+// moves.  m moves only when a score exceeds it by more than 8 (fp16: 15, see kLift;
+// p stays below 2^8 or 2^15, far from overflow), so the accumulators are rarely
+// rescaled.  A range leaves O / l and m + log2 l; ranges are joined by weights
+// 2^(lse_s - max).
 //
 // Bound: HBM, every K / V row of the visible keys read once per KV head
 // (512 bytes a key); the 16-row products are 4 % of what the tensor cores
@@ -327,9 +327,9 @@ paged_token_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
         t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, off));
         t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, off));
       }
-      const bool move0 = t0 > m0 + kMoveBy, move1 = t1 > m1 + kMoveBy;
+      const bool move0 = t0 - m0 > kMoveBy + kLift<T>, move1 = t1 - m1 > kMoveBy + kLift<T>;
       if (__any_sync(0xffffffffu, move0 || move1)) {
-        const float n0 = move0 ? t0 : m0, n1 = move1 ? t1 : m1;
+        const float n0 = move0 ? t0 - kLift<T> : m0, n1 = move1 ? t1 - kLift<T> : m1;
         // an unmoved reference keeps its sums (-inf - -inf would be NaN)
         const float f0 = move0 ? ex2(m0 - n0) : 1.f, f1 = move1 ? ex2(m1 - n1) : 1.f;
         m0 = n0;
@@ -428,13 +428,13 @@ paged_token_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
         if (!(fabsf(y) < CUDART_INF_F)) o[c] += y;
       }
     }
-    const float lse2 = l == 0.f ? -CUDART_INF_F : m + log2f(l);
     if (r < rows) {
       const int t = rq.first + r / R, h = g * R + r % R;
       if (joined)
-        paged_store_row<Out, 16>(a, t, h, d0, o, lse2);
+        paged_store_row<Out, 16>(a, t, h, d0, o, paged_lse(m, l));
       else
-        paged_store_part<16>(w.few, (int64_t)unit * w.few_rows + r, split, d0, o, lse2);
+        paged_store_part<16>(w.few, (int64_t)unit * w.few_rows + r, split, d0, o,
+                             paged_lse2(m, l));
     }
   }
 }
