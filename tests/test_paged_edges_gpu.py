@@ -194,6 +194,21 @@ def test_large_scores(tw, cuda, dtype, size, new, kv):
     assert bool(((lse.double() - top).abs() <= math.log(kv[0]) + slack).all())
 
 
+# ------------------------------------------------------------------ lengths --
+
+def test_a_bound_of_no_tokens_is_kept_to(tw, cuda):
+    """max_q_len 0: a request with one token is longer than that."""
+    b = Batch(cuda, [1, 0], [20, 30], q_heads=8, kv_heads=2, page=16, dtype=torch.float16)
+    out = torch.full_like(b.q, 5.0)
+    _, _, error = b.run(tw, max_q_len=0, out=out)
+    assert error == tw._lib.TW_ERR_BAD_ARG
+    assert bool((out == 5.0).all())
+    b = Batch(cuda, [0, 0], [20, 30], q_heads=8, kv_heads=2, page=16, dtype=torch.float16)
+    b.q = torch.zeros(3, 8, D, dtype=torch.float16, device=cuda)  # padding only
+    out, _, error = b.run(tw)
+    assert error == 0 and bool((out == 0).all())
+
+
 # ------------------------------------------------------- workspace and order --
 
 def test_inputs_that_the_kernel_before_writes(tw, cuda):

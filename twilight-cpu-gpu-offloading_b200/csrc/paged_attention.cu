@@ -38,7 +38,7 @@ paged_merge_kernel(const __grid_constant__ PagedWork w) {
     const int unit = (int)(row / w.few_rows);
     const int b = unit / a.pool.kv_heads;
     rq = paged_request(a, b);
-    if (rq.n > w.few_tokens || r >= rq.n * w.group) return;
+    if (rq.n > w.few_tokens || rq.n > a.max_q_len || r >= rq.n * w.group) return;
     t = rq.first + r / w.group;
     h = (unit - b * a.pool.kv_heads) * w.group + r % w.group;
     keys = paged_keys(a, rq, 0, rq.n);

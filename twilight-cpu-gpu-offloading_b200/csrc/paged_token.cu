@@ -146,7 +146,7 @@ paged_token_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
     page = table[guess / a.pool.page_size];
   const PagedRequest rq = paged_request(a, b);
   if (rq.n == 0) return;
-  if (rq.n > w.few_tokens) {
+  if (rq.n > w.few_tokens || rq.n > a.max_q_len) {
     if (rq.n > a.max_q_len && tid == 0) raise_error(a.error_flag, TW_ERR_BAD_ARG);
     return;
   }
