@@ -555,7 +555,9 @@ int tw_paged_write(const tw_paged_pool* pool, const void* k, int64_t k_token_str
  * with KV head h / (q_heads / kv_heads).  A row that sees no key, and every
  * row at or past cu_q[B], gets out 0 and lse -inf.  What rows the mask hides
  * hold (NaN included) does not reach a result.
- * tokens: rows of q and out, at least cu_q[B] (which may be less: padding).
+ * tokens: rows of q and out, at least cu_q[B] (which may be less: padding); a
+ * request with rows beyond sets *error_flag to TW_ERR_BAD_ARG and is not
+ * computed.
  * max_q_len: an upper bound of the requests' new tokens (it chooses the
  * kernels); a longer request sets *error_flag to TW_ERR_BAD_ARG and its rows
  * are not computed.  max_kv_len: the longest kv_lens, which sizes launch and

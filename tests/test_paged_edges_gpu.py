@@ -209,6 +209,23 @@ def test_a_bound_of_no_tokens_is_kept_to(tw, cuda):
     assert error == 0 and bool((out == 0).all())
 
 
+@pytest.mark.parametrize("new,kv", [([1, 1, 3], [40, 50, 60]), ([40, 70], [50, 200]),
+                                    ([40, 5], [50, 200]), ([300], [300])])
+def test_requests_beyond_the_rows_of_q_are_flagged(tw, cuda, new, kv):
+    """cu_q promises more rows than q has: that request is not computed (its positions would
+    be wrong), the others are."""
+    b = Batch(cuda, new, kv, q_heads=8, kv_heads=2, page=16, dtype=torch.bfloat16)
+    good, _, error = b.run(tw)
+    assert error == 0
+    q = b.q[:-2].contiguous()
+    out = torch.full_like(q, 5.0)
+    _, _, error = b.run(tw, q=q, out=out)
+    assert error == tw._lib.TW_ERR_BAD_ARG
+    first = int(b.cu[-2])
+    assert torch.equal(out[:first], good[:first])
+    assert bool((out[first:] == 5.0).all())
+
+
 # ------------------------------------------------------- workspace and order --
 
 def test_inputs_that_the_kernel_before_writes(tw, cuda):

@@ -38,13 +38,17 @@ struct PagedRequest {
   int kv;        // its tokens, the new ones included
 };
 
-// Lengths as the call gives them, cut to what its buffers hold.
+// Lengths as the call gives them, cut to what its buffers hold.  A request with rows that
+// q does not have is not computed: cut, the rest would be at wrong positions.
 __device__ __forceinline__ PagedRequest paged_request(const tw_paged_attention_args& a, int b) {
   PagedRequest r;
-  r.first = min(max(a.cu_q[b], 0), a.tokens);
-  r.n = max(min(a.cu_q[b + 1], a.tokens) - r.first, 0);
+  const int first = a.cu_q[b], end = a.cu_q[b + 1];
+  r.kv = max(a.kv_lens[b], 0);  // read with them, before a branch
+  const bool held = first >= 0 && end <= a.tokens;
+  if (!held) raise_error(a.error_flag, TW_ERR_BAD_ARG);
+  r.first = min(max(first, 0), a.tokens);
+  r.n = held ? max(end - first, 0) : 0;
   const long long cap = (long long)a.table_width * a.pool.page_size;
-  r.kv = max(a.kv_lens[b], 0);
   if (r.kv > cap) {
     r.kv = (int)cap;
     raise_error(a.error_flag, TW_ERR_INVALID_INDEX);
