@@ -228,6 +228,40 @@ def test_requests_beyond_the_rows_of_q_are_flagged(tw, cuda, new, kv):
 
 # ------------------------------------------------------- workspace and order --
 
+def test_one_long_request_among_many(tw, cuda):
+    """More partial results than the workspace's bound holds at the usual range length."""
+    requests = 700
+    new, kv = [1] * requests, [3] * requests
+    new[1], kv[350], new[350] = 4, 70000, 4
+    kv[1] = 4
+    b = Batch(cuda, new, kv, q_heads=32, kv_heads=8, page=128, dtype=torch.bfloat16)
+    torch.cuda.synchronize()
+    out, lse, error = b.run(tw)
+    assert error == 0
+    first = int(b.cu[350])
+    for r, at, n in ((350, first, 4), (1, int(b.cu[1]), 4), (699, int(b.cu[699]), 1)):
+        o, z, tol, tol_z = paged_ref.attention(
+            b.q[at:at + n], b.k_pages, b.v_pages, b.table[r:r + 1],
+            torch.tensor([0, n], device=cuda), b.kv[r:r + 1])
+        assert bool(((out[at:at + n].double() - o).abs() <= tol).all())
+        assert bool(((lse[at:at + n].double() - z).abs() <= tol_z).all())
+
+
+def test_large_workspaces_go_back_to_the_allocator(tw, cuda):
+    """What a call takes for itself and is large is not kept once it has been used."""
+    b = Batch(cuda, [4] + [1] * 299, [70000] + [3] * 299, q_heads=32, kv_heads=8, page=128,
+              dtype=torch.bfloat16)
+    need = tw.ops.paged_attention_workspace_bytes(300, b.q.shape[0], 32, 8, 4, 70000)
+    assert need > 1 << 27
+    out = torch.empty_like(b.q)
+    call = lambda: tw.ops.paged_attention(  # noqa: E731
+        b.q, b.k_pages, b.v_pages, b.table, b.cu, b.kv, max_q_len=4, max_kv_len=70000, out=out)
+    before = torch.cuda.memory_allocated()
+    call()
+    torch.cuda.synchronize()
+    assert torch.cuda.memory_allocated() - before < 1 << 27
+
+
 def test_inputs_that_the_kernel_before_writes(tw, cuda):
     """Chunks and single tokens in one call, right behind the kernels that write its rows of
     K and V, its table and its lengths."""

@@ -102,3 +102,19 @@ def test_cpu_tensors_are_refused(tw):
     with pytest.raises(ValueError, match="CUDA"):
         tw.ops.paged_step(one, one, one[None], one, one, page_size=16, kv_lens=one, cu_q=one,
                           slots=one.long(), positions=one, free_count_out=one)
+
+
+@pytest.mark.parametrize("q_heads,kv_heads", [(32, 8), (8, 8), (64, 8), (8, 1), (128, 128)])
+@pytest.mark.parametrize("max_kv", [1, 4097, 131072, 1 << 20, 2 ** 31 - 1])
+def test_workspace_has_a_bound(tw, q_heads, kv_heads, max_kv):
+    """Whatever the requests and their longest: 256 MiB of partial results of requests with
+    few tokens (split only as far as that allows), and of the others at most one of 256 rows
+    for each of two CTAs per SM, 132 numbers a row."""
+    lib = tw.load_library()
+    most = (256 << 20) + 2 * 148 * 256 * 132 * 4
+    for requests in (1, 2, 16, 256, 700, 8192):
+        for tokens in (requests, requests + 3000, 16384):
+            for max_q in (1, 2, 4, 16, 3000):
+                need = lib.tw_paged_attention_workspace_size(requests, tokens, q_heads, kv_heads,
+                                                             max_q, max_kv, 0, 128)
+                assert need <= most, (requests, tokens, max_q, need)

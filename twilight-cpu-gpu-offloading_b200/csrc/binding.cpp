@@ -180,12 +180,15 @@ PyObject* paged_write(PyObject*, PyObject* const* o, Py_ssize_t n) {
 
 // The workspace of calls that brought none, kept per stream: calls on one stream
 // follow one another, and a larger one takes the place of a smaller.  A graph under
-// capture gets its own.
+// capture gets its own, and so does a call that needs much, which takes long enough for
+// the allocator's time not to count: what stays is bounded.
+constexpr size_t kKeptBytes = 32 << 20;
 at::Tensor workspace_for(const at::Tensor& like, int dev, void* stream, size_t bytes) {
   const auto fresh = [&] {
     return at::empty({(int64_t)bytes}, like.options().dtype(at::kByte));
   };
-  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None)
+  if (bytes > kKeptBytes ||
+      c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None)
     return fresh();
   // never destroyed: at exit the allocator may be gone first
   static auto* kept = new std::map<std::pair<int, void*>, at::Tensor>;

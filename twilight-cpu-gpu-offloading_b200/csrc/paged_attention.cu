@@ -134,8 +134,9 @@ static PagedSplit cut(int64_t keys, int64_t chunk) {
   return sp;
 }
 
+constexpr int64_t kRowBytes = (kHeadDim + 4) * sizeof(float);  // of a row's partial result
 static size_t part_bytes(int64_t rows, const PagedSplit& sp) {
-  return sp.splits > 1 ? (size_t)rows * sp.splits * (kHeadDim + 4) * sizeof(float) : 0;
+  return sp.splits > 1 ? (size_t)rows * sp.splits * kRowBytes : 0;
 }
 
 // Ranges of the token kernel.  Its 2 CTAs per SM share the device; one request
@@ -143,12 +144,17 @@ static size_t part_bytes(int64_t rows, const PagedSplit& sp) {
 // (the pipeline's fill and the merge cost about that); many requests are cut
 // into twice the CTAs, because their lengths differ; and no range is longer
 // than 4096 keys, so that one long request among many short ones does not
-// leave the others waiting.
-static PagedSplit split_few(int requests, int kv_heads, int64_t max_keys) {
+// leave the others waiting, unless the partial results, which every request has a
+// place for in each range, would take more than kFewBytes (256 requests with up to 4
+// tokens each, one at 131k: 15 ranges of 8832 keys instead of 32).
+constexpr int64_t kFewBytes = 256 << 20;
+static PagedSplit split_few(int requests, int kv_heads, int rows, int64_t max_keys) {
   const int64_t units = (int64_t)requests * kv_heads;
   const int64_t ctas = 2 * 148 * (requests > 1 ? 2 : 1);
   int64_t chunk = div_up(units * max_keys, ctas);
   chunk = chunk < 256 ? 256 : chunk > 4096 ? 4096 : chunk;
+  const int64_t most = kFewBytes / (units * rows * kRowBytes);
+  if (chunk * most < max_keys) chunk = most > 1 ? div_up(max_keys, most) : max_keys;
   return cut(max_keys, chunk);
 }
 
@@ -192,7 +198,7 @@ static PagedPlan plan_paged(PagedWork& w, int requests, int tokens, int q_heads,
   };
   PagedPlan plan = {};
   if (w.few_tokens > 0) {
-    w.few = split_few(requests, kv_heads, seen(w.few_tokens));
+    w.few = split_few(requests, kv_heads, w.few_rows, seen(w.few_tokens));
     plan.few_rows = (int64_t)requests * kv_heads * w.few_rows;
   }
   if (most > w.few_tokens) {

@@ -465,7 +465,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     longest kv_lens (it sizes the launch).  window > 0: each token sees the last
     `window` positions only.  Returns out [T, q_heads, 128] (q's dtype or
     float32); lse [T, q_heads] fp32 receives the log-sum-exp.  Without a
-    workspace one is taken that is kept for the current stream."""
+    workspace (300 MB at most, see paged_attention_workspace_bytes) one is taken: up
+    to 32 MB is kept for the current stream, more goes back to the allocator."""
     rc = _lib.binding().paged_attention(q, k_pages, v_pages, block_table, cu_q, kv_lens, max_q_len,
                                         max_kv_len, window, softmax_scale, out, out_dtype, lse,
                                         workspace, error_flag)
