@@ -94,6 +94,19 @@ def test_capacity_is_checked_before_anything_changes(tw, cuda):
     cache.synchronize()
 
 
+def test_a_plan_keeps_its_numbers(tw, cuda):
+    """Plans that are held while later steps are planned."""
+    cache = make(tw, cuda)
+    plans, want = [], []
+    for new in ([3, 40], [1, 1, 17], [20, -1, 1], [1, 5, 1, 2], [-1, 1, 0, 30]):
+        plans.append(cache.step(new))
+        want.append(list(cache.lengths))
+    for plan, lengths in zip(plans, want):
+        assert plan.kv_lens.tolist() == lengths
+        assert int(plan.cu_q[-1]) == plan.tokens == plan.slots.numel() == plan.positions.numel()
+    cache.synchronize()
+
+
 def test_refusals(tw, cuda):
     for bad in (dict(page_size=12), dict(head_dim=64), dict(dtype=torch.float32), dict(num_pages=0),
                 dict(device="cpu"), dict(max_requests=9000)):

@@ -29,7 +29,8 @@ from .ops import HEAD_DIM
 
 @dataclass(frozen=True)
 class PagedStep:
-    """What one step() planned; device tensors, rows of the step's tokens in request order."""
+    """What one step() planned; device tensors, rows of the step's tokens in request order.
+    Later steps leave them as they are (the cache's block_table moves on)."""
 
     tokens: int
     cu_q: torch.Tensor        # [requests + 1] int32
@@ -77,8 +78,8 @@ class PagedKVCache:
         i32 = dict(dtype=torch.int32, device=device)
         self.block_table = torch.full((max_requests, width), -1, **i32)
         self._free_pages = torch.arange(num_pages - 1, -1, -1, **i32)
-        # lengths and free count before and after a step, in turn
-        self._lens = [torch.zeros(max_requests, **i32) for _ in range(2)]
+        self._lens = torch.zeros(max_requests, **i32)  # those of the last plan
+        # free count before and after a step, in turn
         self._free_count = [torch.full((1,), num_pages, **i32) for _ in range(2)]
         self._turn = 0
         self._error_flag = torch.zeros(1, **i32)
@@ -113,15 +114,16 @@ class PagedKVCache:
         i32 = dict(dtype=torch.int32, device=self.device)
         before, now = self._turn, self._turn ^ 1
         cu_q = torch.empty(self.max_requests + 1, **i32)
+        kv_lens = torch.empty(self.max_requests, **i32)
         slots = torch.empty(tokens, dtype=torch.int64, device=self.device)
         positions = torch.empty(tokens, **i32)
-        ops.paged_step(self._lens[before], torch.tensor(new, **i32), self.block_table,
+        ops.paged_step(self._lens, torch.tensor(new, **i32), self.block_table,
                        self._free_pages, self._free_count[before], page_size=self.page_size,
-                       kv_lens=self._lens[now], cu_q=cu_q, slots=slots, positions=positions,
+                       kv_lens=kv_lens, cu_q=cu_q, slots=slots, positions=positions,
                        free_count_out=self._free_count[now], error_flag=self._error_flag)
-        self._turn = now
+        self._turn, self._lens = now, kv_lens
         self.lengths, self.free_pages = after, free
-        self._step = PagedStep(tokens, cu_q, self._lens[now], slots, positions,
+        self._step = PagedStep(tokens, cu_q, kv_lens, slots, positions,
                                max(0, *new), max(after))
         return self._step
 
