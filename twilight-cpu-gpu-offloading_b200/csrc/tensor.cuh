@@ -158,8 +158,8 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 
 // 2^x of a pair on the FMA pipe, for x <= 126 (below -126: 2^-126; NaN: NaN): n = x
 // rounded to a whole number by adding 1.5 * 2^23, 2^(x - n) on [-1/2, 1/2] by the
-// polynomial of degree 4 with the smallest largest relative error there (2.6e-6;
-// Remez exchange), times 2^n put together from its bits.
+// polynomial of degree 4 with the smallest largest relative error there (Remez
+// exchange; 2.7e-6 with its roundings), times 2^n put together from its bits.
 __device__ __forceinline__ void ex2_fma(uint64_t x2, float& e0, float& e1) {
   float x0, x1;
   unpair(x2, x0, x1);
