@@ -119,15 +119,16 @@ __global__ void __launch_bounds__(kStepThreads) paged_step_kernel(tw_paged_step_
     return !r.wide && (r.want == 0 || (long long)s_wanted[b] <= top);
   };
 
-  const int step = gridDim.x * kStepThreads;
-  const int first = blockIdx.x * kStepThreads + tid;
-  for (int t = first; t < a.tokens_cap; t += step) {
+  // (unsigned counters: a signed one would overflow past counts near 2^31)
+  const unsigned step = gridDim.x * kStepThreads;
+  const unsigned first = blockIdx.x * kStepThreads + tid;
+  for (unsigned t = first; t < (unsigned)a.tokens_cap; t += step) {
     int64_t slot = -1;
     int position = 0;
-    if (t < total) {
-      const int b = first_above(s_tokens, B, t);
+    if (t < (unsigned)total) {
+      const int b = first_above(s_tokens, B, (int)t);
       const StepRequest r = step_request(a.lens[b], a.new_lens[b], a.page_size, a.table_width);
-      position = r.len + (t - (b > 0 ? s_tokens[b - 1] : 0));
+      position = r.len + ((int)t - (b > 0 ? s_tokens[b - 1] : 0));
       if (served(b, r)) {
         const int i = position / a.page_size;
         const int page = i < r.have
@@ -143,14 +144,14 @@ __global__ void __launch_bounds__(kStepThreads) paged_step_kernel(tw_paged_step_
     a.positions[t] = position;
   }
   // pages returned, at their places on the stack
-  for (int k = first; k < returned; k += step) {
+  for (unsigned k = first; k < (unsigned)returned; k += step) {
     if ((long long)count + k < a.num_pages)
-      a.free_pages[count + k] = stack_page((long long)count + k);
+      a.free_pages[(long long)count + k] = stack_page((long long)count + k);
     else
       raise_error(a.error_flag, TW_ERR_CAPACITY);
   }
   // per request: lengths and the pages it takes
-  for (int b = first; b < B; b += step) {
+  for (unsigned b = first; b < (unsigned)B; b += step) {
     const StepRequest r = step_request(a.lens[b], a.new_lens[b], a.page_size, a.table_width);
     const bool ok = served(b, r);
     if (!ok) raise_error(a.error_flag, TW_ERR_CAPACITY);
@@ -158,11 +159,11 @@ __global__ void __launch_bounds__(kStepThreads) paged_step_kernel(tw_paged_step_
     a.cu_q[b + 1] = s_tokens[b];
   }
   const int wanted = saturate(base.wanted);
-  for (int k = first; k < wanted && (long long)k < top; k += step) {
-    const int b = first_above(s_wanted, B, k);
+  for (unsigned k = first; k < (unsigned)wanted && (long long)k < top; k += step) {
+    const int b = first_above(s_wanted, B, (int)k);
     if ((long long)s_wanted[b] > top) break;  // refused, and so are all after it
     const StepRequest r = step_request(a.lens[b], a.new_lens[b], a.page_size, a.table_width);
-    const int i = r.have + (k - (s_wanted[b] - r.want));
+    const int i = r.have + ((int)k - (s_wanted[b] - r.want));
     a.block_table[(int64_t)b * a.table_stride + i] = stack_page(top - 1 - k);
   }
   if (blockIdx.x == 0 && tid == 0) {
