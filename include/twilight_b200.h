@@ -563,7 +563,7 @@ int tw_paged_write(const tw_paged_pool* pool, const void* k, int64_t k_token_str
  * are not computed.  max_kv_len: the longest kv_lens, which sizes launch and
  * workspace; with longer ones the results are the same, later.  A page id
  * outside the pool sets TW_ERR_INVALID_INDEX and is not read (its keys count
- * as zero rows), and so does a kv_len beyond the table (which is cut).
+ * as zero rows), and so does a kv_len beyond the table or 2^30 (which is cut).
  * workspace: >= tw_paged_attention_workspace_size(...) bytes, 16-byte aligned,
  * no initial content; calls that share one must not overlap.  out_dtype: the
  * pool's dtype or TW_F32.  lse, error_flag may be NULL.  page_size a multiple

@@ -226,6 +226,31 @@ def test_requests_beyond_the_rows_of_q_are_flagged(tw, cuda, new, kv):
     assert bool((out[first:] == 5.0).all())
 
 
+@pytest.mark.parametrize("new", [1, 200])
+def test_lengths_beyond_2_30_are_cut_and_flagged(tw, cuda, new):
+    """Pages may be shared, so that a table can hold more positions than 32 bits count."""
+    page, window = 1 << 20, 100
+    b = Batch(cuda, [new], [1], q_heads=8, kv_heads=1, page=8, dtype=torch.bfloat16)
+    g = torch.Generator(cuda).manual_seed(3)
+    b.k_pages, b.v_pages = (torch.randn(1, 1, page, D, generator=g, device=cuda).to(torch.bfloat16)
+                            for _ in range(2))
+    b.table = torch.zeros(1, 2049, dtype=torch.int32, device=cuda)
+    results = []
+    for length in (1 << 30, (1 << 30) + 1, 2 ** 31 - 1):
+        b.kv.fill_(length)
+        out, lse, error = b.run(tw, window=window, max_kv_len=1 << 30)
+        assert error == (tw._lib.TW_ERR_INVALID_INDEX if length > 1 << 30 else 0)
+        results.append((out, lse))
+    for out, lse in results[1:]:
+        assert torch.equal(out, results[0][0]) and torch.equal(lse, results[0][1])
+    # the same keys in a table of one page
+    b.table, b.max_kv = b.table[:, :1].contiguous(), page
+    b.kv.fill_(page)
+    out, lse, error = b.run(tw, window=window)
+    assert error == 0
+    assert torch.equal(out, results[0][0]) and torch.equal(lse, results[0][1])
+
+
 # ------------------------------------------------------- workspace and order --
 
 def test_one_long_request_among_many(tw, cuda):

@@ -48,7 +48,8 @@ __device__ __forceinline__ PagedRequest paged_request(const tw_paged_attention_a
   if (!held) raise_error(a.error_flag, TW_ERR_BAD_ARG);
   r.first = min(max(first, 0), a.tokens);
   r.n = held ? max(end - first, 0) : 0;
-  const long long cap = (long long)a.table_width * a.pool.page_size;
+  // 2^30: positions are 32-bit, and a tile or range past the last key must be one too
+  const long long cap = min((long long)a.table_width * a.pool.page_size, 1ll << 30);
   if (r.kv > cap) {
     r.kv = (int)cap;
     raise_error(a.error_flag, TW_ERR_INVALID_INDEX);
