@@ -281,8 +281,8 @@ extern "C" int tw_paged_attention(const tw_paged_attention_args* args, void* str
   if (st == TW_OK) st = encode_rows_map(&maps.v, a.pool.dtype, 4, a.pool.v_pages, dims, strides, box);
   if (st != TW_OK) return st;
   cudaStream_t s = (cudaStream_t)stream;
-  if (w.many.splits > 0) st = launch_paged_chunk(w, maps, s);
-  if (st == TW_OK && w.few.splits > 0) st = launch_paged_token(w, maps, s);
+  // a mixed call is one launch too: the chunk kernel takes the token kernel's items
+  st = w.many.splits > 0 ? launch_paged_chunk(w, maps, s) : launch_paged_token(w, maps, s);
   if (st == TW_OK && w.few.splits > 1) st = launch_merge<true>(w, plan.few_rows, s);
   if (st == TW_OK && w.many.splits > 1) st = launch_merge<false>(w, plan.many_rows, s);
   return st;

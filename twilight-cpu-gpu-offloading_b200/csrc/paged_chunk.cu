@@ -22,7 +22,7 @@
 // PFLOP/s, at the board's power limit (1.5 to 1.6 GHz); 2048 tokens, 32 / 8
 // heads: 1.0 ms there, 45 us as a prompt of their own.  The tensor pipe is busy
 // 68 % of a busy SM's cycles; a tile takes 1.8 us, and each CTA 6 us more.
-#include "paged_attention.cuh"
+#include "paged_token.cuh"
 #include "tensor.cuh"
 
 #include <type_traits>
@@ -154,7 +154,9 @@ struct ChunkShared {
   ChunkOdd odd;
 };
 
-template <typename T, typename Out>
+// kMixed: some requests may have few tokens, whose items the grid takes too.  (A kernel of
+// its own: with the items' code in it a call of one short chunk takes 0.3 us longer.)
+template <typename T, typename Out, bool kMixed>
 __global__ void __launch_bounds__(kChThreads, 1)
 paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ PagedMaps maps,
                    const __grid_constant__ CUtensorMap q_map) {
@@ -198,6 +200,18 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
   const int g = (int)(cta / w.many.splits % kv_heads);
   const int slots = a.tokens / tokens + a.requests;
   const int64_t ctas = (int64_t)slots * kv_heads * w.many.splits;
+  if constexpr (kMixed) {
+    if (cta >= ctas + kPadCtas) {  // two items
+      static_assert(kChThreads == 2 * kTokThreads);
+      __shared__ TokShared tok[2];
+      const int half = tid >= kTokThreads, at = tid - half * kTokThreads;
+      const int64_t item = (cta - ctas - kPadCtas) * 2 + half;
+      if (item >= (int64_t)a.requests * kv_heads * w.few.splits) return;
+      if (at == 0) token_init(tok[half]);
+      token_item<T, Out>(w, maps, smem + half * kTokRing, tok[half], item, half, at);
+      return;
+    }
+  }
   if (cta >= ctas) {
     paged_clear_padding<Out>(a, (int)(cta - ctas));
     return;
@@ -691,7 +705,7 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
   }
 }
 
-template <typename T, typename Out>
+template <typename T, typename Out, bool kMixed>
 static int launch_chunk(const PagedWork& w, const PagedMaps& maps, cudaStream_t stream) {
   const int tokens = paged_chunk_tokens(w.group);
   CUtensorMap q_map;
@@ -703,15 +717,21 @@ static int launch_chunk(const PagedWork& w, const PagedMaps& maps, cudaStream_t 
   int rc = encode_rows_map(&q_map, w.a.pool.dtype, 3, w.a.q, dims, strides, box);
   if (rc != TW_OK) return rc;
   static DynSmemOptIn opt_in;
-  const auto kernel = paged_chunk_kernel<T, Out>;
+  const auto kernel = paged_chunk_kernel<T, Out, kMixed>;
   rc = ensure_dyn_smem((const void*)kernel, opt_in, kChSmem);
   if (rc != TW_OK) return rc;
   const int64_t ctas = ((int64_t)w.a.tokens / tokens + w.a.requests) * w.a.pool.kv_heads *
                            w.many.splits +
-                       (w.few_tokens > 0 ? 0 : kPadCtas);
+                       kPadCtas + (paged_token_items(w) + 1) / 2;
   if (ctas > INT32_MAX) return TW_ERR_UNSUPPORTED;
   return launch_pdl(kernel, dim3((unsigned)ctas), dim3(kChThreads), (size_t)kChSmem, stream, w,
                     maps, q_map);
+}
+
+template <typename T, typename Out>
+static int launch_chunk(const PagedWork& w, const PagedMaps& maps, cudaStream_t stream) {
+  return w.few.splits > 0 ? launch_chunk<T, Out, true>(w, maps, stream)
+                          : launch_chunk<T, Out, false>(w, maps, stream);
 }
 
 int launch_paged_chunk(const PagedWork& w, const PagedMaps& maps, cudaStream_t stream) {
