@@ -540,7 +540,9 @@ size_t tw_paged_step_args_size(void);
 
 /* Rows k / v [tokens][kv_heads][D] (element strides given, D contiguous) to
  * their slots of the pool.  Slot -1 is skipped; another slot outside the pool
- * is skipped and sets *error_flag.  Two equal slots leave one of the rows. */
+ * is skipped and sets *error_flag.  Slots other than -1 have to differ: of two
+ * rows with the same one it is not fixed what remains, not even whether K and V
+ * are of one row. */
 int tw_paged_write(const tw_paged_pool* pool, const void* k, int64_t k_token_stride,
                    int64_t k_head_stride, const void* v, int64_t v_token_stride,
                    int64_t v_head_stride, const int64_t* slots, int64_t tokens,

@@ -14,9 +14,9 @@ constexpr int kMergeAhead = 10;  // ranges that a warp reads before it knows the
 // Rows of few-token requests have many ranges: four warps a row take every fourth,
 // so that a row's loads are in flight together; the others get a warp each.  The
 // ranges are added in an order that does not depend on which was ready first.
-// Bound: latency; 32 rows of 37 ranges cost about 3 us after the token kernel, 1.6 us
-// less than with loads that wait for the maximum and 5 us less than with one warp a
-// row.
+// Bound: latency; 32 rows of 37 ranges cost about 4 us after the token kernel (one of
+// them for the lengths, read when that has ended), 1.6 us less than with loads that wait
+// for the maximum and 5 us less than with one warp a row.
 template <typename Out, bool kFew>
 __global__ void __launch_bounds__(kMergeWarps * 32)
 paged_merge_kernel(const __grid_constant__ PagedWork w) {
@@ -161,14 +161,14 @@ static PagedSplit split_few(int requests, int kv_heads, int rows, int64_t max_ke
 // Ranges of the chunk kernel: one, unless its CTAs would leave SMs idle.  A single
 // request's CTAs are known: its keys are cut so that about all SMs get one, into
 // ranges of 768 keys or more (a range costs 6 us besides its tiles, and the merge;
-// 560 tokens at 3k, 14 heads: 36 us in three ranges, 29 us in four).
-// Of several requests, those with few tokens get no CTA here, but how many that are
+// 511 tokens at 3k, 14 heads: 47 us whole, 37, 31, 28 us in two, three, four ranges).
+// Of several requests, those with few tokens get no chunk CTA, but how many that are
 // the host does not know: the keys are cut for twice the SMs, into ranges of 1536
-// keys or more (13 requests of 5k to 14k, five of them with up to 8 tokens: 173 us
-// whole, 105 us in two ranges).  More does not pay where all have a CTA (6 requests
-// at 5k to 7k, 64 heads, 160 CTAs: 201 us whole, 259 us in three ranges), nor does
-// evening out the last wave of a single request (256 CTAs at 32k: 1.00 ms whole,
-// 1.13 ms in four): the partial results' traffic costs more.
+// keys or more (13 requests of 5k to 14k, five of them with up to 8 tokens: 184 us
+// whole, 112 us in two ranges, 103 us in three).  Cutting does not pay where all have a
+// CTA (6 requests of 5k to 7k, 645 tokens, 64 heads: 172 us whole, 183, 197 us in two,
+// three ranges), nor does evening out the last wave of a single request (256 CTAs at
+// 32k: 0.99 ms whole, 1.06 ms in four): the partial results' traffic costs more.
 static PagedSplit split_many(int requests, int64_t units, int64_t keys) {
   const int64_t ctas = (requests > 1 ? 2 : 1) * 148;
   int64_t n = units < ctas ? ctas / units : 1;

@@ -18,10 +18,11 @@
 // while one computes its weights, the tensor cores work for the other.  (Two
 // threads a row, or two issuing threads, measured slower.)
 //
-// Measured: 4096 tokens over a 32k context, 64 / 8 heads: 3.56 ms, 1.16
+// Measured: 4096 tokens over a 32k context, 64 / 8 heads: 3.57 ms, 1.15
 // PFLOP/s, at the board's power limit (1.5 to 1.6 GHz); 2048 tokens, 32 / 8
-// heads: 1.0 ms there, 45 us as a prompt of their own.  The tensor pipe is busy
-// 68 % of a busy SM's cycles; a tile takes 1.8 us, and each CTA 6 us more.
+// heads: 1.0 ms there, 47 us as a prompt of their own.  The tensor pipe is busy
+// 67 % of a busy SM's cycles; a tile takes 1.8 us, and each CTA 6 us more.  The
+// looking warp costs a prompt of 2048 tokens 1.5 us, a windowed call 3 of 76.
 #include "paged_token.cuh"
 #include "tensor.cuh"
 

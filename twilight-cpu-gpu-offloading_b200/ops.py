@@ -328,6 +328,7 @@ def qkv_rope(hidden: torch.Tensor, w_q: torch.Tensor, w_k: torch.Tensor, w_v: to
 
 
 # ------------------------------------------------------------- paged cache --
+# No backward passes: as with all ops here, results carry no gradient.
 # Called for every step and layer, so these go through the compiled binding
 # (csrc/binding.cpp), which unpacks and checks the tensors; what is wrong with them is
 # worked out here when it finds that something is.
@@ -424,7 +425,7 @@ def paged_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_pages: 
                 v_pages: torch.Tensor, *, error_flag: torch.Tensor | None = None) -> None:
     """New rows k / v [T, kv_heads, 128] (strided views of a projection are fine) to
     slots [T] int64 of the pool [pages, kv_heads, page_size, 128] (tw_paged_write);
-    slot -1 is skipped."""
+    slot -1 is skipped, all others have to differ."""
     rc = _lib.binding().paged_write(k, v, slots, k_pages, v_pages, error_flag)
     if rc is None:
         return
@@ -461,8 +462,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 
     q [T, q_heads, 128] (token and head strides free), pool [pages, kv_heads,
     page_size, 128], block_table [B, W] int32, cu_q [B+1] and kv_lens [B] int32
-    on the device; max_q_len bounds the requests' new tokens, max_kv_len is their
-    longest kv_lens (it sizes the launch).  window > 0: each token sees the last
+    on the device; max_q_len bounds the requests' new tokens (a longer request, or one
+    whose rows q does not have, sets error_flag and is not computed), max_kv_len is
+    their longest kv_lens (it sizes the launch).  window > 0: each token sees the last
     `window` positions only.  Returns out [T, q_heads, 128] (q's dtype or
     float32); lse [T, q_heads] fp32 receives the log-sum-exp.  Without a
     workspace (300 MB at most, see paged_attention_workspace_bytes) one is taken: up

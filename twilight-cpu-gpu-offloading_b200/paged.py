@@ -12,7 +12,10 @@ A serving step is::
 
 Tables, slots and lengths are built on the device (ops.paged_step); the host keeps
 the lengths it gave, so nothing is read back and capacity is checked before a
-launch.  A finished prompt can move to an offloaded cache for sparse decoding
+launch.  step() copies the numbers it is given to the device and waits for that copy,
+and so for what the stream holds before it.  Kernels see all max_requests rows, those of
+waiting requests too: a cache for many more requests than are served at a time divides
+its work less well than one of the right size.  A finished prompt can move to an offloaded cache for sparse decoding
 (to_offloaded).
 """
 
