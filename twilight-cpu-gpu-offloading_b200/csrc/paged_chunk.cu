@@ -115,22 +115,39 @@ __device__ __forceinline__ void write_rows(const char* smem, int warp, int lane,
   }
 }
 
-// Adds the values of `v` that are not finite to a staged row.
+// Adds what is not finite in a V row, of which the lane holds dimensions 4l .. 4l + 3 in
+// `x`, to the warp's staged rows in `rows` (a bit each), four rows at a time.
 template <typename T, typename Out>
-__device__ __forceinline__ void add_odd_staged(char* smem, int warp, int row, const T* v) {
+__device__ __forceinline__ void add_odd_staged(char* smem, int warp, int lane, uint2 x,
+                                               unsigned rows) {
   constexpr int kVec = 16 / sizeof(Out);
-  Out* base = reinterpret_cast<Out*>(smem + (warp * 32 + row) * (kHeadDim * (int)sizeof(Out)));
+  struct __align__(4 * sizeof(Out)) Four {
+    Out v[4];
+  };
+  if (!(odd_halves<T>(x.x) | odd_halves<T>(x.y))) return;
+  const T* v = reinterpret_cast<const T*>(&x);
+  float y[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) y[c] = to_f32<T>(v[c]);
 #pragma unroll 1
-  for (int c = 0; c < kVecPerRow16; ++c) {
-    const uint4 x = reinterpret_cast<const uint4*>(v)[c];
-    if (!(odd_halves<T>(x.x) | odd_halves<T>(x.y) | odd_halves<T>(x.z) | odd_halves<T>(x.w)))
-      continue;
-#pragma unroll 1
-    for (int e = 0; e < 8; ++e) {
-      const int d = c * 8 + e;
-      const float y = to_f32<T>(v[d]);
-      Out* to = base + ((d / kVec) ^ (row & 7)) * kVec + d % kVec;
-      if (!(fabsf(y) < CUDART_INF_F)) *to = from_f32<Out>(to_f32<Out>(*to) + y);
+  for (int first = 0; first < 32; first += 4, rows >>= 4) {
+    if (!(rows & 15)) continue;
+    Four* at[4];
+    Four o[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int row = first + r;
+      at[r] = reinterpret_cast<Four*>(
+          reinterpret_cast<Out*>(smem + (warp * 32 + row) * (kHeadDim * (int)sizeof(Out))) +
+          ((lane * 4 / kVec) ^ (row & 7)) * kVec + lane * 4 % kVec);
+      o[r] = *at[r];
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (!(fabsf(y[c]) < CUDART_INF_F)) o[r].v[c] = from_f32<Out>(to_f32<Out>(o[r].v[c]) + y[c]);
+      if (rows >> r & 1) *at[r] = o[r];
     }
   }
 }
@@ -399,13 +416,17 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
                              odd_halves<T>(sum[2]) | odd_halves<T>(sum[3]);
         if (__any_sync(0xffffffffu, odd != 0)) {
           if (lane == 0) sh.odd.any = 1;
-          for (int i = c0 * 16 + lane; i < c1 * 16; i += 32) {
-            const int r = i >> 4, k = first + r;
-            uint4 x = *at(i);
-            if ((r < before || r >= after) && clear_odd<T>(x)) {
-              *at(i) = x;
+          for (int r0 = c0; r0 < c1; r0 += 2) {  // two rows of 16 vectors
+            const int r = r0 + (lane >> 4);
+            bool found = false;
+            if (r < c1 && (r < before || r >= after)) {
+              uint4 x = *at(r * 16 + (lane & 15));
+              found = clear_odd<T>(x);
+              if (found) *at(r * 16 + (lane & 15)) = x;
+            }
+            if ((__ballot_sync(0xffffffffu, found) >> (lane & 16) & 0xffff) && (lane & 15) == 0) {
               const int kind = r >= after ? 0 : 1;
-              const int bit = kind == 0 ? k - p_first : k - keys.low;
+              const int bit = first + r - (kind == 0 ? p_first : keys.low);
               atomicOr(&sh.odd.bits[kind][bit >> 5], 1u << (bit & 31));
             }
           }
@@ -652,18 +673,24 @@ paged_chunk_kernel(const __grid_constant__ PagedWork w, const __grid_constant__ 
             stage_row<float>(smem, warp, lane, c, o[c]);
         }
       }
-      // what was cleared before the product and this row does see
+      // what was cleared before the product, for the rows that do see it
+      if (sh.odd.any) {
+        __syncwarp();
 #pragma unroll 1
-      for (int x = 0; sh.odd.any && x < 16; ++x) {
+        for (int x = 0; x < 16; ++x) {
 #pragma unroll 1
-        for (unsigned bits = sh.odd.bits[x >> 3][x & 7]; bits; bits &= bits - 1) {
-          const int k = (x & 7) * 32 + __ffs(bits) - 1 + (x < 8 ? p_first : keys.low);
-          const T* v = live && k >= see && k <= p ? paged_value<T>(a, b, g, k) : nullptr;
-          if (!v) continue;
-          if (joined)
-            add_odd_staged<T, Out>(smem, warp, lane, v);
-          else
-            add_odd_staged<T, float>(smem, warp, lane, v);
+          for (unsigned bits = sh.odd.bits[x >> 3][x & 7]; bits; bits &= bits - 1) {
+            const int k = (x & 7) * 32 + __ffs(bits) - 1 + (x < 8 ? p_first : keys.low);
+            const unsigned rows = __ballot_sync(0xffffffffu, live && k >= see && k <= p);
+            const T* v = paged_value<T>(a, b, g, k);
+            if (!v) continue;
+            const uint2 mine = reinterpret_cast<const uint2*>(v)[lane];
+            if (joined)
+              add_odd_staged<T, Out>(smem, warp, lane, mine, rows);
+            else
+              add_odd_staged<T, float>(smem, warp, lane, mine, rows);
+            __syncwarp();
+          }
         }
       }
       if (live) {
