@@ -603,6 +603,149 @@ size_t tw_paged_attention_workspace_size(int requests, int tokens, int q_heads, 
 int tw_paged_attention(const tw_paged_attention_args* args, void* stream);
 size_t tw_paged_attention_args_size(void);
 
+/* ---- rotary positions, attention weights of cached rows, eviction ------------------------------------
+ * Additions of this library beside the paged cache; no counterpart in the reference. */
+
+/* Rotary positions: pair n of a row at position p turns by the angle p * frequencies[n]
+ * (radians; 64-bit, as is the product), n < pairs <= 64.  interleaved 0: dimensions (n,
+ * n + pairs); 1: (2n, 2n + 1).  (a, b) -> scale * (a cos - b sin, b cos + a sin); inverse 1:
+ * by the negative angle, which with the same scale is the gradient.  Dimensions from
+ * 2 * pairs on pass unchanged and unscaled.  frequencies: device memory. */
+typedef struct tw_rope {
+  const double* frequencies;
+  int32_t pairs;
+  int32_t interleaved;
+  int32_t inverse;
+  float scale;
+} tw_rope;
+size_t tw_rope_size(void);
+
+/* Rows x [tokens][heads][D] (element strides, multiples of 8; 16-byte aligned), turned by
+ * positions [tokens], to out, which may be x with the same strides and must not overlap it
+ * otherwise. */
+int tw_rope_rows(const tw_rope* rope, const void* x, int64_t x_token_stride,
+                 int64_t x_head_stride, const int32_t* positions, int64_t tokens, int heads,
+                 int head_dim, int dtype, void* out, int64_t out_token_stride,
+                 int64_t out_head_stride, void* stream);
+
+/* tw_paged_write with the rotation in front of it, in one launch: q turned to q_out (which
+ * may be q, with the same strides, and must not overlap an input otherwise), k turned and v
+ * as it is to the slots of the pool.  Every row of q is turned, those with slot -1 too.
+ * Where they are given, row_weights / row_positions [num_pages][kv_heads][page_size] get 0
+ * and the token's position at its slot.  q_heads may be 0 (no q). */
+typedef struct tw_paged_rope_write_args {
+  tw_paged_pool pool;
+  tw_rope rope;
+  const void* q;
+  int64_t q_token_stride;
+  int64_t q_head_stride;
+  const void* k;
+  int64_t k_token_stride;
+  int64_t k_head_stride;
+  const void* v;
+  int64_t v_token_stride;
+  int64_t v_head_stride;
+  void* q_out;
+  int64_t q_out_token_stride;
+  int64_t q_out_head_stride;
+  const int32_t* positions;
+  const int64_t* slots;
+  int64_t tokens;
+  int32_t q_heads;
+  int32_t reserved; /* 0 */
+  float* row_weights;
+  int32_t* row_positions;
+  int32_t* error_flag;
+} tw_paged_rope_write_args;
+size_t tw_paged_rope_write_args_size(void);
+int tw_paged_rope_write(const tw_paged_rope_write_args* args, void* stream);
+
+/* tw_paged_step for requests whose cache has lost rows: offsets [requests] counts the tokens
+ * that are gone, a new token's position is its row plus that, and a request that ends gets
+ * offset 0.  offsets NULL: tw_paged_step. */
+int tw_paged_step_at(const tw_paged_step_args* args, int32_t* offsets, void* stream);
+
+/* Adds to each cached row's weight the attention that a call's rows gave it: for request b,
+ * KV head g and key j
+ *   row_weights[slot of j][g] += sum over the rows i of b that see j and the query heads h of
+ *                                g of exp(scale * q[i][h] . k_j - lse[i][h])
+ * with rows, masks, lengths and flags as in tw_paged_attention, whose lse [tokens][q_heads]
+ * this takes.  last > 0: only the last `last` rows of each request count.  A row whose lse is
+ * -inf counts nothing.  Slots that no counted row sees stay as they are.  The sums are 32-bit
+ * and in a fixed order; where requests share a page, both add to it, in either order.
+ * pool.v_pages is not read (it has to be a valid pointer: k_pages will do).  row_weights
+ * [num_pages][kv_heads][page_size]. */
+typedef struct tw_paged_weights_args {
+  tw_paged_pool pool;
+  const void* q;
+  int64_t q_token_stride;
+  int64_t q_head_stride;
+  const int32_t* block_table;
+  int64_t table_stride;
+  int32_t table_width;
+  int32_t requests;
+  const int32_t* cu_q;
+  const int32_t* kv_lens;
+  int32_t tokens;
+  int32_t q_heads;
+  int32_t max_q_len;
+  int32_t max_kv_len;
+  int32_t window;
+  int32_t last;
+  float softmax_scale;
+  int32_t reserved; /* 0 */
+  const float* lse;
+  float* row_weights;
+  int32_t* error_flag;
+} tw_paged_weights_args;
+size_t tw_paged_weights_args_size(void);
+int tw_paged_weights(const tw_paged_weights_args* args, void* stream);
+
+/* Cuts requests to the rows that were given most.  Of request b, when lens[b] > keep[b] >= 0,
+ * keep[b] rows stay in every layer and KV head, chosen for each by itself: first rows at
+ * positions below sink or among the request's last `recent` (position >= lens[b] + offsets[b]
+ * - recent), in row order; then by weight, the largest first, equal ones in row order (NaN
+ * counts as larger than all).  The i-th row at or past keep[b] that stays moves to the i-th
+ * place below it that has become free (K, V, weight, position): rows that were below and stay
+ * do not move, so the order of rows is not kept; row_positions says which is which.
+ *   lens_out = min(lens, keep), offsets_out = offsets + lens - lens_out; the pages past a
+ * request's last row are pushed on the stack free_pages (free_count entries before,
+ * *free_count_out after), requests in order, pages in order; the block table is not changed.
+ * free_pages, free_count and free_count_out may all be NULL.
+ * max_len: an upper bound of lens (it sizes the launch), at most 2^21; a longer request is
+ * left as it is and sets TW_ERR_BAD_ARG, one longer than its table row TW_ERR_INVALID_INDEX.
+ * A page outside the pool sets TW_ERR_INVALID_INDEX; rows in it rank last and are not moved.
+ * Pages must not be shared by requests.  Layer i's pages are at + i * layer_stride elements
+ * (a multiple of 8), its records [num_pages][kv_heads][page_size] at + i *
+ * record_layer_stride.  lens_out, offsets_out, free_pages and free_count_out must not overlap
+ * each other or the inputs.  requests <= 8192. */
+typedef struct tw_paged_evict_args {
+  tw_paged_pool pool; /* of layer 0 */
+  int64_t layer_stride;
+  int64_t record_layer_stride;
+  float* row_weights;
+  int32_t* row_positions;
+  const int32_t* block_table;
+  int64_t table_stride;
+  int32_t table_width;
+  int32_t requests;
+  int32_t layers;
+  int32_t max_len;
+  int32_t sink;
+  int32_t recent;
+  const int32_t* lens;
+  const int32_t* keep;
+  const int32_t* offsets;
+  int32_t* lens_out;
+  int32_t* offsets_out;
+  int32_t* free_pages;
+  const int32_t* free_count;
+  int32_t* free_count_out;
+  int32_t* error_flag;
+} tw_paged_evict_args;
+size_t tw_paged_evict_args_size(void);
+int tw_paged_evict(const tw_paged_evict_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -103,6 +103,51 @@ class PagedAttentionArgs(ctypes.Structure):
     ]
 
 
+class Rope(ctypes.Structure):
+    """tw_rope of include/twilight_b200.h."""
+
+    _fields_ = [("frequencies", P), ("pairs", I32T), ("interleaved", I32T), ("inverse", I32T),
+                ("scale", FLT)]
+
+
+class PagedRopeWriteArgs(ctypes.Structure):
+    """tw_paged_rope_write_args of include/twilight_b200.h."""
+
+    _fields_ = [
+        ("pool", PagedPool), ("rope", Rope), ("q", P), ("q_token_stride", I64),
+        ("q_head_stride", I64), ("k", P), ("k_token_stride", I64), ("k_head_stride", I64),
+        ("v", P), ("v_token_stride", I64), ("v_head_stride", I64), ("q_out", P),
+        ("q_out_token_stride", I64), ("q_out_head_stride", I64), ("positions", P), ("slots", P),
+        ("tokens", I64), ("q_heads", I32T), ("reserved", I32T), ("row_weights", P),
+        ("row_positions", P), ("error_flag", P),
+    ]
+
+
+class PagedWeightsArgs(ctypes.Structure):
+    """tw_paged_weights_args of include/twilight_b200.h."""
+
+    _fields_ = [
+        ("pool", PagedPool), ("q", P), ("q_token_stride", I64), ("q_head_stride", I64),
+        ("block_table", P), ("table_stride", I64), ("table_width", I32T), ("requests", I32T),
+        ("cu_q", P), ("kv_lens", P), ("tokens", I32T), ("q_heads", I32T), ("max_q_len", I32T),
+        ("max_kv_len", I32T), ("window", I32T), ("last", I32T), ("softmax_scale", FLT),
+        ("reserved", I32T), ("lse", P), ("row_weights", P), ("error_flag", P),
+    ]
+
+
+class PagedEvictArgs(ctypes.Structure):
+    """tw_paged_evict_args of include/twilight_b200.h."""
+
+    _fields_ = [
+        ("pool", PagedPool), ("layer_stride", I64), ("record_layer_stride", I64),
+        ("row_weights", P), ("row_positions", P), ("block_table", P), ("table_stride", I64),
+        ("table_width", I32T), ("requests", I32T), ("layers", I32T), ("max_len", I32T),
+        ("sink", I32T), ("recent", I32T), ("lens", P), ("keep", P), ("offsets", P),
+        ("lens_out", P), ("offsets_out", P), ("free_pages", P), ("free_count", P),
+        ("free_count_out", P), ("error_flag", P),
+    ]
+
+
 # name -> (restype, argtypes); mirrors include/twilight_b200.h
 SIGNATURES = {
     "tw_status_string": (ctypes.c_char_p, [I32]),
@@ -149,6 +194,16 @@ SIGNATURES = {
     "tw_paged_attention_workspace_size": (SZ, [I32, I32, I32, I32, I32, I32, I32, I32]),
     "tw_paged_attention": (I32, [ctypes.POINTER(PagedAttentionArgs), P]),
     "tw_paged_attention_args_size": (SZ, []),
+    "tw_rope_size": (SZ, []),
+    "tw_rope_rows": (I32, [ctypes.POINTER(Rope), P, I64, I64, P, I64, I32, I32, I32, P, I64, I64,
+                           P]),
+    "tw_paged_rope_write": (I32, [ctypes.POINTER(PagedRopeWriteArgs), P]),
+    "tw_paged_rope_write_args_size": (SZ, []),
+    "tw_paged_step_at": (I32, [ctypes.POINTER(PagedStepArgs), P, P]),
+    "tw_paged_weights": (I32, [ctypes.POINTER(PagedWeightsArgs), P]),
+    "tw_paged_weights_args_size": (SZ, []),
+    "tw_paged_evict": (I32, [ctypes.POINTER(PagedEvictArgs), P]),
+    "tw_paged_evict_args_size": (SZ, []),
 }
 
 _lib = None

@@ -24,7 +24,7 @@ LIB = PKG / "libtwilight_b200.so"
 BINDING = PKG / "_binding.so"  # Python calls with torch tensors (csrc/binding.cpp)
 SOURCES = ["quest.cu", "int4.cu", "topp_union.cu", "gather.cu", "attention.cu", "frontend.cu",
            "capi.cu", "paged.cu", "paged_attention.cu",
-           "paged_token.cu", "paged_chunk.cu"]
+           "paged_token.cu", "paged_chunk.cu", "rope.cu", "paged_weights.cu", "paged_evict.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",

@@ -117,13 +117,13 @@ template <typename F> PyObject* guarded(Py_ssize_t n, Py_ssize_t want, F f) {
 void* stream_of(int dev) { return c10::cuda::getCurrentCUDAStream(dev).stream(); }
 
 // lens, new_lens, block_table, free_pages, free_count, page_size, kv_lens, cu_q, slots,
-// positions, free_count_out, error_flag
+// positions, free_count_out, error_flag[, offsets]
 PyObject* paged_step(PyObject*, PyObject* const* o, Py_ssize_t n) {
-  return guarded(n, 12, [&]() -> PyObject* {
+  return guarded(n == 13 ? 12 : n, 12, [&]() -> PyObject* {
     const at::Tensor *lens = tensor(o[0]), *fresh = tensor(o[1]), *tab = tensor(o[2]),
                      *stack = tensor(o[3]), *count = tensor(o[4]), *kv = tensor(o[6]),
                      *cu = tensor(o[7]), *slots = tensor(o[8]), *pos = tensor(o[9]),
-                     *left = tensor(o[10]), *err;
+                     *left = tensor(o[10]), *err, *gone = nullptr;
     int page_size;
     if (!whole(o[5], page_size)) return nullptr;
     const int dev = device_of(lens);
@@ -133,7 +133,8 @@ PyObject* paged_step(PyObject*, PyObject* const* o, Py_ssize_t n) {
         !vec(count, dev, at::kInt, 1) || !vec(kv, dev, at::kInt, B) ||
         !vec(cu, dev, at::kInt, B + 1) || !vec(slots, dev, at::kLong, -1) ||
         !vec(pos, dev, at::kInt, slots->size(0)) || !vec(left, dev, at::kInt, 1) ||
-        !optional(o[11], err) || !flag(err, dev) || B > INT32_MAX ||
+        !optional(o[11], err) || !flag(err, dev) || (n == 13 && !optional(o[12], gone)) ||
+        (gone && !vec(gone, dev, at::kInt, B)) || B > INT32_MAX ||
         slots->size(0) > INT32_MAX || tab->size(1) > INT32_MAX)
       return unexpected();
     tw_paged_step_args a = {};
@@ -154,7 +155,7 @@ PyObject* paged_step(PyObject*, PyObject* const* o, Py_ssize_t n) {
     a.positions = ptr<int32_t>(pos);
     a.free_count_out = ptr<int32_t>(left);
     a.error_flag = ptr<int32_t>(err);
-    return status(tw_paged_step(&a, stream_of(dev)));
+    return status(tw_paged_step_at(&a, ptr<int32_t>(gone), stream_of(dev)));
   });
 }
 
@@ -281,7 +282,237 @@ PyObject* paged_attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
   });
 }
 
+// A finite or infinite number; false with a Python error otherwise.
+bool number(PyObject* o, double& x) {
+  x = PyFloat_AsDouble(o);
+  return !(x == -1.0 && PyErr_Occurred());
+}
+
+// frequencies, interleaved, scale, inverse
+bool rope_of(const at::Tensor* f, int dev, int interleaved, double scale, int inverse, tw_rope& r) {
+  if (!vec(f, dev, at::kDouble, -1) || f->size(0) > kHeadDim / 2) return false;
+  r = {ptr<double>(f), (int32_t)f->size(0), interleaved, inverse, (float)scale};
+  return true;
+}
+bool heads_of(const at::Tensor* t, int dev) {
+  return t && t->is_cuda() && t->get_device() == dev && t->dim() == 3 && t->size(2) == kHeadDim;
+}
+// Rows' records: [pages, kv_heads, page_size], or None.
+bool records(const at::Tensor* t, int dev, at::ScalarType type, const tw_paged_pool& p) {
+  return t->is_cuda() && t->get_device() == dev && t->scalar_type() == type && t->dim() == 3 &&
+         t->size(0) == p.num_pages && t->size(1) == p.kv_heads && t->size(2) == p.page_size &&
+         t->is_contiguous();
+}
+
+// x, positions, frequencies, interleaved, scale, inverse, out
+PyObject* rope(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  return guarded(n, 7, [&]() -> PyObject* {
+    const at::Tensor *x = tensor(o[0]), *pos = tensor(o[1]), *out;
+    int interleaved, inverse;
+    double scale;
+    if (!whole(o[3], interleaved) || !number(o[4], scale) || !whole(o[5], inverse)) return nullptr;
+    const int dev = device_of(x);
+    tw_rope r;
+    int64_t xt, xh, ot, oh;
+    if (dev < 0 || !heads_of(x, dev) ||
+        (x->scalar_type() != at::kHalf && x->scalar_type() != at::kBFloat16) ||
+        x->size(1) > INT32_MAX || !vec(pos, dev, at::kInt, x->size(0)) ||
+        !rope_of(tensor(o[2]), dev, interleaved, scale, inverse, r) || !optional(o[6], out) ||
+        !rows(*x, xt, xh))
+      return unexpected();
+    at::Tensor made;
+    if (!out) {
+      made = at::empty({x->size(0), x->size(1), kHeadDim}, x->options());
+      out = &made;
+    }
+    if (!heads_of(out, dev) || out->sizes() != x->sizes() ||
+        out->scalar_type() != x->scalar_type() || !rows(*out, ot, oh))
+      return unexpected();
+    const int rc = tw_rope_rows(&r, x->data_ptr(), xt, xh, ptr<int32_t>(pos), x->size(0),
+                                (int)x->size(1), kHeadDim,
+                                x->scalar_type() == at::kHalf ? TW_F16 : TW_BF16, out->data_ptr(),
+                                ot, oh, stream_of(dev));
+    if (rc != TW_OK) return PyLong_FromLong(rc);
+    if (!made.defined()) {
+      Py_INCREF(o[6]);
+      return o[6];
+    }
+    return THPVariable_Wrap(std::move(made));
+  });
+}
+
+// q, k, v, positions, slots, frequencies, k_pages, v_pages, interleaved, scale, q_out,
+// row_weights, row_positions, error_flag
+PyObject* paged_rope_write(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  return guarded(n, 14, [&]() -> PyObject* {
+    const at::Tensor *q = tensor(o[0]), *k = tensor(o[1]), *v = tensor(o[2]), *pos = tensor(o[3]),
+                     *slots = tensor(o[4]), *out, *weights, *places, *err;
+    int interleaved;
+    double scale;
+    if (!whole(o[8], interleaved) || !number(o[9], scale)) return nullptr;
+    const int dev = device_of(q);
+    tw_paged_rope_write_args a = {};
+    if (dev < 0 || !pool(tensor(o[6]), tensor(o[7]), dev, a.pool) || !heads_of(q, dev) ||
+        !heads_of(k, dev) || !heads_of(v, dev))
+      return unexpected();
+    const at::ScalarType type = tensor(o[6])->scalar_type();
+    const int64_t T = q->size(0);
+    if (q->scalar_type() != type || k->scalar_type() != type || v->scalar_type() != type ||
+        k->size(0) != T || v->size(0) != T || k->size(1) != a.pool.kv_heads ||
+        v->size(1) != a.pool.kv_heads || q->size(1) > INT32_MAX || !vec(pos, dev, at::kInt, T) ||
+        !vec(slots, dev, at::kLong, T) ||
+        !rope_of(tensor(o[5]), dev, interleaved, scale, 0, a.rope) || !optional(o[10], out) ||
+        !optional(o[11], weights) || !optional(o[12], places) || !optional(o[13], err) ||
+        !flag(err, dev) || (weights && !records(weights, dev, at::kFloat, a.pool)) ||
+        (places && !records(places, dev, at::kInt, a.pool)) ||
+        !rows(*q, a.q_token_stride, a.q_head_stride) ||
+        !rows(*k, a.k_token_stride, a.k_head_stride) ||
+        !rows(*v, a.v_token_stride, a.v_head_stride))
+      return unexpected();
+    at::Tensor made;
+    if (!out) {
+      made = at::empty({T, q->size(1), kHeadDim}, q->options());
+      out = &made;
+    }
+    if (!heads_of(out, dev) || out->sizes() != q->sizes() || out->scalar_type() != type ||
+        !rows(*out, a.q_out_token_stride, a.q_out_head_stride))
+      return unexpected();
+    a.q = q->data_ptr();
+    a.k = k->data_ptr();
+    a.v = v->data_ptr();
+    a.q_out = out->data_ptr();
+    a.positions = ptr<int32_t>(pos);
+    a.slots = ptr<int64_t>(slots);
+    a.tokens = T;
+    a.q_heads = (int32_t)q->size(1);
+    a.row_weights = ptr<float>(weights);
+    a.row_positions = ptr<int32_t>(places);
+    a.error_flag = ptr<int32_t>(err);
+    const int rc = tw_paged_rope_write(&a, stream_of(dev));
+    if (rc != TW_OK) return PyLong_FromLong(rc);
+    if (!made.defined()) {
+      Py_INCREF(o[10]);
+      return o[10];
+    }
+    return THPVariable_Wrap(std::move(made));
+  });
+}
+
+// q, k_pages, block_table, cu_q, kv_lens, lse, row_weights, max_q_len, max_kv_len, window,
+// last, softmax_scale, error_flag
+PyObject* paged_weights(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  return guarded(n, 13, [&]() -> PyObject* {
+    const at::Tensor *q = tensor(o[0]), *tab = tensor(o[2]), *cu = tensor(o[3]),
+                     *kv = tensor(o[4]), *lse = tensor(o[5]), *weights = tensor(o[6]), *err;
+    tw_paged_weights_args a = {};
+    if (!whole(o[7], a.max_q_len) || !whole(o[8], a.max_kv_len) || !whole(o[9], a.window) ||
+        !whole(o[10], a.last))
+      return nullptr;
+    a.softmax_scale = 0.08838834764831845f;  // 1 / sqrt(128)
+    if (o[11] != Py_None) {
+      double s;
+      if (!number(o[11], s)) return nullptr;
+      a.softmax_scale = (float)s;
+    }
+    const int dev = device_of(q);
+    if (dev < 0 || !pool(tensor(o[1]), tensor(o[1]), dev, a.pool) || !heads_of(q, dev) ||
+        q->scalar_type() != tensor(o[1])->scalar_type() || q->size(1) == 0 ||
+        q->size(1) % a.pool.kv_heads != 0 || q->size(0) > INT32_MAX || q->size(1) > INT32_MAX ||
+        !vec(kv, dev, at::kInt, -1) || !vec(cu, dev, at::kInt, kv->size(0) + 1) ||
+        !table(tab, dev, kv->size(0)) || kv->size(0) > INT32_MAX || tab->size(1) > INT32_MAX ||
+        !weights || !records(weights, dev, at::kFloat, a.pool) || !optional(o[12], err) ||
+        !flag(err, dev) || !rows(*q, a.q_token_stride, a.q_head_stride))
+      return unexpected();
+    const int64_t T = q->size(0), H = q->size(1), B = kv->size(0);
+    if (!lse || !lse->is_cuda() || lse->get_device() != dev || lse->scalar_type() != at::kFloat ||
+        lse->dim() != 2 || lse->size(0) != T || lse->size(1) != H || !lse->is_contiguous())
+      return unexpected();
+    a.q = q->data_ptr();
+    a.block_table = ptr<int32_t>(tab);
+    a.table_width = (int32_t)tab->size(1);
+    a.table_stride = B > 1 ? tab->stride(0) : a.table_width;
+    a.requests = (int32_t)B;
+    a.cu_q = ptr<int32_t>(cu);
+    a.kv_lens = ptr<int32_t>(kv);
+    a.tokens = (int32_t)T;
+    a.q_heads = (int32_t)H;
+    a.lse = ptr<float>(lse);
+    a.row_weights = ptr<float>(weights);
+    a.error_flag = ptr<int32_t>(err);
+    return status(tw_paged_weights(&a, stream_of(dev)));
+  });
+}
+
+// k_pages, v_pages, row_weights, row_positions, block_table, lens, keep, offsets, max_len,
+// sink, recent, lens_out, offsets_out, free_pages, free_count, free_count_out, error_flag
+PyObject* paged_evict(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  return guarded(n, 17, [&]() -> PyObject* {
+    const at::Tensor *k = tensor(o[0]), *v = tensor(o[1]), *weights = tensor(o[2]),
+                     *places = tensor(o[3]), *tab = tensor(o[4]), *lens = tensor(o[5]),
+                     *keep = tensor(o[6]), *gone = tensor(o[7]), *lens_out = tensor(o[11]),
+                     *gone_out = tensor(o[12]), *stack, *count, *left, *err;
+    tw_paged_evict_args a = {};
+    if (!whole(o[8], a.max_len) || !whole(o[9], a.sink) || !whole(o[10], a.recent)) return nullptr;
+    const int dev = device_of(k);
+    if (dev < 0 || !v || !weights || !places || v->dim() != k->dim() ||
+        weights->dim() != k->dim() - 1 || places->dim() != k->dim() - 1)
+      return unexpected();
+    a.layers = 1;
+    at::Tensor layer[4];  // the first of several
+    if (k->dim() == 5) {
+      const int64_t L = k->size(0);
+      if (L == 0 || L > INT32_MAX || v->size(0) != L || weights->size(0) != L ||
+          places->size(0) != L)
+        return unexpected();
+      if (L > 1) {
+        a.layer_stride = k->stride(0);
+        a.record_layer_stride = weights->stride(0);
+        if (v->stride(0) != a.layer_stride || places->stride(0) != a.record_layer_stride ||
+            !stride_ok(a.layer_stride) || a.record_layer_stride <= 0)
+          return unexpected();
+      }
+      a.layers = (int32_t)L;
+      const at::Tensor** all[4] = {&k, &v, &weights, &places};
+      for (int i = 0; i < 4; ++i) {
+        layer[i] = (*all[i])->select(0, 0);
+        *all[i] = &layer[i];
+      }
+    }
+    if (!pool(k, v, dev, a.pool) || !records(weights, dev, at::kFloat, a.pool) ||
+        !records(places, dev, at::kInt, a.pool) || !vec(lens, dev, at::kInt, -1))
+      return unexpected();
+    const int64_t B = lens->size(0);
+    if (!table(tab, dev, B) || !vec(keep, dev, at::kInt, B) || !vec(gone, dev, at::kInt, B) ||
+        !vec(lens_out, dev, at::kInt, B) || !vec(gone_out, dev, at::kInt, B) || B > INT32_MAX ||
+        tab->size(1) > INT32_MAX || !optional(o[13], stack) || !optional(o[14], count) ||
+        !optional(o[15], left) || !optional(o[16], err) || !flag(err, dev) ||
+        (stack && !vec(stack, dev, at::kInt, a.pool.num_pages)) ||
+        (count && !vec(count, dev, at::kInt, 1)) || (left && !vec(left, dev, at::kInt, 1)))
+      return unexpected();
+    a.row_weights = ptr<float>(weights);
+    a.row_positions = ptr<int32_t>(places);
+    a.block_table = ptr<int32_t>(tab);
+    a.table_width = (int32_t)tab->size(1);
+    a.table_stride = B > 1 ? tab->stride(0) : a.table_width;
+    a.requests = (int32_t)B;
+    a.lens = ptr<int32_t>(lens);
+    a.keep = ptr<int32_t>(keep);
+    a.offsets = ptr<int32_t>(gone);
+    a.lens_out = ptr<int32_t>(lens_out);
+    a.offsets_out = ptr<int32_t>(gone_out);
+    a.free_pages = ptr<int32_t>(stack);
+    a.free_count = ptr<int32_t>(count);
+    a.free_count_out = ptr<int32_t>(left);
+    a.error_flag = ptr<int32_t>(err);
+    return status(tw_paged_evict(&a, stream_of(dev)));
+  });
+}
+
 PyMethodDef kMethods[] = {
+    {"rope", (PyCFunction)(void*)rope, METH_FASTCALL, nullptr},
+    {"paged_rope_write", (PyCFunction)(void*)paged_rope_write, METH_FASTCALL, nullptr},
+    {"paged_weights", (PyCFunction)(void*)paged_weights, METH_FASTCALL, nullptr},
+    {"paged_evict", (PyCFunction)(void*)paged_evict, METH_FASTCALL, nullptr},
     {"paged_step", (PyCFunction)(void*)paged_step, METH_FASTCALL, nullptr},
     {"paged_write", (PyCFunction)(void*)paged_write, METH_FASTCALL, nullptr},
     {"paged_attention", (PyCFunction)(void*)paged_attention, METH_FASTCALL, nullptr},

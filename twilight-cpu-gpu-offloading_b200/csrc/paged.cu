@@ -61,7 +61,7 @@ __device__ __forceinline__ StepRequest step_request(int len, int fresh, int page
   return r;
 }
 
-__global__ void __launch_bounds__(kStepThreads) paged_step_kernel(tw_paged_step_args a) {
+__global__ void __launch_bounds__(kStepThreads) paged_step_kernel(tw_paged_step_args a, int32_t* offsets) {
   extern __shared__ int s_sums[];
   int* s_tokens = s_sums;                // inclusive prefix sums per request
   int* s_wanted = s_tokens + a.requests;
@@ -128,14 +128,15 @@ __global__ void __launch_bounds__(kStepThreads) paged_step_kernel(tw_paged_step_
     if (t < (unsigned)total) {
       const int b = first_above(s_tokens, B, (int)t);
       const StepRequest r = step_request(a.lens[b], a.new_lens[b], a.page_size, a.table_width);
-      position = r.len + ((int)t - (b > 0 ? s_tokens[b - 1] : 0));
+      const int at = r.len + ((int)t - (b > 0 ? s_tokens[b - 1] : 0));  // its row
+      position = offsets ? saturate((long long)at + offsets[b]) : at;
       if (served(b, r)) {
-        const int i = position / a.page_size;
+        const int i = at / a.page_size;
         const int page = i < r.have
                              ? a.block_table[(int64_t)b * a.table_stride + i]
                              : stack_page(top - 1 - (s_wanted[b] - r.want + (i - r.have)));
         if (page >= 0 && page < a.num_pages)
-          slot = (int64_t)page * a.page_size + (position - i * a.page_size);
+          slot = (int64_t)page * a.page_size + (at - i * a.page_size);
         else
           raise_error(a.error_flag, TW_ERR_INVALID_INDEX);
       }
@@ -157,6 +158,7 @@ __global__ void __launch_bounds__(kStepThreads) paged_step_kernel(tw_paged_step_
     if (!ok) raise_error(a.error_flag, TW_ERR_CAPACITY);
     a.kv_lens[b] = a.new_lens[b] < 0 ? 0 : ok ? r.len + r.add : r.len;
     a.cu_q[b + 1] = s_tokens[b];
+    if (offsets && a.new_lens[b] < 0) offsets[b] = 0;
   }
   const int wanted = saturate(base.wanted);
   for (unsigned k = first; k < (unsigned)wanted && (long long)k < top; k += step) {
@@ -226,6 +228,10 @@ extern "C" size_t tw_paged_pool_size(void) { return sizeof(tw_paged_pool); }
 extern "C" size_t tw_paged_step_args_size(void) { return sizeof(tw_paged_step_args); }
 
 extern "C" int tw_paged_step(const tw_paged_step_args* args, void* stream) {
+  return tw_paged_step_at(args, nullptr, stream);
+}
+
+extern "C" int tw_paged_step_at(const tw_paged_step_args* args, int32_t* offsets, void* stream) {
   if (!args) return TW_ERR_BAD_ARG;
   const tw_paged_step_args& a = *args;
   if (!a.lens || !a.new_lens || !a.block_table || !a.free_pages || !a.free_count || !a.kv_lens ||
@@ -235,6 +241,8 @@ extern "C" int tw_paged_step(const tw_paged_step_args* args, void* stream) {
     return TW_ERR_BAD_ARG;
   if (a.kv_lens == a.lens || a.kv_lens == a.new_lens || a.free_count_out == a.free_count)
     return TW_ERR_BAD_ARG;
+  if (offsets && (offsets == a.lens || offsets == a.new_lens || offsets == a.kv_lens))
+    return TW_ERR_BAD_ARG;
   if (a.requests > kStepMaxRequests) return TW_ERR_UNSUPPORTED;
   static DynSmemOptIn opt_in;
   const int smem = 3 * a.requests * (int)sizeof(int);
@@ -242,7 +250,7 @@ extern "C" int tw_paged_step(const tw_paged_step_args* args, void* stream) {
   if (rc != TW_OK) return rc;
   const int ctas = min(148, max(1, (a.tokens_cap + kStepTokensPerCta - 1) / kStepTokensPerCta));
   return launch_pdl(paged_step_kernel, dim3(ctas), dim3(kStepThreads), (size_t)smem,
-                    (cudaStream_t)stream, a);
+                    (cudaStream_t)stream, a, offsets);
 }
 
 extern "C" int tw_paged_write(const tw_paged_pool* pool, const void* k, int64_t k_token_stride,

@@ -1,0 +1,670 @@
+// Attention weights that the cached rows of a paged cache are given.
+//
+// weight[slot of key j][g] += sum over counted rows i that see j and heads r of group g of
+// exp(scale * q_ir . k_j - lse_ir), with the log-sum-exp that the attention left.
+//
+// Bound: for single tokens HBM (K is read once, 256 bytes a key and head); for chunks the
+// special-function unit (one 2^x a pair, 16 a clock and SM) and, less, the tensor cores
+// (2 D flops a pair).
+//
+// Layout: an item is 256 keys of a request and KV head.  The product is taken with keys
+// along the rows of tensor memory, S^T = K Q^T, so that a thread owns a key and the sum over
+// rows needs no exchange: 8 warps read their key's scores of 128 (token, head) rows at a time
+// while the tensor cores make those of the next 128.  One warp issues the products, one
+// copies K (page piece by page piece), one Q, one the log-sum-exps; the next item's K is on
+// its way while one is worked on, so that single tokens stream.  CTAs take every n-th item
+// of all requests'; each warp finds them from the lengths by itself.  Where a call has few
+// items, a cluster takes one, each CTA every n-th tile of its rows, and the first CTA adds
+// their sums in order: a result does not depend on scheduling.
+#include "paged_attention.cuh"
+#include "tensor.cuh"
+
+namespace tw {
+
+constexpr int kWtKeys = 256, kWtCols = 128;
+constexpr int kWtSumThreads = 256, kWtThreads = 384;
+constexpr int kWtMmaWarp = 8, kWtKeyWarp = 9, kWtRowWarp = 10, kWtLseWarp = 11;
+constexpr int kWtHalfTile = 128 * 128;     // bytes: 128 rows of 64 elements
+constexpr int kWtTile = 2 * kWtHalfTile;
+constexpr int kWtSlots = 7;                // of shared memory, a tile each:
+// K of two items and three tiles of q; where a cluster takes an item, K of one, four tiles
+// of q, and the sums of the other CTAs
+template <bool kSplit> constexpr int kWtKeySlots = kSplit ? 1 : 2;
+template <bool kSplit> constexpr int kWtRowSlots = kSplit ? 4 : 3;
+constexpr int kWtLseSlots = 3;
+constexpr int kWtSmem = kWtSlots * kWtTile + 1024;
+constexpr int kWtColumns = 512;            // S^T: 2 halves of the keys, 2 tiles, 128 columns
+constexpr int kWtMaxCluster = 8;
+static_assert((kWtMaxCluster - 1) * kWtKeys * 4 <= kWtTile);
+
+struct WeightWork {
+  tw_paged_weights_args a;
+  tw_paged_attention_args lens;  // what paged_request and paged_low read
+  int group;                     // query heads per KV head
+  int box;                       // rows of one box of K
+  int tile_tokens;               // tokens of 128 columns
+  int few_tokens;                // tokens of 16 columns (or one): a box of their own
+};
+
+struct WeightItem {
+  int request, head;
+  int row0, tokens;       // counted rows of q: [row0, row0 + tokens)
+  int p0;                 // position of the first
+  int key0, begin, end;   // keys [begin, end) of the block from key0 on
+  int from, tiles;        // tokens that see any of them: from `from` on, so many tiles
+  int upto;
+};
+
+// Items are numbered through the requests: every warp walks over them in the same way, 32
+// requests at a time.
+struct WeightWalk {
+  int base = -32;
+  long long before = 0, end = 0;     // items of the requests before these 32; with them
+  // of request base + lane
+  int row0, tokens, p0, low, high;
+  long long upto, items;
+
+  __device__ __forceinline__ void load(const WeightWork& w, int lane) {
+    const int b = base + lane;
+    row0 = tokens = p0 = low = high = 0;
+    items = 0;
+    if (b < w.a.requests) {
+      const PagedRequest r = paged_request(w.lens, b);
+      if (r.n > w.a.max_q_len) {
+        raise_error(w.a.error_flag, TW_ERR_BAD_ARG);
+      } else if (r.n > 0) {
+        const int skip = w.a.last > 0 ? max(0, r.n - w.a.last) : 0;
+        row0 = r.first + skip;
+        tokens = r.n - skip;
+        p0 = r.kv - tokens;
+        const PagedKeys keys = paged_keys(w.lens, r, skip, tokens);
+        low = keys.low;
+        high = keys.high;
+        if (high > low)
+          items = (long long)((high - low / kWtKeys * kWtKeys + kWtKeys - 1) / kWtKeys) *
+                  w.a.pool.kv_heads;
+      }
+    }
+    upto = items;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, upto, off);
+      if (lane >= off) upto += y;
+    }
+    upto += before;
+    end = __shfl_sync(0xffffffffu, upto, 31);
+  }
+
+  // Item `n`; false: there are not so many.  (n never goes down.)
+  __device__ __forceinline__ bool find(const WeightWork& w, int lane, long long n, WeightItem& x) {
+    while (n >= end) {
+      base += 32;
+      if (base >= w.a.requests) return false;
+      before = end;
+      load(w, lane);
+    }
+    const int l = __ffs(__ballot_sync(0xffffffffu, n < upto)) - 1;
+    const long long of = n - (__shfl_sync(0xffffffffu, upto - items, l));
+    x.request = base + l;
+    x.row0 = __shfl_sync(0xffffffffu, row0, l);
+    x.tokens = __shfl_sync(0xffffffffu, tokens, l);
+    x.p0 = __shfl_sync(0xffffffffu, p0, l);
+    const int lo = __shfl_sync(0xffffffffu, low, l), hi = __shfl_sync(0xffffffffu, high, l);
+    // heads of a block follow one another: blocks that most rows see come first
+    const int block = (int)(of / w.a.pool.kv_heads);
+    x.head = (int)(of - (long long)block * w.a.pool.kv_heads);
+    x.key0 = lo / kWtKeys * kWtKeys + block * kWtKeys;
+    x.begin = max(lo, x.key0);
+    x.end = min(hi, x.key0 + kWtKeys);
+    x.from = max(0, x.begin - x.p0);
+    x.upto = x.tokens;
+    if (w.a.window > 0)
+      x.upto = (int)min((long long)x.tokens, (long long)x.end + w.a.window - 1 - x.p0);
+    x.tiles = (max(x.upto - x.from, 0) + w.tile_tokens - 1) / w.tile_tokens;
+    return true;
+  }
+};
+
+struct WeightShared {
+  uint64_t k_full[2], k_empty[2];
+  uint64_t q_full[4], q_empty[4];
+  uint64_t lse_full[kWtLseSlots], lse_empty[kWtLseSlots];
+  uint64_t s_full[2][2], s_free[2][2];  // [half][tile]
+  uint64_t part_full, part_free, drain;
+  uint32_t tmem;
+  volatile int abort;
+  alignas(16) float lse[kWtLseSlots][kWtCols];  // minus the log-sum-exps
+};
+
+// Barriers and memory of another CTA of the cluster.
+__device__ __forceinline__ uint32_t remote(uint32_t addr, int rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void remote_arrive(uint64_t* bar, int rank) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
+                   remote(smem_addr(bar), rank))
+               : "memory");
+}
+__device__ __forceinline__ void remote_store(float* p, int rank, float x) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote(smem_addr(p), rank)), "f"(x)
+               : "memory");
+}
+__device__ __forceinline__ bool cluster_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  return wait_until(
+      [&] {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done)
+            : "r"(smem_addr(bar)), "r"(parity)
+            : "memory");
+        return done != 0;
+      },
+      abort);
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+
+// The lowest n bits (n <= 0: none, n >= 32: all).
+__device__ __forceinline__ uint32_t first_bits(int n) {
+  return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1;
+}
+
+template <bool kBf16, bool kSplit>
+__global__ void __launch_bounds__(kWtThreads, 1)
+paged_weights_kernel(const __grid_constant__ WeightWork w,
+                     const __grid_constant__ CUtensorMap k_map,
+                     const __grid_constant__ CUtensorMap q_map,
+                     const __grid_constant__ CUtensorMap few_map) {
+  extern __shared__ char s_raw[];
+  __shared__ WeightShared sh;
+  pdl_wait();
+  pdl_launch_dependents();
+  const tw_paged_weights_args& a = w.a;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int R = w.group, T = w.tile_tokens;
+  uint32_t cluster_rank, cluster_ctas;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(cluster_rank));
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(cluster_ctas));
+  const int rank = kSplit ? (int)cluster_rank : 0, S = kSplit ? (int)cluster_ctas : 1;
+  constexpr int kKeySlots = kWtKeySlots<kSplit>, kRowSlots = kWtRowSlots<kSplit>;
+  const long long first_item = blockIdx.x / S, step = gridDim.x / S;
+  char* smem = (char*)(((uintptr_t)s_raw + 1023) & ~(uintptr_t)1023);
+  const uint32_t keys_at = smem_addr(smem), rows_at = keys_at + 2 * kKeySlots * kWtTile;
+  float* s_part = reinterpret_cast<float*>(smem + (kWtSlots - 1) * kWtTile);  // kSplit: [rank - 1][key]
+  if (tid == 0) {
+    for (int i = 0; i < kKeySlots; ++i) {
+      mbar_init(&sh.k_full[i], 1);
+      mbar_init(&sh.k_empty[i], 1);
+    }
+    for (int i = 0; i < kRowSlots; ++i) {
+      mbar_init(&sh.q_full[i], 1);
+      mbar_init(&sh.q_empty[i], 1);
+    }
+    for (int i = 0; i < kWtLseSlots; ++i) {
+      mbar_init(&sh.lse_full[i], 1);
+      mbar_init(&sh.lse_empty[i], kWtSumThreads / 32);
+    }
+    for (int i = 0; i < 2; ++i)
+      for (int j = 0; j < 2; ++j) {
+        mbar_init(&sh.s_full[i][j], 1);
+        mbar_init(&sh.s_free[i][j], 4);
+      }
+    if (kSplit) {
+      mbar_init(&sh.part_full, (uint32_t)((S - 1) * (kWtSumThreads / 32)));
+      mbar_init(&sh.part_free, kWtSumThreads / 32);
+    }
+    mbar_init(&sh.drain, 1);
+    sh.abort = 0;
+    mbar_init_fence();
+  }
+  // columns that no token fills (groups that do not divide 128) stay zero rows
+  for (int i = tid; i < kRowSlots * 2 * (kWtCols - T * R) * 8; i += kWtThreads) {
+    const int tile = i / ((kWtCols - T * R) * 8), at = i % ((kWtCols - T * R) * 8);
+    *reinterpret_cast<uint4*>(smem + 2 * kKeySlots * kWtTile + tile * kWtHalfTile +
+                              T * R * 128 + at * 16) = make_uint4(0u, 0u, 0u, 0u);
+  }
+  fence_async_smem();
+  if (warp == kWtMmaWarp) tmem_alloc(&sh.tmem, kWtColumns);
+  tmem_fence_before();
+  __syncthreads();
+  tmem_fence_after();
+  if constexpr (kSplit) cluster_barrier();  // all barriers are there
+  const uint32_t tmem = sh.tmem;
+
+  WeightWalk walk;
+  WeightItem x;
+  bool ok = true;
+  if (warp == kWtKeyWarp) {
+    // ---- K of the items
+    if (elect_one()) prefetch_map(&k_map);
+    __syncwarp();
+    const uint32_t box_bytes = (uint32_t)w.box * 128;  // of 64 dimensions
+    const int boxes = kWtKeys / w.box;                 // at most 32
+    int n = 0;
+    for (long long item = first_item; walk.find(w, lane, item, x); item += step) {
+      if (rank >= x.tiles) continue;
+      const int s = n % kKeySlots;
+      const int key = x.key0 + lane * w.box;
+      const bool wanted = lane < boxes && key < x.end && key + w.box > x.begin;
+      int p = 0, row = 0;
+      if (wanted) {
+        const int i = key / a.pool.page_size;
+        row = key - i * a.pool.page_size;
+        p = a.block_table[(int64_t)x.request * a.table_stride + i];
+        if (p < 0 || p >= a.pool.num_pages) {
+          raise_error(a.error_flag, TW_ERR_INVALID_INDEX);
+          p = (int)a.pool.num_pages;  // out of the map's range: zeros
+        }
+      }
+      const uint32_t all = __ballot_sync(0xffffffffu, wanted);
+      const int from = __ffs(all) - 1, to = 32 - __clz(all);
+      if (n >= kKeySlots) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&sh.k_empty[s],
+                                               (uint32_t)((n / kKeySlots - 1) & 1), &sh.abort));
+        if (!ok) break;
+      }
+      if (elect_one())
+        mbar_arrive_expect(&sh.k_full[s], (uint32_t)(to - from) * box_bytes * 2);
+      for (int y0 = from; y0 < to; y0 += 4) {
+        int px[4], rx[4];
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          px[y] = __shfl_sync(0xffffffffu, p, y0 + y);
+          rx[y] = __shfl_sync(0xffffffffu, row, y0 + y);
+        }
+        if (elect_one()) {
+#pragma unroll
+          for (int y = 0; y < 4; ++y)
+            if (y0 + y < to) {
+              const int r = (y0 + y) * w.box;  // of the block's 256
+              const uint32_t dst = keys_at + (uint32_t)(s * 2 + (r >> 7)) * kWtTile +
+                                   (uint32_t)(r & 127) * 128;
+              tma_load_4d(&k_map, dst, &sh.k_full[s], 0, rx[y], x.head, px[y]);
+              tma_load_4d(&k_map, dst + kWtHalfTile, &sh.k_full[s], 64, rx[y], x.head, px[y]);
+            }
+        }
+        __syncwarp();
+      }
+      ++n;
+    }
+    if (!ok || sh.abort) {  // give up: wait (with the same limit) for the copies in flight
+      volatile int never = 0;
+      for (int i = max(n - kKeySlots, 0); i < n; ++i)
+        mbar_wait(&sh.k_full[i % kKeySlots], (uint32_t)((i / kKeySlots) & 1), &never);
+    }
+  } else if (warp == kWtRowWarp) {
+    // ---- tiles of q
+    if (elect_one()) {
+      prefetch_map(&q_map);
+      prefetch_map(&few_map);
+    }
+    __syncwarp();
+    int n = 0;
+    for (long long item = first_item; ok && walk.find(w, lane, item, x); item += step) {
+      for (int t = rank; t < x.tiles; t += S, ++n) {
+        const int s = n % kRowSlots;
+        if (n >= kRowSlots) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&sh.q_empty[s],
+                                                 (uint32_t)((n / kRowSlots - 1) & 1), &sh.abort));
+          if (!ok) break;
+        }
+        const int i = x.from + t * T, here = min(T, x.upto - i);
+        if (elect_one()) {
+          const uint32_t dst = rows_at + (uint32_t)s * kWtTile;
+          // rows past the last are masked
+          const bool few = here <= w.few_tokens;
+          const CUtensorMap* map = few ? &few_map : &q_map;
+          mbar_arrive_expect(&sh.q_full[s], (uint32_t)((few ? w.few_tokens : T) * R) * 256);
+          tma_load_3d(map, dst, &sh.q_full[s], 0, x.head * R, x.row0 + i);
+          tma_load_3d(map, dst + kWtHalfTile, &sh.q_full[s], 64, x.head * R, x.row0 + i);
+        }
+        __syncwarp();
+      }
+    }
+    if (!ok || sh.abort) {
+      volatile int never = 0;
+      for (int i = max(n - kRowSlots, 0); i < n; ++i)
+        mbar_wait(&sh.q_full[i % kRowSlots], (uint32_t)((i / kRowSlots) & 1), &never);
+    }
+  } else if (warp == kWtLseWarp) {
+    // ---- log-sum-exps of the tiles' rows
+    int n = 0;
+    for (long long item = first_item; ok && walk.find(w, lane, item, x); item += step) {
+      for (int t = rank; t < x.tiles; t += S, ++n) {
+        const int s = n % kWtLseSlots;
+        const int i = x.from + t * T, cols = min(T, x.upto - i) * R;
+        float z[kWtCols / 32];
+#pragma unroll
+        for (int c = 0; c < kWtCols / 32; ++c) {
+          const int col = c * 32 + lane, token = col / R;
+          z[c] = col < cols ? -a.lse[(int64_t)(x.row0 + i + token) * a.q_heads + x.head * R +
+                                     (col - token * R)]
+                            : -CUDART_INF_F;
+          // a row that saw nothing: no weight (its score less -infinity would be infinite)
+          if (z[c] == CUDART_INF_F) z[c] = -CUDART_INF_F;
+        }
+        if (n >= kWtLseSlots) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&sh.lse_empty[s],
+                                                 (uint32_t)((n / kWtLseSlots - 1) & 1), &sh.abort));
+          if (!ok) break;
+        }
+#pragma unroll
+        for (int c = 0; c < kWtCols / 32; ++c) sh.lse[s][c * 32 + lane] = z[c];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.lse_full[s]);
+      }
+    }
+  } else if (warp == kWtMmaWarp) {
+    // ---- products
+    int nk = 0, nq = 0, ns[2] = {0, 0};
+    for (long long item = first_item; ok && walk.find(w, lane, item, x); item += step) {
+      if (rank >= x.tiles) continue;
+      const int ks = nk % kKeySlots;
+      const int halves = x.end - x.key0 > 128 ? 2 : 1;
+      const bool first_half = x.begin < x.key0 + 128;
+      ok = __all_sync(0xffffffffu,
+                      mbar_wait(&sh.k_full[ks], (uint32_t)((nk / kKeySlots) & 1), &sh.abort));
+      for (int t = rank; ok && t < x.tiles; t += S, ++nq) {
+        const int qs = nq % kRowSlots;
+        const int cols = min(T, x.upto - x.from - t * T) * R;
+        const uint32_t desc = product_desc(kBf16, (cols + 15) / 16 * 16, false);
+        ok = __all_sync(0xffffffffu,
+                        mbar_wait(&sh.q_full[qs], (uint32_t)((nq / kRowSlots) & 1), &sh.abort));
+        for (int h = first_half ? 0 : 1; ok && h < halves; ++h) {
+          const int buf = ns[h] & 1;
+          if (ns[h] >= 2)
+            ok = __all_sync(0xffffffffu, mbar_wait(&sh.s_free[h][buf],
+                                                   (uint32_t)((ns[h] / 2 - 1) & 1), &sh.abort));
+          if (!ok) break;
+          tmem_fence_after();
+          if (elect_one()) {
+            const uint32_t ka = keys_at + (uint32_t)(ks * 2 + h) * kWtTile,
+                           qa = rows_at + (uint32_t)qs * kWtTile;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const uint32_t off = (k >> 2) * kWtHalfTile + (k & 3) * 32;
+              mma_smem(tmem + (h * 2 + buf) * 128, operand_desc(ka + off, 16, 1024),
+                       operand_desc(qa + off, 16, 1024), desc, k > 0);
+            }
+            mma_commit(&sh.s_full[h][buf]);
+          }
+          __syncwarp();
+          ++ns[h];
+        }
+        if (ok && elect_one()) mma_commit(&sh.q_empty[qs]);
+        __syncwarp();
+      }
+      if (ok && elect_one()) mma_commit(&sh.k_empty[ks]);
+      __syncwarp();
+      ++nk;
+    }
+    if (!ok || sh.abort) {
+      volatile int never = 0;
+      if (elect_one()) mma_commit(&sh.drain);
+      __syncwarp();
+      mbar_wait(&sh.drain, 0, &never);
+    }
+  } else {
+    // ---- sums: a thread per key
+    const int h = warp >> 2;
+    const uint32_t my = tmem + ((uint32_t)((warp & 3) * 32) << 16) + h * 256;
+    const uint64_t scale2 = pair(a.softmax_scale, a.softmax_scale);
+    const uint64_t log2e2 = pair(1.4426950408889634f, 1.4426950408889634f);
+    int nl = 0, ns = 0, items = 0;
+    for (long long item = first_item; ok && walk.find(w, lane, item, x); item += step, ++items) {
+      const int j = x.key0 + tid;
+      const bool held = j >= x.begin && j < x.end;
+      int64_t place = -1;
+      if (held && rank == 0) {
+        const int i = j / a.pool.page_size;
+        const int page = a.block_table[(int64_t)x.request * a.table_stride + i];
+        if (page >= 0 && page < a.pool.num_pages)
+          place = ((int64_t)page * a.pool.kv_heads + x.head) * a.pool.page_size +
+                  (j - i * a.pool.page_size);
+      }
+      const bool mine = h == 0 ? x.begin < x.key0 + 128 : x.end > x.key0 + 128;
+      float sum = 0.f;
+      for (int t = rank; t < x.tiles; t += S, ++nl) {
+        const int ls = nl % kWtLseSlots;
+        // (also by warps with no keys: they must not hand a slot back twice in a phase)
+        ok = __all_sync(0xffffffffu, mbar_wait(&sh.lse_full[ls],
+                                               (uint32_t)((nl / kWtLseSlots) & 1), &sh.abort));
+        if (!ok) break;
+        if (mine) {
+          const int buf = ns & 1;
+          ok = __all_sync(0xffffffffu,
+                          mbar_wait(&sh.s_full[h][buf], (uint32_t)((ns / 2) & 1), &sh.abort));
+          if (!ok) break;
+          ++ns;
+          tmem_fence_after();
+          const int i = x.from + t * T, here = min(T, x.upto - i);
+          const int cols = here * R, p = x.p0 + i;  // position of the tile's first token
+          const int kh = x.key0 + h * 128;
+          // columns of the tokens that see this key: [from, to)
+          const bool plain = here == T && kh >= x.begin && kh + 128 <= x.end && p >= kh + 127 &&
+                             (a.window <= 0 || (long long)p + T - a.window <= kh);
+          int from = 0, to = cols;
+          if (!plain) {
+            from = held ? max(j - p, 0) * R : 0;
+            to = 0;
+            if (held)
+              to = a.window > 0 ? (int)max(min((long long)here, (long long)j + a.window - p), 0ll) * R
+                                : cols;
+          }
+          const uint32_t at = my + buf * 128;
+          const int chunks = (cols + 31) / 32;
+          float s[2][32];
+          uint64_t sum2[2] = {0ull, 0ull};
+          tmem_ld32(s[0], at);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            if (c >= chunks) break;
+            tmem_wait_ld(s[c & 1]);
+            if (c + 1 < chunks) {
+              tmem_ld32(s[(c + 1) & 1], at + (c + 1) * 32);
+            } else {
+              tmem_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&sh.s_free[h][buf]);
+            }
+            const uint32_t seen = first_bits(to - c * 32) & ~first_bits(from - c * 32);
+            // (columns that no token fills are zero rows: an infinite key would make them NaN)
+            const bool masked = !plain || (c + 1) * 32 > cols;
+            const float4* z = reinterpret_cast<const float4*>(&sh.lse[ls][c * 32]);
+#pragma unroll
+            for (int y = 0; y < 32; y += 4) {
+              const float4 l = z[y / 4];
+              const uint64_t d0 =
+                  mul2(fma2(pair(s[c & 1][y], s[c & 1][y + 1]), scale2, pair(l.x, l.y)), log2e2);
+              const uint64_t d1 = mul2(
+                  fma2(pair(s[c & 1][y + 2], s[c & 1][y + 3]), scale2, pair(l.z, l.w)), log2e2);
+              float e0, e1, e2, e3;
+              unpair(d0, e0, e1);
+              unpair(d1, e2, e3);
+              e0 = ex2(e0);
+              e1 = ex2(e1);
+              e2 = ex2(e2);
+              e3 = ex2(e3);
+              if (masked) {
+                e0 = seen >> y & 1 ? e0 : 0.f;
+                e1 = seen >> (y + 1) & 1 ? e1 : 0.f;
+                e2 = seen >> (y + 2) & 1 ? e2 : 0.f;
+                e3 = seen >> (y + 3) & 1 ? e3 : 0.f;
+              }
+              sum2[0] = add2(sum2[0], pair(e0, e1));
+              sum2[1] = add2(sum2[1], pair(e2, e3));
+            }
+          }
+          float y0, y1;
+          unpair(add2(sum2[0], sum2[1]), y0, y1);
+          sum += y0 + y1;  // a tile's by itself first: beside a large sum each could be nothing
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.lse_empty[ls]);
+      }
+      if (!ok) break;
+      if constexpr (kSplit) {
+        if (rank != 0) {
+          if (items > 0)
+            ok = __all_sync(0xffffffffu,
+                            cluster_wait(&sh.part_free, (uint32_t)((items - 1) & 1), &sh.abort));
+          if (!ok) break;
+          remote_store(s_part + (rank - 1) * kWtKeys + tid, 0, sum);
+          __syncwarp();
+          if (lane == 0) remote_arrive(&sh.part_full, 0);
+        } else {
+          ok = __all_sync(0xffffffffu,
+                          cluster_wait(&sh.part_full, (uint32_t)(items & 1), &sh.abort));
+          if (!ok) break;
+          for (int r = 1; r < S; ++r) sum += s_part[(r - 1) * kWtKeys + tid];
+          __syncwarp();
+          if (lane == 0)
+            for (int r = 1; r < S; ++r) remote_arrive(&sh.part_free, r);
+        }
+      }
+      // no other thread of the call adds to this slot, unless requests share its page
+      if (place >= 0) atomicAdd(a.row_weights + place, sum);
+    }
+    if (!ok && lane == 0) raise_error(a.error_flag, TW_ERR_TIMEOUT);
+    tmem_fence_before();
+  }
+  __syncwarp();
+  __syncthreads();
+  if (warp == kWtMmaWarp) {
+    tmem_fence_after();
+    tmem_free(tmem, kWtColumns);
+  }
+  if constexpr (kSplit) cluster_barrier();  // no CTA is gone while another writes to it
+}
+
+// Clusters of `cluster` CTAs that the device holds at once, asked once per device.
+template <bool kBf16, bool kSplit>
+static int resident_clusters(int cluster, int& n) {
+  static int known[kMaxDevices][4] = {};
+  static std::mutex mu;
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  const int i = cluster == 1 ? 0 : cluster == 2 ? 1 : cluster == 4 ? 2 : 3;
+  if (err == cudaSuccess && dev < kMaxDevices) {
+    std::lock_guard<std::mutex> lk(mu);
+    if (known[dev][i] > 0) {
+      n = known[dev][i];
+      return TW_OK;
+    }
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)cluster);
+  cfg.blockDim = dim3(kWtThreads);
+  cfg.dynamicSmemBytes = kWtSmem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (err == cudaSuccess)
+    err = cudaOccupancyMaxActiveClusters(&n, paged_weights_kernel<kBf16, kSplit>, &cfg);
+  if (err != cudaSuccess) {
+    set_last_cuda_error(err);
+    return TW_ERR_CUDA;
+  }
+  if (n < 1) n = 1;
+  if (dev < kMaxDevices) {
+    std::lock_guard<std::mutex> lk(mu);
+    known[dev][i] = n;
+  }
+  return TW_OK;
+}
+
+template <bool kBf16, bool kSplit>
+static int launch_weights(const WeightWork& w, int cluster, int64_t items, cudaStream_t stream) {
+  const tw_paged_weights_args& a = w.a;
+  CUtensorMap k_map, q_map, few_map;
+  const cuuint64_t dims[4] = {(cuuint64_t)kHeadDim, (cuuint64_t)a.pool.page_size,
+                              (cuuint64_t)a.pool.kv_heads, (cuuint64_t)a.pool.num_pages};
+  const cuuint64_t strides[3] = {(cuuint64_t)a.pool.token_stride * 2,
+                                 (cuuint64_t)a.pool.head_stride * 2,
+                                 (cuuint64_t)a.pool.page_stride * 2};
+  const cuuint32_t box[4] = {64, (cuuint32_t)w.box, 1, 1};
+  int rc = encode_rows_map(&k_map, a.pool.dtype, 4, a.pool.k_pages, dims, strides, box);
+  const cuuint64_t q_dims[3] = {(cuuint64_t)kHeadDim, (cuuint64_t)a.q_heads, (cuuint64_t)a.tokens};
+  const cuuint64_t q_strides[2] = {(cuuint64_t)a.q_head_stride * 2,
+                                   (cuuint64_t)a.q_token_stride * 2};
+  const cuuint32_t q_box[3] = {64, (cuuint32_t)w.group, (cuuint32_t)w.tile_tokens};
+  const cuuint32_t few_box[3] = {64, (cuuint32_t)w.group, (cuuint32_t)w.few_tokens};
+  if (rc == TW_OK) rc = encode_rows_map(&q_map, a.pool.dtype, 3, a.q, q_dims, q_strides, q_box);
+  if (rc == TW_OK) rc = encode_rows_map(&few_map, a.pool.dtype, 3, a.q, q_dims, q_strides, few_box);
+  if (rc != TW_OK) return rc;
+  static DynSmemOptIn opt_in;
+  const auto kernel = paged_weights_kernel<kBf16, kSplit>;
+  rc = ensure_dyn_smem((const void*)kernel, opt_in, kWtSmem);
+  int most = 0;
+  if (rc == TW_OK) rc = resident_clusters<kBf16, kSplit>(cluster, most);
+  if (rc != TW_OK) return rc;
+  const int64_t clusters = items < most ? items : most;
+  return launch_pdl_cluster(kernel, dim3((unsigned)(clusters * cluster)), dim3(kWtThreads), cluster,
+                            (size_t)kWtSmem, stream, w, k_map, q_map, few_map);
+}
+
+}  // namespace tw
+
+using namespace tw;
+
+extern "C" size_t tw_paged_weights_args_size(void) { return sizeof(tw_paged_weights_args); }
+
+extern "C" int tw_paged_weights(const tw_paged_weights_args* args, void* stream) {
+  if (!args) return TW_ERR_BAD_ARG;
+  const tw_paged_weights_args& a = *args;
+  const int rc = check_paged_pool(a.pool);
+  if (rc != TW_OK) return rc;
+  if (a.pool.page_size % 8 != 0) return TW_ERR_UNSUPPORTED;
+  if (a.tokens < 0 || a.requests < 0) return TW_ERR_BAD_ARG;
+  if (a.tokens == 0) return TW_OK;
+  if (!a.q || !a.block_table || !a.cu_q || !a.kv_lens || !a.lse || !a.row_weights ||
+      a.requests <= 0 || a.q_heads <= 0 || a.q_heads % a.pool.kv_heads != 0 ||
+      a.table_width <= 0 || a.table_stride < a.table_width || a.max_q_len < 0 ||
+      a.max_kv_len < 0 || a.window < 0 || a.last < 0 || a.reserved != 0 ||
+      !(a.softmax_scale > 0.f) || !(a.softmax_scale < INFINITY))
+    return TW_ERR_BAD_ARG;
+  if (a.q_heads / a.pool.kv_heads > 64) return TW_ERR_UNSUPPORTED;
+  if (!aligned16(a.q) || !paged_stride_ok(a.q_token_stride) || !paged_stride_ok(a.q_head_stride))
+    return TW_ERR_BAD_ARG;
+  WeightWork w = {};
+  w.a = a;
+  w.lens.pool = a.pool;
+  w.lens.cu_q = a.cu_q;
+  w.lens.kv_lens = a.kv_lens;
+  w.lens.tokens = a.tokens;
+  w.lens.table_width = a.table_width;
+  w.lens.window = a.window;
+  w.lens.error_flag = a.error_flag;
+  w.group = a.q_heads / a.pool.kv_heads;
+  w.tile_tokens = kWtCols / w.group;
+  w.few_tokens = w.group < 16 ? 16 / w.group : 1;
+  w.box = 64;
+  while (a.pool.page_size % w.box != 0) w.box /= 2;
+  // Bounds of the items and of a request's tiles: a cluster an item where CTAs would idle.
+  int64_t most = a.max_q_len < a.tokens ? a.max_q_len : a.tokens;
+  if (a.last > 0 && a.last < most) most = a.last;
+  int64_t keys = a.max_kv_len;
+  if (a.window > 0 && a.window + most < keys) keys = a.window + most;
+  const int64_t items =
+      ((keys + kWtKeys - 1) / kWtKeys + (a.window > 0)) * a.requests * a.pool.kv_heads;
+  const int64_t tiles = (most + w.tile_tokens - 1) / w.tile_tokens;
+  int cluster = 1;
+  while (cluster < kWtMaxCluster && 2 * cluster <= tiles && 2 * cluster * items <= 148) cluster *= 2;
+  cudaStream_t s = (cudaStream_t)stream;
+  const int64_t some = items > 0 ? items : 1;
+  if (a.pool.dtype == TW_F16)
+    return cluster > 1 ? launch_weights<false, true>(w, cluster, some, s)
+                       : launch_weights<false, false>(w, cluster, some, s);
+  return cluster > 1 ? launch_weights<true, true>(w, cluster, some, s)
+                     : launch_weights<true, false>(w, cluster, some, s);
+}

@@ -393,7 +393,8 @@ def paged_step(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Te
                free_pages: torch.Tensor, free_count: torch.Tensor, *, page_size: int,
                kv_lens: torch.Tensor, cu_q: torch.Tensor, slots: torch.Tensor,
                positions: torch.Tensor, free_count_out: torch.Tensor,
-               error_flag: torch.Tensor | None = None) -> None:
+               error_flag: torch.Tensor | None = None,
+               offsets: torch.Tensor | None = None) -> None:
     """Block tables and slot map of one serving step, in one launch (tw_paged_step).
 
     lens / new_lens [B] int32 (tokens held, tokens to add; new < 0: the request
@@ -401,9 +402,12 @@ def paged_step(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Te
     free_pages [num_pages] with free_count [1] entries are updated; outputs
     kv_lens [B], cu_q [B+1], free_count_out [1] and, per new token, slots
     (int64, -1: none) and positions [tokens_cap].  A refused request or a full
-    output sets error_flag to TW_ERR_CAPACITY."""
+    output sets error_flag to TW_ERR_CAPACITY.  offsets [B] int32: tokens that each
+    request's cache has lost (paged_evict); positions count them, and a request that ends
+    gets 0."""
     rc = _lib.binding().paged_step(lens, new_lens, block_table, free_pages, free_count, page_size,
-                                   kv_lens, cu_q, slots, positions, free_count_out, error_flag)
+                                   kv_lens, cu_q, slots, positions, free_count_out, error_flag,
+                                   offsets)
     if rc is None:
         return
     if rc < 0:
@@ -416,7 +420,7 @@ def paged_step(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Te
                  ("slots", slots, torch.int64, (None,)),
                  ("positions", positions, i32, slots.shape[:1]),
                  ("free_count_out", free_count_out, i32, (1,)),
-                 ("error_flag", error_flag, i32, (1,)))
+                 ("error_flag", error_flag, i32, (1,)), ("offsets", offsets, i32, (B,)))
         raise ValueError("paged_step: unexpected tensors")
     _lib.check(rc, "paged_step")
 
@@ -496,3 +500,242 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
             raise ValueError("workspace must be contiguous, on q's device")
         raise ValueError("paged_attention: unexpected tensors")
     _lib.check(rc, "paged_attention")
+
+
+# --------------------------------------------------------- rotary positions --
+
+_LAYOUTS = {"half": 0, "interleaved": 1}
+
+
+def _interleaved(layout: str) -> int:
+    if layout not in _LAYOUTS:
+        raise ValueError(f"layout must be 'half' or 'interleaved', got {layout!r}")
+    return _LAYOUTS[layout]
+
+
+def rope_frequencies(dims: int = HEAD_DIM, *, base: float = 10000.0, scaling: dict | None = None,
+                     device: torch.device | str | None = None) -> tuple[torch.Tensor, float]:
+    """(frequencies [dims / 2] float64, scale) for rope and paged_rope_write: pair n turns by
+    base^(-2n / dims) radians a position.  scaling, for contexts beyond those a model was
+    trained on:
+
+    {"type": "linear", "factor": f}: all f times slower.
+    {"type": "ntk", "factor": f}: the base times f^(dims / (dims - 2)), which slows the slowest
+        pair f times and leaves the fastest.
+    {"type": "bands", "factor": f, "original": n, "low": 1, "high": 4}: pairs that turn fewer
+        than `low` times in `original` positions f times slower, those that turn more than
+        `high` times as they are, between them in proportion.
+    {"type": "yarn", "factor": f, "original": n, "fast": 32, "slow": 1, "scale": None}: the
+        same between the pairs that turn `fast` and `slow` times, in proportion to the pair's
+        number; rotated values are scaled by `scale`, by default 0.1 ln(f) + 1."""
+    if not 0 <= dims <= HEAD_DIM or dims % 2:
+        raise ValueError(f"dims must be even and at most {HEAD_DIM}")
+    if not base > 1.0:
+        raise ValueError("base must be above 1")
+    n = torch.arange(0, dims, 2, dtype=torch.float64)
+    s = dict(scaling or {"type": "none"})
+    kind = s.pop("type", None)
+    known = {"none": (), "linear": ("factor",), "ntk": ("factor",),
+             "bands": ("factor", "original", "low", "high"),
+             "yarn": ("factor", "original", "fast", "slow", "scale")}
+    if kind not in known or not set(s) <= set(known[kind]):
+        raise ValueError(f"unknown scaling {scaling}")
+    factor = float(s.get("factor", 1.0))
+    if kind != "none" and not (factor >= 1.0 and "factor" in s):
+        raise ValueError("scaling needs a factor of at least 1")
+    if kind in ("bands", "yarn") and not s.get("original", 0) > 0:
+        raise ValueError("scaling needs the original length")
+    if kind == "ntk" and dims > 2:
+        base = base * factor ** (dims / (dims - 2))
+    frequencies, scale = base ** (-n / max(dims, 1)), 1.0
+    if kind == "linear":
+        frequencies = frequencies / factor
+    elif kind == "bands":
+        low, high = float(s.get("low", 1.0)), float(s.get("high", 4.0))
+        if not high > low:
+            raise ValueError("high must be above low")
+        turns = s["original"] * frequencies / (2 * math.pi)
+        kept = ((turns - low) / (high - low)).clamp(0, 1)
+        frequencies = frequencies / factor * (1 - kept) + frequencies * kept
+    elif kind == "yarn":
+        fast, slow = float(s.get("fast", 32.0)), float(s.get("slow", 1.0))
+        if not fast > slow > 0:
+            raise ValueError("fast must be above slow")
+
+        def pair(turns: float) -> float:  # the pair that turns so often
+            return dims * math.log(s["original"] / (turns * 2 * math.pi)) / (2 * math.log(base))
+
+        low, high = max(math.floor(pair(fast)), 0), min(math.ceil(pair(slow)), dims - 1)
+        slowed = ((n / 2 - low) / max(high - low, 0.001)).clamp(0, 1)
+        frequencies = frequencies / factor * slowed + frequencies * (1 - slowed)
+        scale = s.get("scale")
+        scale = 0.1 * math.log(factor) + 1.0 if scale is None else float(scale)
+    return frequencies.to(device) if device is not None else frequencies, scale
+
+
+def _explain_rope(dev: int, positions, frequencies, tokens: int, scale: float) -> None:
+    _explain(dev, ("positions", positions, torch.int32, (tokens,)),
+             ("frequencies", frequencies, torch.float64, (None,)))
+    if frequencies.shape[0] > HEAD_DIM // 2:
+        raise ValueError(f"at most {HEAD_DIM // 2} frequencies")
+    if not math.isfinite(scale):
+        raise ValueError("scale must be finite")
+
+
+def rope(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, *,
+         layout: str = "half", scale: float = 1.0, inverse: bool = False,
+         out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotary positions of rows x [T, heads, 128] (strided views of a projection are fine, q
+    and k side by side among them) at positions [T] int32 (tw_rope_rows).
+
+    frequencies [pairs] float64 (rope_frequencies): pair n, dimensions (n, n + pairs) in the
+    "half" layout and (2n, 2n + 1) in the "interleaved" one, turns by position * frequency and
+    is scaled; the other dimensions pass.  inverse: by the negative angle (the gradient of the
+    same call).  out: x itself, or rows that do not overlap it."""
+    rc = _lib.binding().rope(x, positions, frequencies, _interleaved(layout), scale, bool(inverse),
+                             out)
+    if not isinstance(rc, int):
+        return rc
+    if rc < 0:
+        dev = _explain_device(x)
+        _kv_code(x.dtype)
+        _explain_rows(dev, "x", x, x.dtype, None, None, HEAD_DIM)
+        _explain_rope(dev, positions, frequencies, x.shape[0], scale)
+        if out is not None:
+            _explain_rows(dev, "out", out, x.dtype, x.shape[0], x.shape[1], HEAD_DIM)
+        raise ValueError("rope: unexpected tensors")
+    _lib.check(rc, "rope")
+
+
+def _explain_records(dev: int, k_pages: torch.Tensor, row_weights, row_positions) -> None:
+    shape = k_pages.shape[:-1]
+    for name, t, dtype in (("row_weights", row_weights, torch.float32),
+                           ("row_positions", row_positions, torch.int32)):
+        _explain(dev, (name, t, dtype, shape))
+        if t is not None and not (t[0] if t.dim() == 4 else t).is_contiguous():
+            raise ValueError(f"{name} must be contiguous [pages, kv_heads, page_size]")
+
+
+def paged_rope_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
+                     slots: torch.Tensor, frequencies: torch.Tensor, k_pages: torch.Tensor,
+                     v_pages: torch.Tensor, *, layout: str = "half", scale: float = 1.0,
+                     q_out: torch.Tensor | None = None, row_weights: torch.Tensor | None = None,
+                     row_positions: torch.Tensor | None = None,
+                     error_flag: torch.Tensor | None = None) -> torch.Tensor:
+    """rope of q and k and paged_write of k and v in one launch (tw_paged_rope_write).
+
+    q [T, q_heads, 128], k / v [T, kv_heads, 128] (strided views are fine), positions and slots
+    [T] as paged_step plans them (slot -1: nothing is written, q is turned all the same).
+    Returns the turned q: q_out, which may be q itself and must not overlap an input
+    otherwise.  row_weights float32 / row_positions int32 [pages, kv_heads, page_size], what
+    paged_weights and paged_evict work on: the slots get 0 and the token's position."""
+    rc = _lib.binding().paged_rope_write(q, k, v, positions, slots, frequencies, k_pages, v_pages,
+                                         _interleaved(layout), scale, q_out, row_weights,
+                                         row_positions, error_flag)
+    if not isinstance(rc, int):
+        return rc
+    if rc < 0:
+        dev = _explain_device(q)
+        _explain_pool(dev, k_pages, v_pages)
+        dtype, heads, T = k_pages.dtype, k_pages.shape[1], q.shape[0]
+        _explain_rows(dev, "q", q, dtype, None, None, HEAD_DIM)
+        _explain_rows(dev, "k", k, dtype, T, heads, HEAD_DIM)
+        _explain_rows(dev, "v", v, dtype, T, heads, HEAD_DIM)
+        _explain_rope(dev, positions, frequencies, T, scale)
+        _explain(dev, ("slots", slots, torch.int64, (T,)),
+                 ("error_flag", error_flag, torch.int32, (1,)))
+        if q_out is not None:
+            _explain_rows(dev, "q_out", q_out, dtype, T, q.shape[1], HEAD_DIM)
+        _explain_records(dev, k_pages, row_weights, row_positions)
+        raise ValueError("paged_rope_write: unexpected tensors")
+    _lib.check(rc, "paged_rope_write")
+
+
+# ------------------------------------------------- attention weights, eviction --
+
+def paged_weights(q: torch.Tensor, k_pages: torch.Tensor, block_table: torch.Tensor,
+                  cu_q: torch.Tensor, kv_lens: torch.Tensor, lse: torch.Tensor,
+                  row_weights: torch.Tensor, *, max_q_len: int, max_kv_len: int, window: int = 0,
+                  last: int = 0, softmax_scale: float | None = None,
+                  error_flag: torch.Tensor | None = None) -> None:
+    """Adds to row_weights [pages, kv_heads, page_size] float32 what a paged_attention call's
+    tokens gave each row of the cache (tw_paged_weights): the softmax weights, summed over the
+    tokens that see the row and the query heads of its KV head.
+
+    Arguments as of that call, and its lse [T, q_heads].  last > 0: only the last `last` new
+    tokens of each request count."""
+    rc = _lib.binding().paged_weights(q, k_pages, block_table, cu_q, kv_lens, lse, row_weights,
+                                      max_q_len, max_kv_len, window, last, softmax_scale,
+                                      error_flag)
+    if rc is None:
+        return
+    if rc < 0:
+        dev = _explain_device(q)
+        _explain_pool(dev, k_pages, k_pages)
+        if q.dim() != 3 or q.shape[1] == 0 or q.shape[1] % k_pages.shape[1]:
+            raise ValueError("q must be [T, q_heads, 128], q_heads a multiple of kv_heads")
+        _explain_rows(dev, "q", q, k_pages.dtype, None, q.shape[1], HEAD_DIM)
+        i32, B = torch.int32, kv_lens.shape[0] if kv_lens.dim() == 1 else -1
+        _explain(dev, ("kv_lens", kv_lens, i32, (None,)), ("cu_q", cu_q, i32, (B + 1,)),
+                 ("block_table", block_table, i32, (B, None)),
+                 ("lse", lse, torch.float32, q.shape[:2]),
+                 ("error_flag", error_flag, i32, (1,)))
+        if lse is None or not lse.is_contiguous():
+            raise ValueError("lse must be contiguous [T, q_heads] float32")
+        if row_weights is None:
+            raise ValueError("row_weights must be a tensor")
+        _explain_records(dev, k_pages, row_weights, None)
+        raise ValueError("paged_weights: unexpected tensors")
+    _lib.check(rc, "paged_weights")
+
+
+def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, row_weights: torch.Tensor,
+                row_positions: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor,
+                keep: torch.Tensor, offsets: torch.Tensor, *, max_len: int, sink: int, recent: int,
+                lens_out: torch.Tensor, offsets_out: torch.Tensor,
+                free_pages: torch.Tensor | None = None, free_count: torch.Tensor | None = None,
+                free_count_out: torch.Tensor | None = None,
+                error_flag: torch.Tensor | None = None) -> None:
+    """Cuts requests of more than keep [B] rows to those that were given most, in one launch
+    (tw_paged_evict): in each layer and KV head the rows at positions below `sink` and the
+    last `recent` ones, then those of the largest row_weights, ties in row order.
+
+    Pools [pages, kv_heads, page_size, 128] of one layer or [layers, ...] of several that share
+    the block table, records [(layers,) pages, kv_heads, page_size].  lens [B] rows held (at
+    most max_len), keep < 0: the request stays as it is, offsets [B] tokens it has lost before;
+    lens_out and offsets_out are the new ones.  Rows that stay fill the first `keep` places in
+    no fixed order: row_positions says which is which.  With free_pages, free_count and
+    free_count_out (as in paged_step) the pages past the last row go back on the stack; entries
+    of the block table past a request's end are not used.  Pages must not be shared by
+    requests."""
+    rc = _lib.binding().paged_evict(k_pages, v_pages, row_weights, row_positions, block_table,
+                                    lens, keep, offsets, max_len, sink, recent, lens_out,
+                                    offsets_out, free_pages, free_count, free_count_out,
+                                    error_flag)
+    if rc is None:
+        return
+    if rc < 0:
+        dev, i32 = _explain_device(k_pages), torch.int32
+        if k_pages.dim() == 5 and k_pages.shape[0] and v_pages.shape == k_pages.shape:
+            if k_pages.shape[0] > 1 and (k_pages.stride(0) != v_pages.stride(0)
+                                         or k_pages.stride(0) <= 0 or k_pages.stride(0) % 8):
+                raise ValueError("layers of k_pages and v_pages must have one stride, a multiple "
+                                 "of 8")
+            _explain_pool(dev, k_pages[0], v_pages[0])
+        else:
+            _explain_pool(dev, k_pages, v_pages)
+        if row_weights is None or row_positions is None:
+            raise ValueError("row_weights and row_positions must be tensors")
+        _explain_records(dev, k_pages, row_weights, row_positions)
+        if row_weights.dim() == 4 and row_weights.stride(0) != row_positions.stride(0):
+            raise ValueError("layers of row_weights and row_positions must have one stride")
+        B = lens.shape[0] if lens.dim() == 1 else -1
+        pages = k_pages.shape[-4]
+        _explain(dev, ("lens", lens, i32, (None,)), ("keep", keep, i32, (B,)),
+                 ("offsets", offsets, i32, (B,)), ("block_table", block_table, i32, (B, None)),
+                 ("lens_out", lens_out, i32, (B,)), ("offsets_out", offsets_out, i32, (B,)),
+                 ("free_pages", free_pages, i32, (pages,)), ("free_count", free_count, i32, (1,)),
+                 ("free_count_out", free_count_out, i32, (1,)),
+                 ("error_flag", error_flag, i32, (1,)))
+        raise ValueError("paged_evict: unexpected tensors")
+    _lib.check(rc, "paged_evict")
