@@ -25,12 +25,12 @@ def rope(x, positions, frequencies, layout, scale=1.0, inverse=False):
     y[..., i], y[..., j] = a * cos - b * sin, b * cos + a * sin
     both = (a.abs() + b.abs()) * abs(scale)
     big[..., i], big[..., j] = both, both
-    # sine and cosine: 2 units of the last place, the angle's reduction (one rounding of a
-    # part of a turn: 2^-25 turns, and 2^-53 of the 64-bit angle), scale, product, sum: 3
-    # roundings; then the rounding to the type
+    # sine and cosine: 2^-21.19 and 2^-21.41 (CUDA's documents, for [-pi, pi]), the angle's
+    # reduction (two roundings of a part of a turn: 2^-24 turns, 2 pi's: 2^-24 of pi, and
+    # 2^-53 of the 64-bit angle), scale, product, sum: 3 roundings; then the rounding to the type
     turns = (positions.double().abs()[:, None, None] * frequencies.abs().max().clamp(min=1e-9)
              if n else 0.0)
-    arithmetic = big * (2 * 2.0 ** -23 + 2 * math.pi * 2.0 ** -25 + 3 * 2.0 ** -24
+    arithmetic = big * (2.0 ** -21.19 + 3 * math.pi * 2.0 ** -24 + 3 * 2.0 ** -24
                         + turns * 4 * 2.0 ** -53)
     tol = y.abs() * UNIT[x.dtype] + arithmetic * (1 + UNIT[x.dtype]) + smallest(x.dtype)
     tol[..., 2 * n:] = 0.0

@@ -27,15 +27,16 @@ constexpr int kEvThreads = 512, kEvWarps = kEvThreads / 32;
 constexpr int kEvBins = 2048, kEvRounds = 3;
 constexpr int kEvMaxCluster = 8;
 constexpr int kEvMaxRequests = 8192;
-constexpr int kEvRowsPerCta = 2048;        // a cluster is as large as this asks for
+constexpr int kEvRowsPerCta = 4096;        // a cluster is as large as this asks for
 constexpr int kEvMaxRows = 1 << 21;        // of a request: 8 CTAs' bits of its rows
 constexpr int kEvSmem = 160 << 10;         // besides the histograms
-constexpr int kEvBatch = 8;                // rows that a warp copies at a time
+constexpr int kEvBatch = 4;                // rows that a warp copies at a time
 constexpr uint32_t kEvProtected = 0xffffffffu;
 
 struct EvictTask {
   int request, layer, head;
   int len, keep;
+  int more;        // tasks that may follow it
   long long next;  // the position after the request's last
 };
 
@@ -61,35 +62,46 @@ __device__ __forceinline__ int evict_kept(const tw_paged_evict_args& a, int len,
   return held && keep >= 0 && keep < len ? keep : len;
 }
 
-// The place of a row in K / V and in the records; -1: its page is none.  (A row beyond the
-// request has none either: what a call that changes the weights meanwhile could make of the
-// list stays inside the buffers.)
+// Where row j is: page and row of the page; page -1: its page is none.
 struct EvictRow {
-  int64_t row, record;
+  int page, row;
 };
 __device__ __forceinline__ EvictRow evict_row(const tw_paged_evict_args& a, const EvictTask& t,
                                               int j) {
-  if ((unsigned)j >= (unsigned)t.len) return {-1, -1};
   const unsigned i = (unsigned)j / (unsigned)a.pool.page_size;
-  const int o = j - (int)(i * (unsigned)a.pool.page_size);
   const int page = a.block_table[(int64_t)t.request * a.table_stride + i];
   if (page < 0 || page >= a.pool.num_pages) {
     raise_error(a.error_flag, TW_ERR_INVALID_INDEX);
-    return {-1, -1};
+    return {-1, 0};
   }
-  return {(int64_t)t.layer * a.layer_stride + (int64_t)page * a.pool.page_stride +
-              (int64_t)t.head * a.pool.head_stride + (int64_t)o * a.pool.token_stride,
-          (int64_t)t.layer * a.record_layer_stride +
-              ((int64_t)page * a.pool.kv_heads + t.head) * a.pool.page_size + o};
+  return {page, j - (int)(i * (unsigned)a.pool.page_size)};
+}
+// (What a call that changes weights meanwhile could leave in the list stays inside the buffers.)
+__device__ __forceinline__ bool evict_real(const tw_paged_evict_args& a, EvictRow r) {
+  return (unsigned)r.page < (unsigned)a.pool.num_pages &&
+         (unsigned)r.row < (unsigned)a.pool.page_size;
+}
+// In a layer and head's records, and its K or V (in 16-byte vectors).
+__device__ __forceinline__ int64_t evict_record(const tw_paged_evict_args& a, const EvictTask& t,
+                                                EvictRow r) {
+  return (int64_t)t.layer * a.record_layer_stride +
+         ((int64_t)r.page * a.pool.kv_heads + t.head) * a.pool.page_size + r.row;
+}
+__device__ __forceinline__ int64_t evict_vector(const tw_paged_evict_args& a, const EvictTask& t,
+                                                EvictRow r) {
+  return ((int64_t)t.layer * a.layer_stride + (int64_t)r.page * a.pool.page_stride +
+          (int64_t)t.head * a.pool.head_stride + (int64_t)r.row * a.pool.token_stride) /
+         kPagedAlign;
 }
 
 // 32 bits that order as the ranking: a NaN weight above all others, -0 as 0.
 __device__ __forceinline__ uint32_t evict_key(const tw_paged_evict_args& a, const EvictTask& t,
                                               int j) {
   const EvictRow r = evict_row(a, t, j);
-  if (r.record < 0) return 0u;
-  const float w = a.row_weights[r.record] + 0.f;
-  const long long p = a.row_positions[r.record];
+  if (r.page < 0) return 0u;
+  const int64_t at = evict_record(a, t, r);
+  const float w = a.row_weights[at] + 0.f;
+  const long long p = a.row_positions[at];
   if (p < a.sink || p >= t.next - a.recent) return kEvProtected;
   if (w != w) return kEvProtected - 1;
   const uint32_t u = __float_as_uint(w);
@@ -165,10 +177,11 @@ __device__ void evict_lengths(const tw_paged_evict_args& a, uint32_t* s_back,
     *a.free_count_out = (int)min(count + base, (long long)a.pool.num_pages);
 }
 
-__global__ void __launch_bounds__(kEvThreads)
+__global__ void __launch_bounds__(kEvThreads, 2)
 paged_evict_kernel(const __grid_constant__ EvictWork w) {
   extern __shared__ __align__(16) uint32_t s_dyn[];
   __shared__ EvictShared sh;
+  for (int i = threadIdx.x; i < kEvRounds * kEvBins; i += kEvThreads) (&sh.hist[0][0])[i] = 0;
   pdl_wait();
   pdl_launch_dependents();
   const tw_paged_evict_args& a = w.a;
@@ -184,8 +197,9 @@ paged_evict_kernel(const __grid_constant__ EvictWork w) {
   uint32_t* s_eq = s_keep + w.words;      // its key is the keep-th largest
   uint32_t* s_holes = s_eq + w.words;     // free places before a word of rows, of all CTAs
   uint32_t* s_movers = s_holes + w.words; // rows that move before it
-  uint32_t* s_key = s_movers + w.words;   // keys; then free places and rows that move there
-  const uint32_t pairs_held = (uint32_t)w.held / 2;
+  uint32_t* s_key = s_movers + w.words;   // keys; then free places and the rows that move there
+  EvictRow* s_list = reinterpret_cast<EvictRow*>(s_key);
+  const uint32_t pairs_held = (uint32_t)w.held / 4;
 
   const int64_t tasks = (int64_t)a.requests * w.units;
   int64_t at = mine;  // first task that may be next
@@ -193,14 +207,15 @@ paged_evict_kernel(const __grid_constant__ EvictWork w) {
     // ---- the next task that evicts anything: found by the first CTA, so that all of the
     // cluster do the same whatever becomes of the lengths meanwhile
     if (rank == 0 && warp == 0) {
-      EvictTask t = {-1, 0, 0, 0, 0, 0};
+      EvictTask t = {-1, 0, 0, 0, 0, 0, 0};
       while (at < tasks) {
         const int64_t x = at + (int64_t)lane * clusters;
-        int len = 0, kept = 0;
+        int len = 0, kept = 0, gone = 0;
         if (x < tasks) {
           const int b = (int)(x / w.units);
           len = max(a.lens[b], 0);
           kept = evict_kept(a, len, a.keep[b]);
+          gone = a.offsets[b];
         }
         const unsigned found = __ballot_sync(0xffffffffu, kept < len);
         if (!found) {
@@ -215,13 +230,13 @@ paged_evict_kernel(const __grid_constant__ EvictWork w) {
         t.head = unit - t.layer * a.pool.kv_heads;
         t.len = __shfl_sync(0xffffffffu, len, first);
         t.keep = __shfl_sync(0xffffffffu, kept, first);
-        t.next = (long long)t.len + a.offsets[t.request];
+        t.next = (long long)t.len + __shfl_sync(0xffffffffu, gone, first);
         at += clusters;
+        t.more = at < tasks;
         break;
       }
       if (lane == 0) sh.task = t;
     }
-    for (int i = tid; i < kEvRounds * kEvBins; i += kEvThreads) (&sh.hist[0][0])[i] = 0;
     cluster.sync();
     const EvictTask t = *cluster.map_shared_rank(&sh.task, 0);
     if (t.request < 0) break;
@@ -258,7 +273,9 @@ paged_evict_kernel(const __grid_constant__ EvictWork w) {
       constexpr int kEach = kEvBins / kEvThreads;
       uint32_t bin[kEach] = {};
       const int first = kEvBins - kEach * (tid + 1);
-      for (int r = 0; r < C; ++r) {
+#pragma unroll
+      for (int r = 0; r < kEvMaxCluster; ++r) {
+        if (r >= C) break;
         const uint4 x = *reinterpret_cast<const uint4*>(
             cluster.map_shared_rank(&sh.hist[round][first], r));
         bin[0] += x.w;
@@ -374,7 +391,7 @@ paged_evict_kernel(const __grid_constant__ EvictWork w) {
       const auto put = [&](uint32_t list, uint32_t k, int row) {
         if (k < done || k - done >= pairs_held * C) return;
         const uint32_t i = k - done;
-        *cluster.map_shared_rank(&s_key[list * pairs_held + i / C], i % C) = (uint32_t)row;
+        *cluster.map_shared_rank(&s_list[list * pairs_held + i / C], i % C) = evict_row(a, t, row);
       };
       for (int x = warp; x < words; x += kEvWarps) {
         const uint32_t h = holes_of(x), m = movers_of(x), below = (1u << lane) - 1;
@@ -385,36 +402,50 @@ paged_evict_kernel(const __grid_constant__ EvictWork w) {
       cluster.sync();
       const uint32_t here = min(pairs - done, pairs_held * C);  // of all CTAs
       const int count = (int)((here + C - 1 - rank) / C);       // of this one
+      uint4* const pages = reinterpret_cast<uint4*>(lane < kVecPerRow16 ? a.pool.k_pages
+                                                                        : a.pool.v_pages) +
+                           lane % kVecPerRow16;
       for (int first = warp * kEvBatch; first < count; first += kEvWarps * kEvBatch) {
-        const int i = first + lane;
-        EvictRow from = {-1, -1}, to = {-1, -1};
-        if (lane < kEvBatch && i < count) {
-          to = evict_row(a, t, (int)s_key[i]);
-          from = evict_row(a, t, (int)s_key[pairs_held + i]);
-          if (from.row < 0 || to.row < 0) {
-            from.row = to.row = -1;
-          } else {
-            a.row_weights[to.record] = a.row_weights[from.record];
-            a.row_positions[to.record] = a.row_positions[from.record];
-          }
-        }
-        uint4* const pages = reinterpret_cast<uint4*>(lane < kVecPerRow16 ? a.pool.k_pages
-                                                                          : a.pool.v_pages);
-        const int c = lane % kVecPerRow16;
         uint4 x[kEvBatch];
-        int64_t place[kEvBatch];
+        float weight;
+        int position;
+        const bool record = lane < kEvBatch && first + lane < count;
 #pragma unroll
         for (int y = 0; y < kEvBatch; ++y) {
-          const int64_t source = __shfl_sync(0xffffffffu, (long long)from.row, y);
-          place[y] = __shfl_sync(0xffffffffu, (long long)to.row, y);
-          if (place[y] >= 0) x[y] = pages[source / kPagedAlign + c];
+          const EvictRow from =
+              first + y < count ? s_list[pairs_held + first + y] : EvictRow{-1, 0};
+          x[y] = make_uint4(0u, 0u, 0u, 0u);
+          if (evict_real(a, from)) x[y] = pages[evict_vector(a, t, from)];
+        }
+        EvictRow from = {-1, 0}, to = {-1, 0};
+        if (record) {
+          to = s_list[first + lane];
+          from = s_list[pairs_held + first + lane];
+        }
+        const bool moves = evict_real(a, from) && evict_real(a, to);
+        if (moves) {
+          weight = a.row_weights[evict_record(a, t, from)];
+          position = a.row_positions[evict_record(a, t, from)];
         }
 #pragma unroll
-        for (int y = 0; y < kEvBatch; ++y)
-          if (place[y] >= 0) pages[place[y] / kPagedAlign + c] = x[y];
+        for (int y = 0; y < kEvBatch; ++y) {
+          if (first + y < count && evict_real(a, s_list[first + y]) &&
+              evict_real(a, s_list[pairs_held + first + y]))
+            pages[evict_vector(a, t, s_list[first + y])] = x[y];
+        }
+        if (moves) {
+          a.row_weights[evict_record(a, t, to)] = weight;
+          a.row_positions[evict_record(a, t, to)] = position;
+        }
       }
-      cluster.sync();
+      if (pairs - done > pairs_held * C) cluster.sync();
     }
+    if (!t.more) {
+      // (with pairs, a barrier has come after the last access to another CTA's memory)
+      if (pairs == 0) cluster.sync();
+      return;
+    }
+    for (int i = tid; i < kEvRounds * kEvBins; i += kEvThreads) (&sh.hist[0][0])[i] = 0;
   }
   cluster.sync();  // the first CTA's memory has been read
 }
@@ -464,7 +495,7 @@ extern "C" int tw_paged_evict(const tw_paged_evict_args* args, void* stream) {
   w.units = a.layers * a.pool.kv_heads;
   int C = 1;
   while (C < kEvMaxCluster && a.max_len > C * kEvRowsPerCta) C *= 2;
-  const int seg = max(((a.max_len + C - 1) / C + 31) / 32 * 32, 64);
+  const int seg = max(((a.max_len + C - 1) / C + 31) / 32 * 32, 128);
   w.words = seg / 32;
   w.held = min(seg, (kEvSmem - 16 * w.words) / 4);
   const int smem = max(16 * w.words + 4 * w.held, 4 * a.requests);

@@ -19,20 +19,33 @@
 #include "paged_attention.cuh"
 #include "tensor.cuh"
 
+#include <type_traits>
+
 namespace tw {
 
 constexpr int kWtKeys = 256, kWtCols = 128;
-constexpr int kWtSumThreads = 256, kWtThreads = 384;
-constexpr int kWtMmaWarp = 8, kWtKeyWarp = 9, kWtRowWarp = 10, kWtLseWarp = 11;
+constexpr int kWtSumThreads = 512, kWtThreads = 640;  // two groups of 256 sum
+constexpr int kWtMmaWarp = 16, kWtRowWarp = 17, kWtKeyWarp = 18;  // and 19
+constexpr int kWtAhead = 2;                // tiles whose log-sum-exps are read at a time
 constexpr int kWtHalfTile = 128 * 128;     // bytes: 128 rows of 64 elements
 constexpr int kWtTile = 2 * kWtHalfTile;
-constexpr int kWtSlots = 7;                // of shared memory, a tile each:
-// K of two items and three tiles of q; where a cluster takes an item, K of one, four tiles
-// of q, and the sums of the other CTAs
-template <bool kSplit> constexpr int kWtKeySlots = kSplit ? 1 : 2;
-template <bool kSplit> constexpr int kWtRowSlots = kSplit ? 4 : 3;
+constexpr int kWtSlots = 7;                // of shared memory, a tile each
+
+// How a call's items are done.
+enum WeightMode {
+  kWtWhole,  // a CTA takes an item; K of two items and three tiles of q in shared memory
+  kWtSplit,  // a cluster takes one; K of one, four tiles of q, and the sums of the other CTAs
+  kWtFew     // at most 16 (token, head) rows a request: K of three, eight tiles of 16 rows
+};
+template <int kMode> struct WeightLayout {
+  static constexpr int kKeySlots = kMode == kWtFew ? 3 : kMode == kWtSplit ? 1 : 2;
+  static constexpr int kRowSlots = kMode == kWtFew ? 8 : kMode == kWtSplit ? 4 : 3;
+  static constexpr int kCols = kMode == kWtFew ? 16 : kWtCols;   // rows of a tile of q
+  static constexpr int kRowHalf = kCols * 128;                   // bytes: 64 dimensions of them
+  static constexpr int kRowTile = 2 * kRowHalf;
+};
 constexpr int kWtLseSlots = 3;
-constexpr int kWtSmem = kWtSlots * kWtTile + 1024;
+constexpr int kWtFma = 6;                  // one pair in this many on the FMA pipe
 constexpr int kWtColumns = 512;            // S^T: 2 halves of the keys, 2 tiles, 128 columns
 constexpr int kWtMaxCluster = 8;
 static_assert((kWtMaxCluster - 1) * kWtKeys * 4 <= kWtTile);
@@ -126,15 +139,20 @@ struct WeightWalk {
 };
 
 struct WeightShared {
-  uint64_t k_full[2], k_empty[2];
-  uint64_t q_full[4], q_empty[4];
+  uint64_t k_full[3], k_empty[3];
+  uint64_t q_full[8], q_empty[8];
   uint64_t lse_full[kWtLseSlots], lse_empty[kWtLseSlots];
   uint64_t s_full[2][2], s_free[2][2];  // [half][tile]
-  uint64_t part_full, part_free, drain;
+  uint64_t sums_full, sums_free, part_full, part_free, drain;
   uint32_t tmem;
   volatile int abort;
+  float sums[kWtKeys];                          // of the second group's
   alignas(16) float lse[kWtLseSlots][kWtCols];  // minus the log-sum-exps
 };
+
+// No static shared memory beside it: the tiles begin on a boundary of 1024 bytes.
+constexpr int kWtSmem = kWtSlots * kWtTile + (int)sizeof(WeightShared);
+static_assert(kWtSmem <= 232448);
 
 // Barriers and memory of another CTA of the cluster.
 __device__ __forceinline__ uint32_t remote(uint32_t addr, int rank) {
@@ -170,19 +188,48 @@ __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
 
+// 2^x of a pair on the FMA pipe, for all x (below -126.5: 0, from 127.5 on: infinity, NaN:
+// NaN): n = x rounded to a whole number by adding 1.5 * 2^23, 2^(x - n) on [-1/2, 1/2] by the
+// polynomial of degree 5 with the smallest largest relative error there (Remez exchange;
+// 2.2e-7 with its roundings, as the special-function unit's), times 2^n put together from
+// its bits.
+__device__ __forceinline__ void ex2_five(uint64_t x2, float& e0, float& e1) {
+  float x0, x1;
+  unpair(x2, x0, x1);
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x0) : "f"(-127.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x1) : "f"(-127.f));
+  asm("min.NaN.f32 %0, %0, %1;" : "+f"(x0) : "f"(128.f));
+  asm("min.NaN.f32 %0, %0, %1;" : "+f"(x1) : "f"(128.f));
+  x2 = pair(x0, x1);
+  const uint64_t round = pair(12582912.f, 12582912.f), back = pair(-12582912.f, -12582912.f);
+  const uint64_t r = add2(x2, round);
+  const uint64_t f = fma2(add2(r, back), pair(-1.f, -1.f), x2);
+  uint64_t p = pair(0x1.5c08e6p-10f, 0x1.5c08e6p-10f);
+  p = fma2(p, f, pair(0x1.3d0c52p-7f, 0x1.3d0c52p-7f));
+  p = fma2(p, f, pair(0x1.c6b6e4p-5f, 0x1.c6b6e4p-5f));
+  p = fma2(p, f, pair(0x1.ebf918p-3f, 0x1.ebf918p-3f));
+  p = fma2(p, f, pair(0x1.62e428p-1f, 0x1.62e428p-1f));
+  p = fma2(p, f, pair(0x1.000002p+0f, 0x1.000002p+0f));
+  float r0, r1;
+  unpair(r, r0, r1);
+  p = mul2(p, pair(__int_as_float((__float_as_int(r0) << 23) + 0x3f800000),
+                   __int_as_float((__float_as_int(r1) << 23) + 0x3f800000)));
+  unpair(p, e0, e1);
+}
+
 // The lowest n bits (n <= 0: none, n >= 32: all).
 __device__ __forceinline__ uint32_t first_bits(int n) {
   return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1;
 }
 
-template <bool kBf16, bool kSplit>
+template <bool kBf16, int kMode>
 __global__ void __launch_bounds__(kWtThreads, 1)
 paged_weights_kernel(const __grid_constant__ WeightWork w,
                      const __grid_constant__ CUtensorMap k_map,
                      const __grid_constant__ CUtensorMap q_map,
                      const __grid_constant__ CUtensorMap few_map) {
-  extern __shared__ char s_raw[];
-  __shared__ WeightShared sh;
+  extern __shared__ __align__(1024) char smem[];
+  WeightShared& sh = *reinterpret_cast<WeightShared*>(smem + kWtSlots * kWtTile);
   pdl_wait();
   pdl_launch_dependents();
   const tw_paged_weights_args& a = w.a;
@@ -191,15 +238,23 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
   uint32_t cluster_rank, cluster_ctas;
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(cluster_rank));
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(cluster_ctas));
+  constexpr bool kSplit = kMode == kWtSplit;
   const int rank = kSplit ? (int)cluster_rank : 0, S = kSplit ? (int)cluster_ctas : 1;
-  constexpr int kKeySlots = kWtKeySlots<kSplit>, kRowSlots = kWtRowSlots<kSplit>;
+  using Layout = WeightLayout<kMode>;
+  constexpr int kKeySlots = Layout::kKeySlots, kRowSlots = Layout::kRowSlots;
+  constexpr int kCols = Layout::kCols, kRowHalf = Layout::kRowHalf, kRowTile = Layout::kRowTile;
+  static_assert(2 * kKeySlots * kWtTile + kRowSlots * kRowTile <=
+                (kSplit ? kWtSlots - 1 : kWtSlots) * kWtTile);
   const long long first_item = blockIdx.x / S, step = gridDim.x / S;
-  char* smem = (char*)(((uintptr_t)s_raw + 1023) & ~(uintptr_t)1023);
   const uint32_t keys_at = smem_addr(smem), rows_at = keys_at + 2 * kKeySlots * kWtTile;
   float* s_part = reinterpret_cast<float*>(smem + (kWtSlots - 1) * kWtTile);  // kSplit: [rank - 1][key]
+  if (keys_at & 1023) {  // (what the layout of the products rests on)
+    if (tid == 0) raise_error(a.error_flag, TW_ERR_UNSUPPORTED);
+    return;
+  }
   if (tid == 0) {
     for (int i = 0; i < kKeySlots; ++i) {
-      mbar_init(&sh.k_full[i], 1);
+      mbar_init(&sh.k_full[i], 2);
       mbar_init(&sh.k_empty[i], 1);
     }
     for (int i = 0; i < kRowSlots; ++i) {
@@ -208,27 +263,28 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
     }
     for (int i = 0; i < kWtLseSlots; ++i) {
       mbar_init(&sh.lse_full[i], 1);
-      mbar_init(&sh.lse_empty[i], kWtSumThreads / 32);
+      mbar_init(&sh.lse_empty[i], kWtSumThreads / 2 / 32);
     }
     for (int i = 0; i < 2; ++i)
       for (int j = 0; j < 2; ++j) {
         mbar_init(&sh.s_full[i][j], 1);
         mbar_init(&sh.s_free[i][j], 4);
       }
+    mbar_init(&sh.sums_full, kWtKeys / 32);
+    mbar_init(&sh.sums_free, kWtKeys / 32);
     if (kSplit) {
-      mbar_init(&sh.part_full, (uint32_t)((S - 1) * (kWtSumThreads / 32)));
-      mbar_init(&sh.part_free, kWtSumThreads / 32);
+      mbar_init(&sh.part_full, (uint32_t)((S - 1) * (kWtKeys / 32)));
+      mbar_init(&sh.part_free, kWtKeys / 32);
     }
     mbar_init(&sh.drain, 1);
     sh.abort = 0;
     mbar_init_fence();
   }
   // columns that no token fills (groups that do not divide 128) stay zero rows
-  for (int i = tid; i < kRowSlots * 2 * (kWtCols - T * R) * 8; i += kWtThreads) {
-    const int tile = i / ((kWtCols - T * R) * 8), at = i % ((kWtCols - T * R) * 8);
-    *reinterpret_cast<uint4*>(smem + 2 * kKeySlots * kWtTile + tile * kWtHalfTile +
-                              T * R * 128 + at * 16) = make_uint4(0u, 0u, 0u, 0u);
-  }
+  const int spare = (kCols - T * R) * 8;  // 16-byte vectors of 64 dimensions
+  for (int i = tid; i < kRowSlots * 2 * spare; i += kWtThreads)
+    *reinterpret_cast<uint4*>(smem + 2 * kKeySlots * kWtTile + i / spare * kRowHalf + T * R * 128 +
+                              i % spare * 16) = make_uint4(0u, 0u, 0u, 0u);
   fence_async_smem();
   if (warp == kWtMmaWarp) tmem_alloc(&sh.tmem, kWtColumns);
   tmem_fence_before();
@@ -240,17 +296,18 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
   WeightWalk walk;
   WeightItem x;
   bool ok = true;
-  if (warp == kWtKeyWarp) {
-    // ---- K of the items
+  if (warp >= kWtKeyWarp) {
+    // ---- K of the items: a warp for each 128 keys
+    const int h = warp - kWtKeyWarp;
     if (elect_one()) prefetch_map(&k_map);
     __syncwarp();
     const uint32_t box_bytes = (uint32_t)w.box * 128;  // of 64 dimensions
-    const int boxes = kWtKeys / w.box;                 // at most 32
+    const int boxes = 128 / w.box;                     // at most 16
     int n = 0;
     for (long long item = first_item; walk.find(w, lane, item, x); item += step) {
       if (rank >= x.tiles) continue;
       const int s = n % kKeySlots;
-      const int key = x.key0 + lane * w.box;
+      const int key = x.key0 + h * 128 + lane * w.box;
       const bool wanted = lane < boxes && key < x.end && key + w.box > x.begin;
       int p = 0, row = 0;
       if (wanted) {
@@ -263,7 +320,7 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
         }
       }
       const uint32_t all = __ballot_sync(0xffffffffu, wanted);
-      const int from = __ffs(all) - 1, to = 32 - __clz(all);
+      const int from = all ? __ffs(all) - 1 : 0, to = 32 - __clz(all);
       if (n >= kKeySlots) {
         ok = __all_sync(0xffffffffu, mbar_wait(&sh.k_empty[s],
                                                (uint32_t)((n / kKeySlots - 1) & 1), &sh.abort));
@@ -282,9 +339,8 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
 #pragma unroll
           for (int y = 0; y < 4; ++y)
             if (y0 + y < to) {
-              const int r = (y0 + y) * w.box;  // of the block's 256
-              const uint32_t dst = keys_at + (uint32_t)(s * 2 + (r >> 7)) * kWtTile +
-                                   (uint32_t)(r & 127) * 128;
+              const uint32_t dst = keys_at + (uint32_t)(s * 2 + h) * kWtTile +
+                                   (uint32_t)((y0 + y) * w.box) * 128;
               tma_load_4d(&k_map, dst, &sh.k_full[s], 0, rx[y], x.head, px[y]);
               tma_load_4d(&k_map, dst + kWtHalfTile, &sh.k_full[s], 64, rx[y], x.head, px[y]);
             }
@@ -299,32 +355,66 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
         mbar_wait(&sh.k_full[i % kKeySlots], (uint32_t)((i / kKeySlots) & 1), &never);
     }
   } else if (warp == kWtRowWarp) {
-    // ---- tiles of q
+    // ---- tiles of q and their rows' log-sum-exps
     if (elect_one()) {
       prefetch_map(&q_map);
       prefetch_map(&few_map);
     }
     __syncwarp();
-    int n = 0;
+    int n = 0, nl = 0;  // tiles copied; with their log-sum-exps
     for (long long item = first_item; ok && walk.find(w, lane, item, x); item += step) {
-      for (int t = rank; t < x.tiles; t += S, ++n) {
-        const int s = n % kRowSlots;
-        if (n >= kRowSlots) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&sh.q_empty[s],
-                                                 (uint32_t)((n / kRowSlots - 1) & 1), &sh.abort));
-          if (!ok) break;
+      for (int t0 = rank; ok && t0 < x.tiles; t0 += kWtAhead * S) {
+        constexpr int kParts = (kCols + 31) / 32;
+        float z[kWtAhead][kParts];
+#pragma unroll
+        for (int y = 0; y < kWtAhead; ++y) {
+          const int i = x.from + (t0 + y * S) * T, cols = min(T, x.upto - i) * R;
+#pragma unroll
+          for (int c = 0; c < kParts; ++c) {
+            const int col = c * 32 + lane, token = col / R;
+            z[y][c] = col < cols ? -a.lse[(int64_t)(x.row0 + i + token) * a.q_heads + x.head * R +
+                                          (col - token * R)]
+                                 : -CUDART_INF_F;
+          }
         }
-        const int i = x.from + t * T, here = min(T, x.upto - i);
-        if (elect_one()) {
-          const uint32_t dst = rows_at + (uint32_t)s * kWtTile;
-          // rows past the last are masked
-          const bool few = here <= w.few_tokens;
-          const CUtensorMap* map = few ? &few_map : &q_map;
-          mbar_arrive_expect(&sh.q_full[s], (uint32_t)((few ? w.few_tokens : T) * R) * 256);
-          tma_load_3d(map, dst, &sh.q_full[s], 0, x.head * R, x.row0 + i);
-          tma_load_3d(map, dst + kWtHalfTile, &sh.q_full[s], 64, x.head * R, x.row0 + i);
+        for (int y = 0; y < kWtAhead && t0 + y * S < x.tiles; ++y, ++n) {
+          const int s = n % kRowSlots;
+          if (n >= kRowSlots) {
+            ok = __all_sync(0xffffffffu, mbar_wait(&sh.q_empty[s],
+                                                   (uint32_t)((n / kRowSlots - 1) & 1), &sh.abort));
+            if (!ok) break;
+          }
+          const int i = x.from + (t0 + y * S) * T, here = min(T, x.upto - i);
+          if (elect_one()) {
+            const uint32_t dst = rows_at + (uint32_t)s * kRowTile;
+            // rows past the last are masked
+            const bool few = kMode == kWtFew || here <= w.few_tokens;
+            const CUtensorMap* map = few ? &few_map : &q_map;
+            mbar_arrive_expect(&sh.q_full[s], (uint32_t)((few ? w.few_tokens : T) * R) * 256);
+            tma_load_3d(map, dst, &sh.q_full[s], 0, x.head * R, x.row0 + i);
+            tma_load_3d(map, dst + kRowHalf, &sh.q_full[s], 64, x.head * R, x.row0 + i);
+          }
+          __syncwarp();
         }
-        __syncwarp();
+        if (!ok) break;
+#pragma unroll
+        for (int y = 0; y < kWtAhead; ++y) {
+          if (t0 + y * S >= x.tiles) break;
+          const int s = nl % kWtLseSlots;
+          if (nl >= kWtLseSlots) {
+            ok = __all_sync(0xffffffffu,
+                            mbar_wait(&sh.lse_empty[s], (uint32_t)((nl / kWtLseSlots - 1) & 1),
+                                      &sh.abort));
+            if (!ok) break;
+          }
+          // (a row that saw nothing: no weight; its score less -infinity would be infinite)
+#pragma unroll
+          for (int c = 0; c < kParts; ++c)
+            sh.lse[s][c * 32 + lane] = z[y][c] == CUDART_INF_F ? -CUDART_INF_F : z[y][c];
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.lse_full[s]);
+          ++nl;
+        }
       }
     }
     if (!ok || sh.abort) {
@@ -332,37 +422,10 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
       for (int i = max(n - kRowSlots, 0); i < n; ++i)
         mbar_wait(&sh.q_full[i % kRowSlots], (uint32_t)((i / kRowSlots) & 1), &never);
     }
-  } else if (warp == kWtLseWarp) {
-    // ---- log-sum-exps of the tiles' rows
-    int n = 0;
-    for (long long item = first_item; ok && walk.find(w, lane, item, x); item += step) {
-      for (int t = rank; t < x.tiles; t += S, ++n) {
-        const int s = n % kWtLseSlots;
-        const int i = x.from + t * T, cols = min(T, x.upto - i) * R;
-        float z[kWtCols / 32];
-#pragma unroll
-        for (int c = 0; c < kWtCols / 32; ++c) {
-          const int col = c * 32 + lane, token = col / R;
-          z[c] = col < cols ? -a.lse[(int64_t)(x.row0 + i + token) * a.q_heads + x.head * R +
-                                     (col - token * R)]
-                            : -CUDART_INF_F;
-          // a row that saw nothing: no weight (its score less -infinity would be infinite)
-          if (z[c] == CUDART_INF_F) z[c] = -CUDART_INF_F;
-        }
-        if (n >= kWtLseSlots) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&sh.lse_empty[s],
-                                                 (uint32_t)((n / kWtLseSlots - 1) & 1), &sh.abort));
-          if (!ok) break;
-        }
-#pragma unroll
-        for (int c = 0; c < kWtCols / 32; ++c) sh.lse[s][c * 32 + lane] = z[c];
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.lse_full[s]);
-      }
-    }
   } else if (warp == kWtMmaWarp) {
     // ---- products
-    int nk = 0, nq = 0, ns[2] = {0, 0};
+    int nk = 0, nq = 0;
+    uint32_t used = 0, turn = 0;  // a bit per buffer of scores: used before; its phase
     for (long long item = first_item; ok && walk.find(w, lane, item, x); item += step) {
       if (rank >= x.tiles) continue;
       const int ks = nk % kKeySlots;
@@ -377,25 +440,26 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
         ok = __all_sync(0xffffffffu,
                         mbar_wait(&sh.q_full[qs], (uint32_t)((nq / kRowSlots) & 1), &sh.abort));
         for (int h = first_half ? 0 : 1; ok && h < halves; ++h) {
-          const int buf = ns[h] & 1;
-          if (ns[h] >= 2)
-            ok = __all_sync(0xffffffffu, mbar_wait(&sh.s_free[h][buf],
-                                                   (uint32_t)((ns[h] / 2 - 1) & 1), &sh.abort));
+          const int buf = nq & 1, bit = h * 2 + buf;  // a group of sums each
+          if (used >> bit & 1)
+            ok = __all_sync(0xffffffffu,
+                            mbar_wait(&sh.s_free[h][buf], ~(turn >> bit) & 1, &sh.abort));
           if (!ok) break;
+          used |= 1u << bit;
+          turn ^= 1u << bit;
           tmem_fence_after();
           if (elect_one()) {
             const uint32_t ka = keys_at + (uint32_t)(ks * 2 + h) * kWtTile,
-                           qa = rows_at + (uint32_t)qs * kWtTile;
+                           qa = rows_at + (uint32_t)qs * kRowTile;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const uint32_t off = (k >> 2) * kWtHalfTile + (k & 3) * 32;
-              mma_smem(tmem + (h * 2 + buf) * 128, operand_desc(ka + off, 16, 1024),
-                       operand_desc(qa + off, 16, 1024), desc, k > 0);
-            }
+            for (int k = 0; k < 8; ++k)
+              mma_smem(tmem + (h * 2 + buf) * 128,
+                       operand_desc(ka + (k >> 2) * kWtHalfTile + (k & 3) * 32, 16, 1024),
+                       operand_desc(qa + (k >> 2) * kRowHalf + (k & 3) * 32, 16, 1024), desc,
+                       k > 0);
             mma_commit(&sh.s_full[h][buf]);
           }
           __syncwarp();
-          ++ns[h];
         }
         if (ok && elect_one()) mma_commit(&sh.q_empty[qs]);
         __syncwarp();
@@ -411,17 +475,21 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
       mbar_wait(&sh.drain, 0, &never);
     }
   } else {
-    // ---- sums: a thread per key
-    const int h = warp >> 2;
-    const uint32_t my = tmem + ((uint32_t)((warp & 3) * 32) << 16) + h * 256;
+    // ---- sums: a thread per key and group; the groups take tiles in turn
+    const int group = warp >> 3, h = (warp >> 2) & 1, key = tid & (kWtKeys - 1);
+    const uint32_t my = tmem + ((uint32_t)((warp & 3) * 32) << 16) + h * 256 + group * 128;
     const uint64_t scale2 = pair(a.softmax_scale, a.softmax_scale);
     const uint64_t log2e2 = pair(1.4426950408889634f, 1.4426950408889634f);
-    int nl = 0, ns = 0, items = 0;
+    // tiles so far, those that this warp took, items, and those of them that both groups had
+    int nl = 0, ns = 0, items = 0, joins = 0;
     for (long long item = first_item; ok && walk.find(w, lane, item, x); item += step, ++items) {
-      const int j = x.key0 + tid;
+      // this CTA's tiles of the item, and whether the other group has some of them too
+      const int tiles = x.tiles > rank ? (x.tiles - rank - 1) / S + 1 : 0;
+      const bool both = tiles > 1, adds = group == (tiles == 1 ? nl & 1 : 0);
+      const int j = x.key0 + key;
       const bool held = j >= x.begin && j < x.end;
       int64_t place = -1;
-      if (held && rank == 0) {
+      if (held && rank == 0 && adds) {
         const int i = j / a.pool.page_size;
         const int page = a.block_table[(int64_t)x.request * a.table_stride + i];
         if (page >= 0 && page < a.pool.num_pages)
@@ -431,15 +499,15 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
       const bool mine = h == 0 ? x.begin < x.key0 + 128 : x.end > x.key0 + 128;
       float sum = 0.f;
       for (int t = rank; t < x.tiles; t += S, ++nl) {
+        if ((nl & 1) != group) continue;
         const int ls = nl % kWtLseSlots;
         // (also by warps with no keys: they must not hand a slot back twice in a phase)
         ok = __all_sync(0xffffffffu, mbar_wait(&sh.lse_full[ls],
                                                (uint32_t)((nl / kWtLseSlots) & 1), &sh.abort));
         if (!ok) break;
         if (mine) {
-          const int buf = ns & 1;
           ok = __all_sync(0xffffffffu,
-                          mbar_wait(&sh.s_full[h][buf], (uint32_t)((ns / 2) & 1), &sh.abort));
+                          mbar_wait(&sh.s_full[h][group], (uint32_t)(ns & 1), &sh.abort));
           if (!ok) break;
           ++ns;
           tmem_fence_after();
@@ -457,40 +525,32 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
               to = a.window > 0 ? (int)max(min((long long)here, (long long)j + a.window - p), 0ll) * R
                                 : cols;
           }
-          const uint32_t at = my + buf * 128;
-          const int chunks = (cols + 31) / 32;
-          float s[2][32];
+          const uint32_t at = my;
           uint64_t sum2[2] = {0ull, 0ull};
-          tmem_ld32(s[0], at);
+          // the columns [c0, c0 + N) of the tile, in s
+          const auto add_columns = [&](const auto& s, int c0, auto n, auto some) {
+            constexpr int N = decltype(n)::value;
+            constexpr bool masked = decltype(some)::value;
+            const uint32_t seen = first_bits(to - c0) & ~first_bits(from - c0);
+            const float4* z = reinterpret_cast<const float4*>(&sh.lse[ls][c0]);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            if (c >= chunks) break;
-            tmem_wait_ld(s[c & 1]);
-            if (c + 1 < chunks) {
-              tmem_ld32(s[(c + 1) & 1], at + (c + 1) * 32);
-            } else {
-              tmem_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&sh.s_free[h][buf]);
-            }
-            const uint32_t seen = first_bits(to - c * 32) & ~first_bits(from - c * 32);
-            // (columns that no token fills are zero rows: an infinite key would make them NaN)
-            const bool masked = !plain || (c + 1) * 32 > cols;
-            const float4* z = reinterpret_cast<const float4*>(&sh.lse[ls][c * 32]);
-#pragma unroll
-            for (int y = 0; y < 32; y += 4) {
+            for (int y = 0; y < N; y += 4) {
               const float4 l = z[y / 4];
-              const uint64_t d0 =
-                  mul2(fma2(pair(s[c & 1][y], s[c & 1][y + 1]), scale2, pair(l.x, l.y)), log2e2);
-              const uint64_t d1 = mul2(
-                  fma2(pair(s[c & 1][y + 2], s[c & 1][y + 3]), scale2, pair(l.z, l.w)), log2e2);
+              const uint64_t d0 = mul2(fma2(pair(s[y], s[y + 1]), scale2, pair(l.x, l.y)), log2e2);
+              const uint64_t d1 =
+                  mul2(fma2(pair(s[y + 2], s[y + 3]), scale2, pair(l.z, l.w)), log2e2);
               float e0, e1, e2, e3;
-              unpair(d0, e0, e1);
-              unpair(d1, e2, e3);
-              e0 = ex2(e0);
-              e1 = ex2(e1);
-              e2 = ex2(e2);
-              e3 = ex2(e3);
+              const auto weigh = [&](uint64_t d, int number, float& u, float& v) {
+                if (!masked && number % kWtFma == kWtFma - 1) {
+                  ex2_five(d, u, v);
+                } else {
+                  unpair(d, u, v);
+                  u = ex2(u);
+                  v = ex2(v);
+                }
+              };
+              weigh(d0, y / 2, e0, e1);
+              weigh(d1, y / 2 + 1, e2, e3);
               if (masked) {
                 e0 = seen >> y & 1 ? e0 : 0.f;
                 e1 = seen >> (y + 1) & 1 ? e1 : 0.f;
@@ -499,6 +559,36 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
               }
               sum2[0] = add2(sum2[0], pair(e0, e1));
               sum2[1] = add2(sum2[1], pair(e2, e3));
+            }
+          };
+          // (two pieces of code: in one, the compiler masks always)
+          const auto add = [&](const auto& s, int c0, auto n) {
+            // (columns that no token fills are zero rows: an infinite key would make them NaN)
+            if (plain && c0 + decltype(n)::value <= cols)
+              add_columns(s, c0, n, std::false_type{});
+            else
+              add_columns(s, c0, n, std::true_type{});
+          };
+          const auto read_all = [&] {  // the scores are in registers: the next tile's may come
+            tmem_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.s_free[h][group]);
+          };
+          if constexpr (kMode == kWtFew) {
+            float s[16];
+            tmem_ld16(s, at);
+            tmem_wait_ld(s);
+            read_all();
+            add(s, 0, std::integral_constant<int, 16>{});
+          } else {
+            const int chunks = (cols + 31) / 32;
+#pragma unroll 1
+            for (int c = 0; c < chunks; ++c) {
+              float s[32];
+              tmem_ld32(s, at + c * 32);
+              tmem_wait_ld(s);
+              if (c == chunks - 1) read_all();
+              add(s, c * 32, std::integral_constant<int, 32>{});
             }
           }
           float y0, y1;
@@ -509,20 +599,40 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
         if (lane == 0) mbar_arrive(&sh.lse_empty[ls]);
       }
       if (!ok) break;
+      if (both) {
+        if (group == 1) {
+          if (joins > 0)
+            ok = __all_sync(0xffffffffu,
+                            mbar_wait(&sh.sums_free, (uint32_t)((joins - 1) & 1), &sh.abort));
+          if (!ok) break;
+          sh.sums[key] = sum;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.sums_full);
+        } else {
+          ok = __all_sync(0xffffffffu,
+                          mbar_wait(&sh.sums_full, (uint32_t)(joins & 1), &sh.abort));
+          if (!ok) break;
+          sum += sh.sums[key];
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.sums_free);
+        }
+        ++joins;
+      }
+      if (!adds) continue;
       if constexpr (kSplit) {
         if (rank != 0) {
           if (items > 0)
             ok = __all_sync(0xffffffffu,
                             cluster_wait(&sh.part_free, (uint32_t)((items - 1) & 1), &sh.abort));
           if (!ok) break;
-          remote_store(s_part + (rank - 1) * kWtKeys + tid, 0, sum);
+          remote_store(s_part + (rank - 1) * kWtKeys + key, 0, sum);
           __syncwarp();
           if (lane == 0) remote_arrive(&sh.part_full, 0);
         } else {
           ok = __all_sync(0xffffffffu,
                           cluster_wait(&sh.part_full, (uint32_t)(items & 1), &sh.abort));
           if (!ok) break;
-          for (int r = 1; r < S; ++r) sum += s_part[(r - 1) * kWtKeys + tid];
+          for (int r = 1; r < S; ++r) sum += s_part[(r - 1) * kWtKeys + key];
           __syncwarp();
           if (lane == 0)
             for (int r = 1; r < S; ++r) remote_arrive(&sh.part_free, r);
@@ -544,7 +654,7 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
 }
 
 // Clusters of `cluster` CTAs that the device holds at once, asked once per device.
-template <bool kBf16, bool kSplit>
+template <bool kBf16, int kMode>
 static int resident_clusters(int cluster, int& n) {
   static int known[kMaxDevices][4] = {};
   static std::mutex mu;
@@ -570,7 +680,7 @@ static int resident_clusters(int cluster, int& n) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   if (err == cudaSuccess)
-    err = cudaOccupancyMaxActiveClusters(&n, paged_weights_kernel<kBf16, kSplit>, &cfg);
+    err = cudaOccupancyMaxActiveClusters(&n, paged_weights_kernel<kBf16, kMode>, &cfg);
   if (err != cudaSuccess) {
     set_last_cuda_error(err);
     return TW_ERR_CUDA;
@@ -583,7 +693,7 @@ static int resident_clusters(int cluster, int& n) {
   return TW_OK;
 }
 
-template <bool kBf16, bool kSplit>
+template <bool kBf16, int kMode>
 static int launch_weights(const WeightWork& w, int cluster, int64_t items, cudaStream_t stream) {
   const tw_paged_weights_args& a = w.a;
   CUtensorMap k_map, q_map, few_map;
@@ -603,10 +713,10 @@ static int launch_weights(const WeightWork& w, int cluster, int64_t items, cudaS
   if (rc == TW_OK) rc = encode_rows_map(&few_map, a.pool.dtype, 3, a.q, q_dims, q_strides, few_box);
   if (rc != TW_OK) return rc;
   static DynSmemOptIn opt_in;
-  const auto kernel = paged_weights_kernel<kBf16, kSplit>;
+  const auto kernel = paged_weights_kernel<kBf16, kMode>;
   rc = ensure_dyn_smem((const void*)kernel, opt_in, kWtSmem);
   int most = 0;
-  if (rc == TW_OK) rc = resident_clusters<kBf16, kSplit>(cluster, most);
+  if (rc == TW_OK) rc = resident_clusters<kBf16, kMode>(cluster, most);
   if (rc != TW_OK) return rc;
   const int64_t clusters = items < most ? items : most;
   return launch_pdl_cluster(kernel, dim3((unsigned)(clusters * cluster)), dim3(kWtThreads), cluster,
@@ -662,9 +772,14 @@ extern "C" int tw_paged_weights(const tw_paged_weights_args* args, void* stream)
   while (cluster < kWtMaxCluster && 2 * cluster <= tiles && 2 * cluster * items <= 148) cluster *= 2;
   cudaStream_t s = (cudaStream_t)stream;
   const int64_t some = items > 0 ? items : 1;
+  if (w.group <= 16 && most <= w.few_tokens) {
+    w.tile_tokens = w.few_tokens;
+    return a.pool.dtype == TW_F16 ? launch_weights<false, kWtFew>(w, 1, some, s)
+                                  : launch_weights<true, kWtFew>(w, 1, some, s);
+  }
   if (a.pool.dtype == TW_F16)
-    return cluster > 1 ? launch_weights<false, true>(w, cluster, some, s)
-                       : launch_weights<false, false>(w, cluster, some, s);
-  return cluster > 1 ? launch_weights<true, true>(w, cluster, some, s)
-                     : launch_weights<true, false>(w, cluster, some, s);
+    return cluster > 1 ? launch_weights<false, kWtSplit>(w, cluster, some, s)
+                       : launch_weights<false, kWtWhole>(w, 1, some, s);
+  return cluster > 1 ? launch_weights<true, kWtSplit>(w, cluster, some, s)
+                     : launch_weights<true, kWtWhole>(w, 1, some, s);
 }
