@@ -27,10 +27,13 @@ constexpr int kEvThreads = 512, kEvWarps = kEvThreads / 32;
 constexpr int kEvBins = 2048, kEvRounds = 3;
 constexpr int kEvMaxCluster = 8;
 constexpr int kEvMaxRequests = 8192;
-constexpr int kEvRowsPerCta = 4096;        // a cluster is as large as this asks for
+// A cluster is as large as this many rows a CTA ask for, if the device holds them all at once;
+// in any case so large that a CTA has no more than kEvMostRows.
+constexpr int kEvRowsPerCta = 4096, kEvCtas = 2 * 148, kEvMostRows = 16384;
 constexpr int kEvMaxRows = 1 << 21;        // of a request: 8 CTAs' bits of its rows
 constexpr int kEvSmem = 160 << 10;         // besides the histograms
-constexpr int kEvBatch = 4;                // rows that a warp copies at a time
+constexpr int kEvAhead = 8;                // rows whose records a thread reads at a time
+constexpr int kEvBatch = 8;                // rows that a warp copies at a time
 constexpr uint32_t kEvProtected = 0xffffffffu;
 
 struct EvictTask {
@@ -42,8 +45,9 @@ struct EvictTask {
 
 struct EvictShared {
   alignas(16) uint32_t hist[kEvRounds][kEvBins];
-  uint32_t warp_sum[2][kEvWarps];
-  EvictTask task;           // the cluster's: that of its first CTA
+  uint32_t warp_sum[kEvWarps];
+  unsigned long long warp_sums[kEvWarps];
+  EvictTask task, own;      // the cluster's is that of its first CTA; a copy of it
   uint32_t bin, above, in;  // where a round's bins reach the rank; keys above it, in it
   uint32_t ties;            // of the CTA
   uint32_t holes, movers;   // of the CTA
@@ -62,12 +66,15 @@ __device__ __forceinline__ int evict_kept(const tw_paged_evict_args& a, int len,
   return held && keep >= 0 && keep < len ? keep : len;
 }
 
-// Where row j is: page and row of the page; page -1: its page is none.
+// Where row j is: page and row of the page; page -1: its page is none.  (Nor has a row beyond
+// the request one: what a call that changes weights meanwhile could leave in the list stays
+// inside the buffers.)
 struct EvictRow {
   int page, row;
 };
 __device__ __forceinline__ EvictRow evict_row(const tw_paged_evict_args& a, const EvictTask& t,
                                               int j) {
+  if ((unsigned)j >= (unsigned)t.len) return {-1, 0};
   const unsigned i = (unsigned)j / (unsigned)a.pool.page_size;
   const int page = a.block_table[(int64_t)t.request * a.table_stride + i];
   if (page < 0 || page >= a.pool.num_pages) {
@@ -75,11 +82,6 @@ __device__ __forceinline__ EvictRow evict_row(const tw_paged_evict_args& a, cons
     return {-1, 0};
   }
   return {page, j - (int)(i * (unsigned)a.pool.page_size)};
-}
-// (What a call that changes weights meanwhile could leave in the list stays inside the buffers.)
-__device__ __forceinline__ bool evict_real(const tw_paged_evict_args& a, EvictRow r) {
-  return (unsigned)r.page < (unsigned)a.pool.num_pages &&
-         (unsigned)r.row < (unsigned)a.pool.page_size;
 }
 // In a layer and head's records, and its K or V (in 16-byte vectors).
 __device__ __forceinline__ int64_t evict_record(const tw_paged_evict_args& a, const EvictTask& t,
@@ -95,17 +97,40 @@ __device__ __forceinline__ int64_t evict_vector(const tw_paged_evict_args& a, co
 }
 
 // 32 bits that order as the ranking: a NaN weight above all others, -0 as 0.
-__device__ __forceinline__ uint32_t evict_key(const tw_paged_evict_args& a, const EvictTask& t,
-                                              int j) {
-  const EvictRow r = evict_row(a, t, j);
-  if (r.page < 0) return 0u;
-  const int64_t at = evict_record(a, t, r);
-  const float w = a.row_weights[at] + 0.f;
-  const long long p = a.row_positions[at];
+__device__ __forceinline__ uint32_t evict_order(const tw_paged_evict_args& a, const EvictTask& t,
+                                                float w, long long p) {
   if (p < a.sink || p >= t.next - a.recent) return kEvProtected;
   if (w != w) return kEvProtected - 1;
-  const uint32_t u = __float_as_uint(w);
+  const uint32_t u = __float_as_uint(w + 0.f);
   return u >> 31 ? ~u : u | 0x80000000u;
+}
+// N rows `step` apart: all their pages are read at once, then all their records (without
+// branches between, or each read would wait for the one before; a row past the end reads the
+// last one's, a page that is none the first record).
+template <int N>
+__device__ __forceinline__ void evict_keys(const tw_paged_evict_args& a, const EvictTask& t, int j,
+                                           int step, int end, uint32_t (&key)[N]) {
+  const int32_t* table = a.block_table + (int64_t)t.request * a.table_stride;
+  const unsigned size = (unsigned)a.pool.page_size;
+  int page[N];
+  float w[N];
+  int p[N];
+  bool bad = false;
+#pragma unroll
+  for (int y = 0; y < N; ++y) page[y] = table[(unsigned)min(j + y * step, end - 1) / size];
+#pragma unroll
+  for (int y = 0; y < N; ++y) {
+    const bool real = (unsigned)page[y] < (unsigned)a.pool.num_pages;
+    const int row = (int)((unsigned)min(j + y * step, end - 1) % size);
+    const int64_t at = real ? evict_record(a, t, {page[y], row}) : 0;
+    w[y] = a.row_weights[at];
+    p[y] = a.row_positions[at];
+    bad |= !real;
+  }
+#pragma unroll
+  for (int y = 0; y < N; ++y)
+    key[y] = (unsigned)page[y] < (unsigned)a.pool.num_pages ? evict_order(a, t, w[y], p[y]) : 0u;
+  if (bad) raise_error(a.error_flag, TW_ERR_INVALID_INDEX);
 }
 
 // Sum of x over the threads before this one; total: over all.
@@ -124,6 +149,31 @@ __device__ __forceinline__ uint32_t block_before(uint32_t x, uint32_t* s_warp, u
 #pragma unroll
   for (int i = 0; i < kEvWarps; ++i) {
     const uint32_t y = s_warp[i];
+    if (i < warp) before += y;
+    total += y;
+  }
+  __syncthreads();
+  return before + sum - x;
+}
+
+// The same for two counts of less than 2^31 in all.
+__device__ __forceinline__ unsigned long long block_before(unsigned long long x,
+                                                           unsigned long long* s_warp,
+                                                           unsigned long long& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  unsigned long long sum = x;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const unsigned long long y = __shfl_up_sync(0xffffffffu, sum, off);
+    if (lane >= off) sum += y;
+  }
+  if (lane == 31) s_warp[warp] = sum;
+  __syncthreads();
+  unsigned long long before = 0;
+  total = 0;
+#pragma unroll
+  for (int i = 0; i < kEvWarps; ++i) {
+    const unsigned long long y = s_warp[i];
     if (i < warp) before += y;
     total += y;
   }
@@ -190,7 +240,7 @@ paged_evict_kernel(const __grid_constant__ EvictWork w) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int clusters = (int)(gridDim.x / C) - 1, mine = (int)(blockIdx.x / C);
   if (mine == clusters) {  // the last one
-    evict_lengths(a, s_dyn, sh.warp_sum[0], rank, C);
+    evict_lengths(a, s_dyn, sh.warp_sum, rank, C);
     return;
   }
   uint32_t* s_keep = s_dyn;               // a bit per row: it stays
@@ -198,8 +248,7 @@ paged_evict_kernel(const __grid_constant__ EvictWork w) {
   uint32_t* s_holes = s_eq + w.words;     // free places before a word of rows, of all CTAs
   uint32_t* s_movers = s_holes + w.words; // rows that move before it
   uint32_t* s_key = s_movers + w.words;   // keys; then free places and the rows that move there
-  EvictRow* s_list = reinterpret_cast<EvictRow*>(s_key);
-  const uint32_t pairs_held = (uint32_t)w.held / 4;
+  const uint32_t pairs_held = (uint32_t)w.held / 2;
 
   const int64_t tasks = (int64_t)a.requests * w.units;
   int64_t at = mine;  // first task that may be next
@@ -238,28 +287,41 @@ paged_evict_kernel(const __grid_constant__ EvictWork w) {
       if (lane == 0) sh.task = t;
     }
     cluster.sync();
-    const EvictTask t = *cluster.map_shared_rank(&sh.task, 0);
+    if (tid == 0) sh.own = *cluster.map_shared_rank(&sh.task, 0);
+    __syncthreads();
+    const EvictTask& t = sh.own;
     if (t.request < 0) break;
 
     const int seg = ((t.len + C - 1) / C + 31) / 32 * 32;
     const int row0 = min(rank * seg, t.len), n = min(seg, t.len - row0);
     const int words = (n + 31) / 32;
-    const auto key = [&](int i) { return i < w.held ? s_key[i] : evict_key(a, t, row0 + i); };
+    const auto key = [&](int i) {
+      if (i < w.held) return s_key[i];
+      uint32_t k[1];
+      evict_keys(a, t, row0 + i, 1, row0 + n, k);
+      return k[0];
+    };
 
     // ---- the keep-th largest key
     uint32_t prefix = 0;              // its bits found so far
     uint32_t need = (uint32_t)t.keep; // its rank among the keys with these
-    uint32_t same = 0;                // keys that equal it
+    uint32_t same = 0;                // keys that equal it in these
+    int low = 0;                      // bits that were not needed
 #pragma unroll 1
     for (int round = 0; round < kEvRounds; ++round) {
       const int shift = round == 0 ? 21 : round == 1 ? 10 : 0;
       const int bits = round == 2 ? 10 : 11;
       if (round == 0) {
-#pragma unroll 4
-        for (int i = tid; i < n; i += kEvThreads) {
-          const uint32_t k = evict_key(a, t, row0 + i);
-          if (i < w.held) s_key[i] = k;
-          atomicAdd(&sh.hist[0][k >> shift], 1u);
+        for (int i = tid; i < n; i += kEvAhead * kEvThreads) {
+          uint32_t k[kEvAhead];
+          evict_keys(a, t, row0 + i, kEvThreads, row0 + n, k);
+#pragma unroll
+          for (int y = 0; y < kEvAhead; ++y) {
+            const int at = i + y * kEvThreads;
+            if (at >= n) break;
+            if (at < w.held) s_key[at] = k[y];
+            atomicAdd(&sh.hist[0][k[y] >> shift], 1u);
+          }
         }
       } else {
         const int top = shift + bits;
@@ -285,7 +347,7 @@ paged_evict_kernel(const __grid_constant__ EvictWork w) {
       }
       static_assert(kEach == 4);
       uint32_t total;
-      uint32_t before = block_before(bin[0] + bin[1] + bin[2] + bin[3], sh.warp_sum[0], total);
+      uint32_t before = block_before(bin[0] + bin[1] + bin[2] + bin[3], sh.warp_sum, total);
 #pragma unroll
       for (int i = 0; i < kEach; ++i) {
         if (before < need && need <= before + bin[i]) {
@@ -302,14 +364,17 @@ paged_evict_kernel(const __grid_constant__ EvictWork w) {
         same = sh.in;
       }
       __syncthreads();
+      low = shift;
+      if (need == same) break;
     }
     const bool all = need == same;  // all that equal it stay (nothing at all: keep is 0)
+    prefix >>= low;
 
     // ---- which rows stay
     uint32_t ties = 0;
     for (int x = warp; x < words; x += kEvWarps) {
       const int i = x * 32 + lane;
-      const uint32_t k = i < n ? key(i) : 0u;
+      const uint32_t k = i < n ? key(i) >> low : 0u;
       const unsigned above = __ballot_sync(0xffffffffu, i < n && t.keep > 0 && k > prefix);
       const unsigned equal = __ballot_sync(0xffffffffu, i < n && t.keep > 0 && k == prefix);
       if (lane == 0) {
@@ -329,7 +394,7 @@ paged_evict_kernel(const __grid_constant__ EvictWork w) {
         const int x = x0 + tid;
         const uint32_t equal = x < words ? s_eq[x] : 0u;
         uint32_t total;
-        const uint32_t first = before + block_before(__popc(equal), sh.warp_sum[0], total);
+        const uint32_t first = before + block_before(__popc(equal), sh.warp_sum, total);
         before += total;
         int stay = (int)min(max((long long)need - first, 0ll), 32ll);
         if (stay >= __popc(equal)) {
@@ -360,15 +425,15 @@ paged_evict_kernel(const __grid_constant__ EvictWork w) {
       const int x = x0 + tid;
       const uint32_t h = x < words ? __popc(holes_of(x)) : 0u;
       const uint32_t m = x < words ? __popc(movers_of(x)) : 0u;
-      uint32_t total_h, total_m;
-      const uint32_t h_first = holes + block_before(h, sh.warp_sum[0], total_h);
-      const uint32_t m_first = movers + block_before(m, sh.warp_sum[1], total_m);
+      unsigned long long total;
+      const unsigned long long before =
+          block_before((unsigned long long)m << 32 | h, sh.warp_sums, total);
       if (x < words) {
-        s_holes[x] = h_first;
-        s_movers[x] = m_first;
+        s_holes[x] = holes + (uint32_t)before;
+        s_movers[x] = movers + (uint32_t)(before >> 32);
       }
-      holes += total_h;
-      movers += total_m;
+      holes += (uint32_t)total;
+      movers += (uint32_t)(total >> 32);
     }
     if (tid == 0) {
       sh.holes = holes;
@@ -391,7 +456,7 @@ paged_evict_kernel(const __grid_constant__ EvictWork w) {
       const auto put = [&](uint32_t list, uint32_t k, int row) {
         if (k < done || k - done >= pairs_held * C) return;
         const uint32_t i = k - done;
-        *cluster.map_shared_rank(&s_list[list * pairs_held + i / C], i % C) = evict_row(a, t, row);
+        *cluster.map_shared_rank(&s_key[list * pairs_held + i / C], i % C) = (uint32_t)row;
       };
       for (int x = warp; x < words; x += kEvWarps) {
         const uint32_t h = holes_of(x), m = movers_of(x), below = (1u << lane) - 1;
@@ -402,40 +467,39 @@ paged_evict_kernel(const __grid_constant__ EvictWork w) {
       cluster.sync();
       const uint32_t here = min(pairs - done, pairs_held * C);  // of all CTAs
       const int count = (int)((here + C - 1 - rank) / C);       // of this one
+      // A warp takes up to 32 rows: a thread finds where one comes from and goes to and moves
+      // its record, then the warp copies them, half of it K and half V.  (64-bit products for
+      // each row by the whole warp took longer than the copies.)
       uint4* const pages = reinterpret_cast<uint4*>(lane < kVecPerRow16 ? a.pool.k_pages
                                                                         : a.pool.v_pages) +
                            lane % kVecPerRow16;
-      for (int first = warp * kEvBatch; first < count; first += kEvWarps * kEvBatch) {
-        uint4 x[kEvBatch];
-        float weight;
-        int position;
-        const bool record = lane < kEvBatch && first + lane < count;
+      const int per = min((count + kEvWarps - 1) / kEvWarps, 32);
+      for (int first = warp * per; first < count; first += kEvWarps * per) {
+        const int rows = min(per, count - first);
+        int64_t source = 0, place = -1;  // -1: not to move; it reads the pool's first row
+        if (lane < rows) {
+          const EvictRow to = evict_row(a, t, (int)s_key[first + lane]);
+          const EvictRow from = evict_row(a, t, (int)s_key[pairs_held + first + lane]);
+          if (to.page >= 0 && from.page >= 0) {
+            source = evict_vector(a, t, from);
+            place = evict_vector(a, t, to);
+            const int64_t i = evict_record(a, t, from), o = evict_record(a, t, to);
+            const float weight = a.row_weights[i];
+            const int position = a.row_positions[i];
+            a.row_weights[o] = weight;
+            a.row_positions[o] = position;
+          }
+        }
+        for (int y0 = 0; y0 < rows; y0 += kEvBatch) {
+          uint4 x[kEvBatch];
 #pragma unroll
-        for (int y = 0; y < kEvBatch; ++y) {
-          const EvictRow from =
-              first + y < count ? s_list[pairs_held + first + y] : EvictRow{-1, 0};
-          x[y] = make_uint4(0u, 0u, 0u, 0u);
-          if (evict_real(a, from)) x[y] = pages[evict_vector(a, t, from)];
-        }
-        EvictRow from = {-1, 0}, to = {-1, 0};
-        if (record) {
-          to = s_list[first + lane];
-          from = s_list[pairs_held + first + lane];
-        }
-        const bool moves = evict_real(a, from) && evict_real(a, to);
-        if (moves) {
-          weight = a.row_weights[evict_record(a, t, from)];
-          position = a.row_positions[evict_record(a, t, from)];
-        }
+          for (int y = 0; y < kEvBatch; ++y)
+            x[y] = __ldcs(pages + __shfl_sync(0xffffffffu, (long long)source, y0 + y));
 #pragma unroll
-        for (int y = 0; y < kEvBatch; ++y) {
-          if (first + y < count && evict_real(a, s_list[first + y]) &&
-              evict_real(a, s_list[pairs_held + first + y]))
-            pages[evict_vector(a, t, s_list[first + y])] = x[y];
-        }
-        if (moves) {
-          a.row_weights[evict_record(a, t, to)] = weight;
-          a.row_positions[evict_record(a, t, to)] = position;
+          for (int y = 0; y < kEvBatch; ++y) {
+            const long long to = __shfl_sync(0xffffffffu, (long long)place, y0 + y);
+            if (to >= 0) pages[to] = x[y];
+          }
         }
       }
       if (pairs - done > pairs_held * C) cluster.sync();
@@ -493,8 +557,11 @@ extern "C" int tw_paged_evict(const tw_paged_evict_args* args, void* stream) {
   EvictWork w = {};
   w.a = a;
   w.units = a.layers * a.pool.kv_heads;
+  const int64_t tasks = (int64_t)a.requests * w.units;
   int C = 1;
-  while (C < kEvMaxCluster && a.max_len > C * kEvRowsPerCta) C *= 2;
+  while (C < kEvMaxCluster && a.max_len > C * kEvRowsPerCta &&
+         (2 * C * tasks <= kEvCtas || a.max_len > C * kEvMostRows))
+    C *= 2;
   const int seg = max(((a.max_len + C - 1) / C + 31) / 32 * 32, 128);
   w.words = seg / 32;
   w.held = min(seg, (kEvSmem - 16 * w.words) / 4);
@@ -503,8 +570,7 @@ extern "C" int tw_paged_evict(const tw_paged_evict_args* args, void* stream) {
   const int st = ensure_dyn_smem((const void*)paged_evict_kernel, opt_in, smem);
   if (st != TW_OK) return st;
   // (one more for the lengths)
-  const int64_t tasks = (int64_t)a.requests * w.units;
-  const int clusters = (int)min(tasks, (int64_t)(4 * 148 / C)) + 1;
+  const int clusters = (int)min(tasks, (int64_t)(2 * kEvCtas / C)) + 1;
   return launch_pdl_cluster(paged_evict_kernel, dim3((unsigned)(clusters * C)), dim3(kEvThreads),
                             C, (size_t)smem, (cudaStream_t)stream, w);
 }
