@@ -36,15 +36,12 @@ class Stack:
                       for _ in range(LAYERS)]
         self.w_out = [(torch.randn(HIDDEN, Q_HEADS * D, generator=g, device=dev)
                        / (Q_HEADS * D) ** 0.5).to(dtype) for _ in range(LAYERS)]
-        self.inv = 500000.0 ** (-torch.arange(0, D, 2, device=dev) / D)
+        self.rotary = tw.RotaryPositions(D, base=500000.0, device=dev)
 
     def qkv(self, layer: int, x: torch.Tensor, positions: torch.Tensor):
         """q, k (rotated) and v, views of one projection."""
         y = (x @ self.w_qkv[layer].T).view(-1, Q_HEADS + 2 * KV_HEADS, D)
-        angle = (positions[:, None] * self.inv).repeat(1, 2)[:, None]
-        qk = y[:, :-KV_HEADS]
-        half = torch.cat((-qk[..., D // 2:], qk[..., :D // 2]), -1)
-        y[:, :-KV_HEADS] = (qk * angle.cos() + half * angle.sin()).to(y.dtype)
+        self.rotary(y[:, :-KV_HEADS], positions, out=y[:, :-KV_HEADS])
         return y[:, :Q_HEADS], y[:, Q_HEADS:-KV_HEADS], y[:, -KV_HEADS:]
 
     def step(self, cache, plan, x: torch.Tensor) -> torch.Tensor:

@@ -17,6 +17,19 @@ and so for what the stream holds before it.  Kernels see all max_requests rows, 
 waiting requests too: a cache for many more requests than are served at a time divides
 its work less well than one of the right size.  A finished prompt can move to an offloaded cache for sparse decoding
 (to_offloaded).
+
+write_rotated turns q and k by their positions on the way.  With track_weights the cache
+keeps, for every row, its token's position and the attention weight that it has been given,
+and evict() cuts long requests to the rows that were given most::
+
+    cache = PagedKVCache(..., track_weights=True)
+    ...
+        q = cache.write_rotated(layer, q, k, v, rotary)
+        out = cache.attend(layer, q)
+    cache.evict(4096, sink=4, recent=256)        # after the step's last layer
+
+Each layer and KV head keeps rows of its own; positions go on from the tokens seen, not
+from the rows held.
 """
 
 from __future__ import annotations
@@ -28,6 +41,7 @@ import torch
 
 from . import _lib, ops
 from .ops import HEAD_DIM
+from .rope import RotaryPositions
 
 
 @dataclass(frozen=True)
@@ -52,7 +66,7 @@ class PagedKVCache:
     def __init__(self, *, num_layers: int, num_kv_heads: int, num_pages: int,
                  max_requests: int, max_tokens_per_request: int, page_size: int = 16,
                  head_dim: int = HEAD_DIM, dtype: torch.dtype = torch.bfloat16,
-                 device: torch.device | str = "cuda") -> None:
+                 device: torch.device | str = "cuda", track_weights: bool = False) -> None:
         device = torch.device(device)
         if device.type != "cuda" or not torch.cuda.is_available():
             raise ValueError("an operational CUDA device is required")
@@ -87,6 +101,15 @@ class PagedKVCache:
         self._turn = 0
         self._error_flag = torch.zeros(1, **i32)
         self.lengths = [0] * max_requests  # the host's copy
+        self.evicted = [0] * max_requests  # tokens that the requests' rows no longer hold
+        self.row_weights: Optional[torch.Tensor] = None    # [layer][page][head][row]
+        self.row_positions: Optional[torch.Tensor] = None
+        self._offsets: Optional[torch.Tensor] = None       # `evicted` on the device
+        if track_weights:
+            shape = (num_layers, num_pages, num_kv_heads, page_size)
+            self.row_weights = torch.zeros(shape, dtype=torch.float32, device=device)
+            self.row_positions = torch.zeros(shape, **i32)
+            self._offsets = torch.zeros(max_requests, **i32)
         self.free_pages = num_pages
         self._step: Optional[PagedStep] = None
 
@@ -123,9 +146,11 @@ class PagedKVCache:
         ops.paged_step(self._lens, torch.tensor(new, **i32), self.block_table,
                        self._free_pages, self._free_count[before], page_size=self.page_size,
                        kv_lens=kv_lens, cu_q=cu_q, slots=slots, positions=positions,
-                       free_count_out=self._free_count[now], error_flag=self._error_flag)
+                       free_count_out=self._free_count[now], error_flag=self._error_flag,
+                       offsets=self._offsets)
         self._turn, self._lens = now, kv_lens
         self.lengths, self.free_pages = after, free
+        self.evicted = [0 if n < 0 else e for e, n in zip(self.evicted, new)]
         self._step = PagedStep(tokens, cu_q, kv_lens, slots, positions,
                                max(0, *new), max(after))
         return self._step
@@ -137,29 +162,120 @@ class PagedKVCache:
             raise ValueError("plan a step first")
         return self.pool[layer, 0], self.pool[layer, 1], self._step
 
+    def _records(self, layer: int) -> dict:
+        if self.row_weights is None:
+            return {}
+        return dict(row_weights=self.row_weights[layer], row_positions=self.row_positions[layer])
+
     def write(self, layer: int, k: torch.Tensor, v: torch.Tensor) -> None:
         """The step's new K / V rows [tokens, kv_heads, 128] of one layer."""
         k_pages, v_pages, step = self._layer(layer)
         if k.shape[0] != step.tokens:
             raise ValueError(f"the step has {step.tokens} tokens, got {k.shape[0]} rows")
-        if step.tokens:
+        if not step.tokens:
+            return
+        if self.row_weights is None:
             ops.paged_write(k, v, step.slots, k_pages, v_pages, error_flag=self._error_flag)
+        else:  # the records too: no rows of q, nothing turns
+            ops.paged_rope_write(k[:, :0], k, v, step.positions, step.slots,
+                                 torch.empty(0, dtype=torch.float64, device=self.device), k_pages,
+                                 v_pages, error_flag=self._error_flag, **self._records(layer))
 
-    def attend(self, layer: int, q: torch.Tensor, *, window: int = 0, **kw) -> torch.Tensor:
-        """Attention of the step's tokens, whose rows have been written: q and the result
-        [tokens, q_heads, 128].  Keywords of ops.paged_attention (out, out_dtype, lse,
-        softmax_scale, workspace)."""
+    def write_rotated(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                      rotary: RotaryPositions, *,
+                      q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """write() with q [tokens, q_heads, 128] and k turned by the step's positions, in one
+        launch; returns the turned q (q_out, which may be q itself)."""
         k_pages, v_pages, step = self._layer(layer)
         if q.shape[0] != step.tokens:
             raise ValueError(f"the step has {step.tokens} tokens, got {q.shape[0]} rows")
-        return ops.paged_attention(q, k_pages, v_pages, self.block_table, step.cu_q, step.kv_lens,
-                                   max_q_len=step.max_q_len, max_kv_len=step.max_kv_len,
-                                   window=window, error_flag=self._error_flag, **kw)
+        return ops.paged_rope_write(q, k, v, step.positions, step.slots, rotary.frequencies,
+                                    k_pages, v_pages, layout=rotary.layout, scale=rotary.scale,
+                                    q_out=q_out, error_flag=self._error_flag,
+                                    **self._records(layer))
+
+    def attend(self, layer: int, q: torch.Tensor, *, window: int = 0, last: int = 0,
+               lse: Optional[torch.Tensor] = None, **kw) -> torch.Tensor:
+        """Attention of the step's tokens, whose rows have been written: q and the result
+        [tokens, q_heads, 128].  Keywords of ops.paged_attention (out, out_dtype, lse,
+        softmax_scale, workspace).  With track_weights it adds what the tokens (last > 0: the
+        last `last` of each request) gave each row; a window goes by rows, so it is refused
+        while any request that holds rows has lost some."""
+        k_pages, v_pages, step = self._layer(layer)
+        if q.shape[0] != step.tokens:
+            raise ValueError(f"the step has {step.tokens} tokens, got {q.shape[0]} rows")
+        tracked = self.row_weights is not None
+        if last and not tracked:
+            raise ValueError("last: the cache does not track weights")
+        if window and any(e and l for e, l in zip(self.evicted, self.lengths)):
+            raise ValueError("no window over requests that have lost rows")
+        if tracked and lse is None:
+            lse = torch.empty(q.shape[:2], dtype=torch.float32, device=self.device)
+        lengths = dict(max_q_len=step.max_q_len, max_kv_len=step.max_kv_len, window=window,
+                       error_flag=self._error_flag)
+        out = ops.paged_attention(q, k_pages, v_pages, self.block_table, step.cu_q, step.kv_lens,
+                                  lse=lse, **lengths, **kw)
+        if tracked:
+            ops.paged_weights(q, k_pages, self.block_table, step.cu_q, step.kv_lens, lse,
+                              self.row_weights[layer], last=last,
+                              softmax_scale=kw.get("softmax_scale"), **lengths)
+        return out
+
+    # -------------------------------------------------------------- eviction --
+    def evict(self, keep: int | Sequence[int], *, sink: int = 4, recent: int = 64) -> None:
+        """Cuts every request of more than `keep` rows (one number, or one for each request;
+        negative: leave it) to that many, in each layer and KV head those at the first `sink`
+        positions, the last `recent` and then those of the largest weights; the pages past
+        them are free from here on.  To be called when a step's last layer has attended; the
+        next step has to be planned before more is written."""
+        if self.row_weights is None:
+            raise ValueError("the cache does not track weights")
+        if sink < 0 or recent < 0:
+            raise ValueError("sink and recent must not be negative")
+        one = isinstance(keep, int)
+        wanted = [keep] * self.max_requests if one else [int(n) for n in keep]
+        if len(wanted) > self.max_requests:
+            raise ValueError(f"{len(wanted)} requests in a cache for {self.max_requests}")
+        wanted += [-1] * (self.max_requests - len(wanted))
+        if any(0 <= n < sink + recent for n in wanted):
+            raise ValueError(f"keep must hold sink + recent = {sink + recent} rows")
+        after = [n if 0 <= n < l else l for l, n in zip(self.lengths, wanted)]
+        if after == self.lengths:
+            return
+        i32 = dict(dtype=torch.int32, device=self.device)
+        before, now = self._turn, self._turn ^ 1
+        lens, offsets = (torch.empty(self.max_requests, **i32) for _ in range(2))
+        ops.paged_evict(self.pool[:, 0], self.pool[:, 1], self.row_weights, self.row_positions,
+                        self.block_table, self._lens, torch.tensor(wanted, **i32), self._offsets,
+                        max_len=max(self.lengths), sink=sink, recent=recent, lens_out=lens,
+                        offsets_out=offsets, free_pages=self._free_pages,
+                        free_count=self._free_count[before],
+                        free_count_out=self._free_count[now], error_flag=self._error_flag)
+        self._turn, self._lens, self._offsets = now, lens, offsets
+        self.evicted = [e + l - a for e, l, a in zip(self.evicted, self.lengths, after)]
+        self.free_pages += sum(self._pages(l) - self._pages(a)
+                               for l, a in zip(self.lengths, after))
+        self.lengths = after
+        self._step = None  # its lengths are no longer those of the requests
+
+    def request_positions(self, layer: int, request: int) -> torch.Tensor:
+        """Positions of the rows that a request holds, [kv_heads, rows] int32 in the order of
+        request_kv."""
+        if self.row_positions is None:
+            raise ValueError("the cache does not track weights")
+        j = torch.arange(self.lengths[request], device=self.device)
+        pages = self.block_table[request, j // self.page_size].long()
+        return self.row_positions[layer][pages, :, j % self.page_size].T.contiguous()
 
     # ---------------------------------------------------------------- export --
     def request_kv(self, layer: int, request: int) -> tuple[torch.Tensor, torch.Tensor]:
-        """K and V of one request and layer, [kv_heads, tokens, 128] each."""
-        k_pages, v_pages, _ = self._layer(layer)
+        """K and V of one request and layer, [kv_heads, tokens, 128] each.  (After an eviction
+        the rows are in no fixed order: request_positions.)"""
+        if not 0 <= layer < self.num_layers:
+            raise IndexError("layer out of range")
+        if self._step is None and not any(self.evicted):
+            raise ValueError("plan a step first")
+        k_pages, v_pages = self.pool[layer, 0], self.pool[layer, 1]
         n, G, P = self.lengths[request], self.num_kv_heads, self.page_size
         out = torch.empty((2, G, n, HEAD_DIM), dtype=self.dtype, device=self.device)
         if n:
@@ -173,7 +289,10 @@ class PagedKVCache:
 
     def to_offloaded(self, request: int, cache) -> None:
         """Hands a request's tokens to an offloaded cache as its prompt (its slab rows,
-        page metadata and INT4 codes): layer i to entries i*kv_heads .. of `cache`."""
+        page metadata and INT4 codes): layer i to entries i*kv_heads .. of `cache`.  Not after
+        an eviction: that cache goes by the order of its rows."""
+        if self.evicted[request]:
+            raise ValueError("the request has lost rows")
         G = self.num_kv_heads
         for layer in range(self.num_layers):
             k, v = self.request_kv(layer, request)
