@@ -295,3 +295,20 @@ def test_graph_and_stream(tw, cuda):
         graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(w, want)
+
+
+@pytest.mark.parametrize("q_heads,kv_heads", [(4, 1), (8, 2), (6, 2), (32, 2)])
+def test_clusters_of_several_items(tw, cuda, q_heads, kv_heads):
+    """Few items that clusters take, more of them than clusters, so that each takes several:
+    a tile or two for a CTA, or none.  Many times, for what depends on who is first."""
+    new = [70, 1, 257, 33, 0, 129, 300, 2, 90, 65, 40, 128]
+    s = state(cuda, 14, new, [3, 500, 40, 256, 9, 0, 200, 700, 1, 511, 90, 128], q_heads=q_heads,
+              kv_heads=kv_heads, dtype=torch.float16)
+    first = check(tw, s)
+    for _ in range(20):
+        assert torch.equal(first, check(tw, s))
+    for seed in range(8):
+        rng = random.Random(seed)
+        new = [rng.choice((0, 1, rng.randint(2, 300))) for _ in range(rng.randint(4, 14))]
+        check(tw, state(cuda, seed, new + [64], [rng.randint(0, 600) for _ in new] + [5],
+                        q_heads=q_heads, kv_heads=kv_heads), last=rng.choice((0, 0, 100)))

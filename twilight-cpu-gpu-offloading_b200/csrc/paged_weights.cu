@@ -24,7 +24,7 @@
 namespace tw {
 
 constexpr int kWtKeys = 256, kWtCols = 128;
-constexpr int kWtSumThreads = 512, kWtThreads = 640;  // two groups of 256 sum
+constexpr int kWtThreads = 640;            // 512 of them sum, in two groups
 constexpr int kWtMmaWarp = 16, kWtRowWarp = 17, kWtKeyWarp = 18;  // and 19
 constexpr int kWtAhead = 2;                // tiles whose log-sum-exps are read at a time
 constexpr int kWtHalfTile = 128 * 128;     // bytes: 128 rows of 64 elements
@@ -245,7 +245,12 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
   constexpr int kCols = Layout::kCols, kRowHalf = Layout::kRowHalf, kRowTile = Layout::kRowTile;
   static_assert(2 * kKeySlots * kWtTile + kRowSlots * kRowTile <=
                 (kSplit ? kWtSlots - 1 : kWtSlots) * kWtTile);
-  const long long first_item = blockIdx.x / S, step = gridDim.x / S;
+  // Its items: back and forth through them, so that the long ones at the beginning (keys that
+  // most rows see) and the short ones at the end come together.
+  const long long mine = blockIdx.x / S, others = gridDim.x / S;
+  const auto item = [&](int round) {
+    return round * others + (round & 1 ? others - 1 - mine : mine);
+  };
   const uint32_t keys_at = smem_addr(smem), rows_at = keys_at + 2 * kKeySlots * kWtTile;
   float* s_part = reinterpret_cast<float*>(smem + (kWtSlots - 1) * kWtTile);  // kSplit: [rank - 1][key]
   if (keys_at & 1023) {  // (what the layout of the products rests on)
@@ -263,7 +268,7 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
     }
     for (int i = 0; i < kWtLseSlots; ++i) {
       mbar_init(&sh.lse_full[i], 1);
-      mbar_init(&sh.lse_empty[i], kWtSumThreads / 2 / 32);
+      mbar_init(&sh.lse_empty[i], kWtKeys / 32);
     }
     for (int i = 0; i < 2; ++i)
       for (int j = 0; j < 2; ++j) {
@@ -303,23 +308,34 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
     __syncwarp();
     const uint32_t box_bytes = (uint32_t)w.box * 128;  // of 64 dimensions
     const int boxes = 128 / w.box;                     // at most 16
-    int n = 0;
-    for (long long item = first_item; walk.find(w, lane, item, x); item += step) {
-      if (rank >= x.tiles) continue;
-      const int s = n % kKeySlots;
+    // lane l < boxes knows the page of box l, and looks the next item's up before it waits
+    int p = 0, row = 0;
+    bool wanted = false;
+    const auto look_up = [&](const WeightItem& x) {
       const int key = x.key0 + h * 128 + lane * w.box;
-      const bool wanted = lane < boxes && key < x.end && key + w.box > x.begin;
-      int p = 0, row = 0;
+      wanted = lane < boxes && key < x.end && key + w.box > x.begin;
       if (wanted) {
         const int i = key / a.pool.page_size;
         row = key - i * a.pool.page_size;
         p = a.block_table[(int64_t)x.request * a.table_stride + i];
-        if (p < 0 || p >= a.pool.num_pages) {
-          raise_error(a.error_flag, TW_ERR_INVALID_INDEX);
-          p = (int)a.pool.num_pages;  // out of the map's range: zeros
-        }
       }
+    };
+    int n = 0, round = 0;
+    bool more = walk.find(w, lane, item(0), x);
+    if (more) look_up(x);
+    while (more) {
+      const bool skip = rank >= x.tiles;
+      const int head = x.head, now_row = row;
+      int now = p;
       const uint32_t all = __ballot_sync(0xffffffffu, wanted);
+      if (wanted && (now < 0 || now >= a.pool.num_pages)) {
+        raise_error(a.error_flag, TW_ERR_INVALID_INDEX);
+        now = (int)a.pool.num_pages;  // out of the map's range: zeros
+      }
+      more = walk.find(w, lane, item(++round), x);
+      if (more) look_up(x);
+      if (skip) continue;
+      const int s = n % kKeySlots;
       const int from = all ? __ffs(all) - 1 : 0, to = 32 - __clz(all);
       if (n >= kKeySlots) {
         ok = __all_sync(0xffffffffu, mbar_wait(&sh.k_empty[s],
@@ -332,8 +348,8 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
         int px[4], rx[4];
 #pragma unroll
         for (int y = 0; y < 4; ++y) {
-          px[y] = __shfl_sync(0xffffffffu, p, y0 + y);
-          rx[y] = __shfl_sync(0xffffffffu, row, y0 + y);
+          px[y] = __shfl_sync(0xffffffffu, now, y0 + y);
+          rx[y] = __shfl_sync(0xffffffffu, now_row, y0 + y);
         }
         if (elect_one()) {
 #pragma unroll
@@ -341,8 +357,8 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
             if (y0 + y < to) {
               const uint32_t dst = keys_at + (uint32_t)(s * 2 + h) * kWtTile +
                                    (uint32_t)((y0 + y) * w.box) * 128;
-              tma_load_4d(&k_map, dst, &sh.k_full[s], 0, rx[y], x.head, px[y]);
-              tma_load_4d(&k_map, dst + kWtHalfTile, &sh.k_full[s], 64, rx[y], x.head, px[y]);
+              tma_load_4d(&k_map, dst, &sh.k_full[s], 0, rx[y], head, px[y]);
+              tma_load_4d(&k_map, dst + kWtHalfTile, &sh.k_full[s], 64, rx[y], head, px[y]);
             }
         }
         __syncwarp();
@@ -362,7 +378,7 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
     }
     __syncwarp();
     int n = 0, nl = 0;  // tiles copied; with their log-sum-exps
-    for (long long item = first_item; ok && walk.find(w, lane, item, x); item += step) {
+    for (int round = 0; ok && walk.find(w, lane, item(round), x); ++round) {
       for (int t0 = rank; ok && t0 < x.tiles; t0 += kWtAhead * S) {
         constexpr int kParts = (kCols + 31) / 32;
         float z[kWtAhead][kParts];
@@ -426,7 +442,7 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
     // ---- products
     int nk = 0, nq = 0;
     uint32_t used = 0, turn = 0;  // a bit per buffer of scores: used before; its phase
-    for (long long item = first_item; ok && walk.find(w, lane, item, x); item += step) {
+    for (int round = 0; ok && walk.find(w, lane, item(round), x); ++round) {
       if (rank >= x.tiles) continue;
       const int ks = nk % kKeySlots;
       const int halves = x.end - x.key0 > 128 ? 2 : 1;
@@ -440,7 +456,7 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
         ok = __all_sync(0xffffffffu,
                         mbar_wait(&sh.q_full[qs], (uint32_t)((nq / kRowSlots) & 1), &sh.abort));
         for (int h = first_half ? 0 : 1; ok && h < halves; ++h) {
-          const int buf = nq & 1, bit = h * 2 + buf;  // a group of sums each
+          const int buf = nq & 1, bit = h * 2 + buf;
           if (used >> bit & 1)
             ok = __all_sync(0xffffffffu,
                             mbar_wait(&sh.s_free[h][buf], ~(turn >> bit) & 1, &sh.abort));
@@ -475,31 +491,33 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
       mbar_wait(&sh.drain, 0, &never);
     }
   } else {
-    // ---- sums: a thread per key and group; the groups take tiles in turn
+    // ---- sums: a thread per key and group; the groups take tiles in turn.  (64 columns of
+    // each tile: 680 us instead of 626 for 2048 tokens at 32k, a tile has its costs.)
+    constexpr bool kFew = kMode == kWtFew;
     const int group = warp >> 3, h = (warp >> 2) & 1, key = tid & (kWtKeys - 1);
-    const uint32_t my = tmem + ((uint32_t)((warp & 3) * 32) << 16) + h * 256 + group * 128;
+    const uint32_t my = tmem + ((uint32_t)((warp & 3) * 32) << 16) + h * 256;
     const uint64_t scale2 = pair(a.softmax_scale, a.softmax_scale);
     const uint64_t log2e2 = pair(1.4426950408889634f, 1.4426950408889634f);
-    // tiles so far, those that this warp took, items, and those of them that both groups had
-    int nl = 0, ns = 0, items = 0, joins = 0;
-    for (long long item = first_item; ok && walk.find(w, lane, item, x); item += step, ++items) {
-      // this CTA's tiles of the item, and whether the other group has some of them too
+    int nl = 0, joins = 0;  // tiles so far; items whose sums the groups joined
+    uint32_t turn = 0;      // a bit per buffer of scores: its phase
+    for (int round = 0; ok && walk.find(w, lane, item(round), x); ++round) {
+      // This CTA's tiles of the item; which group goes on with the sums, and whether the other
+      // has some for it.  Of a single tile it is the one that has it; with a cluster always the
+      // first, which so sees every phase of the barriers between CTAs (a group that left one out
+      // would take an older phase for the one it waits for).
       const int tiles = x.tiles > rank ? (x.tiles - rank - 1) / S + 1 : 0;
-      const bool both = tiles > 1, adds = group == (tiles == 1 ? nl & 1 : 0);
+      const int last = kSplit || tiles != 1 ? 0 : nl & 1;
+      const bool both = tiles > 1 || (tiles == 1 && (nl & 1) != last), adds = group == last;
       const int j = x.key0 + key;
       const bool held = j >= x.begin && j < x.end;
-      int64_t place = -1;
-      if (held && rank == 0 && adds) {
-        const int i = j / a.pool.page_size;
-        const int page = a.block_table[(int64_t)x.request * a.table_stride + i];
-        if (page >= 0 && page < a.pool.num_pages)
-          place = ((int64_t)page * a.pool.kv_heads + x.head) * a.pool.page_size +
-                  (j - i * a.pool.page_size);
-      }
+      int page = -1;
+      if (held && rank == 0 && adds)
+        page = a.block_table[(int64_t)x.request * a.table_stride + j / a.pool.page_size];
       const bool mine = h == 0 ? x.begin < x.key0 + 128 : x.end > x.key0 + 128;
       float sum = 0.f;
       for (int t = rank; t < x.tiles; t += S, ++nl) {
-        if ((nl & 1) != group) continue;
+        const int buf = nl & 1;
+        if (buf != group) continue;
         const int ls = nl % kWtLseSlots;
         // (also by warps with no keys: they must not hand a slot back twice in a phase)
         ok = __all_sync(0xffffffffu, mbar_wait(&sh.lse_full[ls],
@@ -507,9 +525,9 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
         if (!ok) break;
         if (mine) {
           ok = __all_sync(0xffffffffu,
-                          mbar_wait(&sh.s_full[h][group], (uint32_t)(ns & 1), &sh.abort));
+                          mbar_wait(&sh.s_full[h][buf], turn >> buf & 1, &sh.abort));
           if (!ok) break;
-          ++ns;
+          turn ^= 1u << buf;
           tmem_fence_after();
           const int i = x.from + t * T, here = min(T, x.upto - i);
           const int cols = here * R, p = x.p0 + i;  // position of the tile's first token
@@ -525,7 +543,7 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
               to = a.window > 0 ? (int)max(min((long long)here, (long long)j + a.window - p), 0ll) * R
                                 : cols;
           }
-          const uint32_t at = my;
+          const uint32_t at = my + buf * 128;
           uint64_t sum2[2] = {0ull, 0ull};
           // the columns [c0, c0 + N) of the tile, in s
           const auto add_columns = [&](const auto& s, int c0, auto n, auto some) {
@@ -572,23 +590,24 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
           const auto read_all = [&] {  // the scores are in registers: the next tile's may come
             tmem_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.s_free[h][group]);
+            if (lane == 0) mbar_arrive(&sh.s_free[h][buf]);
           };
-          if constexpr (kMode == kWtFew) {
+          if constexpr (kFew) {
             float s[16];
             tmem_ld16(s, at);
             tmem_wait_ld(s);
             read_all();
             add(s, 0, std::integral_constant<int, 16>{});
           } else {
-            const int chunks = (cols + 31) / 32;
+            // (each read is followed by its wait: a branch between them, and the compiler
+            // may move the registers before they hold anything)
 #pragma unroll 1
-            for (int c = 0; c < chunks; ++c) {
+            for (int c0 = 0; c0 < cols; c0 += 32) {
               float s[32];
-              tmem_ld32(s, at + c * 32);
+              tmem_ld32(s, at + c0);
               tmem_wait_ld(s);
-              if (c == chunks - 1) read_all();
-              add(s, c * 32, std::integral_constant<int, 32>{});
+              if (c0 + 32 >= cols) read_all();
+              add(s, c0, std::integral_constant<int, 32>{});
             }
           }
           float y0, y1;
@@ -621,16 +640,16 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
       if (!adds) continue;
       if constexpr (kSplit) {
         if (rank != 0) {
-          if (items > 0)
+          if (round > 0)
             ok = __all_sync(0xffffffffu,
-                            cluster_wait(&sh.part_free, (uint32_t)((items - 1) & 1), &sh.abort));
+                            cluster_wait(&sh.part_free, (uint32_t)((round - 1) & 1), &sh.abort));
           if (!ok) break;
           remote_store(s_part + (rank - 1) * kWtKeys + key, 0, sum);
           __syncwarp();
           if (lane == 0) remote_arrive(&sh.part_full, 0);
         } else {
           ok = __all_sync(0xffffffffu,
-                          cluster_wait(&sh.part_full, (uint32_t)(items & 1), &sh.abort));
+                          cluster_wait(&sh.part_full, (uint32_t)(round & 1), &sh.abort));
           if (!ok) break;
           for (int r = 1; r < S; ++r) sum += s_part[(r - 1) * kWtKeys + key];
           __syncwarp();
@@ -639,7 +658,10 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
         }
       }
       // no other thread of the call adds to this slot, unless requests share its page
-      if (place >= 0) atomicAdd(a.row_weights + place, sum);
+      if (page >= 0 && page < a.pool.num_pages)
+        atomicAdd(a.row_weights + ((int64_t)page * a.pool.kv_heads + x.head) * a.pool.page_size +
+                      j % a.pool.page_size,
+                  sum);
     }
     if (!ok && lane == 0) raise_error(a.error_flag, TW_ERR_TIMEOUT);
     tmem_fence_before();
@@ -769,7 +791,7 @@ extern "C" int tw_paged_weights(const tw_paged_weights_args* args, void* stream)
       ((keys + kWtKeys - 1) / kWtKeys + (a.window > 0)) * a.requests * a.pool.kv_heads;
   const int64_t tiles = (most + w.tile_tokens - 1) / w.tile_tokens;
   int cluster = 1;
-  while (cluster < kWtMaxCluster && 2 * cluster <= tiles && 2 * cluster * items <= 148) cluster *= 2;
+  while (cluster < kWtMaxCluster && 2 * cluster <= tiles && cluster * items < 148) cluster *= 2;
   cudaStream_t s = (cudaStream_t)stream;
   const int64_t some = items > 0 ? items : 1;
   if (w.group <= 16 && most <= w.few_tokens) {
