@@ -272,3 +272,78 @@ def test_graph_and_stream(tw, cuda):
     side.synchronize()
     for n in ("k", "v", "w", "p", "stack"):
         assert torch.equal(a[n], want[n]), n
+
+
+@pytest.mark.parametrize("n,keep,max_len", [(400_003, 399_700, None), (700_001, 350_000, None),
+                                            (90_001, 60_000, 1 << 21), (5000, 2500, 1 << 21)])
+def test_long_requests(tw, cuda, n, keep, max_len):
+    """Keys that shared memory does not hold, lists that take several turns, a bound far above
+    the lengths: against a stable sort."""
+    page = 64
+    g = torch.Generator(cuda).manual_seed(n)
+    pages = -(-n // page) + 2
+    i32 = dict(dtype=torch.int32, device=cuda)
+    table = torch.randperm(pages, generator=g, device=cuda)[:-2].to(torch.int32)[None].contiguous()
+    k, v = (torch.randint(-30000, 30000, (pages, 1, page, D), generator=g, device=cuda,
+                          dtype=torch.int16) for _ in range(2))
+    w = torch.rand(pages, 1, page, generator=g, device=cuda)
+    w[torch.rand(w.shape, generator=g, device=cuda) < 0.2] = 0.5
+    p = torch.randint(0, 2 * n, (pages, 1, page), generator=g, device=cuda, dtype=torch.int32)
+    j = torch.arange(n, device=cuda)
+    at = table[0, j // page].long(), torch.zeros_like(j), j % page
+    fixed = (p[at] < 50) | (p[at] >= 2 * n - 100)
+    order = torch.where(fixed, 2.0, w[at].double()).sort(descending=True, stable=True).indices
+    stays = torch.zeros(n, dtype=torch.bool, device=cuda)
+    stays[order[:keep]] = True
+    to, source = torch.nonzero(~stays[:keep])[:, 0], torch.nonzero(stays[keep:])[:, 0] + keep
+    spot = lambda x: (table[0, x // page].long(), torch.zeros_like(x), x % page)  # noqa: E731
+    want = [t.clone() for t in (k, v, w, p)]
+    for t in want:
+        t[spot(to)] = t[spot(source)]
+    lens_out, gone_out = torch.zeros(1, **i32), torch.zeros(1, **i32)
+    err = torch.zeros(1, **i32)
+    tw.ops.paged_evict(k.view(torch.float16), v.view(torch.float16), w, p, table,
+                       torch.tensor([n], **i32), torch.tensor([keep], **i32),
+                       torch.tensor([n], **i32), max_len=n if max_len is None else max_len, sink=50,
+                       recent=100, lens_out=lens_out, offsets_out=gone_out, error_flag=err)
+    assert int(err) == 0 and int(lens_out) == keep and int(gone_out) == 2 * n - keep
+    for got, t in zip((k, v, w, p), want):
+        assert torch.equal(got, t)
+
+
+def test_far_pages(tw, cuda):
+    """Places beyond 2^31 elements of a pool: written, weighed and moved there."""
+    heads, page, pages = 8, 16, 140_000  # 2.3e9 elements
+    g = torch.Generator().manual_seed(1)
+    i32 = dict(dtype=torch.int32, device=cuda)
+    k, v = (torch.zeros(pages, heads, page, D, dtype=torch.float16, device=cuda) for _ in range(2))
+    w = torch.zeros(pages, heads, page, device=cuda)
+    p = torch.zeros(pages, heads, page, **i32)
+    ids = torch.tensor([pages - 1, 3, pages - 7, pages - 2], **i32)
+    table = ids[None].contiguous()
+    rows = torch.randn(60, 2 * heads, D, generator=g).to(torch.float16).to(cuda)
+    kk, vv = rows[:, :heads], rows[:, heads:]
+    j = torch.arange(60, device=cuda)
+    slots = table[0, j // page].long() * page + j % page
+    f, _ = tw.ops.rope_frequencies(128, device=cuda)
+    q = tw.ops.paged_rope_write(kk, kk, vv, j.int(), slots, f, k, v, row_weights=w,
+                                row_positions=p)
+    at = table[0, j // page].long(), slice(None), j % page
+    assert torch.equal(k[at], q) and torch.equal(v[at], vv)
+    cu, kv = torch.tensor([0, 60], **i32), torch.tensor([60], **i32)
+    lse = evict_ref.attention_lse(q, k, table, cu, kv)
+    ref, tol = evict_ref.weights(q, k, table, cu, kv, lse, w)
+    tw.ops.paged_weights(q, k, table, cu, kv, lse, w, max_q_len=60, max_kv_len=60)
+    assert bool(((w.double() - ref).abs() <= tol).all()) and bool((w[at] > 0).all())
+    had = [w[at].T.clone(), k[at].transpose(0, 1).clone(), v[at].transpose(0, 1).clone()]
+    out = [torch.zeros(1, **i32) for _ in range(2)]
+    tw.ops.paged_evict(k, v, w, p, table, kv, torch.tensor([33], **i32), torch.zeros(1, **i32),
+                       max_len=60, sink=2, recent=5, lens_out=out[0], offsets_out=out[1])
+    at = table[0, j[:33] // page].long(), slice(None), j[:33] % page
+    places = p[at].T.long()  # [heads, 33]
+    for h in range(heads):
+        fixed = (j < 2) | (j >= 55)
+        best = torch.where(fixed, torch.inf, had[0][h]).sort(descending=True, stable=True).indices
+        assert sorted(places[h].tolist()) == sorted(best[:33].tolist())
+        assert torch.equal(k[at][:, h], had[1][h][places[h]])
+        assert torch.equal(v[at][:, h], had[2][h][places[h]])

@@ -230,8 +230,6 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
                      const __grid_constant__ CUtensorMap few_map) {
   extern __shared__ __align__(1024) char smem[];
   WeightShared& sh = *reinterpret_cast<WeightShared*>(smem + kWtSlots * kWtTile);
-  pdl_wait();
-  pdl_launch_dependents();
   const tw_paged_weights_args& a = w.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int R = w.group, T = w.tile_tokens;
@@ -245,18 +243,8 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
   constexpr int kCols = Layout::kCols, kRowHalf = Layout::kRowHalf, kRowTile = Layout::kRowTile;
   static_assert(2 * kKeySlots * kWtTile + kRowSlots * kRowTile <=
                 (kSplit ? kWtSlots - 1 : kWtSlots) * kWtTile);
-  // Its items: back and forth through them, so that the long ones at the beginning (keys that
-  // most rows see) and the short ones at the end come together.
-  const long long mine = blockIdx.x / S, others = gridDim.x / S;
-  const auto item = [&](int round) {
-    return round * others + (round & 1 ? others - 1 - mine : mine);
-  };
   const uint32_t keys_at = smem_addr(smem), rows_at = keys_at + 2 * kKeySlots * kWtTile;
   float* s_part = reinterpret_cast<float*>(smem + (kWtSlots - 1) * kWtTile);  // kSplit: [rank - 1][key]
-  if (keys_at & 1023) {  // (what the layout of the products rests on)
-    if (tid == 0) raise_error(a.error_flag, TW_ERR_UNSUPPORTED);
-    return;
-  }
   if (tid == 0) {
     for (int i = 0; i < kKeySlots; ++i) {
       mbar_init(&sh.k_full[i], 2);
@@ -297,11 +285,22 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
   tmem_fence_after();
   if constexpr (kSplit) cluster_barrier();  // all barriers are there
   const uint32_t tmem = sh.tmem;
+  // (so far nothing but shared and tensor memory: while the kernel before this one ends)
+  pdl_wait();
+  pdl_launch_dependents();
 
+  // Its items: back and forth through them, so that the long ones at the beginning (keys that
+  // most rows see) and the short ones at the end come together.
+  const long long mine = blockIdx.x / S, others = gridDim.x / S;
+  const auto item = [&](int round) {
+    return round * others + (round & 1 ? others - 1 - mine : mine);
+  };
   WeightWalk walk;
   WeightItem x;
   bool ok = true;
-  if (warp >= kWtKeyWarp) {
+  if (keys_at & 1023) {  // (what the layout of the products rests on)
+    if (tid == 0) raise_error(a.error_flag, TW_ERR_UNSUPPORTED);
+  } else if (warp >= kWtKeyWarp) {
     // ---- K of the items: a warp for each 128 keys
     const int h = warp - kWtKeyWarp;
     if (elect_one()) prefetch_map(&k_map);
