@@ -310,18 +310,23 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
     // lane l < boxes knows the page of box l, and looks the next item's up before it waits
     int p = 0, row = 0;
     bool wanted = false;
-    const auto look_up = [&](const WeightItem& x) {
+    const auto look_up = [&](const WeightItem& x, bool known, int page) {
       const int key = x.key0 + h * 128 + lane * w.box;
       wanted = lane < boxes && key < x.end && key + w.box > x.begin;
       if (wanted) {
         const int i = key / a.pool.page_size;
         row = key - i * a.pool.page_size;
-        p = a.block_table[(int64_t)x.request * a.table_stride + i];
+        p = known ? page : a.block_table[(int64_t)x.request * a.table_stride + i];
       }
     };
     int n = 0, round = 0;
+    // a single request's first pages are read together with its lengths
+    const long long guess = item(0) / a.pool.kv_heads * kWtKeys + h * 128 + lane * w.box;
+    const bool guesses = a.requests == 1 && a.window == 0 && lane < boxes &&
+                         guess / a.pool.page_size < a.table_width;
+    const int first_page = guesses ? a.block_table[guess / a.pool.page_size] : 0;
     bool more = walk.find(w, lane, item(0), x);
-    if (more) look_up(x);
+    if (more) look_up(x, guesses, first_page);
     while (more) {
       const bool skip = rank >= x.tiles;
       const int head = x.head, now_row = row;
@@ -332,7 +337,7 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
         now = (int)a.pool.num_pages;  // out of the map's range: zeros
       }
       more = walk.find(w, lane, item(++round), x);
-      if (more) look_up(x);
+      if (more) look_up(x, false, 0);
       if (skip) continue;
       const int s = n % kKeySlots;
       const int from = all ? __ffs(all) - 1 : 0, to = 32 - __clz(all);
@@ -439,6 +444,7 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
     }
   } else if (warp == kWtMmaWarp) {
     // ---- products
+    const uint64_t k_desc = operand_desc(keys_at, 16, 1024), q_desc = operand_desc(rows_at, 16, 1024);
     int nk = 0, nq = 0;
     uint32_t used = 0, turn = 0;  // a bit per buffer of scores: used before; its phase
     for (int round = 0; ok && walk.find(w, lane, item(round), x); ++round) {
@@ -464,14 +470,15 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
           turn ^= 1u << bit;
           tmem_fence_after();
           if (elect_one()) {
-            const uint32_t ka = keys_at + (uint32_t)(ks * 2 + h) * kWtTile,
-                           qa = rows_at + (uint32_t)qs * kRowTile;
+            // (addresses count in 16 bytes in the low bits of a descriptor; worked out for each
+            // product, they took this thread longer than the tensor cores need)
+            const uint64_t ka = k_desc + (uint64_t)((ks * 2 + h) * (kWtTile >> 4)),
+                           qa = q_desc + (uint64_t)(qs * (kRowTile >> 4));
+            const uint32_t d = tmem + (h * 2 + buf) * 128;
 #pragma unroll
             for (int k = 0; k < 8; ++k)
-              mma_smem(tmem + (h * 2 + buf) * 128,
-                       operand_desc(ka + (k >> 2) * kWtHalfTile + (k & 3) * 32, 16, 1024),
-                       operand_desc(qa + (k >> 2) * kRowHalf + (k & 3) * 32, 16, 1024), desc,
-                       k > 0);
+              mma_smem(d, ka + (k >> 2) * (kWtHalfTile >> 4) + (k & 3) * 2,
+                       qa + (k >> 2) * (kRowHalf >> 4) + (k & 3) * 2, desc, k > 0);
             mma_commit(&sh.s_full[h][buf]);
           }
           __syncwarp();
