@@ -382,21 +382,15 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
     }
     __syncwarp();
     int n = 0, nl = 0;  // tiles copied; with their log-sum-exps
+    constexpr int kParts = (kCols + 31) / 32;
+    int64_t place[kParts];  // of the lane's columns in a.lse
+#pragma unroll
+    for (int c = 0; c < kParts; ++c) {
+      const int col = c * 32 + lane, token = col / R;
+      place[c] = (int64_t)token * a.q_heads + (col - token * R);
+    }
     for (int round = 0; ok && walk.find(w, lane, item(round), x); ++round) {
       for (int t0 = rank; ok && t0 < x.tiles; t0 += kWtAhead * S) {
-        constexpr int kParts = (kCols + 31) / 32;
-        float z[kWtAhead][kParts];
-#pragma unroll
-        for (int y = 0; y < kWtAhead; ++y) {
-          const int i = x.from + (t0 + y * S) * T, cols = min(T, x.upto - i) * R;
-#pragma unroll
-          for (int c = 0; c < kParts; ++c) {
-            const int col = c * 32 + lane, token = col / R;
-            z[y][c] = col < cols ? -a.lse[(int64_t)(x.row0 + i + token) * a.q_heads + x.head * R +
-                                          (col - token * R)]
-                                 : -CUDART_INF_F;
-          }
-        }
         for (int y = 0; y < kWtAhead && t0 + y * S < x.tiles; ++y, ++n) {
           const int s = n % kRowSlots;
           if (n >= kRowSlots) {
@@ -417,6 +411,15 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
           __syncwarp();
         }
         if (!ok) break;
+        float z[kWtAhead][kParts];
+#pragma unroll
+        for (int y = 0; y < kWtAhead; ++y) {
+          const int i = x.from + (t0 + y * S) * T, cols = min(T, x.upto - i) * R;
+          const float* lse = a.lse + (int64_t)(x.row0 + i) * a.q_heads + x.head * R;
+#pragma unroll
+          for (int c = 0; c < kParts; ++c)
+            z[y][c] = c * 32 + lane < cols ? -lse[place[c]] : -CUDART_INF_F;
+        }
 #pragma unroll
         for (int y = 0; y < kWtAhead; ++y) {
           if (t0 + y * S >= x.tiles) break;
@@ -458,22 +461,29 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
         const int qs = nq % kRowSlots;
         const int cols = min(T, x.upto - x.from - t * T) * R;
         const uint32_t desc = product_desc(kBf16, (cols + 15) / 16 * 16, false);
-        ok = __all_sync(0xffffffffu,
-                        mbar_wait(&sh.q_full[qs], (uint32_t)((nq / kRowSlots) & 1), &sh.abort));
-        for (int h = first_half ? 0 : 1; ok && h < halves; ++h) {
-          const int buf = nq & 1, bit = h * 2 + buf;
-          if (used >> bit & 1)
-            ok = __all_sync(0xffffffffu,
-                            mbar_wait(&sh.s_free[h][buf], ~(turn >> bit) & 1, &sh.abort));
-          if (!ok) break;
+        // q and both places of scores, before the first product: a wait between them would come
+        // to more than the products take
+        const int buf = nq & 1;
+        bool there = mbar_wait(&sh.q_full[qs], (uint32_t)((nq / kRowSlots) & 1), &sh.abort);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int bit = h * 2 + buf;
+          if (h < (first_half ? 0 : 1) || h >= halves) continue;
+          if (there && (used >> bit & 1))
+            there = mbar_wait(&sh.s_free[h][buf], ~(turn >> bit) & 1, &sh.abort);
           used |= 1u << bit;
           turn ^= 1u << bit;
-          tmem_fence_after();
-          if (elect_one()) {
-            // (addresses count in 16 bytes in the low bits of a descriptor; worked out for each
-            // product, they took this thread longer than the tensor cores need)
-            const uint64_t ka = k_desc + (uint64_t)((ks * 2 + h) * (kWtTile >> 4)),
-                           qa = q_desc + (uint64_t)(qs * (kRowTile >> 4));
+        }
+        ok = __all_sync(0xffffffffu, there);
+        if (!ok) break;
+        tmem_fence_after();
+        if (elect_one()) {
+          // (addresses count in 16 bytes in the low bits of a descriptor)
+          const uint64_t qa = q_desc + (uint64_t)(qs * (kRowTile >> 4));
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (h < (first_half ? 0 : 1) || h >= halves) continue;
+            const uint64_t ka = k_desc + (uint64_t)((ks * 2 + h) * (kWtTile >> 4));
             const uint32_t d = tmem + (h * 2 + buf) * 128;
 #pragma unroll
             for (int k = 0; k < 8; ++k)
@@ -481,9 +491,8 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
                        qa + (k >> 2) * (kRowHalf >> 4) + (k & 3) * 2, desc, k > 0);
             mma_commit(&sh.s_full[h][buf]);
           }
-          __syncwarp();
+          mma_commit(&sh.q_empty[qs]);
         }
-        if (ok && elect_one()) mma_commit(&sh.q_empty[qs]);
         __syncwarp();
       }
       if (ok && elect_one()) mma_commit(&sh.k_empty[ks]);
