@@ -4,18 +4,28 @@
 // exp(scale * q_ir . k_j - lse_ir), with the log-sum-exp that the attention left.
 //
 // Bound: for single tokens HBM (K is read once, 256 bytes a key and head); for chunks the
-// special-function unit (one 2^x a pair, 16 a clock and SM) and, less, the tensor cores
-// (2 D flops a pair).
+// special-function unit (one 2^x a pair, 16 a clock and SM), then the tensor cores (2 D flops
+// a pair) and the board's power limit.
 //
 // Layout: an item is 256 keys of a request and KV head.  The product is taken with keys
 // along the rows of tensor memory, S^T = K Q^T, so that a thread owns a key and the sum over
-// rows needs no exchange: 8 warps read their key's scores of 128 (token, head) rows at a time
-// while the tensor cores make those of the next 128.  One warp issues the products, one
-// copies K (page piece by page piece), one Q, one the log-sum-exps; the next item's K is on
-// its way while one is worked on, so that single tokens stream.  CTAs take every n-th item
-// of all requests'; each warp finds them from the lengths by itself.  Where a call has few
-// items, a cluster takes one, each CTA every n-th tile of its rows, and the first CTA adds
-// their sums in order: a result does not depend on scheduling.
+// rows needs no exchange.  Sixteen warps sum, in two groups that take tiles of 128 (token,
+// head) rows in turn: while a group reads its keys' scores and adds up their exponentials, the
+// tensor cores make the next tile's for the other.  One warp issues the products, one copies
+// tiles of q and reads their log-sum-exps, two copy K, page piece by page piece, with the next
+// items' on its way while one is worked on, so that single tokens stream.  Clusters of one CTA
+// take every n-th item of all requests', back and forth; each warp finds them from the lengths
+// by itself.  Where a call has few items, larger clusters take them, each CTA every n-th tile,
+// and the first CTA adds their sums in order: a result does not depend on scheduling.
+//
+// Measured: 16 requests of 8k to 131k, a token each, 32 / 8 heads: 362 us, 6.5 TB/s (all that
+// the device copies); one at 32k: 18 us, of which 10.6 are its bytes' and the rest the way to
+// the first tile (lengths, page, K: 4 us), and from the last; 2048 tokens over 30720: 597 us,
+// 0.89 PFLOP/s at 990 W (a tile takes 2.4k clocks, of which its exponentials are 1.7k); a
+// prompt of 2048: 38 us, 17 of them in 16 tiles a CTA at 1.4 us, 8 before the first.
+// Tried: 8 warps that sum (880 us for the last but one), 64 columns of a tile for each group
+// (680 us), products of 64 columns that follow each other sooner (960 us: the tensor cores read
+// K again for each), two warps that issue (613 us, and 469 instead of 394 for single tokens).
 #include "paged_attention.cuh"
 #include "tensor.cuh"
 
@@ -36,6 +46,7 @@ enum WeightMode {
   kWtWhole,  // a CTA takes an item; K of two items and three tiles of q in shared memory
   kWtSplit,  // a cluster takes one; K of one, four tiles of q, and the sums of the other CTAs
   kWtFew     // at most 16 (token, head) rows a request: K of three, eight tiles of 16 rows
+             // (16 requests of 8k to 131k: 362 us; with K of two, as above, 545)
 };
 template <int kMode> struct WeightLayout {
   static constexpr int kKeySlots = kMode == kWtFew ? 3 : kMode == kWtSplit ? 1 : 2;
@@ -45,7 +56,8 @@ template <int kMode> struct WeightLayout {
   static constexpr int kRowTile = 2 * kRowHalf;
 };
 constexpr int kWtLseSlots = 3;
-constexpr int kWtFma = 6;                  // one pair in this many on the FMA pipe
+constexpr int kWtFma = 6;  // one pair in this many on the FMA pipe (none: 629 us, 12: 618, 8: 595,
+                           // 4: 652 and 3: 660 before the products were waited for in one go)
 constexpr int kWtColumns = 512;            // S^T: 2 halves of the keys, 2 tiles, 128 columns
 constexpr int kWtMaxCluster = 8;
 static_assert((kWtMaxCluster - 1) * kWtKeys * 4 <= kWtTile);
@@ -506,8 +518,7 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
       mbar_wait(&sh.drain, 0, &never);
     }
   } else {
-    // ---- sums: a thread per key and group; the groups take tiles in turn.  (64 columns of
-    // each tile: 680 us instead of 626 for 2048 tokens at 32k, a tile has its costs.)
+    // ---- sums: a thread per key and group; the groups take tiles in turn
     constexpr bool kFew = kMode == kWtFew;
     const int group = warp >> 3, h = (warp >> 2) & 1, key = tid & (kWtKeys - 1);
     const uint32_t my = tmem + ((uint32_t)((warp & 3) * 32) << 16) + h * 256;
@@ -797,7 +808,9 @@ extern "C" int tw_paged_weights(const tw_paged_weights_args* args, void* stream)
   w.few_tokens = w.group < 16 ? 16 / w.group : 1;
   w.box = 64;
   while (a.pool.page_size % w.box != 0) w.box /= 2;
-  // Bounds of the items and of a request's tiles: a cluster an item where CTAs would idle.
+  // Bounds of the items and of a request's tiles: a cluster an item where CTAs would idle (a
+  // prompt of 2048 tokens, 64 items: clusters of two 55 us, of four 38, of eight, of which the
+  // device holds 15, 55).
   int64_t most = a.max_q_len < a.tokens ? a.max_q_len : a.tokens;
   if (a.last > 0 && a.last < most) most = a.last;
   int64_t keys = a.max_kv_len;
