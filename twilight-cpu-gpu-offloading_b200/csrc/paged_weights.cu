@@ -19,9 +19,9 @@
 // and the first CTA adds their sums in order: a result does not depend on scheduling.
 //
 // Measured: 16 requests of 8k to 131k, a token each, 32 / 8 heads: 362 us, 6.5 TB/s (all that
-// the device copies); one at 32k: 18 us, of which 10.6 are its bytes' and the rest the way to
+// the device copies), 417 us in a run of a second, at 1010 W and 1.7 GHz; one at 32k: 18 us, of which 10.6 are its bytes' and the rest the way to
 // the first tile (lengths, page, K: 4 us), and from the last; 2048 tokens over 30720: 597 us,
-// 0.89 PFLOP/s at 990 W (a tile takes 2.4k clocks, of which its exponentials are 1.7k); a
+// 0.89 PFLOP/s, 669 us in a run of a second, at 1.78 GHz (a tile takes 2.4k clocks, of which its exponentials are 1.7k); a
 // prompt of 2048: 38 us, 17 of them in 16 tiles a CTA at 1.4 us, 8 before the first.
 // Tried: 8 warps that sum (880 us for the last but one), 64 columns of a tile for each group
 // (680 us), products of 64 columns that follow each other sooner (960 us: the tensor cores read
@@ -619,11 +619,27 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
             if (lane == 0) mbar_arrive(&sh.s_free[h][buf]);
           };
           if constexpr (kFew) {
-            float s[16];
-            tmem_ld16(s, at);
-            tmem_wait_ld(s);
-            read_all();
-            add(s, 0, std::integral_constant<int, 16>{});
+            // (no more columns than there are: in a long run, at the power limit, 16 requests take
+            // 417 us instead of 424)
+            if (cols <= 4) {
+              float s[4];
+              tmem_ld4(s, at);
+              tmem_wait_ld(s);
+              read_all();
+              add(s, 0, std::integral_constant<int, 4>{});
+            } else if (cols <= 8) {
+              float s[8];
+              tmem_ld8(s, at);
+              tmem_wait_ld(s);
+              read_all();
+              add(s, 0, std::integral_constant<int, 8>{});
+            } else {
+              float s[16];
+              tmem_ld16(s, at);
+              tmem_wait_ld(s);
+              read_all();
+              add(s, 0, std::integral_constant<int, 16>{});
+            }
           } else {
             // (each read is followed by its wait: a branch between them, and the compiler
             // may move the registers before they hold anything)

@@ -53,7 +53,30 @@ __device__ __forceinline__ void tmem_ld32(float (&r)[32], uint32_t tmem) {
         "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
       : "r"(tmem));
 }
-// 16 columns, and the wait for them.
+// 4, 8 and 16 columns, and the waits for them.
+__device__ __forceinline__ void tmem_ld4(float (&r)[4], uint32_t tmem) {
+  uint32_t* u = reinterpret_cast<uint32_t*>(r);
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3])
+               : "r"(tmem));
+}
+__device__ __forceinline__ void tmem_wait_ld(float (&r)[4]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3])::"memory");
+}
+__device__ __forceinline__ void tmem_ld8(float (&r)[8], uint32_t tmem) {
+  uint32_t* u = reinterpret_cast<uint32_t*>(r);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]),
+        "=r"(u[7])
+      : "r"(tmem));
+}
+__device__ __forceinline__ void tmem_wait_ld(float (&r)[8]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]),
+                 "+f"(r[6]), "+f"(r[7])::"memory");
+}
 __device__ __forceinline__ void tmem_ld16(float (&r)[16], uint32_t tmem) {
   uint32_t* u = reinterpret_cast<uint32_t*>(r);
   asm volatile(
