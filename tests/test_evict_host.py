@@ -102,7 +102,8 @@ def test_weights_checks(tw, change, status):
 
 @pytest.mark.parametrize("change,status", [
     (dict(requests=0), "TW_OK"), (dict(requests=-1), "TW_ERR_BAD_ARG"),
-    (dict(requests=8193), "TW_ERR_UNSUPPORTED"), (dict(max_len=(1 << 21) + 1), "TW_ERR_UNSUPPORTED"),
+    (dict(requests=8193), "TW_ERR_UNSUPPORTED"),
+    (dict(max_len=(1 << 21) + 1), "TW_ERR_UNSUPPORTED"),
     (dict(max_len=-1), "TW_ERR_BAD_ARG"), (dict(sink=-1), "TW_ERR_BAD_ARG"),
     (dict(recent=-1), "TW_ERR_BAD_ARG"), (dict(layers=0), "TW_ERR_BAD_ARG"),
     (dict(layers=2), "TW_ERR_BAD_ARG"), (dict(layers=2, layer_stride=12, record_layer_stride=320),
@@ -185,7 +186,10 @@ def test_frequencies(tw):
     got, scale = f(dims, base=base, scaling={"type": "yarn", "factor": factor,
                                              "original": original})
     assert scale == pytest.approx(0.1 * math.log(factor) + 1)
-    at = lambda t: dims * math.log(original / (t * 2 * math.pi)) / (2 * math.log(base))  # noqa: E731
+
+    def at(turns):
+        return dims * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(base))
+
     low, high = math.floor(at(32)), math.ceil(at(1))
     for n, (x, y) in enumerate(zip(plain, got.tolist())):
         slowed = min(1.0, max(0.0, (n - low) / (high - low)))

@@ -45,7 +45,8 @@ def test_far_positions(tw, cuda, layout):
     pos = torch.tensor([0, 1, -1, (1 << 24) + 1, 2 ** 31 - 1, -2 ** 31, 999_999_937],
                        dtype=torch.int32, device=cuda)
     x = normal(g, cuda, len(pos), 4, D, dtype=torch.float16)
-    f = torch.cat((torch.tensor([7.5, 1.0, 0.3]), torch.rand(61, generator=g) / 100)).double().to(cuda)
+    f = torch.cat((torch.tensor([7.5, 1.0, 0.3]), torch.rand(61, generator=g) / 100))
+    f = f.double().to(cuda)
     ref, tol = evict_ref.rope(x, pos, f, layout)
     assert within(tw.ops.rope(x, pos, f, layout=layout), ref, tol)
 

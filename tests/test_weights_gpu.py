@@ -34,7 +34,10 @@ def state(dev, seed, new, before, *, q_heads=8, kv_heads=2, page=16, dtype=torch
     if pool == "token":
         k = k.transpose(1, 2)
     k[..., 3] *= loud
-    k = k.to(dtype).to(dev) if pool == "head" else k.transpose(1, 2).to(dtype).to(dev).transpose(1, 2)
+    if pool == "token":  # [pages, rows, heads, D] in memory
+        k = k.transpose(1, 2).to(dtype).to(dev).transpose(1, 2)
+    else:
+        k = k.to(dtype).to(dev)
     q = torch.randn(sum(new) + pad, q_heads, D, generator=g).to(dtype).to(dev)
     i32 = dict(dtype=torch.int32, device=dev)
     cu = torch.tensor([0] + [sum(new[:i + 1]) for i in range(len(new))], **i32)

@@ -36,9 +36,9 @@ constexpr int kEvBins = 2048, kEvRounds = 3;
 constexpr int kEvMaxCluster = 8;
 constexpr int kEvMaxRequests = 8192;
 // A cluster is as large as this many rows a CTA ask for, if the device holds them all at once;
-// in any case so large that a CTA has no more than kEvMostRows.  (4160 rows: one CTA 22 us, two
-// 17, four 18, eight 22; the four layers above, 128 clusters: two CTAs 44 us, four 66, eight
-// 120 when all of these still took half as long again.)
+// in any case so large that a CTA has no more than kEvMostRows.  (4160 rows: one CTA 19 us, two
+// 17, four 18, eight 22; the four layers above, 128 clusters: two CTAs 44 us, four, of which
+// the device holds about half at once, 51, eight 93.)
 constexpr int kEvRowsPerCta = 4096, kEvCtas = 2 * 148, kEvMostRows = 16384;
 constexpr int kEvMaxRows = 1 << 21;        // of a request: 8 CTAs' bits of its rows
 constexpr int kEvSmem = 160 << 10;         // besides the histograms
@@ -197,7 +197,9 @@ __device__ void evict_lengths(const tw_paged_evict_args& a, uint32_t* s_back,
                               uint32_t* s_warp, int rank, int ctas) {
   const int tid = threadIdx.x;
   const int page = a.pool.page_size;
-  const auto pages = [&](int n) { return (int)(((unsigned)n + (unsigned)page - 1) / (unsigned)page); };
+  const auto pages = [&](int n) {
+    return (int)(((unsigned)n + (unsigned)page - 1) / (unsigned)page);
+  };
   long long base = 0;
   for (int b0 = 0; b0 < a.requests; b0 += kEvThreads) {
     const int b = b0 + tid;
@@ -337,7 +339,8 @@ paged_evict_kernel(const __grid_constant__ EvictWork w) {
         const int top = shift + bits;
         for (int i = tid; i < n; i += kEvThreads) {
           const uint32_t k = key(i);
-          if (k >> top == prefix >> top) atomicAdd(&sh.hist[round][k >> shift & ((1u << bits) - 1)], 1u);
+          if (k >> top == prefix >> top)
+            atomicAdd(&sh.hist[round][k >> shift & ((1u << bits) - 1)], 1u);
         }
       }
       cluster.sync();

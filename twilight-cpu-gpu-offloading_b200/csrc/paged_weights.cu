@@ -19,10 +19,11 @@
 // and the first CTA adds their sums in order: a result does not depend on scheduling.
 //
 // Measured: 16 requests of 8k to 131k, a token each, 32 / 8 heads: 362 us, 6.5 TB/s (all that
-// the device copies), 417 us in a run of a second, at 1010 W and 1.7 GHz; one at 32k: 18 us, of which 10.6 are its bytes' and the rest the way to
-// the first tile (lengths, page, K: 4 us), and from the last; 2048 tokens over 30720: 597 us,
-// 0.89 PFLOP/s, 669 us in a run of a second, at 1.78 GHz (a tile takes 2.4k clocks, of which its exponentials are 1.7k); a
-// prompt of 2048: 38 us, 17 of them in 16 tiles a CTA at 1.4 us, 8 before the first.
+// the device copies), and 412 us in a run of a second, at 1010 W and 1.7 GHz; one at 32k: 18
+// us, of which 10.6 are its bytes' and the rest the way to the first tile (lengths, page, K)
+// and from the last; 2048 tokens at 32k: 597 us, 0.89 PFLOP/s, and 668 us in a run of a
+// second, at 1.78 GHz (a tile takes 2.4k clocks, of which its exponentials are 1.7k); a prompt
+// of 2048: 38 us, of which 8 come before the first tile and 16 tiles a CTA take 1.5 each.
 // Tried: 8 warps that sum (880 us for the last but one), 64 columns of a tile for each group
 // (680 us), products of 64 columns that follow each other sooner (960 us: the tensor cores read
 // K again for each), two warps that issue (613 us, and 469 instead of 394 for single tokens).
@@ -256,7 +257,8 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
   static_assert(2 * kKeySlots * kWtTile + kRowSlots * kRowTile <=
                 (kSplit ? kWtSlots - 1 : kWtSlots) * kWtTile);
   const uint32_t keys_at = smem_addr(smem), rows_at = keys_at + 2 * kKeySlots * kWtTile;
-  float* s_part = reinterpret_cast<float*>(smem + (kWtSlots - 1) * kWtTile);  // kSplit: [rank - 1][key]
+  // kSplit: the other CTAs' sums, [rank - 1][key]
+  float* s_part = reinterpret_cast<float*>(smem + (kWtSlots - 1) * kWtTile);
   if (tid == 0) {
     for (int i = 0; i < kKeySlots; ++i) {
       mbar_init(&sh.k_full[i], 2);
@@ -459,7 +461,8 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
     }
   } else if (warp == kWtMmaWarp) {
     // ---- products
-    const uint64_t k_desc = operand_desc(keys_at, 16, 1024), q_desc = operand_desc(rows_at, 16, 1024);
+    const uint64_t k_desc = operand_desc(keys_at, 16, 1024);
+    const uint64_t q_desc = operand_desc(rows_at, 16, 1024);
     int nk = 0, nq = 0;
     uint32_t used = 0, turn = 0;  // a bit per buffer of scores: used before; its phase
     for (int round = 0; ok && walk.find(w, lane, item(round), x); ++round) {
@@ -564,10 +567,9 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
           int from = 0, to = cols;
           if (!plain) {
             from = held ? max(j - p, 0) * R : 0;
-            to = 0;
-            if (held)
-              to = a.window > 0 ? (int)max(min((long long)here, (long long)j + a.window - p), 0ll) * R
-                                : cols;
+            to = held ? cols : 0;
+            if (held && a.window > 0)
+              to = (int)max(min((long long)here, (long long)j + a.window - p), 0ll) * R;
           }
           const uint32_t at = my + buf * 128;
           uint64_t sum2[2] = {0ull, 0ull};
