@@ -220,3 +220,40 @@ def test_example(tw, cuda):
                           capture_output=True, text=True, timeout=300)
     assert done.returncode == 0, done.stderr[-2000:]
     assert "rows of 990 tokens" in done.stdout
+
+
+def test_two_caches_at_once(tw, cuda):
+    """Two caches on two streams, their kernels side by side: each gets what it gets alone."""
+    rotary = tw.RotaryPositions(128, base=10000.0, device=cuda)
+
+    def run(seed, stream):
+        g = torch.Generator().manual_seed(seed)
+        rows = torch.randn(700, 10, D, generator=g).to(torch.float16).to(cuda)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            cache = make(tw, cuda, num_layers=3, num_pages=120, max_tokens_per_request=800)
+            cache.pool.zero_()
+            at, outs = 0, []
+            for new in ([300, 1], [5, 260], [1, 1], [1, 40]):
+                n = sum(new)
+                cache.step(new)
+                for layer in range(3):
+                    q, k, v = rows[at:at + n].split((6, 2, 2), 1)
+                    q = cache.write_rotated(layer, q, k, v, rotary)
+                    outs.append(cache.attend(layer, q))
+                at += n
+                cache.evict(160, sink=2, recent=30)
+            return cache, outs
+
+    alone = [run(seed, torch.cuda.Stream(cuda)) for seed in (1, 2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(cuda) for _ in range(2)]
+    for _ in range(3):
+        both = [run(seed, s) for seed, s in zip((1, 2), streams)]
+        torch.cuda.synchronize()
+        for (a, x), (b, y) in zip(alone, both):
+            b.synchronize()
+            assert all(torch.equal(s, t) for s, t in zip(x, y))
+            assert torch.equal(a.row_weights, b.row_weights) and torch.equal(a.pool, b.pool)
+            assert torch.equal(a.row_positions, b.row_positions)
+            assert a.lengths == b.lengths and a.evicted == b.evicted

@@ -47,7 +47,8 @@ enum WeightMode {
   kWtWhole,  // a CTA takes an item; K of two items and three tiles of q in shared memory
   kWtSplit,  // a cluster takes one; K of one, four tiles of q, and the sums of the other CTAs
   kWtFew     // at most 16 (token, head) rows a request: K of three, eight tiles of 16 rows
-             // (16 requests of 8k to 131k: 362 us; with K of two, as above, 545)
+             // (the first kernel, K of two: 16 requests of 8k to 131k in 545 us; K of three
+             // and a second warp that copies it: 427)
 };
 template <int kMode> struct WeightLayout {
   static constexpr int kKeySlots = kMode == kWtFew ? 3 : kMode == kWtSplit ? 1 : 2;
