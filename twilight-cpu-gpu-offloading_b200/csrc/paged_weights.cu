@@ -11,15 +11,16 @@
 // along the rows of tensor memory, S^T = K Q^T, so that a thread owns a key and the sum over
 // rows needs no exchange.  Sixteen warps sum, in two groups that take tiles of 128 (token,
 // head) rows in turn: while a group reads its keys' scores and adds up their exponentials, the
-// tensor cores make the next tile's for the other.  One warp issues the products, one copies
+// tensor cores make the next tile's for the other.  (Of tiles of 16 rows one group takes all:
+// eight warps more that wait cost power, 405 us instead of 399 below.)  One warp issues the products, one copies
 // tiles of q and reads their log-sum-exps, two copy K, page piece by page piece, with the next
 // items' on its way while one is worked on, so that single tokens stream.  Clusters of one CTA
 // take every n-th item of all requests', back and forth; each warp finds them from the lengths
 // by itself.  Where a call has few items, larger clusters take them, each CTA every n-th tile,
 // and the first CTA adds their sums in order: a result does not depend on scheduling.
 //
-// Measured: 16 requests of 8k to 131k, a token each, 32 / 8 heads: 362 us, 6.5 TB/s (all that
-// the device copies), and 412 us in a run of a second, at 1010 W and 1.7 GHz; one at 32k: 18
+// Measured: 16 requests of 8k to 131k, a token each, 32 / 8 heads: 354 us, 6.7 TB/s (all that
+// the device copies), and 399 us in a run of a second, at 1010 W and 1.7 GHz; one at 32k: 17
 // us, of which 10.6 are its bytes' and the rest the way to the first tile (lengths, page, K)
 // and from the last; 2048 tokens at 32k: 597 us, 0.89 PFLOP/s, and 668 us in a run of a
 // second, at 1.78 GHz (a tile takes 2.4k clocks, of which its exponentials are 1.7k); a prompt
@@ -35,8 +36,6 @@
 namespace tw {
 
 constexpr int kWtKeys = 256, kWtCols = 128;
-constexpr int kWtThreads = 640;            // 512 of them sum, in two groups
-constexpr int kWtMmaWarp = 16, kWtRowWarp = 17, kWtKeyWarp = 18;  // and 19
 constexpr int kWtAhead = 2;                // tiles whose log-sum-exps are read at a time
 constexpr int kWtHalfTile = 128 * 128;     // bytes: 128 rows of 64 elements
 constexpr int kWtTile = 2 * kWtHalfTile;
@@ -56,6 +55,10 @@ template <int kMode> struct WeightLayout {
   static constexpr int kCols = kMode == kWtFew ? 16 : kWtCols;   // rows of a tile of q
   static constexpr int kRowHalf = kCols * 128;                   // bytes: 64 dimensions of them
   static constexpr int kRowTile = 2 * kRowHalf;
+  static constexpr int kGroups = kMode == kWtFew ? 1 : 2;        // of 256 threads that sum
+  static constexpr int kMmaWarp = 8 * kGroups, kRowWarp = kMmaWarp + 1;
+  static constexpr int kKeyWarp = kMmaWarp + 2;                  // and the next
+  static constexpr int kThreads = (kMmaWarp + 4) * 32;
 };
 constexpr int kWtLseSlots = 3;
 constexpr int kWtFma = 6;  // one pair in this many on the FMA pipe (none: 629 us, 12: 618, 8: 595,
@@ -237,7 +240,7 @@ __device__ __forceinline__ uint32_t first_bits(int n) {
 }
 
 template <bool kBf16, int kMode>
-__global__ void __launch_bounds__(kWtThreads, 1)
+__global__ void __launch_bounds__(WeightLayout<kMode>::kThreads, 1)
 paged_weights_kernel(const __grid_constant__ WeightWork w,
                      const __grid_constant__ CUtensorMap k_map,
                      const __grid_constant__ CUtensorMap q_map,
@@ -254,6 +257,7 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
   const int rank = kSplit ? (int)cluster_rank : 0, S = kSplit ? (int)cluster_ctas : 1;
   using Layout = WeightLayout<kMode>;
   constexpr int kKeySlots = Layout::kKeySlots, kRowSlots = Layout::kRowSlots;
+  constexpr int kMmaWarp = Layout::kMmaWarp, kKeyWarp = Layout::kKeyWarp;
   constexpr int kCols = Layout::kCols, kRowHalf = Layout::kRowHalf, kRowTile = Layout::kRowTile;
   static_assert(2 * kKeySlots * kWtTile + kRowSlots * kRowTile <=
                 (kSplit ? kWtSlots - 1 : kWtSlots) * kWtTile);
@@ -290,11 +294,11 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
   }
   // columns that no token fills (groups that do not divide 128) stay zero rows
   const int spare = (kCols - T * R) * 8;  // 16-byte vectors of 64 dimensions
-  for (int i = tid; i < kRowSlots * 2 * spare; i += kWtThreads)
+  for (int i = tid; i < kRowSlots * 2 * spare; i += Layout::kThreads)
     *reinterpret_cast<uint4*>(smem + 2 * kKeySlots * kWtTile + i / spare * kRowHalf + T * R * 128 +
                               i % spare * 16) = make_uint4(0u, 0u, 0u, 0u);
   fence_async_smem();
-  if (warp == kWtMmaWarp) tmem_alloc(&sh.tmem, kWtColumns);
+  if (warp == kMmaWarp) tmem_alloc(&sh.tmem, kWtColumns);
   tmem_fence_before();
   __syncthreads();
   tmem_fence_after();
@@ -315,9 +319,9 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
   bool ok = true;
   if (keys_at & 1023) {  // (what the layout of the products rests on)
     if (tid == 0) raise_error(a.error_flag, TW_ERR_UNSUPPORTED);
-  } else if (warp >= kWtKeyWarp) {
+  } else if (warp >= kKeyWarp) {
     // ---- K of the items: a warp for each 128 keys
-    const int h = warp - kWtKeyWarp;
+    const int h = warp - kKeyWarp;
     if (elect_one()) prefetch_map(&k_map);
     __syncwarp();
     const uint32_t box_bytes = (uint32_t)w.box * 128;  // of 64 dimensions
@@ -389,7 +393,7 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
       for (int i = max(n - kKeySlots, 0); i < n; ++i)
         mbar_wait(&sh.k_full[i % kKeySlots], (uint32_t)((i / kKeySlots) & 1), &never);
     }
-  } else if (warp == kWtRowWarp) {
+  } else if (warp == Layout::kRowWarp) {
     // ---- tiles of q and their rows' log-sum-exps
     if (elect_one()) {
       prefetch_map(&q_map);
@@ -460,7 +464,7 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
       for (int i = max(n - kRowSlots, 0); i < n; ++i)
         mbar_wait(&sh.q_full[i % kRowSlots], (uint32_t)((i / kRowSlots) & 1), &never);
     }
-  } else if (warp == kWtMmaWarp) {
+  } else if (warp == kMmaWarp) {
     // ---- products
     const uint64_t k_desc = operand_desc(keys_at, 16, 1024);
     const uint64_t q_desc = operand_desc(rows_at, 16, 1024);
@@ -536,8 +540,9 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
       // first, which so sees every phase of the barriers between CTAs (a group that left one out
       // would take an older phase for the one it waits for).
       const int tiles = x.tiles > rank ? (x.tiles - rank - 1) / S + 1 : 0;
-      const int last = kSplit || tiles != 1 ? 0 : nl & 1;
-      const bool both = tiles > 1 || (tiles == 1 && (nl & 1) != last), adds = group == last;
+      const int last = kSplit || kFew || tiles != 1 ? 0 : nl & 1;
+      const bool both = !kFew && (tiles > 1 || (tiles == 1 && (nl & 1) != last));
+      const bool adds = group == last;
       const int j = x.key0 + key;
       const bool held = j >= x.begin && j < x.end;
       int page = -1;
@@ -547,7 +552,7 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
       float sum = 0.f;
       for (int t = rank; t < x.tiles; t += S, ++nl) {
         const int buf = nl & 1;
-        if (buf != group) continue;
+        if (!kFew && buf != group) continue;
         const int ls = nl % kWtLseSlots;
         // (also by warps with no keys: they must not hand a slot back twice in a phase)
         ok = __all_sync(0xffffffffu, mbar_wait(&sh.lse_full[ls],
@@ -622,8 +627,7 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
             if (lane == 0) mbar_arrive(&sh.s_free[h][buf]);
           };
           if constexpr (kFew) {
-            // (no more columns than there are: in a long run, at the power limit, 16 requests take
-            // 417 us instead of 424)
+            // (no more columns than there are: 417 us instead of 424 in a run of a second)
             if (cols <= 4) {
               float s[4];
               tmem_ld4(s, at);
@@ -713,7 +717,7 @@ paged_weights_kernel(const __grid_constant__ WeightWork w,
   }
   __syncwarp();
   __syncthreads();
-  if (warp == kWtMmaWarp) {
+  if (warp == kMmaWarp) {
     tmem_fence_after();
     tmem_free(tmem, kWtColumns);
   }
@@ -737,7 +741,7 @@ static int resident_clusters(int cluster, int& n) {
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)cluster);
-  cfg.blockDim = dim3(kWtThreads);
+  cfg.blockDim = dim3(WeightLayout<kMode>::kThreads);
   cfg.dynamicSmemBytes = kWtSmem;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -786,7 +790,8 @@ static int launch_weights(const WeightWork& w, int cluster, int64_t items, cudaS
   if (rc == TW_OK) rc = resident_clusters<kBf16, kMode>(cluster, most);
   if (rc != TW_OK) return rc;
   const int64_t clusters = items < most ? items : most;
-  return launch_pdl_cluster(kernel, dim3((unsigned)(clusters * cluster)), dim3(kWtThreads), cluster,
+  return launch_pdl_cluster(kernel, dim3((unsigned)(clusters * cluster)),
+                            dim3(WeightLayout<kMode>::kThreads), cluster,
                             (size_t)kWtSmem, stream, w, k_map, q_map, few_map);
 }
 
