@@ -3,12 +3,14 @@
 // longer for one (16 us for an attention, 8.5 us for the others) than the device for a
 // short one.  Each call checks its tensors in one expression.  What it returns:
 //   None or the output tensor: done; an int > 0: the status of the C ABI;
-//   an int < 0: a tensor is not as wanted (the caller works out which).
+//   -1: a tensor is not as wanted (the caller works out which);
+//   -2: a tensor asks for a gradient, which this call does not give (rope only).
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAStream.h>
@@ -88,6 +90,7 @@ PyObject* status(int rc) {
   return PyLong_FromLong(rc);
 }
 PyObject* unexpected() { return PyLong_FromLong(-1); }
+PyObject* wants_gradient() { return PyLong_FromLong(-2); }
 
 // A whole number that fits the C ABI's int; false with a Python error otherwise.
 bool whole(PyObject* o, int& x) {
@@ -307,7 +310,7 @@ bool records(const at::Tensor* t, int dev, at::ScalarType type, const tw_paged_p
 // x, positions, frequencies, interleaved, scale, inverse, out
 PyObject* rope(PyObject*, PyObject* const* o, Py_ssize_t n) {
   return guarded(n, 7, [&]() -> PyObject* {
-    const at::Tensor *x = tensor(o[0]), *pos = tensor(o[1]), *out;
+    const at::Tensor *x = tensor(o[0]), *pos = tensor(o[1]), *f = tensor(o[2]), *out;
     int interleaved, inverse;
     double scale;
     if (!whole(o[3], interleaved) || !number(o[4], scale) || !whole(o[5], inverse)) return nullptr;
@@ -317,9 +320,12 @@ PyObject* rope(PyObject*, PyObject* const* o, Py_ssize_t n) {
     if (dev < 0 || !heads_of(x, dev) ||
         (x->scalar_type() != at::kHalf && x->scalar_type() != at::kBFloat16) ||
         x->size(1) > INT32_MAX || !vec(pos, dev, at::kInt, x->size(0)) ||
-        !rope_of(tensor(o[2]), dev, interleaved, scale, inverse, r) || !optional(o[6], out) ||
+        !rope_of(f, dev, interleaved, scale, inverse, r) || !optional(o[6], out) ||
         !rows(*x, xt, xh))
       return unexpected();
+    if (c10::GradMode::is_enabled() &&
+        (x->requires_grad() || f->requires_grad() || (out && out->requires_grad())))
+      return wants_gradient();
     at::Tensor made;
     if (!out) {
       made = at::empty({x->size(0), x->size(1), kHeadDim}, x->options());

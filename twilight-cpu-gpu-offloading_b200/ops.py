@@ -328,7 +328,7 @@ def qkv_rope(hidden: torch.Tensor, w_q: torch.Tensor, w_k: torch.Tensor, w_v: to
 
 
 # ------------------------------------------------------------- paged cache --
-# No backward passes: as with all ops here, results carry no gradient.
+# No backward passes: as with all ops here but rope, results carry no gradient.
 # Called for every step and layer, so these go through the compiled binding
 # (csrc/binding.cpp), which unpacks and checks the tensors; what is wrong with them is
 # worked out here when it finds that something is.
@@ -590,12 +590,20 @@ def rope(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, *,
 
     frequencies [pairs] float64 (rope_frequencies): pair n, dimensions (n, n + pairs) in the
     "half" layout and (2n, 2n + 1) in the "interleaved" one, turns by position * frequency and
-    is scaled; the other dimensions pass.  inverse: by the negative angle (the gradient of the
-    same call).  out: x itself, or rows that do not overlap it."""
+    is scaled; the other dimensions pass.  inverse: by the negative angle.  out: x itself, or
+    rows that do not overlap it.
+
+    Differentiable in x: the gradient is the same turn by the other angle.  With out, and by
+    frequencies, there is none: where one is asked for, the call is refused."""
     rc = _lib.binding().rope(x, positions, frequencies, _interleaved(layout), scale, bool(inverse),
                              out)
     if not isinstance(rc, int):
         return rc
+    if rc == -2:
+        if out is not None or frequencies.requires_grad:
+            raise ValueError("rope: no gradient goes through out or to the frequencies (leave out "
+                             "away, detach them, or call it under torch.no_grad)")
+        return _Rope.apply(x, positions, frequencies, layout, scale, bool(inverse))
     if rc < 0:
         dev = _explain_device(x)
         _kv_code(x.dtype)
@@ -605,6 +613,24 @@ def rope(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, *,
             _explain_rows(dev, "out", out, x.dtype, x.shape[0], x.shape[1], HEAD_DIM)
         raise ValueError("rope: unexpected tensors")
     _lib.check(rc, "rope")
+
+
+class _Rope(torch.autograd.Function):
+    """rope of rows that ask for a gradient."""
+
+    @staticmethod
+    def forward(ctx, x, positions, frequencies, layout, scale, inverse):
+        ctx.save_for_backward(positions, frequencies)
+        ctx.how = dict(layout=layout, scale=scale, inverse=not inverse)
+        return rope(x, positions, frequencies, layout=layout, scale=scale, inverse=inverse)
+
+    @staticmethod
+    def backward(ctx, dy):
+        positions, frequencies = ctx.saved_tensors
+        dy = dy.contiguous()  # (a sum's has strides of 0)
+        if dy.data_ptr() % 16:
+            dy = dy.clone()
+        return rope(dy, positions, frequencies, **ctx.how), None, None, None, None, None
 
 
 def _explain_records(dev: int, k_pages: torch.Tensor, row_weights, row_positions) -> None:

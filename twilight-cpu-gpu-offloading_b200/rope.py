@@ -26,6 +26,6 @@ class RotaryPositions:
 
     def __call__(self, x: torch.Tensor, positions: torch.Tensor, *, inverse: bool = False,
                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """Rows x [T, heads, 128] turned by positions [T] int32 (ops.rope)."""
+        """Rows x [T, heads, 128] turned by positions [T] int32 (ops.rope, differentiable in x)."""
         return ops.rope(x, positions, self.frequencies, layout=self.layout, scale=self.scale,
                         inverse=inverse, out=out)
