@@ -307,6 +307,12 @@ bool records(const at::Tensor* t, int dev, at::ScalarType type, const tw_paged_p
          t->is_contiguous();
 }
 
+// Autograd learns that a tensor of the caller's has been overwritten (inference tensors keep
+// no count).
+void overwritten(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // x, positions, frequencies, interleaved, scale, inverse, out
 PyObject* rope(PyObject*, PyObject* const* o, Py_ssize_t n) {
   return guarded(n, 7, [&]() -> PyObject* {
@@ -340,6 +346,7 @@ PyObject* rope(PyObject*, PyObject* const* o, Py_ssize_t n) {
                                 ot, oh, stream_of(dev));
     if (rc != TW_OK) return PyLong_FromLong(rc);
     if (!made.defined()) {
+      overwritten(*out);
       Py_INCREF(o[6]);
       return o[6];
     }
@@ -397,6 +404,7 @@ PyObject* paged_rope_write(PyObject*, PyObject* const* o, Py_ssize_t n) {
     const int rc = tw_paged_rope_write(&a, stream_of(dev));
     if (rc != TW_OK) return PyLong_FromLong(rc);
     if (!made.defined()) {
+      overwritten(*out);
       Py_INCREF(o[10]);
       return o[10];
     }
