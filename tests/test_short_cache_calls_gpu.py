@@ -1,11 +1,12 @@
-"""PagedKVCache kept short: a run in which rows are lost, and two caches whose kernels run at
-the same time."""
+"""PagedKVCache kept short: windows beside requests that wait, a run in which rows are
+lost, and two caches whose kernels run at the same time."""
 
 from __future__ import annotations
 
 import pytest
 import torch
 
+import evict_ref
 import paged_ref
 
 pytestmark = pytest.mark.gpu
@@ -30,6 +31,42 @@ def feed(cache, g, dev, new, **kw):
     x = rows(g, dev, plan.tokens)
     cache.write(0, x[:, :2], x[:, 2:4])
     return plan, x[:, 4:], cache.attend(0, x[:, 4:], **kw)
+
+
+def test_window_while_a_cut_request_waits(tw, cuda):
+    """A window is refused for tokens of a request that has lost rows, not for those of others
+    while it waits; and outputs and weights are then those of the window."""
+    g = torch.Generator().manual_seed(1)
+    cache = make(tw, cuda)
+    feed(cache, g, cuda, [90, 40])
+    cache.evict([50], sink=2, recent=8)
+    assert cache.evicted == [40, 0, 0]
+    weights = cache.row_weights[0].clone()
+    plan = cache.step([0, 30, 25])
+    x = rows(g, cuda, 55)
+    cache.write(0, x[:, :2], x[:, 2:4])
+    for r, i, n in ((1, 40, 30), (2, 0, 25)):
+        j = torch.arange(i, i + n, device=cuda)
+        weights[cache.block_table[r, j // 16].long(), :, j % 16] = 0
+    q, lse = x[:, 4:], torch.empty(55, 4, device=cuda)
+    out = cache.attend(0, q, window=20, lse=lse)
+    args = (q, cache.pool[0, 0], cache.pool[0, 1], cache.block_table, plan.cu_q, plan.kv_lens)
+    ref, _, tol, _ = paged_ref.attention(*args, window=20)
+    assert bool(((out.double() - ref).abs() <= tol).all())
+    wref, wtol = evict_ref.weights(args[0], args[1], *args[3:], lse, weights, window=20)
+    assert bool(((cache.row_weights[0].double() - wref).abs() <= wtol).all())
+    cache.step([1, 1])  # now it has a token
+    x = rows(g, cuda, 2)
+    cache.write(0, x[:, :2], x[:, 2:4])
+    with pytest.raises(ValueError, match="window"):
+        cache.attend(0, x[:, 4:], window=20)
+    cache.attend(0, x[:, 4:])
+    cache.step([-1, 1])  # it ends, another begins in its place
+    cache.step([5])
+    x = rows(g, cuda, 5)
+    cache.write(0, x[:, :2], x[:, 2:4])
+    cache.attend(0, x[:, 4:], window=3)
+    cache.synchronize()
 
 
 def test_a_run_loses_rows(tw, cuda):

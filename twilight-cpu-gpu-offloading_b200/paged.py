@@ -112,6 +112,7 @@ class PagedKVCache:
             self._offsets = torch.zeros(max_requests, **i32)
         self.free_pages = num_pages
         self._step: Optional[PagedStep] = None
+        self._step_lost = False  # some token of the step is of a request that has lost rows
 
     def _pages(self, tokens: int) -> int:
         return -(-tokens // self.page_size)
@@ -151,6 +152,7 @@ class PagedKVCache:
         self._turn, self._lens = now, kv_lens
         self.lengths, self.free_pages = after, free
         self.evicted = [0 if n < 0 else e for e, n in zip(self.evicted, new)]
+        self._step_lost = any(e and n > 0 for e, n in zip(self.evicted, new))
         self._step = PagedStep(tokens, cu_q, kv_lens, slots, positions,
                                max(0, *new), max(after))
         return self._step
@@ -200,14 +202,14 @@ class PagedKVCache:
         [tokens, q_heads, 128].  Keywords of ops.paged_attention (out, out_dtype, lse,
         softmax_scale, workspace).  With track_weights it adds what the tokens (last > 0: the
         last `last` of each request) gave each row; a window goes by rows, so it is refused
-        while any request that holds rows has lost some."""
+        for tokens of a request that has lost some (one that waits does not matter)."""
         k_pages, v_pages, step = self._layer(layer)
         if q.shape[0] != step.tokens:
             raise ValueError(f"the step has {step.tokens} tokens, got {q.shape[0]} rows")
         tracked = self.row_weights is not None
         if last and not tracked:
             raise ValueError("last: the cache does not track weights")
-        if window and any(e and l for e, l in zip(self.evicted, self.lengths)):
+        if window and self._step_lost:
             raise ValueError("no window over requests that have lost rows")
         if tracked and lse is None:
             lse = torch.empty(q.shape[:2], dtype=torch.float32, device=self.device)
