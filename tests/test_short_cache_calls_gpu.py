@@ -1,5 +1,5 @@
-"""PagedKVCache kept short: windows beside requests that wait, a run in which rows are
-lost, and two caches whose kernels run at the same time."""
+"""PagedKVCache kept short: windows beside requests that wait, budgets as numbers of any kind,
+a run in which rows are lost, and two caches whose kernels run at the same time."""
 
 from __future__ import annotations
 
@@ -67,6 +67,23 @@ def test_window_while_a_cut_request_waits(tw, cuda):
     cache.write(0, x[:, :2], x[:, 2:4])
     cache.attend(0, x[:, 4:], window=3)
     cache.synchronize()
+
+
+def test_budgets_of_any_kind(tw, cuda):
+    """One number for all requests, also one of NumPy's; numbers for each, in any sequence."""
+    np = pytest.importorskip("numpy")
+    for keep, want in ((np.int64(40), [40, 30, 40]), (np.int32(40), [40, 30, 40]),
+                       (np.array([40, -1], dtype=np.int64), [40, 30, 70]),
+                       (torch.tensor([-1, 20]), [90, 20, 70]), ((50,), [50, 30, 70])):
+        cache = make(tw, cuda)
+        feed(cache, torch.Generator().manual_seed(2), cuda, [90, 30, 70])
+        cache.evict(keep, sink=2, recent=8)
+        assert cache.lengths == want
+        cache.synchronize()
+        assert cache._lens.tolist() == want
+    cache = make(tw, cuda)
+    with pytest.raises(TypeError):
+        cache.evict(40.0, sink=2, recent=8)
 
 
 def test_a_run_loses_rows(tw, cuda):

@@ -34,6 +34,7 @@ from the rows held.
 
 from __future__ import annotations
 
+import numbers
 from dataclasses import dataclass
 from typing import Optional, Sequence
 
@@ -234,8 +235,8 @@ class PagedKVCache:
             raise ValueError("the cache does not track weights")
         if sink < 0 or recent < 0:
             raise ValueError("sink and recent must not be negative")
-        one = isinstance(keep, int)
-        wanted = [keep] * self.max_requests if one else [int(n) for n in keep]
+        one = isinstance(keep, numbers.Integral)  # (NumPy's too)
+        wanted = [int(keep)] * self.max_requests if one else [int(n) for n in keep]
         if len(wanted) > self.max_requests:
             raise ValueError(f"{len(wanted)} requests in a cache for {self.max_requests}")
         wanted += [-1] * (self.max_requests - len(wanted))
