@@ -61,7 +61,8 @@ __device__ __forceinline__ StepRequest step_request(int len, int fresh, int page
   return r;
 }
 
-__global__ void __launch_bounds__(kStepThreads) paged_step_kernel(tw_paged_step_args a, int32_t* offsets) {
+__global__ void __launch_bounds__(kStepThreads) paged_step_kernel(tw_paged_step_args a,
+                                                                  int32_t* offsets) {
   extern __shared__ int s_sums[];
   int* s_tokens = s_sums;                // inclusive prefix sums per request
   int* s_wanted = s_tokens + a.requests;

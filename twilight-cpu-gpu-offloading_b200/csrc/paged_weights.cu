@@ -4,27 +4,30 @@
 // exp(scale * q_ir . k_j - lse_ir), with the log-sum-exp that the attention left.
 //
 // Bound: for single tokens HBM (K is read once, 256 bytes a key and head); for chunks the
-// special-function unit (one 2^x a pair, 16 a clock and SM), then the tensor cores (2 D flops
-// a pair) and the board's power limit.
+// special-function unit (one 2^x a pair, 16 a clock and SM, but for the pairs in six whose 2^x
+// the FMA pipe works out where all of a piece is seen), then the tensor cores (2 D flops a
+// pair) and the board's power limit.
 //
 // Layout: an item is 256 keys of a request and KV head.  The product is taken with keys
 // along the rows of tensor memory, S^T = K Q^T, so that a thread owns a key and the sum over
 // rows needs no exchange.  Sixteen warps sum, in two groups that take tiles of 128 (token,
 // head) rows in turn: while a group reads its keys' scores and adds up their exponentials, the
 // tensor cores make the next tile's for the other.  (Of tiles of 16 rows one group takes all:
-// eight warps more that wait cost power, 405 us instead of 399 below.)  One warp issues the products, one copies
-// tiles of q and reads their log-sum-exps, two copy K, page piece by page piece, with the next
-// items' on its way while one is worked on, so that single tokens stream.  Clusters of one CTA
-// take every n-th item of all requests', back and forth; each warp finds them from the lengths
-// by itself.  Where a call has few items, larger clusters take them, each CTA every n-th tile,
-// and the first CTA adds their sums in order: a result does not depend on scheduling.
+// eight warps more that wait cost power, 405 us instead of 399 below.)  One warp issues the
+// products, one copies tiles of q and reads their log-sum-exps, two copy K, page piece by page
+// piece, with the next items' on its way while one is worked on, so that single tokens stream.
+// Clusters of one CTA take every n-th item of all requests', back and forth; each warp finds
+// them from the lengths by itself.  Where a call has few items, larger clusters take them, each
+// CTA every n-th tile, and the first CTA adds their sums in order: a result does not depend on
+// scheduling.
 //
-// Measured: 16 requests of 8k to 131k, a token each, 32 / 8 heads: 354 us, 6.7 TB/s (all that
-// the device copies), and 399 us in a run of a second, at 1010 W and 1.7 GHz; one at 32k: 17
-// us, of which 10.6 are its bytes' and the rest the way to the first tile (lengths, page, K)
-// and from the last; 2048 tokens at 32k: 597 us, 0.89 PFLOP/s, and 668 us in a run of a
-// second, at 1.78 GHz (a tile takes 2.4k clocks, of which its exponentials are 1.7k); a prompt
-// of 2048: 38 us, of which 8 come before the first tile and 16 tiles a CTA take 1.5 each.
+// Measured: 16 requests of 8k to 131k, a token each, 32 / 8 heads: 398 us in a run of a
+// second, 5.9 TB/s, at 1005 W and 1.73 GHz, and 355 to 367 in a few calls by themselves, 6.4
+// to 6.7 TB/s (reads alone; a copy moves 6.55); one at 32k: 17.4 us, of which 10.6 are its
+// bytes' and the rest the way to the first tile (lengths, page, K) and from the last; 2048
+// tokens at 32k: 665 us in a run of a second, 0.80 PFLOP/s, at 1.78 GHz, and 597 to 638 in a
+// few calls (a tile takes 2.4k clocks, of which its exponentials are 1.7k); a prompt of 2048:
+// 37.5 us, of which 8 come before the first tile and 16 tiles a CTA take 1.5 each.
 // Tried: 8 warps that sum (880 us for the last but one), 64 columns of a tile for each group
 // (680 us), products of 64 columns that follow each other sooner (960 us: the tensor cores read
 // K again for each), two warps that issue (613 us, and 469 instead of 394 for single tokens).
@@ -61,8 +64,10 @@ template <int kMode> struct WeightLayout {
   static constexpr int kThreads = (kMmaWarp + 4) * 32;
 };
 constexpr int kWtLseSlots = 3;
-constexpr int kWtFma = 6;  // one pair in this many on the FMA pipe (none: 629 us, 12: 618, 8: 595,
-                           // 4: 652 and 3: 660 before the products were waited for in one go)
+// One pair in this many on the FMA pipe.  2048 tokens at 32k, in a run of a second: none 671
+// us, 12: 671, 8: 666, 6: 664, 4: 698; in a few calls (two runs each): 641 and 645, 652 and
+// 616, 596 and 613, 638 and 638, 675 and 640.  A prompt of 2048: 38.6, 37.9, 38.0, 37.5, 38.0.
+constexpr int kWtFma = 6;
 constexpr int kWtColumns = 512;            // S^T: 2 halves of the keys, 2 tiles, 128 columns
 constexpr int kWtMaxCluster = 8;
 static_assert((kWtMaxCluster - 1) * kWtKeys * 4 <= kWtTile);
@@ -833,9 +838,15 @@ extern "C" int tw_paged_weights(const tw_paged_weights_args* args, void* stream)
   w.few_tokens = w.group < 16 ? 16 / w.group : 1;
   w.box = 64;
   while (a.pool.page_size % w.box != 0) w.box /= 2;
-  // Bounds of the items and of a request's tiles: a cluster an item where CTAs would idle (a
-  // prompt of 2048 tokens, 64 items: clusters of two 55 us, of four 38, of eight, of which the
-  // device holds 15, 55).
+  // Bounds of the items and of a request's tiles: a cluster an item where CTAs would idle.
+  // Prompts, us with clusters of two, four, eight (of which the device holds 15):
+  //   heads    256             512             1024            2048            4096 tokens
+  //   32 / 8   14  11 *11      19  14 *16      29  20 *25      52 *37  50     *95 110 137
+  //   16 / 4   13  11 *10      19  13 *11      29  19 *16      50  31 *30      93 *58  74
+  //   64 / 8   19  14 *12      30  19 *20      51  31 *33      96 *62  78    *180 206 231
+  // * what the rule takes.  It does not ask how many clusters the device holds, and where
+  // those of eight come in more than one round it loses (512 and 1024 tokens of 32 / 8 heads);
+  // single CTAs take 1.3 to 2 times as long as clusters of two.
   int64_t most = a.max_q_len < a.tokens ? a.max_q_len : a.tokens;
   if (a.last > 0 && a.last < most) most = a.last;
   int64_t keys = a.max_kv_len;

@@ -278,8 +278,12 @@ static int launch_rope(RopeWork& w, cudaStream_t stream) {
 }
 
 // Few rows: four a warp, so that they spread over more SMs; many: 16 a warp, which share its
-// angles.  701 tokens of 40 rows: 5.9 us with four, 4.6 with eight, 5.1 with 16; 8192 of 32
-// rows: 19.8 with eight, 18.4 with 16, 21.1 with 32.
+// angles.  us with four, eight, 16 a warp, in a graph of calls (up to 150k rows mostly in L2):
+//   rows         2.4k         9.4k         38k          75k          110k           300k
+//   40 a token   1.9 2.1 2.7  2.2 2.3 2.8  5.0 4.3 4.3  8.5 6.8 7.7  12  9.1  9.8   33 26 26
+//   48, written  2.1 2.2 2.4  2.4 2.3 2.5  5.1 4.3 3.8  9.3 7.6 7.6  13 10.2 10.3   36 27 27
+// 8192 tokens of 32 rows (262k), half of each turned: 19.8 with eight, 18.4 with 16, 21.1 with
+// 32, which is what 16 are for.
 template <typename T, bool kWrite>
 static int launch_rope(RopeWork& w, cudaStream_t stream) {
   const int64_t rows = w.tokens * (w.heads + (kWrite ? 2 * w.pool.kv_heads : 0));

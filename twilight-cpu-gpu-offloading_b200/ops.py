@@ -653,8 +653,9 @@ def paged_rope_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, position
     q [T, q_heads, 128], k / v [T, kv_heads, 128] (strided views are fine), positions and slots
     [T] as paged_step plans them (slot -1: nothing is written, q is turned all the same).
     Returns the turned q: q_out, which may be q itself and must not overlap an input
-    otherwise.  row_weights float32 / row_positions int32 [pages, kv_heads, page_size], what
-    paged_weights and paged_evict work on: the slots get 0 and the token's position."""
+    otherwise; no gradient goes through it (one does through rope).  row_weights float32 /
+    row_positions int32 [pages, kv_heads, page_size], what paged_weights and paged_evict work
+    on: the slots get 0 and the token's position."""
     rc = _lib.binding().paged_rope_write(q, k, v, positions, slots, frequencies, k_pages, v_pages,
                                          _interleaved(layout), scale, q_out, row_weights,
                                          row_positions, error_flag)

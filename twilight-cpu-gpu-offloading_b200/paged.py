@@ -12,11 +12,11 @@ A serving step is::
 
 Tables, slots and lengths are built on the device (ops.paged_step); the host keeps
 the lengths it gave, so nothing is read back and capacity is checked before a
-launch.  step() copies the numbers it is given to the device and waits for that copy,
-and so for what the stream holds before it.  Kernels see all max_requests rows, those of
-waiting requests too: a cache for many more requests than are served at a time divides
-its work less well than one of the right size.  A finished prompt can move to an offloaded cache for sparse decoding
-(to_offloaded).
+launch.  step() and evict() copy the numbers they are given to the device and wait for
+that copy, and so for what the stream holds before it.  Kernels see all max_requests rows,
+those of waiting requests too: a cache for many more requests than are served at a time
+divides its work less well than one of the right size.  A finished prompt can move to an
+offloaded cache for sparse decoding (to_offloaded).
 
 write_rotated turns q and k by their positions on the way.  With track_weights the cache
 keeps, for every row, its token's position and the attention weight that it has been given,
@@ -188,7 +188,8 @@ class PagedKVCache:
                       rotary: RotaryPositions, *,
                       q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """write() with q [tokens, q_heads, 128] and k turned by the step's positions, in one
-        launch; returns the turned q (q_out, which may be q itself)."""
+        launch; returns the turned q (q_out, which may be q itself).  No gradient goes
+        through it."""
         k_pages, v_pages, step = self._layer(layer)
         if q.shape[0] != step.tokens:
             raise ValueError(f"the step has {step.tokens} tokens, got {q.shape[0]} rows")
